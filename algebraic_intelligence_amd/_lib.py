@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_PKG, "_build", "libafa_hip.so")
 AFA_F32, AFA_BF16, AFA_F16, AFA_F64 = 0, 1, 2, 3
 FLAG_EXACT_TAIL, FLAG_GENERIC, FLAG_EXACT_REF, FLAG_SIMPLE_SCHEDULE = 0x1, 0x2, 0x4, 0x8
 FLAG_ACCUMULATE, FLAG_PARTIAL = 0x100, 0x200
+FLAG_ZERO_TAIL = 0x400
 
 (OK, ERR_NULL, ERR_DTYPE, ERR_SHAPE, ERR_HEAD_DIM, ERR_SINK, ERR_VALID_LEN, ERR_EPS, ERR_ROTARY,
  ERR_ALIGN, ERR_WORKSPACE, ERR_UNSUPPORTED, ERR_GAMMA, ERR_SCRATCH_LIMIT) = range(14)
@@ -49,6 +50,13 @@ SIGNATURES = {
     "ago_build_tables": (_int, [_int, _i64, _i64, _vp, _dbl, _vp, _vp, _vp]),
     "ago_rotate": (_int, [_int, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _i64, _vp]),
     "ago_rotate_qk": (_int, [_int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _vp, _vp, _i64, _int, _vp]),
+    "ago_rotate_axes": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int,
+                               _i64, _int, _vp, _int, _vp]),
+    "afa_paged_schedule_bytes": (_sz, [_vp]),
+    "afa_paged_build": (_int, [_vp, _vp, _vp, _vp, _vp]),
+    "afa_paged_append": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _vp]),
+    "afa_paged_workspace_size": (_sz, [_vp]),
+    "afa_paged_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _uint, _vp, _sz, _vp]),
     "oace_workspace_size": (_sz, [_int, _i64, _i64, _i64, _int, _uint]),
     "oace_linear_fwd": (_int, [_int, _i64, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _dbl, _dbl, _vp, _vp,
                                _uint, _vp, _sz, _vp]),

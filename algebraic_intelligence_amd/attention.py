@@ -7,6 +7,7 @@ Every computation runs in the gfx950 kernels of libafa_hip.so (include/afa.h).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -16,7 +17,7 @@ from . import _lib
 
 __all__ = [
     "octic_kernel", "algebraic_softmax", "CayleyRotary", "build_cayley_rotary_matrix",
-    "apply_ago_rotations", "rotate_tensor",
+    "apply_ago_rotations", "apply_ago_axis_rotations", "rotate_tensor",
 ]
 
 
@@ -363,3 +364,131 @@ def apply_ago_rotations(q, k, rotary_params=None, seq_axis=None):
         return rotate_tensor(q, c_raw, s_raw, seq_axis), rotate_tensor(k, c_raw, s_raw, seq_axis)
     c, s = _tables_for(q, c_raw, s_raw, seq_axis)
     return _RotatePair.apply(_float_input(q), _float_input(k), c, s, seq_axis % ndim)
+
+
+# ------------------------------------------------------------------- AGO by positions of several axes
+def _axis_tables(rotary_params, head_dim, dtype, dev):
+    """(c, s) device tables in fp32 (fp64 for fp64 inputs), contiguous, of one shape."""
+    c, s = _extract_cs(rotary_params)
+    want = torch.float64 if dtype == torch.float64 else torch.float32
+    if (isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype == want and s.dtype == want and c.ndim == 2
+            and head_dim % 2 == 0 and c.shape[1] == head_dim // 2 and c.shape == s.shape and c.device == dev
+            and s.device == dev and c.is_contiguous() and s.is_contiguous()):
+        return c, s  # as the kernel takes them
+    c, s = (_lib.table_2d(torch.as_tensor(t, device=dev), head_dim) for t in (c, s))
+    if c.shape != s.shape:
+        raise ValueError(f"rotary tables must match, got {tuple(c.shape)} and {tuple(s.shape)}")
+    return c.to(want).contiguous(), s.to(want).contiguous()
+
+
+def _axis_sections(sections, axes, pairs):
+    """The pairs of each axis as a C array; None (all pairs) where there is one axis and no sections."""
+    if not 1 <= axes <= 4:
+        raise ValueError(f"positions must have between 1 and 4 axes, got {axes}")
+    if sections is None:
+        if axes != 1:
+            raise ValueError("positions of several axes need sections, the feature pairs of each axis")
+        return None
+    sections = tuple(sections)
+    if len(sections) != axes or any(int(n) != n or n < 0 for n in sections) or sum(sections) > pairs:
+        raise ValueError(f"sections must be {axes} nonnegative integers with a sum of at most {pairs}, got {sections}")
+    return (ctypes.c_int32 * axes)(*(int(n) for n in sections))
+
+
+def _dense_like(x):
+    """An empty tensor of x's shape whose axes lie in memory in x's order, without gaps."""
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 or y.shape[-1] == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _axes_launch(xs, c, s, positions, cuts, axes, transpose):
+    """Each (B, H, L, D) tensor of xs (one or two of one dtype, batch and length) rotated, or back."""
+    dev = xs[0].device
+    xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
+    ys = [_dense_like(x) for x in xs]
+    B, H, L, D = xs[0].shape
+    k = xs[1] if len(xs) == 2 else None
+    strides = []
+    for pair in (xs, ys):
+        for t in pair:
+            strides.extend(t.stride()[:3])
+        if k is None:
+            strides.extend((0, 0, 0))
+    with _lib.on_device(dev):
+        rc = _lib.lib().ago_rotate_axes(
+            _lib.dtype_code(xs[0].dtype), B, H, 0 if k is None else k.shape[1], L, D, xs[0].data_ptr(), _lib.ptr(k),
+            ys[0].data_ptr(), None if k is None else ys[1].data_ptr(), (ctypes.c_int64 * 12)(*strides), c.data_ptr(),
+            s.data_ptr(), c.shape[0], positions.data_ptr(), positions.element_size(),
+            0 if positions.ndim == 2 else positions.stride(0), axes, cuts, int(transpose), _lib.stream_ptr(dev))
+    _lib.check(rc, "ago_rotate_axes")
+    return ys
+
+
+class _RotateAxes(torch.autograd.Function):
+    """Rotation of q, and of k where there is one, by positions of several axes; the VJP is the
+    transposed rotation of the cotangents, in one launch where both are there."""
+
+    @staticmethod
+    def forward(ctx, q, k, c, s, positions, cuts, axes, transpose):
+        ctx.save_for_backward(c, s, positions)
+        ctx.cfg = (cuts, axes, transpose)
+        ctx.set_materialize_grads(False)
+        if k is None:
+            return _axes_launch([q], c, s, positions, cuts, axes, transpose)[0]
+        out = _axes_launch([q, k], c, s, positions, cuts, axes, transpose)
+        fixed = [y for y, need in zip(out, ctx.needs_input_grad) if not need]
+        if fixed:
+            ctx.mark_non_differentiable(*fixed)
+        return tuple(out)
+
+    @staticmethod
+    def backward(ctx, gq, gk=None):
+        c, s, positions = ctx.saved_tensors
+        cuts, axes, transpose = ctx.cfg
+        args = (c, s, positions, cuts, axes, not transpose)
+        if gq is not None and gk is not None:
+            gq, gk = _RotateAxes.apply(gq, gk, *args)
+        else:
+            gq, gk = (None if g is None else _RotateAxes.apply(g, None, *args) for g in (gq, gk))
+        return gq, gk, None, None, None, None, None, None
+
+
+def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
+    """Cayley rotation by positions of several axes, such as time, height and width of a patch: beside
+    apply_ago_rotations (src/attention.py:207-240), which knows one position per row.
+
+    q (B, H, L, D) and k (B, H_kv, L, D) (None: q alone).  ``positions`` (B, L, A), or (L, A) for every
+    batch entry, int32 or int64, A up to 4: rows of the tables ``rotary_params``, a CayleyRotary or a
+    (c, s) pair of (rows, D / 2) tables.  ``sections`` names how many of the D / 2 feature pairs turn by each axis, in
+    order; pairs behind the last section stay as they are, and with one axis None means all.  Two axes with
+    frequencies of their own are columns of one table (``freqs`` of build_cayley_rotary_matrix).
+
+    Returns (q_rot, k_rot) (q_rot alone without k) in the inputs' dtype and axis order, formed in fp32
+    (fp64) from the tables as they are, with one rounding; a position outside the tables gives NaN.
+    Differentiable with respect to q and k, twice too."""
+    q = _float_input(q)
+    if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+        raise ValueError("q and k must have shapes (batch, heads, sequence, dimension), alike but for the heads, got "
+                         f"{tuple(q.shape)} and {None if k is None else tuple(k.shape)}")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
+    B, _, L, D = q.shape
+    if D % 2 != 0:
+        raise ValueError(f"Feature dimension must be even, got {D}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    if positions.ndim not in (2, 3) or positions.shape[-2] != L or (positions.ndim == 3 and positions.shape[0] not in (1, B)):
+        raise ValueError(f"positions must have shape ({B}, {L}, axes) or ({L}, axes), got {tuple(positions.shape)}")
+    axes = positions.shape[-1]
+    cuts = _axis_sections(sections, axes, D // 2)
+    _lib.dtype_code(q.dtype)
+    dev = _lib.require_device(q, k, positions)
+    c, s = _axis_tables(rotary_params, D, q.dtype, dev)
+    if positions.ndim == 3 and positions.shape[0] == 1:
+        positions = positions[0]
+    positions = positions.contiguous()
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        if q.numel() == 0:
+            return q.clone() if k is None else (q.clone(), k.clone())
+        return _RotateAxes.apply(q, None, c, s, positions, cuts, axes, False), k.clone()
+    return _RotateAxes.apply(q, k, c, s, positions, cuts, axes, False)

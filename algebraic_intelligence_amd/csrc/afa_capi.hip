@@ -101,6 +101,8 @@ int check_rotary(const void* rc, const void* rs, int64_t rot_len, int64_t L, int
 
 namespace afa {
 int hip_status_code(hipError_t e) { return hip_status(e); }
+int device_cus() { return cu_count(); }
+void* workspace_alloc(size_t bytes, hipStream_t s) { return scratch_alloc(bytes, s); }
 }  // namespace afa
 
 extern "C" {

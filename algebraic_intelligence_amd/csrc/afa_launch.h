@@ -97,6 +97,9 @@ struct GenArgs {
 
 // afa_status code of a HIP error (AFA_ERR_HIP, recording it for afa_last_hip_error).
 int hip_status_code(hipError_t e);
+// Compute units of the current device, and stream-ordered scratch from the library's pool (afa_capi.hip).
+int device_cus();
+void* workspace_alloc(size_t bytes, hipStream_t s);
 
 bool mfma_fwd_supported(int dtype, int head_dim);
 int mfma_fwd_queries_per_block(int head_dim);

@@ -261,6 +261,108 @@ int oace_softmax_loss_bwd(int dtype, int64_t rows, int64_t vocab, const void* lo
                           const int64_t* targets, double gamma, const void* row_cache,
                           const void* g_loss, void* dlogits, void* stream);
 
+/*
+ * Serving over a paged key/value cache: block tables and slots from request lengths, the cache
+ * write, and AFA of a tree of drafted tokens over the cached ones.  No counterpart in the
+ * reference, which trains only.
+ *
+ * Keys and values lie in pages (num_pages, kv_heads, page_size, head_dim) of one layer; the pages of
+ * request r are block_tables[r][0..held[r]).  `ring` holds the ids of the free pages as a queue of
+ * capacity num_pages: ring_state = {head, count}, free page i at ring[(head + i) % num_pages].
+ * A step packs the new tokens of all requests one after the other: request r's are rows
+ * starts[r] .. starts[r+1) of q, k and v, and token i of them has cache index cached[r] + i.
+ *
+ * afa_paged_plan describes the pool and one step's plan: sizes and device pointers, all owned by the
+ * caller.  afa_paged_build fills the plan's arrays for a step; afa_paged_append and afa_paged_fwd
+ * read them, for any number of layers.  Calls that share a plan must be ordered on one stream.
+ */
+typedef struct afa_paged_plan {
+  int64_t num_pages, page_size;      /* num_pages * page_size < 2^31; page_size any positive size */
+  int64_t requests, table_width;     /* block_tables (requests, table_width) */
+  int64_t max_tokens;                /* rows of q, k, v and of the arrays per token */
+  int64_t max_new;                   /* most new tokens of one request, <= max_tokens */
+  int64_t max_tree;                  /* 0: no trees; else 64, 128, 192 or 256: most nodes of a tree */
+  int64_t heads, kv_heads, head_dim; /* heads a multiple of kv_heads */
+  int64_t dtype;                     /* of q, k, v and the pages */
+  int32_t* block_tables;             /* entries outside [0, held) are -1 */
+  int32_t* held;                     /* (requests,) */
+  int32_t* ring;                     /* (num_pages,) */
+  int32_t* ring_state;               /* {head, count} */
+  int32_t* slots;                    /* (max_tokens,) page * page_size + offset; -1: none */
+  int32_t* positions;                /* (max_tokens,) cached + depth in the tree */
+  int32_t* token_request;            /* (max_tokens,) -1 behind the last request's tokens */
+  int32_t* starts;                   /* (requests + 1,) */
+  int32_t* status;                   /* (requests,) AFA_PAGED_* */
+  int64_t* masks;                    /* (max_tokens, max_tree / 64) bit i: sees drafted token i */
+  int32_t* schedule;                 /* afa_paged_schedule_bytes() bytes, 16-byte aligned */
+} afa_paged_plan;
+
+/* status of a request after afa_paged_build.  Any but OK: the request keeps the pages it held, its
+ * tokens have no slots and see no keys. */
+enum afa_paged_status {
+  AFA_PAGED_OK = 0,
+  AFA_PAGED_NO_PAGES = 1,  /* fewer pages are free than this and the earlier requests need */
+  AFA_PAGED_TOO_LONG = 2,  /* cached + new tokens exceed table_width pages */
+  AFA_PAGED_TOO_MANY = 3,  /* more than max_new new tokens */
+  AFA_PAGED_PAST_END = 4,  /* the packed tokens run past max_tokens */
+  AFA_PAGED_NEGATIVE = 5   /* a negative length */
+};
+
+/* Bytes of plan->schedule, or 0 where a size of the plan is not supported. */
+size_t afa_paged_schedule_bytes(const afa_paged_plan* plan);
+/*
+ * One step's plan from request lengths: cached (requests,) tokens in the cache, fresh (requests,) new
+ * tokens.  Every request is given the pages of cached + fresh tokens, from the head of the ring in
+ * request order; pages it holds beyond them go to the ring's end (and can be taken from the next
+ * call on), so a request of length 0 gives all back.  parents (max_tokens,), nullable: the index
+ * among its request's new tokens of the token that each drafted token follows, or -1 where it
+ * follows the cached ones; a value that is no earlier token counts as -1.  A token sees the cached tokens, itself
+ * and its ancestors.  Without parents, and in requests of more than max_tree new tokens, each token
+ * follows the one before it.
+ */
+int afa_paged_build(const afa_paged_plan* plan, const int32_t* cached, const int32_t* fresh,
+                    const int32_t* parents, void* stream);
+/*
+ * Rotates q and k of the step's tokens and stores k and v at the tokens' slots (a token without a
+ * slot is not stored).  q (max_tokens, heads, head_dim), k and v (max_tokens, kv_heads, head_dim) with
+ * strides {q_t, q_h, k_t, k_h, v_t, v_h} in elements (NULL: contiguous); q_out contiguous, nullable
+ * without tables.  page_strides {k_page, k_head, k_slot, v_page, v_head, v_slot} (NULL: contiguous).
+ * rot_cos, rot_sin (rot_len, head_dim / 2) in fp32 (fp64 for AFA_F64), nullable: no rotation.
+ * positions (max_tokens, axes) or NULL for the plan's (axes 1); sections: as in ago_rotate_axes.
+ */
+int afa_paged_append(const afa_paged_plan* plan, const void* q, const void* k, const void* v, const int64_t* strides,
+                     void* q_out, void* k_pages, void* v_pages, const int64_t* page_strides, const void* rot_cos,
+                     const void* rot_sin, int64_t rot_len, const int32_t* positions, int axes, const int32_t* sections,
+                     void* stream);
+/*
+ * AFA of the step's tokens over the cache: out_i = sum_j w_ij v_j / (sum_j w_ij + sink), w = rho(s)^8,
+ * over the cached tokens and the drafted ones that token i's mask shows.  q (max_tokens, heads, head_dim)
+ * with strides {q_t, q_h} (NULL: contiguous); masks: nullable, the plan's; out and denom (nullable,
+ * (max_tokens, heads), accumulation type) contiguous.  A row without a visible key is 0.  Rows behind the
+ * last request's are left as they were, or with AFA_FLAG_ZERO_TAIL set to 0.  A page id outside the
+ * pool holds no keys.  workspace: afa_paged_workspace_size() bytes, 16-byte aligned, or NULL.
+ */
+#define AFA_FLAG_ZERO_TAIL 0x400u
+size_t afa_paged_workspace_size(const afa_paged_plan* plan);
+int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
+                  const void* v_pages, const int64_t* page_strides, const int64_t* masks, void* out, void* denom,
+                  double sink_omega, unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Cayley rotation by positions of several axes (time, height, width): pair p of q and k at (b, l) is
+ * turned by row positions[b][l][a] of the tables, a the axis whose section holds p.  sections (host, axes of
+ * them, 1 to 4): pairs per axis, in order; pairs behind the last section stay as they are.  q (batch,
+ * q_heads, seq_len, head_dim), k (batch, k_heads, ...) nullable with k_heads 0; strides {q_b, q_h, q_l, k.., yq.., yk..}
+ * in elements, NULL: contiguous.  positions: int32 or int64 (pos_bytes 4 or 8), batch stride pos_b in positions
+ * (0: shared).  Tables (rot_len, head_dim / 2) fp32 (fp64 for AFA_F64), used as they are in fp32
+ * arithmetic, one rounding; a position outside them gives NaN.  transpose != 0: the inverse rotation,
+ * the VJP.
+ */
+int ago_rotate_axes(int dtype, int64_t batch, int64_t q_heads, int64_t k_heads, int64_t seq_len, int64_t head_dim,
+                    const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* rot_cos,
+                    const void* rot_sin, int64_t rot_len, const void* positions, int pos_bytes, int64_t pos_b, int axes,
+                    const int32_t* sections, int transpose, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
