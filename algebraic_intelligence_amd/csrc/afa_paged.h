@@ -96,6 +96,10 @@ struct PagedFwdArgs {
   int group, zero_tail;
 };
 hipError_t paged_fwd_generic_launch(const PagedFwdArgs& a, hipStream_t st);
+// Matrix-core path (afa_paged_mfma.hip): 16-byte aligned rows of q, pages and out.  ws: paged_fast_workspace bytes.
+bool paged_fast_supported(const afa_paged_plan& p);
+size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c);
+hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int cus, void* ws, hipStream_t st);
 
 struct RotateAxesArgs {
   const void *x[2];

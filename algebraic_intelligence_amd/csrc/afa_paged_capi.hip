@@ -1,6 +1,7 @@
 // C ABI of the paged-cache serving operators (include/afa.h): argument checks and dispatch.
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/afa.h"
 #include "afa_launch.h"
@@ -127,28 +128,26 @@ int afa_paged_append(const afa_paged_plan* plan, const void* q, const void* k, c
   a.tokens = (int)p.max_tokens; a.heads = (int)p.heads; a.kv_heads = (int)p.kv_heads; a.dim = (int)p.head_dim;
   a.page_size = (int)p.page_size;
   a.capacity = p.num_pages * p.page_size;
-  if (p.max_tokens * (p.heads + 2 * p.kv_heads) * ((p.head_dim + 1) / 2) > kLaunchThreads - 256) return AFA_ERR_SHAPE;
+  if (p.max_tokens > (kLaunchThreads - 256) / ((p.heads + 2 * p.kv_heads) * ((p.head_dim + 1) / 2))) return AFA_ERR_SHAPE;
   const hipError_t e = afa::paged_append_launch((int)p.dtype, a, (hipStream_t)stream);
   return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
 }
 
 size_t afa_paged_workspace_size(const afa_paged_plan* plan) {
-  if (plan == nullptr || check_sizes(*plan) != AFA_OK) return 0;
-  return 0;
+  if (plan == nullptr || check_sizes(*plan) != AFA_OK || !afa::paged_fast_supported(*plan)) return 0;
+  return afa::paged_fast_workspace(*plan, afa::paged_cut(*plan, afa::device_cus()));
 }
 
 int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
                   const void* v_pages, const int64_t* page_strides, const int64_t* masks, void* out, void* denom,
                   double sink_omega, unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   const int rc = check_plan(plan);
   if (rc != AFA_OK) return rc;
   if (q == nullptr || k_pages == nullptr || v_pages == nullptr || out == nullptr) return AFA_ERR_NULL;
   if (!(sink_omega >= 0.0 && sink_omega < INFINITY)) return AFA_ERR_SINK;
   const afa_paged_plan& p = *plan;
   if (masks != nullptr && p.max_tree == 0) return AFA_ERR_UNSUPPORTED;
-  if (p.max_tokens * p.heads > (kLaunchThreads - 1) / 256) return AFA_ERR_SHAPE;
+  if (p.max_tokens > (kLaunchThreads - 1) / 256 / p.heads) return AFA_ERR_SHAPE;
   afa::PagedFwdArgs a = {};
   a.plan = p;
   a.sched = afa::paged_schedule(p);
@@ -162,7 +161,33 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
   a.omega = sink_omega;
   a.group = (int)(p.heads / p.kv_heads);
   a.zero_tail = (flags & AFA_FLAG_ZERO_TAIL) != 0;
-  const hipError_t e = afa::paged_fwd_generic_launch(a, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  // 16-byte rows of q and of the pages, whose offsets within a tile take 31 bits
+  const int64_t unit = p.dtype == AFA_F32 ? 4 : 8;
+  bool fast = (flags & AFA_FLAG_GENERIC) == 0 && afa::paged_fast_supported(p) && aligned16(q) && aligned16(k_pages) &&
+              aligned16(v_pages) && aligned16(out) && a.q_t % unit == 0 && a.q_h % unit == 0;
+  for (int64_t v : {a.ps.k_page, a.ps.k_head, a.ps.k_slot, a.ps.v_page, a.ps.v_head, a.ps.v_slot}) fast = fast && v % unit == 0;
+  if (!fast) {
+    const hipError_t e = afa::paged_fwd_generic_launch(a, s);
+    return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
+  }
+  const int cus = afa::device_cus();
+  const afa::PagedCut cut = afa::paged_cut(p, cus);
+  const size_t need = afa::paged_fast_workspace(p, cut);
+  void* ws = workspace;
+  if (ws == nullptr) {
+    ws = afa::workspace_alloc(need, s);
+    if (ws == nullptr) return afa::hip_status_code(hipErrorOutOfMemory);
+  } else if (workspace_bytes < need) {
+    return AFA_ERR_WORKSPACE;
+  } else if (!aligned16(ws)) {
+    return AFA_ERR_ALIGN;
+  }
+  hipError_t e = afa::paged_fwd_fast_launch(a, cut, cus, ws, s);
+  if (workspace == nullptr) {
+    const hipError_t e2 = hipFreeAsync(ws, s);
+    if (e == hipSuccess) e = e2;
+  }
   return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
 }
 

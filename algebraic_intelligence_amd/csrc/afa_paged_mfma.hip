@@ -1,0 +1,510 @@
+// AFA of a serving step's tokens over the paged cache on the matrix cores (bf16, fp16, fp32; head_dim 32,
+// 48, 64, 96, 128, 256; pages of a power of two, 8 tokens or more).
+//
+//   out_i = sum_j w_ij v_j / (sum_j w_ij + Omega),  w_ij = rho(q_i.k_j / sqrt(D))^8
+//
+// The few query rows of a request that share a key/value head (its new tokens times the heads of the
+// group) meet every cached key once: the bytes of K and V bound the work.  A workgroup takes an item of
+// the plan, 16 QB rows and a run of 32-key tiles of one head, and its four waves a quarter of the run
+// each.  A wave needs no other until its end:
+//
+//   S^T = K Q^T    A = 16 keys, B = 16 rows; a lane ends with 8 keys' scores of row lane % 16
+//   w = rho^8      in place; they are the B operand of
+//   O^T += V^T w   A = the feature columns of V, formed in registers
+//
+// The order of the keys within a tile is free, so K's rows are handed to the lanes such that the 8 scores
+// of a lane belong to the 8 consecutive keys that it holds of V (16-bit types: keys 8g..8g+7 for lane
+// group g = lane / 16).  Likewise feature d = EPL * row + j is row `row` of product j: a lane reads EPL
+// consecutive features of 8 V rows, 16 lanes a whole row, and forms the columns by 4 byte permutes each.
+// No LDS, no barrier and no cross-lane step in the loop.
+//
+// The sums are additive: rows split over waves, and over workgroups where the plan cut the keys, are
+// joined by adding numerators and denominators in a fixed order (LDS; fp32 partials and a second launch).
+//
+// Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
+// the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
+// a row's weights are scaled by a power of two, lowered when a larger weight comes.
+#include "afa_common.h"
+#include "afa_paged.h"
+
+namespace afa {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+
+template <int DT>
+struct Paged16 {
+  static constexpr bool F32 = DT == AFA_F32;
+  static constexpr int ESZ = F32 ? 4 : 2;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (DT == AFA_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                  0);
+}
+
+// rho(s)^8 in fp32 with the square root and the reciprocal refined by one Newton step each: the
+// hardware's are off by 1 ulp, which three squarings make 8.
+__device__ __forceinline__ float rho8_refined(float s) {
+  const float a = __builtin_fabsf(s);
+  const float t = __builtin_fmaf(a, a, 1.0f);
+  const float r = __builtin_amdgcn_rsqf(t);
+  const float root = t * r;
+  const float rho = __builtin_fmaf(0.5f * r, __builtin_fmaf(-root, root, t), root) + a;
+  const float p2 = rho * rho;
+  const float p4 = p2 * p2;
+  const float p8 = p4 * p4;
+  const float i0 = __builtin_amdgcn_rcpf(p8);
+  const float inv = __builtin_fmaf(i0, __builtin_fmaf(-p8, i0, 1.0f), i0);
+  return s < 0.0f ? inv : p8;
+}
+
+// Bits of `len` consecutive drafted tokens from index i0 on (negative: cached, seen) that the row sees.
+// words: the row's masks, nullptr for a chain whose row is token `self`; n: the request's new tokens.
+__device__ __forceinline__ unsigned sees_bits(int i0, int len, int n, int self, const int64_t* words, int W) {
+  const unsigned all = (1u << len) - 1;
+  if (i0 + len <= 0) return all;
+  unsigned bits;
+  if (words != nullptr) {
+    const int at = max(i0, 0), w = at >> 6, sh = at & 63;
+    uint64_t x = 0;
+    if (w < W) x = (uint64_t)words[w] >> sh;
+    if (sh > 64 - len && w + 1 < W) x |= (uint64_t)words[w + 1] << (64 - sh);
+    bits = (unsigned)x & all;
+    if (i0 < 0) bits = (bits << -i0) | ((1u << -i0) - 1);
+  } else {
+    const int c = min(max(self + 1 - i0, 0), len);
+    bits = (1u << c) - 1;
+  }
+  const int live = min(max(n - i0, 0), len);
+  return bits & ((1u << live) - 1);
+}
+
+template <int DT>
+__device__ __forceinline__ bool nonfinite(unsigned w) {
+  if constexpr (DT == AFA_F32) return (w & 0x7f800000u) == 0x7f800000u;
+  constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
+  return (w & E) == E || (w >> 16 & E) == E;
+}
+
+struct PagedFast {
+  PagedFwdArgs a;
+  float* part;       // (kv_heads, max_parts, rows, D) numerators, then (kv_heads, max_parts, rows) sums
+  float* part_den;
+  int64_t max_parts;
+  int log_page, dim;
+};
+
+template <int DT, int DP, bool FULL, int QB>
+__global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) {
+  constexpr bool F32 = DT == AFA_F32;
+  constexpr int ESZ = F32 ? 4 : 2;
+  constexpr int EPL = DP / 16;            // features of V a lane, and products of O
+  constexpr int VW = EPL * ESZ / 4;       // their 32-bit words
+  constexpr int KS = F32 ? DP / 16 : DP / 32;  // 16-byte chunks of a K row a lane
+  constexpr int KB = F32 ? 16 : 32;       // features of a chunk over the four lane groups
+  constexpr int ROWS = 16 * QB, LD = DP + 4;
+  __shared__ float red[2][ROWS][LD];
+  __shared__ float red_den[4][ROWS];
+  const PagedFwdArgs& a = f.a;
+  const afa_paged_plan& p = a.plan;
+  const int D = FULL ? DP : f.dim;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64);
+  const float scale = (float)a.scale;
+  const int items = a.sched.header[PS_ITEMS];
+  const int64_t total = (int64_t)items * p.kv_heads;
+
+  for (int64_t w0 = blockIdx.x; w0 < total; w0 += gridDim.x) {
+    const int hk = (int)(w0 / items);
+    const PagedItem it = a.sched.items[w0 - (int64_t)hk * items];
+    if (it.tile0 >= it.tile1) continue;
+    const int c = it.cached, n = it.fresh, keys = c + n, nrows = n * G;
+    const bool tree = a.masks != nullptr && n <= p.max_tree;
+    const int32_t* table = p.block_tables + (int64_t)it.request * p.table_width;
+
+    // the rows of Q: chunk ks of a lane holds features KB ks + (16 / ESZ) g ..
+    u32x4_t qf[QB][KS];
+    int token[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const int row = it.row0 + 16 * b + m;
+      token[b] = min(row, nrows - 1) / G;
+      const int head = hk * G + min(row, nrows - 1) % G;
+      const char* q = (const char*)a.q + ((int64_t)(it.start + token[b]) * a.q_t + head * a.q_h) * ESZ;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = KB * ks + 16 / ESZ * g;
+        qf[b][ks] = FULL || d < D ? *(const u32x4_t*)(q + d * ESZ) : u32x4_t{0, 0, 0, 0};
+      }
+    }
+
+    f32x4_t acc[QB][EPL];
+    float den[QB], sc[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      den[b] = 0.0f;
+      sc[b] = 0x1p60f;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) acc[b][j] = f32x4_t{0, 0, 0, 0};
+    }
+
+    const int per = (it.tile1 - it.tile0 + 3) / 4;
+    const int t0 = it.tile0 + wave * per, t1 = min(t0 + per, it.tile1);
+    for (int t = t0; t < t1; ++t) {
+      const int kb = t * kPagedTile;
+      // Where a lane's K rows and V rows lie: groups of 8 consecutive keys (16-bit types: one of each;
+      // fp32: the two halves of the tile), each within a page.
+      constexpr int GR = F32 ? 2 : 1;
+      const char *kp[GR], *vp[GR];
+      bool lost[GR];  // the V group's page is none of the pool's
+#pragma unroll
+      for (int u = 0; u < GR; ++u) {
+        const int kk = F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3);
+        const int vk = F32 ? 16 * u + 4 * g : 8 * g;
+        const int kpos = min(kb + kk, keys - 1), vpos = min(kb + vk, keys - 1);
+        int kpage = table[kpos >> f.log_page], vpage = table[vpos >> f.log_page];
+        lost[u] = (unsigned)vpage >= (unsigned)p.num_pages;
+        if (lost[u]) vpage = 0;
+        if ((unsigned)kpage >= (unsigned)p.num_pages) kpage = 0;
+        const int mask = (1 << f.log_page) - 1;
+        kp[u] = (const char*)a.k_pages +
+                (kpage * a.ps.k_page + hk * a.ps.k_head + ((kb + kk) & mask) * a.ps.k_slot + 16 / ESZ * g) * ESZ;
+        vp[u] = (const char*)a.v_pages +
+                (vpage * a.ps.v_page + hk * a.ps.v_head + ((kb + vk) & mask) * a.ps.v_slot + EPL * m) * ESZ;
+      }
+      u32x4_t kf[2][KS];
+      unsigned vf[8][VW];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const char* r = F32 ? kp[F32 ? u : 0] : kp[0] + 4 * u * a.ps.k_slot * ESZ;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          kf[u][ks] = FULL || KB * ks + 16 / ESZ * g < D ? *(const u32x4_t*)(r + KB * ks * ESZ) : u32x4_t{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const char* r = F32 ? vp[F32 ? i >> 2 : 0] + (i & 3) * a.ps.v_slot * ESZ : vp[0] + i * a.ps.v_slot * ESZ;
+        if constexpr (VW == 2) {
+          u32x2_t x = {0, 0};
+          if (FULL || EPL * m < D) x = *(const u32x2_t*)r;
+          vf[i][0] = x[0];
+          vf[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int q4 = 0; q4 < VW / 4; ++q4) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (FULL || EPL * m + 16 / ESZ * q4 < D) x = *(const u32x4_t*)(r + 16 * q4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = x[e];
+          }
+        }
+      }
+
+      // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
+      // drafted values that are not finite are taken out of the product, in which a weight of 0 would
+      // not hide them, and added below to the rows that see them.
+      bool any_lost = lost[0];
+      if constexpr (F32) any_lost = any_lost || lost[GR - 1];
+      const bool masked = kb + kPagedTile > c || __ballot(any_lost) != 0;
+      bool odd = false;
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int pos = kb + (F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i);
+          const bool gone = pos >= keys || lost[F32 ? i >> 2 : 0];
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            const bool bad = pos >= c && nonfinite<DT>(vf[i][e]);
+            if (gone) {
+              vf[i][e] = 0;
+            } else if (bad) {
+              odd = true;
+              if constexpr (F32) {
+                vf[i][e] = 0;
+              } else {
+                constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
+                if ((vf[i][e] & E) == E) vf[i][e] &= 0xffff0000u;
+                if ((vf[i][e] >> 16 & E) == E) vf[i][e] &= 0xffffu;
+              }
+            }
+          }
+        }
+      }
+      const bool any_odd = masked && __ballot(odd) != 0;
+
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
+        f32x4_t s4[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s4[u] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const unsigned x = kf[u][ks][e], y = qf[b][ks][e];
+                s4[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y),
+                                                             s4[u], 0, 0, 0);
+              }
+            } else {
+              s4[u] = mma16<DT>(kf[u][ks], qf[b][ks], s4[u]);
+            }
+          }
+        }
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = s4[e >> 2][e & 3] * scale;
+          w[e] = F32 ? rho8_refined(s) : rho8_exact(s);
+        }
+        unsigned sees = 0xff;
+        if (masked) {
+          const int64_t* words = tree ? a.masks + (int64_t)(it.start + token[b]) * W : nullptr;
+          if constexpr (F32) {
+            sees = sees_bits(kb - c + 4 * g, 4, n, token[b], words, W) |
+                   sees_bits(kb - c + 16 + 4 * g, 4, n, token[b], words, W) << 4;
+            if (lost[0]) sees &= 0xf0;
+            if (lost[GR - 1]) sees &= 0x0f;
+          } else {
+            sees = lost[0] ? 0 : sees_bits(kb - c + 8 * g, 8, n, token[b], words, W);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = sees >> e & 1 ? w[e] : 0.0f;
+        }
+        den[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int j = 0; j < EPL; ++j)
+              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[e][j]), w[e], acc[b][j], 0, 0, 0);
+        } else {
+          if constexpr (DT == AFA_F16) {
+            float top = w[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, w[e]);
+            if (__ballot(!(top * sc[b] <= 32768.0f)) != 0) {
+              // a row's largest weight so far now lies in [16, 32)
+              top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+              top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+              if (top * sc[b] > 32768.0f && top < __builtin_inff()) {
+                const int e = (__builtin_bit_cast(int, top) >> 23) - 127;
+                const float to = __builtin_bit_cast(float, (127 + 4 - e) << 23);
+                const float ratio = to / sc[b];
+                sc[b] = to;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) acc[b][j] *= ratio;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] *= sc[b];
+          }
+          u32x4_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned x = Elem<DT>::pack(w[2 * e], w[2 * e + 1]);
+            hi[e] = x;
+            lo[e] = Elem<DT>::pack(w[2 * e] - Elem<DT>::lo(x), w[2 * e + 1] - Elem<DT>::hi(x));
+          }
+#pragma unroll
+          for (int j = 0; j < EPL; ++j) {
+            u32x4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+            acc[b][j] = mma16<DT>(v, hi, acc[b][j]);
+            acc[b][j] = mma16<DT>(v, lo, acc[b][j]);
+          }
+        }
+        if (any_odd) {
+          // the values that are not finite, key by key, from the pages
+          for (int from = 0; from < 4; ++from) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = kb + (F32 ? 16 * (e >> 2) + 4 * from + (e & 3) : 8 * from + e);
+              const float we = __shfl(w[e], 16 * from + m);
+              const bool see = __shfl((int)(sees >> e & 1), 16 * from + m) != 0;
+              if (key < c || key >= keys) continue;
+              const int page = table[key >> f.log_page];
+              if ((unsigned)page >= (unsigned)p.num_pages) continue;
+              const int64_t row = page * a.ps.v_page + hk * a.ps.v_head + (key & ((1 << f.log_page) - 1)) * a.ps.v_slot;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                  const int d = EPL * (4 * g + i) + j;
+                  if (!FULL && d >= D) continue;
+                  const float v = Elem<DT>::load(a.v_pages, row + d);
+                  if (see && !(__builtin_fabsf(v) < __builtin_inff())) acc[b][j][i] += we * v;
+                }
+            }
+          }
+        }
+      }
+    }
+
+    // join the waves: 0 and 1 store, 2 and 3 add to theirs
+    __syncthreads();  // red is free of the item before
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      den[b] += __shfl_xor(den[b], 16);
+      den[b] += __shfl_xor(den[b], 32);
+      if (g == 0) red_den[wave][16 * b + m] = den[b];
+      if constexpr (DT == AFA_F16) {
+        const float back = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc[b]));
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[b][j] *= back;
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if ((wave >> 1) == half) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < EPL; j += 4) {
+              f32x4_t* to = (f32x4_t*)&red[wave & 1][16 * b + m][EPL * (4 * g + i) + j];
+              f32x4_t x = {acc[b][j][i], acc[b][j + 1][i], acc[b][j + 2][i], acc[b][j + 3][i]};
+              *to = half ? *to + x : x;
+            }
+      }
+      __syncthreads();
+    }
+    const int mine = min(ROWS, nrows - it.row0), quads = D / 4;
+    for (int e = tid; e < mine * quads; e += 256) {
+      const int row = e / quads, d = 4 * (e - row * quads);
+      f32x4_t x = *(const f32x4_t*)&red[0][row][d] + *(const f32x4_t*)&red[1][row][d];
+      const float sum = (red_den[0][row] + red_den[1][row]) + (red_den[2][row] + red_den[3][row]);
+      if (it.part >= 0) {
+        const int64_t to = ((int64_t)hk * f.max_parts + it.part) * ROWS + row;
+        *(f32x4_t*)&f.part[to * D + d] = x;
+        if (d == 0) f.part_den[to] = sum;
+      } else {
+        const int64_t at = (int64_t)(it.start + (it.row0 + row) / G) * H + hk * G + (it.row0 + row) % G;
+        const float all = sum + (float)a.omega;
+        const float inv_zero = all == 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = inv_zero == 0.0f ? 0.0f : x[i] / all;
+        if constexpr (F32) {
+          *(f32x4_t*)((float*)a.out + at * D + d) = x;
+        } else {
+          u32x2_t y = {Elem<DT>::pack(x[0], x[1]), Elem<DT>::pack(x[2], x[3])};
+          *(u32x2_t*)((unsigned short*)a.out + at * D + d) = y;
+        }
+        if (d == 0 && a.denom != nullptr) ((float*)a.denom)[at] = all;
+      }
+    }
+  }
+}
+
+// The rows that no single item finished: those of cut requests from their parts, in the order of the
+// keys; those of requests that were not served (0); those behind the last request's (0, where asked for).
+// One wave a row.
+template <int DT>
+__global__ __launch_bounds__(256) void afa_paged_join_kernel(const PagedFast f, const int rows) {
+  const PagedFwdArgs& a = f.a;
+  const afa_paged_plan& p = a.plan;
+  const int lane = threadIdx.x & 63, H = (int)p.heads, G = a.group, D = f.dim;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= p.max_tokens * H) return;
+  const int t = (int)(at / H), h = (int)(at - (int64_t)t * H), hk = h / G, r = p.token_request[t];
+  if (r < 0 && !a.zero_tail) return;
+  const bool dead = r < 0 || p.status[r] != AFA_PAGED_OK;
+  int parts = 0;
+  int64_t from = 0;
+  if (!dead) {
+    const int chunks = a.sched.chunks[r];
+    if (chunks <= 1) return;
+    const int start = p.starts[r], n = p.starts[r + 1] - start, row = (t - start) * G + h % G;
+    const int block = row / rows, chunk = a.sched.header[PS_CHUNK];
+    const PagedItem& it = a.sched.items[a.sched.item[r]];
+    // the parts that hold keys: a chain's rows see none behind the last token of their block
+    const bool tree = p.max_tree > 0 && n <= p.max_tree;
+    const int last = tree ? n - 1 : min(n - 1, (block * rows + rows - 1) / G);
+    const int tiles = (it.cached + last + kPagedTile) / kPagedTile;
+    parts = (tiles + chunk - 1) / chunk;
+    from = ((int64_t)hk * f.max_parts + a.sched.part[r] + (int64_t)block * chunks) * rows + (row - block * rows);
+  }
+  float sum = 0.0f;
+  for (int i = 0; i < parts; ++i) sum += f.part_den[from + (int64_t)i * rows];
+  const float all = sum + (float)a.omega;
+  for (int d = lane; d < D; d += 64) {
+    float x = 0.0f;
+    for (int i = 0; i < parts; ++i) x += f.part[(from + (int64_t)i * rows) * D + d];
+    Elem<DT>::store(a.out, at * D + d, all == 0.0f || parts == 0 ? 0.0f : x / all);
+  }
+  if (lane == 0 && a.denom != nullptr) ((float*)a.denom)[at] = r < 0 ? 0.0f : all;
+}
+
+template <int DT, int DP, bool FULL>
+hipError_t tile_go(const PagedFast& f, int rows, unsigned grid, hipStream_t st) {
+  if (rows == 16) hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 1>), dim3(grid), dim3(256), 0, st, f);
+  else if (rows == 32) {
+    if constexpr (DT != AFA_F32 || DP < 256)
+      hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 2>), dim3(grid), dim3(256), 0, st, f);
+  } else {
+    if constexpr (DP <= (DT == AFA_F32 ? 64 : 128))
+      hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 4>), dim3(grid), dim3(256), 0, st, f);
+  }
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t fast_go(const PagedFast& f, int rows, unsigned grid, hipStream_t st) {
+  hipError_t e;
+  switch (f.dim) {
+    case 64: e = tile_go<DT, 64, true>(f, rows, grid, st); break;
+    case 128: e = tile_go<DT, 128, true>(f, rows, grid, st); break;
+    case 256: e = tile_go<DT, 256, true>(f, rows, grid, st); break;
+    case 96: e = tile_go<DT, 128, false>(f, rows, grid, st); break;
+    default: e = tile_go<DT, 64, false>(f, rows, grid, st); break;
+  }
+  if (e != hipSuccess) return e;
+  const int64_t out_rows = f.a.plan.max_tokens * f.a.plan.heads;
+  hipLaunchKernelGGL((afa_paged_join_kernel<DT>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, f, rows);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+bool paged_fast_supported(const afa_paged_plan& p) {
+  const int64_t d = p.head_dim;
+  return p.dtype != AFA_F64 && (d == 32 || d == 48 || d == 64 || d == 96 || d == 128 || d == 256) && p.page_size >= 8 &&
+         (p.page_size & (p.page_size - 1)) == 0;
+}
+
+size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c) {
+  return (size_t)(p.kv_heads * c.max_parts * c.rows) * (size_t)(p.head_dim + 1) * 4;
+}
+
+hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int cus, void* ws, hipStream_t st) {
+  PagedFast f;
+  f.a = a;
+  f.part = (float*)ws;
+  f.part_den = f.part + a.plan.kv_heads * c.max_parts * c.rows * a.plan.head_dim;
+  f.max_parts = c.max_parts;
+  f.dim = (int)a.plan.head_dim;
+  f.log_page = __builtin_ctzll((unsigned long long)a.plan.page_size);
+  const int64_t most = c.max_items * a.plan.kv_heads, fill = 4 * (int64_t)cus;
+  const unsigned grid = (unsigned)(most < fill ? most : fill);
+  switch ((int)a.plan.dtype) {
+    case AFA_F32: return fast_go<AFA_F32>(f, c.rows, grid, st);
+    case AFA_BF16: return fast_go<AFA_BF16>(f, c.rows, grid, st);
+    default: return fast_go<AFA_F16>(f, c.rows, grid, st);
+  }
+}
+
+}  // namespace afa

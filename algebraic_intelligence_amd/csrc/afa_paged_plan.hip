@@ -19,7 +19,9 @@ namespace afa {
 PagedCut paged_cut(const afa_paged_plan& p, int cus) {
   PagedCut c;
   const int64_t group = p.heads / p.kv_heads, most = p.max_new * group;
-  c.rows = most <= 16 ? 16 : most <= 32 ? 32 : 64;
+  // as many rows as a wave's registers hold beside a tile of K and V
+  const int64_t bytes = p.head_dim * (p.dtype == AFA_F32 ? 4 : 2), limit = bytes <= 256 ? 64 : bytes <= 512 ? 32 : 16;
+  c.rows = most <= 16 || limit == 16 ? 16 : most <= 32 || limit == 32 ? 32 : 64;
   const int64_t want = 2 * (int64_t)cus;
   c.target = (want + p.kv_heads - 1) / p.kv_heads;
   // Keys are cut into chunks of at least total / target tiles, total the sum of tiles over the row blocks.

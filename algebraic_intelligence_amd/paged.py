@@ -104,12 +104,11 @@ class DraftPlan:
     def __init__(self, pool: PagePool, max_tokens: int, *, heads: int, kv_heads: Optional[int] = None, head_dim: int,
                  dtype: torch.dtype, max_new: Optional[int] = None, max_tree: int = 64):
         kv_heads = heads if kv_heads is None else kv_heads
-        max_new = max_tokens if max_new is None else max_new
+        max_new = max_tokens if max_new is None else max_new  # a request cannot have more than all
         _positive(max_tokens=max_tokens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, max_new=max_new)
         if heads % kv_heads != 0:
             raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-        if max_new > max_tokens:
-            raise ValueError(f"max_new ({max_new}) must not exceed max_tokens ({max_tokens})")
+        max_new = min(max_new, max_tokens)
         if max_tree not in (0, 64, 128, 192, 256):
             raise ValueError(f"max_tree must be 0, 64, 128, 192 or 256, got {max_tree}")
         self.pool, self.dtype = pool, dtype

@@ -141,7 +141,7 @@ def test_pool_and_plan_sizes():
     with pytest.raises(ValueError, match="multiple"):
         A.DraftPlan(Pool(), 8, **{**new, "kv_heads": 3})
     with pytest.raises(ValueError, match="max_new"):
-        A.DraftPlan(Pool(), 8, max_new=9, **new)
+        A.DraftPlan(Pool(), 8, max_new=0, **new)
     with pytest.raises(ValueError, match="max_tree"):
         A.DraftPlan(Pool(), 8, max_tree=32, **new)
     with pytest.raises(ValueError, match="max_tokens"):
