@@ -162,11 +162,15 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
   a.group = (int)(p.heads / p.kv_heads);
   a.zero_tail = (flags & AFA_FLAG_ZERO_TAIL) != 0;
   hipStream_t s = (hipStream_t)stream;
-  // 16-byte rows of q and of the pages, whose offsets within a tile take 31 bits
+  // 16-byte rows of q and of the pages; byte offsets within a page, and its stride, in 32 bits
   const int64_t unit = p.dtype == AFA_F32 ? 4 : 8;
   bool fast = (flags & AFA_FLAG_GENERIC) == 0 && afa::paged_fast_supported(p) && aligned16(q) && aligned16(k_pages) &&
               aligned16(v_pages) && aligned16(out) && a.q_t % unit == 0 && a.q_h % unit == 0;
-  for (int64_t v : {a.ps.k_page, a.ps.k_head, a.ps.k_slot, a.ps.v_page, a.ps.v_head, a.ps.v_slot}) fast = fast && v % unit == 0;
+  for (int64_t v : {a.ps.k_page, a.ps.k_head, a.ps.k_slot, a.ps.v_page, a.ps.v_head, a.ps.v_slot})
+    fast = fast && v % unit == 0 && v >= 0;
+  const int64_t reach = (int64_t(1) << 30) / p.page_size;  // elements, of 4 bytes at most
+  for (int64_t v : {a.ps.k_slot, a.ps.v_slot}) fast = fast && v < reach - p.head_dim;
+  for (int64_t v : {a.ps.k_page, a.ps.v_page}) fast = fast && v < int64_t(1) << 30;
   if (!fast) {
     const hipError_t e = afa::paged_fwd_generic_launch(a, s);
     return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);

@@ -31,14 +31,6 @@ namespace afa {
 
 namespace {
 
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-
-template <int DT>
-struct Paged16 {
-  static constexpr bool F32 = DT == AFA_F32;
-  static constexpr int ESZ = F32 ? 4 : 2;
-};
-
 template <int DT>
 __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   if constexpr (DT == AFA_BF16)
@@ -99,25 +91,32 @@ struct PagedFast {
   float* part_den;
   int64_t max_parts;
   int log_page, dim;
+  uint32_t k_page, k_slot, v_page, v_slot;  // strides in bytes
 };
 
+// Waves for each SIMD that the registers are kept to: two where Q, the sums and a tile of K and V leave
+// room for them, one wave's loads then run under another's arithmetic.
+constexpr int paged_waves(bool f32, int dp, int qb) { return dp < 256 && dp * (f32 ? 2 : 1) * qb <= 256 ? 2 : 1; }
+
 template <int DT, int DP, bool FULL, int QB>
-__global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) {
+__global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_paged_tile_kernel(const PagedFast f) {
   constexpr bool F32 = DT == AFA_F32;
   constexpr int ESZ = F32 ? 4 : 2;
   constexpr int EPL = DP / 16;            // features of V a lane, and products of O
   constexpr int VW = EPL * ESZ / 4;       // their 32-bit words
   constexpr int KS = F32 ? DP / 16 : DP / 32;  // 16-byte chunks of a K row a lane
   constexpr int KB = F32 ? 16 : 32;       // features of a chunk over the four lane groups
+  constexpr int GR = F32 ? 2 : 1;         // groups of 8 keys that a lane reads of K, and of V
   constexpr int ROWS = 16 * QB, LD = DP + 4;
   __shared__ float red[2][ROWS][LD];
   __shared__ float red_den[4][ROWS];
+  __shared__ int red_odd[4];
   const PagedFwdArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
   const int D = FULL ? DP : f.dim;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64);
+  const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64), lp = f.log_page, in_page = (1 << lp) - 1;
   const float scale = (float)a.scale;
   const int items = a.sched.header[PS_ITEMS];
   const int64_t total = (int64_t)items * p.kv_heads;
@@ -129,16 +128,82 @@ __global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) 
     const int c = it.cached, n = it.fresh, keys = c + n, nrows = n * G;
     const bool tree = a.masks != nullptr && n <= p.max_tree;
     const int32_t* table = p.block_tables + (int64_t)it.request * p.table_width;
+    const char* k_base = (const char*)a.k_pages + hk * a.ps.k_head * ESZ;
+    const char* v_base = (const char*)a.v_pages + hk * a.ps.v_head * ESZ;
+    const int per = (it.tile1 - it.tile0 + 3) / 4;
+    const int t0 = it.tile0 + wave * per, t1 = min(t0 + per, it.tile1);
+
+    // 64 entries of the table, one a lane, from the page of the wave's first tile on
+    int entry0 = 0, entry = 0;
+    auto load_entries = [&](int t) {
+      entry0 = (t * kPagedTile) >> lp;
+      entry = table[min(entry0 + lane, (keys - 1) >> lp)];
+      if ((unsigned)entry >= (unsigned)p.num_pages) entry = -1;
+    };
+    // Where a lane's K and V rows of a tile lie: groups of 8 consecutive keys, each within a page.  lost: the
+    // V group's page is none of the pool's.
+    const char *kp[GR], *vp[GR];
+    bool lost[GR], lost_next[GR];
+    auto locate = [&](int t) {
+      const int kb = t * kPagedTile;
+      if (((kb + kPagedTile - 1) >> lp) - entry0 > 63) load_entries(t);
+#pragma unroll
+      for (int u = 0; u < GR; ++u) {
+        const int kpos = kb + (F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3)), vpos = kb + (F32 ? 16 * u + 4 * g : 8 * g);
+        const int kpage = __shfl(entry, (min(kpos, keys - 1) >> lp) - entry0);
+        const int vpage = __shfl(entry, (min(vpos, keys - 1) >> lp) - entry0);
+        lost_next[u] = vpage < 0;
+        kp[u] = k_base + (uint64_t)(uint32_t)max(kpage, 0) * f.k_page + ((uint32_t)(kpos & in_page) * f.k_slot + 16 * g);
+        vp[u] = v_base + (uint64_t)(uint32_t)max(vpage, 0) * f.v_page +
+                ((uint32_t)(vpos & in_page) * f.v_slot + EPL * ESZ * m);
+      }
+    };
+    u32x4_t kf[2][KS];
+    unsigned vf[8][VW];
+    auto load_k = [&]() {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const char* r = F32 ? kp[F32 ? u : 0] : kp[0] + 4 * u * f.k_slot;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          kf[u][ks] = FULL || KB * ks + 16 / ESZ * g < D ? *(const u32x4_t*)(r + KB * ks * ESZ) : u32x4_t{0, 0, 0, 0};
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const char* r = F32 ? vp[F32 ? i >> 2 : 0] + (i & 3) * f.v_slot : vp[0] + i * f.v_slot;
+        if constexpr (VW == 2) {
+          u32x2_t x = {0, 0};
+          if (FULL || EPL * m < D) x = *(const u32x2_t*)r;
+          vf[i][0] = x[0];
+          vf[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int q4 = 0; q4 < VW / 4; ++q4) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (FULL || EPL * m + 16 / ESZ * q4 < D) x = *(const u32x4_t*)(r + 16 * q4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = x[e];
+          }
+        }
+      }
+    };
+    if (t0 < t1) {
+      load_entries(t0);
+      locate(t0);
+      load_k();
+      load_v();
+    }
 
     // the rows of Q: chunk ks of a lane holds features KB ks + (16 / ESZ) g ..
     u32x4_t qf[QB][KS];
     int token[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-      const int row = it.row0 + 16 * b + m;
-      token[b] = min(row, nrows - 1) / G;
-      const int head = hk * G + min(row, nrows - 1) % G;
-      const char* q = (const char*)a.q + ((int64_t)(it.start + token[b]) * a.q_t + head * a.q_h) * ESZ;
+      const int row = min(it.row0 + 16 * b + m, nrows - 1);
+      token[b] = row / G;
+      const char* q = (const char*)a.q + ((int64_t)(it.start + token[b]) * a.q_t + (hk * G + row - token[b] * G) * a.q_h) * ESZ;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = KB * ks + 16 / ESZ * g;
@@ -155,121 +220,85 @@ __global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) 
 #pragma unroll
       for (int j = 0; j < EPL; ++j) acc[b][j] = f32x4_t{0, 0, 0, 0};
     }
+    bool any_odd = false;
 
-    const int per = (it.tile1 - it.tile0 + 3) / 4;
-    const int t0 = it.tile0 + wave * per, t1 = min(t0 + per, it.tile1);
     for (int t = t0; t < t1; ++t) {
       const int kb = t * kPagedTile;
-      // Where a lane's K rows and V rows lie: groups of 8 consecutive keys (16-bit types: one of each;
-      // fp32: the two halves of the tile), each within a page.
-      constexpr int GR = F32 ? 2 : 1;
-      const char *kp[GR], *vp[GR];
-      bool lost[GR];  // the V group's page is none of the pool's
 #pragma unroll
-      for (int u = 0; u < GR; ++u) {
-        const int kk = F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3);
-        const int vk = F32 ? 16 * u + 4 * g : 8 * g;
-        const int kpos = min(kb + kk, keys - 1), vpos = min(kb + vk, keys - 1);
-        int kpage = table[kpos >> f.log_page], vpage = table[vpos >> f.log_page];
-        lost[u] = (unsigned)vpage >= (unsigned)p.num_pages;
-        if (lost[u]) vpage = 0;
-        if ((unsigned)kpage >= (unsigned)p.num_pages) kpage = 0;
-        const int mask = (1 << f.log_page) - 1;
-        kp[u] = (const char*)a.k_pages +
-                (kpage * a.ps.k_page + hk * a.ps.k_head + ((kb + kk) & mask) * a.ps.k_slot + 16 / ESZ * g) * ESZ;
-        vp[u] = (const char*)a.v_pages +
-                (vpage * a.ps.v_page + hk * a.ps.v_head + ((kb + vk) & mask) * a.ps.v_slot + EPL * m) * ESZ;
-      }
-      u32x4_t kf[2][KS];
-      unsigned vf[8][VW];
+      for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
+      // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
+      f32x4_t s4[QB][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const char* r = F32 ? kp[F32 ? u : 0] : kp[0] + 4 * u * a.ps.k_slot * ESZ;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          kf[u][ks] = FULL || KB * ks + 16 / ESZ * g < D ? *(const u32x4_t*)(r + KB * ks * ESZ) : u32x4_t{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const char* r = F32 ? vp[F32 ? i >> 2 : 0] + (i & 3) * a.ps.v_slot * ESZ : vp[0] + i * a.ps.v_slot * ESZ;
-        if constexpr (VW == 2) {
-          u32x2_t x = {0, 0};
-          if (FULL || EPL * m < D) x = *(const u32x2_t*)r;
-          vf[i][0] = x[0];
-          vf[i][1] = x[1];
-        } else {
-#pragma unroll
-          for (int q4 = 0; q4 < VW / 4; ++q4) {
-            u32x4_t x = {0, 0, 0, 0};
-            if (FULL || EPL * m + 16 / ESZ * q4 < D) x = *(const u32x4_t*)(r + 16 * q4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = x[e];
-          }
-        }
-      }
-
-      // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
-      // drafted values that are not finite are taken out of the product, in which a weight of 0 would
-      // not hide them, and added below to the rows that see them.
-      bool any_lost = lost[0];
-      if constexpr (F32) any_lost = any_lost || lost[GR - 1];
-      const bool masked = kb + kPagedTile > c || __ballot(any_lost) != 0;
-      bool odd = false;
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int pos = kb + (F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i);
-          const bool gone = pos >= keys || lost[F32 ? i >> 2 : 0];
-#pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            const bool bad = pos >= c && nonfinite<DT>(vf[i][e]);
-            if (gone) {
-              vf[i][e] = 0;
-            } else if (bad) {
-              odd = true;
-              if constexpr (F32) {
-                vf[i][e] = 0;
-              } else {
-                constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
-                if ((vf[i][e] & E) == E) vf[i][e] &= 0xffff0000u;
-                if ((vf[i][e] >> 16 & E) == E) vf[i][e] &= 0xffffu;
-              }
-            }
-          }
-        }
-      }
-      const bool any_odd = masked && __ballot(odd) != 0;
-
-#pragma unroll
-      for (int b = 0; b < QB; ++b) {
-        // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
-        f32x4_t s4[2];
+      for (int b = 0; b < QB; ++b)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          s4[u] = f32x4_t{0, 0, 0, 0};
+          s4[b][u] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
             if constexpr (F32) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const unsigned x = kf[u][ks][e], y = qf[b][ks][e];
-                s4[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y),
-                                                             s4[u], 0, 0, 0);
+                s4[b][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y),
+                                                                s4[b][u], 0, 0, 0);
               }
             } else {
-              s4[u] = mma16<DT>(kf[u][ks], qf[b][ks], s4[u]);
+              s4[b][u] = mma16<DT>(kf[u][ks], qf[b][ks], s4[b][u]);
             }
           }
         }
+      // K of the next tile comes while this one's weights are formed, V while the next one's scores are
+      const bool more = t + 1 < t1;
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) {
+        locate(t + 1);
+        load_k();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
+      // drafted values that are not finite are taken out of the product, in which a weight of 0 would
+      // not hide them; the rows that see them get them at the end.
+      bool any_lost = lost[0];
+      if constexpr (F32) any_lost = any_lost || lost[GR - 1];
+      const bool masked = kb + kPagedTile > c || __ballot(any_lost) != 0;
+      if (masked) {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int pos = kb + (F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i);
+          const bool gone = pos >= keys || lost[F32 ? i >> 2 : 0];
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            unsigned x = gone ? 0u : vf[i][e];
+            if (pos >= c && nonfinite<DT>(x)) {
+              odd = true;
+              if constexpr (F32) {
+                x = 0;
+              } else {
+                constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
+                x &= ((x & E) == E ? 0xffff0000u : ~0u) & ((x >> 16 & E) == E ? 0xffffu : ~0u);
+              }
+            }
+            vf[i][e] = x;
+          }
+        }
+        any_odd = any_odd || __ballot(odd) != 0;
+      }
+
+      // Weights, in place of the scores in fp32, as planes otherwise.
+      u32x4_t hi[F32 ? 1 : QB], lo[F32 ? 1 : QB];
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float s = s4[e >> 2][e & 3] * scale;
+          const float s = s4[b][e >> 2][e & 3] * scale;
           w[e] = F32 ? rho8_refined(s) : rho8_exact(s);
         }
-        unsigned sees = 0xff;
         if (masked) {
           const int64_t* words = tree ? a.masks + (int64_t)(it.start + token[b]) * W : nullptr;
+          unsigned sees;
           if constexpr (F32) {
             sees = sees_bits(kb - c + 4 * g, 4, n, token[b], words, W) |
                    sees_bits(kb - c + 16 + 4 * g, 4, n, token[b], words, W) << 4;
@@ -282,13 +311,9 @@ __global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) 
           for (int e = 0; e < 8; ++e) w[e] = sees >> e & 1 ? w[e] : 0.0f;
         }
         den[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-
         if constexpr (F32) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int j = 0; j < EPL; ++j)
-              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[e][j]), w[e], acc[b][j], 0, 0, 0);
+          for (int e = 0; e < 8; ++e) s4[b][e >> 2][e & 3] = w[e];
         } else {
           if constexpr (DT == AFA_F16) {
             float top = w[0];
@@ -310,52 +335,42 @@ __global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) 
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] *= sc[b];
           }
-          u32x4_t hi, lo;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const unsigned x = Elem<DT>::pack(w[2 * e], w[2 * e + 1]);
-            hi[e] = x;
-            lo[e] = Elem<DT>::pack(w[2 * e] - Elem<DT>::lo(x), w[2 * e + 1] - Elem<DT>::hi(x));
-          }
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            u32x4_t v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-            acc[b][j] = mma16<DT>(v, hi, acc[b][j]);
-            acc[b][j] = mma16<DT>(v, lo, acc[b][j]);
-          }
-        }
-        if (any_odd) {
-          // the values that are not finite, key by key, from the pages
-          for (int from = 0; from < 4; ++from) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int key = kb + (F32 ? 16 * (e >> 2) + 4 * from + (e & 3) : 8 * from + e);
-              const float we = __shfl(w[e], 16 * from + m);
-              const bool see = __shfl((int)(sees >> e & 1), 16 * from + m) != 0;
-              if (key < c || key >= keys) continue;
-              const int page = table[key >> f.log_page];
-              if ((unsigned)page >= (unsigned)p.num_pages) continue;
-              const int64_t row = page * a.ps.v_page + hk * a.ps.v_head + (key & ((1 << f.log_page) - 1)) * a.ps.v_slot;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) {
-                  const int d = EPL * (4 * g + i) + j;
-                  if (!FULL && d >= D) continue;
-                  const float v = Elem<DT>::load(a.v_pages, row + d);
-                  if (see && !(__builtin_fabsf(v) < __builtin_inff())) acc[b][j][i] += we * v;
-                }
-            }
+            hi[b][e] = x;
+            lo[b][e] = Elem<DT>::pack(w[2 * e] - Elem<DT>::lo(x), w[2 * e + 1] - Elem<DT>::hi(x));
           }
         }
       }
+
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[e][j]), s4[b][e >> 2][e & 3],
+                                                               acc[b][j], 0, 0, 0);
+        } else {
+          u32x4_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int b = 0; b < QB; ++b) acc[b][j] = mma16<DT>(v, hi[b], acc[b][j]);
+#pragma unroll
+          for (int b = 0; b < QB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) load_v();
     }
 
     // join the waves: 0 and 1 store, 2 and 3 add to theirs
     __syncthreads();  // red is free of the item before
+    if (lane == 0) red_odd[wave] = any_odd;
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
       den[b] += __shfl_xor(den[b], 16);
@@ -383,21 +398,36 @@ __global__ __launch_bounds__(256) void afa_paged_tile_kernel(const PagedFast f) 
       }
       __syncthreads();
     }
+    const bool odd = (red_odd[0] | red_odd[1] | red_odd[2] | red_odd[3]) != 0;
     const int mine = min(ROWS, nrows - it.row0), quads = D / 4;
     for (int e = tid; e < mine * quads; e += 256) {
-      const int row = e / quads, d = 4 * (e - row * quads);
+      const int row = e / quads, d = 4 * (e - row * quads), who = (it.row0 + row) / G;
       f32x4_t x = *(const f32x4_t*)&red[0][row][d] + *(const f32x4_t*)&red[1][row][d];
       const float sum = (red_den[0][row] + red_den[1][row]) + (red_den[2][row] + red_den[3][row]);
+      if (odd) {
+        // drafted values that are not finite, of weights above 0: the value itself
+        const int64_t* words = a.masks + (int64_t)(it.start + who) * W;
+        for (int pos = max(it.tile0 * kPagedTile, c); pos < min(it.tile1 * kPagedTile, keys); ++pos) {
+          const bool sees = tree ? words[(pos - c) >> 6] >> ((pos - c) & 63) & 1 : pos - c <= who;
+          const int page = table[pos >> lp];
+          if (!sees || (unsigned)page >= (unsigned)p.num_pages) continue;
+          const char* v = v_base + (uint64_t)(uint32_t)page * f.v_page + (uint32_t)(pos & in_page) * f.v_slot;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = Elem<DT>::load(v, d + i);
+            if (!(__builtin_fabsf(y) < __builtin_inff())) x[i] += y;
+          }
+        }
+      }
       if (it.part >= 0) {
         const int64_t to = ((int64_t)hk * f.max_parts + it.part) * ROWS + row;
         *(f32x4_t*)&f.part[to * D + d] = x;
         if (d == 0) f.part_den[to] = sum;
       } else {
-        const int64_t at = (int64_t)(it.start + (it.row0 + row) / G) * H + hk * G + (it.row0 + row) % G;
+        const int64_t at = (int64_t)(it.start + who) * H + hk * G + (it.row0 + row - who * G);
         const float all = sum + (float)a.omega;
-        const float inv_zero = all == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = inv_zero == 0.0f ? 0.0f : x[i] / all;
+        for (int i = 0; i < 4; ++i) x[i] = all == 0.0f ? 0.0f : x[i] / all;
         if constexpr (F32) {
           *(f32x4_t*)((float*)a.out + at * D + d) = x;
         } else {
@@ -497,6 +527,11 @@ hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int c
   f.part_den = f.part + a.plan.kv_heads * c.max_parts * c.rows * a.plan.head_dim;
   f.max_parts = c.max_parts;
   f.dim = (int)a.plan.head_dim;
+  const uint32_t esz = a.plan.dtype == AFA_F32 ? 4 : 2;
+  f.k_page = (uint32_t)a.ps.k_page * esz;
+  f.k_slot = (uint32_t)a.ps.k_slot * esz;
+  f.v_page = (uint32_t)a.ps.v_page * esz;
+  f.v_slot = (uint32_t)a.ps.v_slot * esz;
   f.log_page = __builtin_ctzll((unsigned long long)a.plan.page_size);
   const int64_t most = c.max_items * a.plan.kv_heads, fill = 4 * (int64_t)cus;
   const unsigned grid = (unsigned)(most < fill ? most : fill);
