@@ -18,8 +18,16 @@ struct PagedItem {
   int request, row0, tile0, tile1, part, cached, fresh, start;
 };
 
-// plan->schedule: a header, five ints per request, then the items.
-enum { PS_ITEMS = 0, PS_CHUNK = 1, PS_HEAD = 2, PS_COUNT = 3, PS_INTS = 16 };
+// Key tiles that row block `block` of a request's n new tokens sees: all, or in a chain those up to the
+// block's last token.
+__host__ __device__ inline int paged_block_tiles(int c, int n, bool tree, int block, int rows, int group) {
+  const int64_t last = ((int64_t)block * rows + rows - 1) / group;
+  return (c + (tree || last >= n ? n - 1 : (int)last) + kPagedTile) / kPagedTile;
+}
+
+// plan->schedule: a header, six ints per request, the items, then a counter for each part of each key/value head.
+// The ticket and the counters are 0 between calls.
+enum { PS_ITEMS = 0, PS_CHUNK = 1, PS_TICKET = 2, PS_INTS = 16 };
 struct PagedSchedule {
   int* header;
   int *pop, *push, *held, *chunks, *part, *item;  // per request

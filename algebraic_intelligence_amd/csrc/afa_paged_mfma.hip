@@ -19,7 +19,8 @@
 // No LDS, no barrier and no cross-lane step in the loop.
 //
 // The sums are additive: rows split over waves, and over workgroups where the plan cut the keys, are
-// joined by adding numerators and denominators in a fixed order (LDS; fp32 partials and a second launch).
+// joined by adding numerators and denominators in a fixed order (LDS; fp32 parts that the last workgroup of a
+// row block to finish adds up).
 //
 // Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
 // the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
@@ -30,6 +31,8 @@
 namespace afa {
 
 namespace {
+
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 
 template <int DT>
 __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -87,12 +90,69 @@ __device__ __forceinline__ bool nonfinite(unsigned w) {
 
 struct PagedFast {
   PagedFwdArgs a;
-  float* part;       // (kv_heads, max_parts, rows, D) numerators, then (kv_heads, max_parts, rows) sums
-  float* part_den;
+  float* part;       // (kv_heads, max_parts, rows, D) numerators
+  float *part_den, *part_sum;  // (kv_heads, max_parts, rows) row sums of the parts, and of their groups
+  int* count;        // (kv_heads, max_parts), 0 between calls
   int64_t max_parts;
   int log_page, dim;
   uint32_t k_page, k_slot, v_page, v_slot;  // strides in bytes
 };
+
+// ------------------------------------------------------------------ parts of cut keys
+// Parts pass between workgroups by device-scope relaxed stores and loads, which go to where every XCD sees
+// them: a part's stores are complete (vmcnt 0) before its count, and the last to count reads after its
+// own.  An acquire and release edge would write back and invalidate the whole L2 for each part.
+typedef unsigned long long u64;
+__device__ __forceinline__ void put1(float* p, float x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get1(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put4(float* p, f32x4_t x) {
+  const f32x2_t a = {x[0], x[1]}, b = {x[2], x[3]};
+  __hip_atomic_store((u64*)p, __builtin_bit_cast(u64, a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((u64*)p + 1, __builtin_bit_cast(u64, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4_t get4(const float* p) {
+  const u64 x = __hip_atomic_load((const u64*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const u64 y = __hip_atomic_load((const u64*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const f32x2_t a = __builtin_bit_cast(f32x2_t, x), b = __builtin_bit_cast(f32x2_t, y);
+  return f32x4_t{a[0], a[1], b[0], b[1]};
+}
+
+// Whether this workgroup is the last of `n` to get here; its stores are complete before it counts.  The last
+// one leaves the count at 0.
+__device__ __forceinline__ bool arrived(int* count, int n, int* flag) {
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *flag = atomicAdd(count, 1) == n - 1;
+    if (*flag) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// Sum of four features and of the row sums over `n` parts, `stride` rows apart, in their order.
+__device__ __forceinline__ f32x4_t sum_parts(const float* part, const float* den, int n, int64_t stride, int D, float& sum) {
+  f32x4_t x = {0, 0, 0, 0};
+  sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    x += get4(part + i * stride * D);
+    sum += get1(den + i * stride);
+  }
+  return x;
+}
+
+// Parts are summed in groups, these by the last of each, and the groups by the last of them: one
+// workgroup reads at most about 2 sqrt(parts).
+__device__ __forceinline__ int group_size(int parts) {
+  if (parts <= 8) return parts;
+  const int s = (int)__builtin_sqrtf((float)parts);
+  return s * s < parts ? s + 1 : s;
+}
 
 // Waves for each SIMD that the registers are kept to: two where Q, the sums and a tile of K and V leave
 // room for them, one wave's loads then run under another's arithmetic.
@@ -110,7 +170,7 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   constexpr int ROWS = 16 * QB, LD = DP + 4;
   __shared__ float red[2][ROWS][LD];
   __shared__ float red_den[4][ROWS];
-  __shared__ int red_odd[4];
+  __shared__ int red_odd[4], flag;
   const PagedFwdArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
   const int D = FULL ? DP : f.dim;
@@ -120,6 +180,19 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   const float scale = (float)a.scale;
   const int items = a.sched.header[PS_ITEMS];
   const int64_t total = (int64_t)items * p.kv_heads;
+  // a row's four features d.. from its sums
+  auto store4 = [&](int64_t at, int d, f32x4_t x, float sum) {
+    const float all = sum + (float)a.omega;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = all == 0.0f ? 0.0f : x[i] / all;
+    if constexpr (F32) {
+      *(f32x4_t*)((float*)a.out + at * D + d) = x;
+    } else {
+      u32x2_t y = {Elem<DT>::pack(x[0], x[1]), Elem<DT>::pack(x[2], x[3])};
+      *(u32x2_t*)((unsigned short*)a.out + at * D + d) = y;
+    }
+    if (d == 0 && a.denom != nullptr) ((float*)a.denom)[at] = all;
+  };
 
   for (int64_t w0 = blockIdx.x; w0 < total; w0 += gridDim.x) {
     const int hk = (int)(w0 / items);
@@ -398,14 +471,19 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       }
       __syncthreads();
     }
+    auto out_row = [&](int row) {
+      const int who = (it.row0 + row) / G;
+      return (int64_t)(it.start + who) * H + hk * G + (it.row0 + row - who * G);
+    };
     const bool odd = (red_odd[0] | red_odd[1] | red_odd[2] | red_odd[3]) != 0;
     const int mine = min(ROWS, nrows - it.row0), quads = D / 4;
     for (int e = tid; e < mine * quads; e += 256) {
-      const int row = e / quads, d = 4 * (e - row * quads), who = (it.row0 + row) / G;
+      const int row = e / quads, d = 4 * (e - row * quads);
       f32x4_t x = *(const f32x4_t*)&red[0][row][d] + *(const f32x4_t*)&red[1][row][d];
       const float sum = (red_den[0][row] + red_den[1][row]) + (red_den[2][row] + red_den[3][row]);
       if (odd) {
         // drafted values that are not finite, of weights above 0: the value itself
+        const int who = (it.row0 + row) / G;
         const int64_t* words = a.masks + (int64_t)(it.start + who) * W;
         for (int pos = max(it.tile0 * kPagedTile, c); pos < min(it.tile1 * kPagedTile, keys); ++pos) {
           const bool sees = tree ? words[(pos - c) >> 6] >> ((pos - c) & 63) & 1 : pos - c <= who;
@@ -421,62 +499,64 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       }
       if (it.part >= 0) {
         const int64_t to = ((int64_t)hk * f.max_parts + it.part) * ROWS + row;
-        *(f32x4_t*)&f.part[to * D + d] = x;
-        if (d == 0) f.part_den[to] = sum;
+        put4(f.part + to * D + d, x);
+        if (d == 0) put1(f.part_den + to, sum);
       } else {
-        const int64_t at = (int64_t)(it.start + who) * H + hk * G + (it.row0 + row - who * G);
-        const float all = sum + (float)a.omega;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = all == 0.0f ? 0.0f : x[i] / all;
-        if constexpr (F32) {
-          *(f32x4_t*)((float*)a.out + at * D + d) = x;
-        } else {
-          u32x2_t y = {Elem<DT>::pack(x[0], x[1]), Elem<DT>::pack(x[2], x[3])};
-          *(u32x2_t*)((unsigned short*)a.out + at * D + d) = y;
-        }
-        if (d == 0 && a.denom != nullptr) ((float*)a.denom)[at] = all;
+        store4(out_row(row), d, x, sum);
       }
     }
-  }
-}
+    if (it.part < 0) continue;
 
-// The rows that no single item finished: those of cut requests from their parts, in the order of the
-// keys; those of requests that were not served (0); those behind the last request's (0, where asked for).
-// One wave a row.
-template <int DT>
-__global__ __launch_bounds__(256) void afa_paged_join_kernel(const PagedFast f, const int rows) {
-  const PagedFwdArgs& a = f.a;
-  const afa_paged_plan& p = a.plan;
-  const int lane = threadIdx.x & 63, H = (int)p.heads, G = a.group, D = f.dim;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= p.max_tokens * H) return;
-  const int t = (int)(at / H), h = (int)(at - (int64_t)t * H), hk = h / G, r = p.token_request[t];
-  if (r < 0 && !a.zero_tail) return;
-  const bool dead = r < 0 || p.status[r] != AFA_PAGED_OK;
-  int parts = 0;
-  int64_t from = 0;
-  if (!dead) {
-    const int chunks = a.sched.chunks[r];
-    if (chunks <= 1) return;
-    const int start = p.starts[r], n = p.starts[r + 1] - start, row = (t - start) * G + h % G;
-    const int block = row / rows, chunk = a.sched.header[PS_CHUNK];
-    const PagedItem& it = a.sched.items[a.sched.item[r]];
-    // the parts that hold keys: a chain's rows see none behind the last token of their block
-    const bool tree = p.max_tree > 0 && n <= p.max_tree;
-    const int last = tree ? n - 1 : min(n - 1, (block * rows + rows - 1) / G);
-    const int tiles = (it.cached + last + kPagedTile) / kPagedTile;
-    parts = (tiles + chunk - 1) / chunk;
-    from = ((int64_t)hk * f.max_parts + a.sched.part[r] + (int64_t)block * chunks) * rows + (row - block * rows);
+    const int chunk = a.sched.header[PS_CHUNK], ch = it.tile0 / chunk;
+    const int parts = (paged_block_tiles(c, n, tree, it.row0 / ROWS, ROWS, G) + chunk - 1) / chunk;
+    const int size = group_size(parts), groups = (parts + size - 1) / size, group = ch / size;
+    const int64_t base = (int64_t)hk * f.max_parts + it.part - ch, from = base + group * size;
+    const int here = min(size, parts - group * size);
+    if (!arrived(f.count + base + group, here, &flag)) continue;
+    for (int e = tid; e < mine * quads; e += 256) {
+      const int row = e / quads, d = 4 * (e - row * quads);
+      const int64_t at = from * ROWS + row;
+      float sum;
+      const f32x4_t x = sum_parts(f.part + at * D + d, f.part_den + at, here, ROWS, D, sum);
+      if (groups == 1) {
+        store4(out_row(row), d, x, sum);
+      } else {
+        // over the group's first part, of which this thread alone reads these features
+        put4(f.part + at * D + d, x);
+        if (d == 0) put1(f.part_sum + at, sum);
+      }
+    }
+    // 9 parts or more: fewer groups than parts - 1, so that this counter is none of theirs
+    if (groups == 1 || !arrived(f.count + base + parts - 1, groups, &flag)) continue;
+    for (int e = tid; e < mine * quads; e += 256) {
+      const int row = e / quads, d = 4 * (e - row * quads);
+      const int64_t at = base * ROWS + row;
+      float sum;
+      const f32x4_t x = sum_parts(f.part + at * D + d, f.part_sum + at, groups, (int64_t)size * ROWS, D, sum);
+      store4(out_row(row), d, x, sum);
+    }
   }
-  float sum = 0.0f;
-  for (int i = 0; i < parts; ++i) sum += f.part_den[from + (int64_t)i * rows];
-  const float all = sum + (float)a.omega;
-  for (int d = lane; d < D; d += 64) {
-    float x = 0.0f;
-    for (int i = 0; i < parts; ++i) x += f.part[(from + (int64_t)i * rows) * D + d];
-    Elem<DT>::store(a.out, at * D + d, all == 0.0f || parts == 0 ? 0.0f : x / all);
+
+  // The rows that no item has: those of requests that were not served, and those behind the last
+  // request's where they are asked for.  A lane looks at a token, its wave writes the row.
+  const int64_t waves = (int64_t)gridDim.x * 4, me = (int64_t)blockIdx.x * 4 + wave;
+  for (int64_t t0 = me; t0 < p.max_tokens; t0 += 64 * waves) {
+    const int64_t t = t0 + lane * waves;
+    int r = -1;
+    bool dead = false;
+    if (t < p.max_tokens) {
+      r = p.token_request[t];
+      dead = r < 0 ? a.zero_tail != 0 : p.status[r] != AFA_PAGED_OK;
+    }
+    for (u64 left = __ballot(dead); left != 0; left &= left - 1) {
+      const int which = __ffsll(left) - 1;
+      const int64_t row = (t0 + which * waves) * H;
+      const float all = __shfl(r, which) < 0 ? 0.0f : (float)a.omega;
+      for (int64_t e = lane; e < (int64_t)H * D; e += 64) Elem<DT>::store(a.out, row * D + e, 0.0f);
+      if (a.denom != nullptr)
+        for (int h = lane; h < H; h += 64) ((float*)a.denom)[row + h] = all;
+    }
   }
-  if (lane == 0 && a.denom != nullptr) ((float*)a.denom)[at] = r < 0 ? 0.0f : all;
 }
 
 template <int DT, int DP, bool FULL>
@@ -502,10 +582,7 @@ hipError_t fast_go(const PagedFast& f, int rows, unsigned grid, hipStream_t st) 
     case 96: e = tile_go<DT, 128, false>(f, rows, grid, st); break;
     default: e = tile_go<DT, 64, false>(f, rows, grid, st); break;
   }
-  if (e != hipSuccess) return e;
-  const int64_t out_rows = f.a.plan.max_tokens * f.a.plan.heads;
-  hipLaunchKernelGGL((afa_paged_join_kernel<DT>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, f, rows);
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace
@@ -517,7 +594,7 @@ bool paged_fast_supported(const afa_paged_plan& p) {
 }
 
 size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c) {
-  return (size_t)(p.kv_heads * c.max_parts * c.rows) * (size_t)(p.head_dim + 1) * 4;
+  return (size_t)(p.kv_heads * c.max_parts * c.rows) * (size_t)(p.head_dim + 2) * 4;
 }
 
 hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int cus, void* ws, hipStream_t st) {
@@ -525,6 +602,8 @@ hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int c
   f.a = a;
   f.part = (float*)ws;
   f.part_den = f.part + a.plan.kv_heads * c.max_parts * c.rows * a.plan.head_dim;
+  f.part_sum = f.part_den + a.plan.kv_heads * c.max_parts * c.rows;
+  f.count = (int*)(a.sched.items + c.max_items);
   f.max_parts = c.max_parts;
   f.dim = (int)a.plan.head_dim;
   const uint32_t esz = a.plan.dtype == AFA_F32 ? 4 : 2;

@@ -9,8 +9,8 @@
 // Popped places lie within the ring's free pages and pushed ones outside them, so that the two never
 // meet and each request can be served by its own workgroup, once the sums are known.
 //
-// The amounts of data are small and launches bound the work: one workgroup forms the sums over the
-// requests, then one workgroup per request does the rest.
+// The amounts of data are small and launches bound the work: one launch, in which every request's
+// workgroup forms the sums over all requests again (two launches beyond 1024 requests).
 #include "afa_common.h"
 #include "afa_paged.h"
 
@@ -33,187 +33,303 @@ PagedCut paged_cut(const afa_paged_plan& p, int cus) {
 
 size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c) {
   const int64_t ints = (PS_INTS + 6 * p.requests + 3) & ~(int64_t)3;
-  return (size_t)ints * 4 + (size_t)c.max_items * sizeof(PagedItem);
+  return (size_t)ints * 4 + (size_t)c.max_items * sizeof(PagedItem) + (size_t)(p.kv_heads * c.max_parts) * 4;
 }
 
 namespace {
 
-constexpr int SCAN = 1024;
 // Fewest tiles of a chunk: one for each wave of the attention's workgroups.
 constexpr int kMinChunk = 4;
+// Most requests whose sums every workgroup forms for itself, four a thread at most.
+constexpr int kOwnSums = 4 * kMaxTree;
 
-// Inclusive sum of v over the workgroup's threads, in thread order; `total` the sum of all.
-__device__ int64_t block_scan(int64_t v, int64_t* lds, int64_t& total) {
+struct Sums {
+  int64_t v[3];
+};
+
+// Sums of x over the threads before this one; `all` over all THREADS of the workgroup.
+template <int THREADS, int N>
+__device__ Sums block_before(Sums x, int64_t (*lds)[3], Sums& all) {
+  constexpr int WAVES = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Sums s = x;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t u = __shfl_up(s.v[k], o);
+      if (lane >= o) s.v[k] += u;
+    }
   __syncthreads();  // earlier reads of lds are over
-  if (lane == 63) lds[wave] = v;
+  if (lane == 63)
+#pragma unroll
+    for (int k = 0; k < N; ++k) lds[wave][k] = s.v[k];
   __syncthreads();
-  total = 0;
-  int64_t before = 0;
-  for (int w = 0; w < SCAN / 64; ++w) {
-    if (w == wave) before = total;
-    total += lds[w];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    int64_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w == wave) before = total;
+      total += lds[w][k];
+    }
+    s.v[k] += before - x.v[k];
+    all.v[k] = total;
   }
-  return before + v;
+  return s;
 }
 
-__global__ __launch_bounds__(SCAN) void afa_paged_scan_kernel(const afa_paged_plan p, const int rows, const int64_t target,
-                                                              const int32_t* cached, const int32_t* fresh) {
-  __shared__ int64_t lds[SCAN / 64];
-  const PagedSchedule s = paged_schedule(p);
-  const int R = (int)p.requests, P = (int)p.page_size, group = (int)(p.heads / p.kv_heads);
-  // within the ring whatever the arrays hold
-  const int NP = (int)p.num_pages, count = min(max(p.ring_state[1], 0), NP);
-  const int head = (int)((unsigned)p.ring_state[0] % (unsigned)NP);
-  int64_t tokens = 0, grown = 0, shrunk = 0, taken = 0, tiles = 0;
-  for (int base = 0; base < R; base += SCAN) {
-    const int r = base + threadIdx.x;
-    int c = 0, n = 0, held = 0, status = AFA_PAGED_OK;
-    if (r < R) {
-      c = cached[r];
-      n = fresh[r];
-      held = min(max(p.held[r], 0), (int)p.table_width);
-      if (c < 0 || n < 0) status = AFA_PAGED_NEGATIVE;
-      else if (n > p.max_new) status = AFA_PAGED_TOO_MANY;
-      else if ((int64_t)c + n > p.table_width * P) status = AFA_PAGED_TOO_LONG;
-    }
-    int64_t all;
-    const int64_t end = tokens + block_scan(max(n, 0), lds, all);
-    tokens += all;
-    if (status == AFA_PAGED_OK && n > 0 && end > p.max_tokens) status = AFA_PAGED_PAST_END;
-    int need = status == AFA_PAGED_OK ? (int)(((int64_t)c + n + P - 1) / P) : held;
-    const int grow = max(need - held, 0), shrink = max(held - need, 0);
-    const int64_t grow_end = grown + block_scan(grow, lds, all);
-    grown += all;
-    const int64_t shrink_end = shrunk + block_scan(shrink, lds, all);
-    shrunk += all;
-    if (grow > 0 && grow_end > count) {
-      status = AFA_PAGED_NO_PAGES;
-      need = held;
-    }
-    // the pages that are taken: the sum up to the last request that is served
-    block_scan(status == AFA_PAGED_OK ? grow : 0, lds, all);
-    taken += all;
-    const bool live = r < R && status == AFA_PAGED_OK && n > 0;
-    const int64_t blocks = live ? ((int64_t)n * group + rows - 1) / rows : 0;
-    block_scan(live ? blocks * ((c + n + kPagedTile - 1) / kPagedTile) : 0, lds, all);
-    tiles += all;
-    if (r < R) {
-      s.pop[r] = (int)((head + grow_end - grow) % NP);
-      s.push[r] = (int)((head + count + shrink_end - shrink) % NP);
-      s.held[r] = held;
-      p.held[r] = need;
-      p.status[r] = status;
-      p.starts[r + 1] = (int)min(end, p.max_tokens);
-      if (r == 0) p.starts[0] = 0;
-    }
-  }
-  const int64_t even = (tiles + target - 1) / target;
-  const int chunk = (int)max(even, (int64_t)kMinChunk);
-  int64_t items = 0, parts = 0;
-  for (int base = 0; base < R; base += SCAN) {
-    const int r = base + threadIdx.x;
-    int64_t blocks = 0, chunks = 0;
-    if (r < R && p.status[r] == AFA_PAGED_OK && fresh[r] > 0) {
-      blocks = ((int64_t)fresh[r] * group + rows - 1) / rows;
-      chunks = ((cached[r] + fresh[r] + kPagedTile - 1) / kPagedTile + chunk - 1) / chunk;
-    }
-    int64_t all;
-    const int64_t mine = blocks * chunks, split = chunks > 1 ? mine : 0;
-    const int64_t item_end = items + block_scan(mine, lds, all);
-    items += all;
-    const int64_t part_end = parts + block_scan(split, lds, all);
-    parts += all;
-    if (r < R) {
-      s.item[r] = (int)(item_end - mine);
-      s.part[r] = (int)(part_end - split);
-      s.chunks[r] = (int)chunks;
-    }
-  }
-  if (threadIdx.x == 0) {
-    s.header[PS_ITEMS] = (int)items;
-    s.header[PS_CHUNK] = chunk;
-    s.header[PS_HEAD] = head;
-    s.header[PS_COUNT] = count;
-    p.ring_state[0] = (int)((head + taken) % NP);
-    p.ring_state[1] = (int)(count - taken + shrunk);
-  }
+struct Lengths {
+  int c, n, held;
+};
+
+// One request: what it asks for and what it gets.
+struct Request {
+  int c, n, held, need, status;
+  int64_t blocks, tiles;  // row blocks and key tiles of its attention, 0 where it has none
+};
+
+__device__ __forceinline__ Request request(const afa_paged_plan& p, const Lengths& x) {
+  Request q;
+  q.c = x.c;
+  q.n = x.n;
+  q.held = min(max(x.held, 0), (int)p.table_width);
+  const int P = (int)p.page_size;
+  q.status = AFA_PAGED_OK;
+  if (q.c < 0 || q.n < 0) q.status = AFA_PAGED_NEGATIVE;
+  else if (q.n > p.max_new) q.status = AFA_PAGED_TOO_MANY;
+  else if ((int64_t)q.c + q.n > p.table_width * P) q.status = AFA_PAGED_TOO_LONG;
+  q.need = q.status == AFA_PAGED_OK ? (int)((unsigned)(q.c + q.n + P - 1) / (unsigned)P) : q.held;
+  q.blocks = q.tiles = 0;
+  return q;
 }
 
-// Workgroups (r, y) of request r share its tokens, pages and items; r = requests: the rows behind the
-// last request's.
-__global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_paged_plan p, const int rows,
-                                                                  const int32_t* cached, const int32_t* fresh,
-                                                                  const int32_t* parents) {
+// Places in the ring, from sums below three times its length.
+__device__ __forceinline__ int ring_place(int64_t i, int pages) {
+  if (i >= pages) i -= pages;
+  if (i >= pages) i -= pages;
+  return (int)i;
+}
+
+// What request r's workgroup has to know.
+struct Mine {
+  Request q;
+  int start, pop, push, chunk, chunks, part, item;
+};
+
+// The sums over all requests, formed by a whole workgroup; thread i has requests [i k, i k + k).  `mine` is that
+// of request `which`; where `store` is set all requests' values go to the plan and the schedule.  The
+// pages held and the ring's state are brought up to date only by `finish`.  K: the most requests of a thread,
+// whose lengths it keeps; 0: any number, read again in every pass.
+template <int THREADS, int K>
+struct PlanSums {
+  const afa_paged_plan& p;
+  const int rows;
+  const int64_t target;
+  const int32_t *cached, *fresh;
+  int64_t (*lds)[3];
+  int pages, head, count, r0, r1, end;
+  Lengths own[K > 0 ? K : 1];
+  Sums all, first;  // of all requests, and of those before this thread's
+  int64_t taken;
+
+  __device__ Lengths lengths(int r) const { return Lengths{cached[r], fresh[r], p.held[r]}; }
+  template <typename F>
+  __device__ void each_length(const F& f) {
+    if constexpr (K > 0) {
+#pragma unroll
+      for (int u = 0; u < K; ++u)
+        if (r0 + u < r1) f(r0 + u, own[u]);
+    } else {
+      for (int r = r0; r < r1; ++r) f(r, lengths(r));
+    }
+  }
+
+  // Calls f(r, request, sums before it) of this thread's requests, in order, with status and need as they end.
+  // free: the pages that there are to have.
+  template <typename F>
+  __device__ void each(Sums before, int64_t free, const F& f) {
+    each_length([&](int r, const Lengths& x) {
+      Request q = request(p, x);
+      const int64_t stop = before.v[0] + max(q.n, 0);
+      if (q.status == AFA_PAGED_OK && q.n > 0 && stop > p.max_tokens) {
+        q.status = AFA_PAGED_PAST_END;
+        q.need = q.held;
+      }
+      const int grow = max(q.need - q.held, 0), shrink = max(q.held - q.need, 0);
+      const Sums at = before;
+      before.v[0] = stop;
+      before.v[1] += grow;
+      before.v[2] += shrink;
+      if (grow > 0 && before.v[1] > free) {
+        q.status = AFA_PAGED_NO_PAGES;
+        q.need = q.held;
+      }
+      if (q.status == AFA_PAGED_OK && q.n > 0) {
+        q.blocks = ((int64_t)q.n * (p.heads / p.kv_heads) + rows - 1) / rows;
+        q.tiles = (q.c + q.n + kPagedTile - 1) / kPagedTile;
+      }
+      f(r, q, at);
+    });
+  }
+
+  // Two scans: the pages that are asked for depend on where the tokens end.
+  __device__ void prepare() {
+    const int R = (int)p.requests, k = (R + THREADS - 1) / THREADS;
+    pages = (int)p.num_pages;
+    count = min(max(p.ring_state[1], 0), pages);
+    head = (int)((unsigned)p.ring_state[0] % (unsigned)pages);
+    r0 = min((int)threadIdx.x * k, R);
+    r1 = min(r0 + k, R);
+    if constexpr (K > 0) {
+#pragma unroll
+      for (int u = 0; u < K; ++u)
+        if (r0 + u < r1) own[u] = lengths(r0 + u);
+    }
+    Sums x = {{0, 0, 0}}, total;
+    each_length([&](int, const Lengths& l) { x.v[0] += max(l.n, 0); });
+    first = block_before<THREADS, 1>(x, lds, total);
+    all.v[0] = total.v[0];
+    first.v[1] = first.v[2] = 0;
+    Sums change = {{0, 0, 0}};
+    each(first, INT64_MAX, [&](int, const Request& q, const Sums&) {
+      change.v[0] += max(q.need - q.held, 0);
+      change.v[1] += max(q.held - q.need, 0);
+    });
+    const Sums pg = block_before<THREADS, 2>(change, lds, total);
+    all.v[1] = total.v[0];
+    all.v[2] = total.v[1];
+    first.v[1] = pg.v[0];
+    first.v[2] = pg.v[1];
+  }
+
+  __device__ Mine run(int which, bool store, Mine* shared) {
+    const PagedSchedule s = paged_schedule(p);
+    prepare();
+    Sums work = {{0, 0, 0}}, total;
+    each(first, count, [&](int, const Request& q, const Sums&) {
+      work.v[0] += q.blocks * q.tiles;
+      if (q.status == AFA_PAGED_OK) work.v[1] += max(q.need - q.held, 0);
+    });
+    block_before<THREADS, 2>(work, lds, total);
+    taken = total.v[1];
+    const int64_t even = (total.v[0] + target - 1) / target;
+    const int chunk = (int)max(even, (int64_t)kMinChunk);
+    auto cut = [&](const Request& q) { return (q.tiles + chunk - 1) / chunk; };
+    Sums cuts = {{0, 0, 0}};
+    each(first, count, [&](int, const Request& q, const Sums&) {
+      const int64_t items = q.blocks * cut(q);
+      cuts.v[0] += items;
+      if (cut(q) > 1) cuts.v[1] += items;
+    });
+    Sums at = block_before<THREADS, 2>(cuts, lds, total);
+    each(first, count, [&](int r, const Request& q, const Sums& b) {
+      const int64_t chunks = cut(q), items = q.blocks * chunks;
+      Mine m;
+      m.q = q;
+      m.start = (int)min(b.v[0], p.max_tokens);
+      m.pop = ring_place(head + b.v[1], pages);
+      m.push = ring_place(head + count + b.v[2], pages);
+      m.chunk = chunk;
+      m.chunks = (int)chunks;
+      m.item = (int)at.v[0];
+      m.part = (int)at.v[1];
+      at.v[0] += items;
+      if (chunks > 1) at.v[1] += items;
+      if (r == which) *shared = m;
+      if (store || r == which) {
+        s.item[r] = m.item;
+        s.part[r] = m.part;
+        s.chunks[r] = m.chunks;
+        p.status[r] = q.status;
+        p.starts[r + 1] = (int)min(b.v[0] + max(q.n, 0), p.max_tokens);
+      }
+      if (store) {
+        s.pop[r] = m.pop;
+        s.push[r] = m.push;
+        s.held[r] = q.held;
+      }
+    });
+    end = (int)min(all.v[0], p.max_tokens);
+    if (threadIdx.x == 0 && (store || which == 0)) {
+      s.header[PS_ITEMS] = (int)total.v[0];
+      s.header[PS_CHUNK] = chunk;
+      p.starts[0] = 0;
+    }
+    __syncthreads();
+    return *shared;
+  }
+
+  // Only once no workgroup reads held and ring_state any more.
+  __device__ void finish() {
+    each(first, count, [&](int r, const Request& q, const Sums&) { p.held[r] = q.need; });
+    if (threadIdx.x == 0) {
+      p.ring_state[0] = ring_place(head + taken, pages);
+      p.ring_state[1] = (int)(count - taken + all.v[2]);
+    }
+  }
+};
+
+// Request r's tokens, pages and items by one or more workgroups (gridDim.y); r = requests: the rows behind
+// the last request's, from row `end` on.
+__device__ void fill(const afa_paged_plan& p, const int rows, const int32_t* parents, const int r, const Mine& mine,
+                     const int end) {
   const PagedSchedule s = paged_schedule(p);
-  const int R = (int)p.requests, P = (int)p.page_size, r = blockIdx.x, words = (int)(p.max_tree / 64);
+  const int P = (int)p.page_size, words = (int)(p.max_tree / 64), pages = (int)p.num_pages;
   const int tid = threadIdx.x, step = gridDim.y * kMaxTree, first = blockIdx.y * kMaxTree + tid;
-  if (r == R) {
-    for (int64_t t = p.starts[R] + first; t < p.max_tokens; t += step) {
+  const int c = mine.q.c, n = mine.q.n, held = mine.q.held, need = mine.q.need, start = mine.start;
+  const bool rest = r == (int)p.requests;
+  if (rest || mine.q.status != AFA_PAGED_OK) {
+    const int64_t from = rest ? end : start, to = rest ? p.max_tokens : min((int64_t)start + max(n, 0), p.max_tokens);
+    for (int64_t t = from + first; t < to; t += step) {
       p.slots[t] = -1;
       p.positions[t] = 0;
-      p.token_request[t] = -1;
+      p.token_request[t] = rest ? -1 : r;
       for (int w = 0; w < words; ++w) p.masks[t * words + w] = 0;
     }
     return;
   }
-  const int start = p.starts[r], status = p.status[r];
-  if (status != AFA_PAGED_OK) {
-    for (int64_t t = start + first; t < p.starts[r + 1]; t += step) {
-      p.slots[t] = -1;
-      p.positions[t] = 0;
-      p.token_request[t] = r;
-      for (int w = 0; w < words; ++w) p.masks[t * words + w] = 0;
-    }
-    return;
-  }
-  const int c = cached[r], n = fresh[r], held = s.held[r], need = p.held[r];
   int32_t* table = p.block_tables + (int64_t)r * p.table_width;
-  // page b of the request, also before this launch has written it into the table
-  auto page = [&](int b) { return b < held ? table[b] : p.ring[(s.pop[r] + (int64_t)(b - held)) % p.num_pages]; };
+  // page b of the request, also before it is written into the table
+  auto page = [&](int b) { return b < held ? table[b] : p.ring[ring_place((int64_t)mine.pop + (b - held), pages)]; };
   for (int b = held + first; b < need; b += step) table[b] = page(b);
   for (int b = need + first; b < held; b += step) {
-    p.ring[(s.push[r] + (int64_t)(b - need)) % p.num_pages] = table[b];
+    p.ring[ring_place((int64_t)mine.push + (b - need), pages)] = table[b];
     table[b] = -1;
   }
   const bool tree = n <= p.max_tree;  // masks are written; a chain's where there are no parents
   for (int i = first; i < n; i += step) {
     const int64_t t = start + i;
-    const int at = c + i;
-    p.slots[t] = page(at / P) * P + at % P;
+    const unsigned at = c + i;
+    p.slots[t] = page((int)(at / (unsigned)P)) * P + (int)(at % (unsigned)P);
     p.token_request[t] = r;
     if (!tree) {
-      p.positions[t] = at;
+      p.positions[t] = (int)at;
       for (int w = 0; w < words; ++w) p.masks[t * words + w] = 0;
     }
   }
-  if (tree && blockIdx.y == 0) {
+  if (tree && blockIdx.y == 0 && n > 0) {
     // Ancestors by doubling: after k rounds a node's set holds its 2^k nearest ancestors and `up` is the
     // one behind them.
     __shared__ int up[kMaxTree];
     __shared__ uint64_t set[kMaxTree / 64][kMaxTree];
-    int mine = -1;
+    int above = -1;
     uint64_t seen[kMaxTree / 64];
 #pragma unroll
     for (int w = 0; w < kMaxTree / 64; ++w) seen[w] = tid >> 6 == w ? uint64_t(1) << (tid & 63) : 0;
     if (tid < n) {
-      mine = parents != nullptr ? parents[start + tid] : tid - 1;
-      if (mine < 0 || mine >= tid) mine = -1;
+      above = parents != nullptr ? parents[start + tid] : tid - 1;
+      if (above < 0 || above >= tid) above = -1;
     }
     for (int span = 1; span < n; span <<= 1) {
-      up[tid] = mine;
+      up[tid] = above;
 #pragma unroll
       for (int w = 0; w < kMaxTree / 64; ++w) set[w][tid] = seen[w];
       __syncthreads();
-      if (mine >= 0) {
+      if (above >= 0) {
 #pragma unroll
-        for (int w = 0; w < kMaxTree / 64; ++w) seen[w] |= set[w][mine];
-        mine = up[mine];
+        for (int w = 0; w < kMaxTree / 64; ++w) seen[w] |= set[w][above];
+        above = up[above];
       }
       __syncthreads();
     }
@@ -228,40 +344,93 @@ __global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_page
     }
   }
   if (n == 0) return;
-  const int group = (int)(p.heads / p.kv_heads), chunk = s.header[PS_CHUNK], chunks = s.chunks[r];
-  const int blocks = (int)(((int64_t)n * group + rows - 1) / rows), all = (c + n + kPagedTile - 1) / kPagedTile;
+  const int group = (int)(p.heads / p.kv_heads), chunk = mine.chunk, chunks = mine.chunks, blocks = (int)mine.q.blocks;
   for (int64_t j = first; j < (int64_t)blocks * chunks; j += step) {
     // row blocks run fastest: those that read the same keys follow one another
     const int block = (int)(j % blocks), ch = (int)(j / blocks);
-    int end = all;
-    if (!tree || p.max_tree == 0) {
-      // a chain's rows see no key behind their own token
-      const int last = min(n - 1, (int)(((int64_t)block * rows + rows - 1) / group));
-      end = (c + last + kPagedTile) / kPagedTile;
-    }
     PagedItem it;
     it.request = r;
     it.row0 = block * rows;
     it.tile0 = ch * chunk;
-    it.tile1 = min(it.tile0 + chunk, end);
-    it.part = chunks > 1 ? s.part[r] + block * chunks + ch : -1;
+    it.tile1 = min(it.tile0 + chunk, paged_block_tiles(c, n, n <= p.max_tree, block, rows, group));
+    it.part = chunks > 1 ? mine.part + block * chunks + ch : -1;
     it.cached = c;
     it.fresh = n;
     it.start = start;
-    s.items[s.item[r] + j] = it;
+    s.items[mine.item + j] = it;
   }
+}
+
+// Every workgroup forms the sums over all requests for itself and fills in its own request.  The last
+// one to have read the lengths held brings them up to date.
+template <int K>
+__global__ __launch_bounds__(kMaxTree) void afa_paged_plan_kernel(const afa_paged_plan p, const int rows, const int64_t target,
+                                                                  const int32_t* cached, const int32_t* fresh,
+                                                                  const int32_t* parents) {
+  __shared__ int64_t lds[kMaxTree / 64][3];
+  __shared__ Mine shared;
+  __shared__ bool last;
+  PlanSums<kMaxTree, K> sums{p, rows, target, cached, fresh, lds};
+  const Mine mine = sums.run(blockIdx.x, false, &shared);
+  if (threadIdx.x == 0) {
+    int* ticket = paged_schedule(p).header + PS_TICKET;
+    last = atomicAdd(ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
+    if (last) *ticket = 0;
+  }
+  fill(p, rows, parents, blockIdx.x, mine, sums.end);
+  __syncthreads();
+  if (last) sums.finish();
+}
+
+// The same in two launches, for more requests.
+constexpr int SCAN = 1024;
+__global__ __launch_bounds__(SCAN) void afa_paged_scan_kernel(const afa_paged_plan p, const int rows, const int64_t target,
+                                                              const int32_t* cached, const int32_t* fresh) {
+  __shared__ int64_t lds[SCAN / 64][3];
+  __shared__ Mine shared;
+  PlanSums<SCAN, 0> sums{p, rows, target, cached, fresh, lds};
+  sums.run(-1, true, &shared);
+  sums.finish();
+}
+
+__global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_paged_plan p, const int rows,
+                                                                  const int32_t* cached, const int32_t* fresh,
+                                                                  const int32_t* parents) {
+  const PagedSchedule s = paged_schedule(p);
+  const int r = blockIdx.x, R = (int)p.requests;
+  Mine m = {};
+  if (r < R) {
+    m.start = p.starts[r];
+    m.pop = s.pop[r];
+    m.push = s.push[r];
+    m.chunk = s.header[PS_CHUNK];
+    m.chunks = s.chunks[r];
+    m.part = s.part[r];
+    m.item = s.item[r];
+    m.q = Request{cached[r], fresh[r], s.held[r], p.held[r], p.status[r], 0, 0};
+    m.q.blocks = ((int64_t)max(m.q.n, 0) * (p.heads / p.kv_heads) + rows - 1) / rows;
+  }
+  fill(p, rows, parents, r, m, p.starts[R]);
 }
 
 }  // namespace
 
 hipError_t paged_build_launch(const afa_paged_plan& p, const PagedCut& c, const int32_t* cached, const int32_t* fresh,
                               const int32_t* parents, hipStream_t st) {
-  hipLaunchKernelGGL(afa_paged_scan_kernel, dim3(1), dim3(SCAN), 0, st, p, c.rows, c.target, cached, fresh);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  // a workgroup of long prompts takes about 1024 of their tokens
   const int64_t y = (p.max_new + 1023) / 1024;
-  hipLaunchKernelGGL(afa_paged_fill_kernel, dim3((unsigned)(p.requests + 1), (unsigned)(y < 64 ? y : 64)),
-                     dim3(kMaxTree), 0, st, p, c.rows, cached, fresh, parents);
+  const dim3 grid((unsigned)(p.requests + 1), (unsigned)(y < 64 ? y : 64));
+  if (p.requests <= kOwnSums) {
+    if (p.requests <= kMaxTree)
+      hipLaunchKernelGGL((afa_paged_plan_kernel<1>), grid, dim3(kMaxTree), 0, st, p, c.rows, c.target, cached, fresh, parents);
+    else
+      hipLaunchKernelGGL((afa_paged_plan_kernel<4>), grid, dim3(kMaxTree), 0, st, p, c.rows, c.target, cached, fresh, parents);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(afa_paged_scan_kernel, dim3(1), dim3(SCAN), 0, st, p, c.rows, c.target, cached, fresh);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(afa_paged_fill_kernel, grid, dim3(kMaxTree), 0, st, p, c.rows, cached, fresh, parents);
   return hipGetLastError();
 }
 

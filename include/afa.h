@@ -294,7 +294,8 @@ typedef struct afa_paged_plan {
   int32_t* starts;                   /* (requests + 1,) */
   int32_t* status;                   /* (requests,) AFA_PAGED_* */
   int64_t* masks;                    /* (max_tokens, max_tree / 64) bit i: sees drafted token i */
-  int32_t* schedule;                 /* afa_paged_schedule_bytes() bytes, 16-byte aligned */
+  int32_t* schedule;                 /* afa_paged_schedule_bytes() bytes, 16-byte aligned, set to 0
+                                        once, before the plan's first afa_paged_build */
 } afa_paged_plan;
 
 /* status of a request after afa_paged_build.  Any but OK: the request keeps the pages it held, its
