@@ -21,8 +21,8 @@ struct PagedItem {
 // Key tiles that row block `block` of a request's n new tokens sees: all, or in a chain those up to the
 // block's last token.
 __host__ __device__ inline int paged_block_tiles(int c, int n, bool tree, int block, int rows, int group) {
-  const int64_t last = ((int64_t)block * rows + rows - 1) / group;
-  return (c + (tree || last >= n ? n - 1 : (int)last) + kPagedTile) / kPagedTile;
+  const unsigned last = (unsigned)(block * rows + rows - 1) / (unsigned)group;
+  return (int)((unsigned)(c + (tree || last >= (unsigned)n ? n - 1 : (int)last) + kPagedTile) / kPagedTile);
 }
 
 // plan->schedule: a header, six ints per request, the items, then a counter for each part of each key/value head.
@@ -75,6 +75,7 @@ struct AxisRotation {
   int pairs;
   const void* positions;
   int pos64;             // positions are int64
+  int wide;              // aligned runs of four fp32 table entries are 16-byte aligned
   int axes;
   int end[kMaxAxes];     // first pair behind each axis's section
 };

@@ -58,6 +58,7 @@ int check_rotation(afa::AxisRotation& r, const void* rc, const void* rs, int64_t
   r.pairs = (int)(head_dim / 2);
   r.positions = positions;
   r.pos64 = pos64;
+  r.wide = r.pairs % 4 == 0 && aligned16(rc) && aligned16(rs);
   r.axes = axes;
   if (sections == nullptr) {
     if (axes != 1) return AFA_ERR_NULL;

@@ -43,6 +43,13 @@ constexpr int kMinChunk = 4;
 // Most requests whose sums every workgroup forms for itself, four a thread at most.
 constexpr int kOwnSums = 4 * kMaxTree;
 
+// The attention's cut as the kernels take it: rows of an item (a power of two), query heads a key head, and
+// items per head that fill the device.
+struct Cut {
+  int log_rows, group, target;
+  __device__ int blocks(int n) const { return (n * group + (1 << log_rows) - 1) >> log_rows; }
+};
+
 struct Sums {
   int64_t v[3];
 };
@@ -79,28 +86,18 @@ __device__ Sums block_before(Sums x, int64_t (*lds)[3], Sums& all) {
   return s;
 }
 
-struct Lengths {
-  int c, n, held;
-};
-
-// One request: what it asks for and what it gets.
+// One request: what it asks for, and in the end what it gets.
 struct Request {
   int c, n, held, need, status;
-  int64_t blocks, tiles;  // row blocks and key tiles of its attention, 0 where it has none
 };
 
-__device__ __forceinline__ Request request(const afa_paged_plan& p, const Lengths& x) {
-  Request q;
-  q.c = x.c;
-  q.n = x.n;
-  q.held = min(max(x.held, 0), (int)p.table_width);
-  const int P = (int)p.page_size;
-  q.status = AFA_PAGED_OK;
-  if (q.c < 0 || q.n < 0) q.status = AFA_PAGED_NEGATIVE;
-  else if (q.n > p.max_new) q.status = AFA_PAGED_TOO_MANY;
-  else if ((int64_t)q.c + q.n > p.table_width * P) q.status = AFA_PAGED_TOO_LONG;
-  q.need = q.status == AFA_PAGED_OK ? (int)((unsigned)(q.c + q.n + P - 1) / (unsigned)P) : q.held;
-  q.blocks = q.tiles = 0;
+__device__ __forceinline__ Request request(const afa_paged_plan& p, int c, int n, int held) {
+  Request q{c, n, min(max(held, 0), (int)p.table_width), 0, AFA_PAGED_OK};
+  if (c < 0 || n < 0) q.status = AFA_PAGED_NEGATIVE;
+  else if (n > p.max_new) q.status = AFA_PAGED_TOO_MANY;
+  else if ((unsigned)c + (unsigned)n > (unsigned)p.table_width * (unsigned)p.page_size) q.status = AFA_PAGED_TOO_LONG;
+  const unsigned P = (unsigned)p.page_size;
+  q.need = q.status == AFA_PAGED_OK ? (int)(((unsigned)(c + n) + P - 1) / P) : q.held;
   return q;
 }
 
@@ -114,34 +111,33 @@ __device__ __forceinline__ int ring_place(int64_t i, int pages) {
 // What request r's workgroup has to know.
 struct Mine {
   Request q;
-  int start, pop, push, chunk, chunks, part, item;
+  int start, pop, push, chunk, chunks, part, item;  // chunks 0: no attention
 };
 
 // The sums over all requests, formed by a whole workgroup; thread i has requests [i k, i k + k).  `mine` is that
 // of request `which`; where `store` is set all requests' values go to the plan and the schedule.  The
 // pages held and the ring's state are brought up to date only by `finish`.  K: the most requests of a thread,
-// whose lengths it keeps; 0: any number, read again in every pass.
+// which keeps them; 0: any number, read again in every pass.
 template <int THREADS, int K>
 struct PlanSums {
   const afa_paged_plan& p;
-  const int rows;
-  const int64_t target;
+  const Cut& cut;
   const int32_t *cached, *fresh;
   int64_t (*lds)[3];
   int pages, head, count, r0, r1, end;
-  Lengths own[K > 0 ? K : 1];
+  Request own[K > 0 ? K : 1];
   Sums all, first;  // of all requests, and of those before this thread's
   int64_t taken;
 
-  __device__ Lengths lengths(int r) const { return Lengths{cached[r], fresh[r], p.held[r]}; }
+  __device__ Request read(int r) const { return request(p, cached[r], fresh[r], p.held[r]); }
   template <typename F>
-  __device__ void each_length(const F& f) {
+  __device__ void each_request(const F& f) {
     if constexpr (K > 0) {
 #pragma unroll
       for (int u = 0; u < K; ++u)
         if (r0 + u < r1) f(r0 + u, own[u]);
     } else {
-      for (int r = r0; r < r1; ++r) f(r, lengths(r));
+      for (int r = r0; r < r1; ++r) f(r, read(r));
     }
   }
 
@@ -149,8 +145,7 @@ struct PlanSums {
   // free: the pages that there are to have.
   template <typename F>
   __device__ void each(Sums before, int64_t free, const F& f) {
-    each_length([&](int r, const Lengths& x) {
-      Request q = request(p, x);
+    each_request([&](int r, Request q) {
       const int64_t stop = before.v[0] + max(q.n, 0);
       if (q.status == AFA_PAGED_OK && q.n > 0 && stop > p.max_tokens) {
         q.status = AFA_PAGED_PAST_END;
@@ -164,10 +159,6 @@ struct PlanSums {
       if (grow > 0 && before.v[1] > free) {
         q.status = AFA_PAGED_NO_PAGES;
         q.need = q.held;
-      }
-      if (q.status == AFA_PAGED_OK && q.n > 0) {
-        q.blocks = ((int64_t)q.n * (p.heads / p.kv_heads) + rows - 1) / rows;
-        q.tiles = (q.c + q.n + kPagedTile - 1) / kPagedTile;
       }
       f(r, q, at);
     });
@@ -184,10 +175,10 @@ struct PlanSums {
     if constexpr (K > 0) {
 #pragma unroll
       for (int u = 0; u < K; ++u)
-        if (r0 + u < r1) own[u] = lengths(r0 + u);
+        if (r0 + u < r1) own[u] = read(r0 + u);
     }
     Sums x = {{0, 0, 0}}, total;
-    each_length([&](int, const Lengths& l) { x.v[0] += max(l.n, 0); });
+    each_request([&](int, const Request& q) { x.v[0] += max(q.n, 0); });
     first = block_before<THREADS, 1>(x, lds, total);
     all.v[0] = total.v[0];
     first.v[1] = first.v[2] = 0;
@@ -203,35 +194,41 @@ struct PlanSums {
     first.v[2] = pg.v[1];
   }
 
+  static __device__ int tiles(const Request& q) { return (q.c + q.n + kPagedTile - 1) / kPagedTile; }
+
   __device__ Mine run(int which, bool store, Mine* shared) {
     const PagedSchedule s = paged_schedule(p);
     prepare();
     Sums work = {{0, 0, 0}}, total;
     each(first, count, [&](int, const Request& q, const Sums&) {
-      work.v[0] += q.blocks * q.tiles;
-      if (q.status == AFA_PAGED_OK) work.v[1] += max(q.need - q.held, 0);
+      if (q.status != AFA_PAGED_OK) return;
+      work.v[0] += (int64_t)cut.blocks(q.n) * tiles(q);
+      work.v[1] += max(q.need - q.held, 0);
     });
     block_before<THREADS, 2>(work, lds, total);
     taken = total.v[1];
-    const int64_t even = (total.v[0] + target - 1) / target;
-    const int chunk = (int)max(even, (int64_t)kMinChunk);
-    auto cut = [&](const Request& q) { return (q.tiles + chunk - 1) / chunk; };
+    // at least an equal share, and no longer than any request
+    const double share = (double)total.v[0] / (double)cut.target;
+    const int chunk = max((int)(share < 0x1p26 ? share : 0x1p26) + 1, kMinChunk);
+    auto chunks_of = [&](const Request& q) {
+      return q.status == AFA_PAGED_OK && q.n > 0 ? (int)((unsigned)(tiles(q) + chunk - 1) / (unsigned)chunk) : 0;
+    };
     Sums cuts = {{0, 0, 0}};
     each(first, count, [&](int, const Request& q, const Sums&) {
-      const int64_t items = q.blocks * cut(q);
+      const int chunks = chunks_of(q), items = chunks > 0 ? cut.blocks(q.n) * chunks : 0;
       cuts.v[0] += items;
-      if (cut(q) > 1) cuts.v[1] += items;
+      if (chunks > 1) cuts.v[1] += items;
     });
     Sums at = block_before<THREADS, 2>(cuts, lds, total);
     each(first, count, [&](int r, const Request& q, const Sums& b) {
-      const int64_t chunks = cut(q), items = q.blocks * chunks;
+      const int chunks = chunks_of(q), items = chunks > 0 ? cut.blocks(q.n) * chunks : 0;
       Mine m;
       m.q = q;
       m.start = (int)min(b.v[0], p.max_tokens);
       m.pop = ring_place(head + b.v[1], pages);
       m.push = ring_place(head + count + b.v[2], pages);
       m.chunk = chunk;
-      m.chunks = (int)chunks;
+      m.chunks = chunks;
       m.item = (int)at.v[0];
       m.part = (int)at.v[1];
       at.v[0] += items;
@@ -272,7 +269,7 @@ struct PlanSums {
 
 // Request r's tokens, pages and items by one or more workgroups (gridDim.y); r = requests: the rows behind
 // the last request's, from row `end` on.
-__device__ void fill(const afa_paged_plan& p, const int rows, const int32_t* parents, const int r, const Mine& mine,
+__device__ void fill(const afa_paged_plan& p, const Cut& cut, const int32_t* parents, const int r, const Mine& mine,
                      const int end) {
   const PagedSchedule s = paged_schedule(p);
   const int P = (int)p.page_size, words = (int)(p.max_tree / 64), pages = (int)p.num_pages;
@@ -344,15 +341,15 @@ __device__ void fill(const afa_paged_plan& p, const int rows, const int32_t* par
     }
   }
   if (n == 0) return;
-  const int group = (int)(p.heads / p.kv_heads), chunk = mine.chunk, chunks = mine.chunks, blocks = (int)mine.q.blocks;
-  for (int64_t j = first; j < (int64_t)blocks * chunks; j += step) {
+  const int chunk = mine.chunk, chunks = mine.chunks, blocks = cut.blocks(n), rows = 1 << cut.log_rows;
+  for (int j = first; j < blocks * chunks; j += step) {
     // row blocks run fastest: those that read the same keys follow one another
-    const int block = (int)(j % blocks), ch = (int)(j / blocks);
+    const int ch = (int)((unsigned)j / (unsigned)blocks), block = j - ch * blocks;
     PagedItem it;
     it.request = r;
     it.row0 = block * rows;
     it.tile0 = ch * chunk;
-    it.tile1 = min(it.tile0 + chunk, paged_block_tiles(c, n, n <= p.max_tree, block, rows, group));
+    it.tile1 = min(it.tile0 + chunk, paged_block_tiles(c, n, n <= p.max_tree, block, rows, cut.group));
     it.part = chunks > 1 ? mine.part + block * chunks + ch : -1;
     it.cached = c;
     it.fresh = n;
@@ -364,38 +361,36 @@ __device__ void fill(const afa_paged_plan& p, const int rows, const int32_t* par
 // Every workgroup forms the sums over all requests for itself and fills in its own request.  The last
 // one to have read the lengths held brings them up to date.
 template <int K>
-__global__ __launch_bounds__(kMaxTree) void afa_paged_plan_kernel(const afa_paged_plan p, const int rows, const int64_t target,
-                                                                  const int32_t* cached, const int32_t* fresh,
-                                                                  const int32_t* parents) {
+__global__ __launch_bounds__(kMaxTree) void afa_paged_plan_kernel(const afa_paged_plan p, const Cut cut, const int32_t* cached,
+                                                                  const int32_t* fresh, const int32_t* parents) {
   __shared__ int64_t lds[kMaxTree / 64][3];
   __shared__ Mine shared;
   __shared__ bool last;
-  PlanSums<kMaxTree, K> sums{p, rows, target, cached, fresh, lds};
+  PlanSums<kMaxTree, K> sums{p, cut, cached, fresh, lds};
   const Mine mine = sums.run(blockIdx.x, false, &shared);
   if (threadIdx.x == 0) {
     int* ticket = paged_schedule(p).header + PS_TICKET;
     last = atomicAdd(ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
     if (last) *ticket = 0;
   }
-  fill(p, rows, parents, blockIdx.x, mine, sums.end);
+  fill(p, cut, parents, blockIdx.x, mine, sums.end);
   __syncthreads();
   if (last) sums.finish();
 }
 
 // The same in two launches, for more requests.
 constexpr int SCAN = 1024;
-__global__ __launch_bounds__(SCAN) void afa_paged_scan_kernel(const afa_paged_plan p, const int rows, const int64_t target,
-                                                              const int32_t* cached, const int32_t* fresh) {
+__global__ __launch_bounds__(SCAN) void afa_paged_scan_kernel(const afa_paged_plan p, const Cut cut, const int32_t* cached,
+                                                              const int32_t* fresh) {
   __shared__ int64_t lds[SCAN / 64][3];
   __shared__ Mine shared;
-  PlanSums<SCAN, 0> sums{p, rows, target, cached, fresh, lds};
+  PlanSums<SCAN, 0> sums{p, cut, cached, fresh, lds};
   sums.run(-1, true, &shared);
   sums.finish();
 }
 
-__global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_paged_plan p, const int rows,
-                                                                  const int32_t* cached, const int32_t* fresh,
-                                                                  const int32_t* parents) {
+__global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_paged_plan p, const Cut cut, const int32_t* cached,
+                                                                  const int32_t* fresh, const int32_t* parents) {
   const PagedSchedule s = paged_schedule(p);
   const int r = blockIdx.x, R = (int)p.requests;
   Mine m = {};
@@ -407,10 +402,9 @@ __global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_page
     m.chunks = s.chunks[r];
     m.part = s.part[r];
     m.item = s.item[r];
-    m.q = Request{cached[r], fresh[r], s.held[r], p.held[r], p.status[r], 0, 0};
-    m.q.blocks = ((int64_t)max(m.q.n, 0) * (p.heads / p.kv_heads) + rows - 1) / rows;
+    m.q = Request{cached[r], fresh[r], s.held[r], p.held[r], p.status[r]};
   }
-  fill(p, rows, parents, r, m, p.starts[R]);
+  fill(p, cut, parents, r, m, p.starts[R]);
 }
 
 }  // namespace
@@ -420,17 +414,18 @@ hipError_t paged_build_launch(const afa_paged_plan& p, const PagedCut& c, const 
   // a workgroup of long prompts takes about 1024 of their tokens
   const int64_t y = (p.max_new + 1023) / 1024;
   const dim3 grid((unsigned)(p.requests + 1), (unsigned)(y < 64 ? y : 64));
+  const Cut cut{c.rows == 16 ? 4 : c.rows == 32 ? 5 : 6, (int)(p.heads / p.kv_heads), (int)c.target};
   if (p.requests <= kOwnSums) {
     if (p.requests <= kMaxTree)
-      hipLaunchKernelGGL((afa_paged_plan_kernel<1>), grid, dim3(kMaxTree), 0, st, p, c.rows, c.target, cached, fresh, parents);
+      hipLaunchKernelGGL((afa_paged_plan_kernel<1>), grid, dim3(kMaxTree), 0, st, p, cut, cached, fresh, parents);
     else
-      hipLaunchKernelGGL((afa_paged_plan_kernel<4>), grid, dim3(kMaxTree), 0, st, p, c.rows, c.target, cached, fresh, parents);
+      hipLaunchKernelGGL((afa_paged_plan_kernel<4>), grid, dim3(kMaxTree), 0, st, p, cut, cached, fresh, parents);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(afa_paged_scan_kernel, dim3(1), dim3(SCAN), 0, st, p, c.rows, c.target, cached, fresh);
+  hipLaunchKernelGGL(afa_paged_scan_kernel, dim3(1), dim3(SCAN), 0, st, p, cut, cached, fresh);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(afa_paged_fill_kernel, grid, dim3(kMaxTree), 0, st, p, c.rows, cached, fresh, parents);
+  hipLaunchKernelGGL(afa_paged_fill_kernel, grid, dim3(kMaxTree), 0, st, p, cut, cached, fresh, parents);
   return hipGetLastError();
 }
 

@@ -4,6 +4,8 @@
 // order) and is turned by table row m = positions[b][l][a]: (x0, x1) -> (c x0 - s x1, s x0 + c x1), c and s
 // the entries (m, p).  Pairs behind the last section stay as they are.  The tables enter in fp32 (fp64)
 // and each result is rounded once.
+#include <initializer_list>
+
 #include "afa_common.h"
 #include "afa_paged.h"
 
@@ -30,7 +32,7 @@ __device__ __forceinline__ void turn(const AxisRotation& r, int64_t m, int p, T 
   y1 = s * x0 + c * x1;
 }
 
-// One thread a pair, q's rows before k's.
+// One thread a pair, q's rows before k's: fp64, rows that are no whole 16-byte chunks, and any alignment.
 template <int DT>
 __global__ __launch_bounds__(256) void ago_axes_kernel(const RotateAxesArgs a, int64_t total) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -58,7 +60,151 @@ __global__ __launch_bounds__(256) void ago_axes_kernel(const RotateAxesArgs a, i
   }
 }
 
-// The cache write: one thread a pair (or the last element of an odd head_dim) of a token's q, k and v
+// The same in 16-byte chunks: a thread owns one chunk of a token's rows, holds its table entries and turns
+// it in up to HG heads, `groups` apart, whose loads are in flight together.  Where the heads of a token lie
+// nearer to one another than its neighbours do, lanes run over heads before tokens, so that a wave's
+// accesses stay whole lines side by side either way.
+template <int DT>
+struct ChunkTurn {
+  using R = RowChunk<DT>;
+  static constexpr int NP = R::EPC / 2;
+  float c[NP], s[NP];
+  bool keep[NP];
+
+  __device__ __forceinline__ void load(const AxisRotation& r, int64_t token, int p0, float sign) {
+    const int first = pair_axis(r, p0), last = pair_axis(r, p0 + NP - 1);
+    if (first == last && first >= 0 && r.wide) {
+      const int64_t m = position(r, token + first), at = m * r.pairs + p0;
+      const bool in = m >= 0 && m < r.len;
+      typedef __attribute__((ext_vector_type(NP))) float vec;
+      const vec nan = __builtin_nanf("");
+      const vec cv = in ? *(const vec*)((const float*)r.rc + at) : nan, sv = in ? *(const vec*)((const float*)r.rs + at) : nan;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        c[p] = cv[p];
+        s[p] = sv[p] * sign;
+        keep[p] = false;
+      }
+      return;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int axis = pair_axis(r, p0 + p);
+      const int64_t m = axis < 0 ? 0 : position(r, token + axis), at = m * r.pairs + p0 + p;
+      const bool in = m >= 0 && m < r.len;
+      keep[p] = axis < 0;
+      c[p] = in ? ((const float*)r.rc)[at] : __builtin_nanf("");
+      s[p] = in ? ((const float*)r.rs)[at] * sign : __builtin_nanf("");
+    }
+  }
+
+  __device__ __forceinline__ u32x4_t turned(u32x4_t w) const {
+#pragma clang fp contract(off)
+    float v[R::EPC];
+    R::unpack(w, v);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const float x0 = v[2 * p], x1 = v[2 * p + 1];
+      v[2 * p] = keep[p] ? x0 : c[p] * x0 - s[p] * x1;
+      v[2 * p + 1] = keep[p] ? x1 : s[p] * x0 + c[p] * x1;
+    }
+    return R::pack(v);
+  }
+};
+
+// Thread i of tokens * groups * chunks: its chunk of a row, its token and its first head.
+struct ChunkPlace {
+  uint32_t chunk, token, group;
+};
+struct ChunkGrid {
+  uint32_t chunks, tokens, groups, total;
+  int heads_inner;
+};
+__device__ __forceinline__ ChunkPlace chunk_place(const ChunkGrid& g, uint32_t i) {
+  const uint32_t rest = i / g.chunks, inner = g.heads_inner ? g.groups : g.tokens;
+  const uint32_t in = rest % inner, out = rest / inner;
+  return ChunkPlace{i - rest * g.chunks, g.heads_inner ? out : in, g.heads_inner ? in : out};
+}
+
+template <int DT, int HG>
+__global__ __launch_bounds__(256) void ago_axes_chunk_kernel(const RotateAxesArgs a, const ChunkGrid g) {
+  constexpr int EPC = RowChunk<DT>::EPC;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= g.total) return;
+  const ChunkPlace at = chunk_place(g, i);
+  const uint32_t b = at.token / (uint32_t)a.seq, l = at.token - b * (uint32_t)a.seq;
+  const int all = a.heads[0] + a.heads[1];
+  u32x4_t w[HG];
+  int64_t to[HG];
+#pragma unroll
+  for (int u = 0; u < HG; ++u) {
+    const int h = (int)(at.group + u * g.groups);
+    if (h >= all) break;
+    const int which = h >= a.heads[0], hh = which ? h - a.heads[0] : h;
+    w[u] = *(const u32x4_t*)((const typename Elem<DT>::storage*)a.x[which] + b * a.sx[which][0] + hh * a.sx[which][1] +
+                             l * a.sx[which][2] + at.chunk * EPC);
+    to[u] = b * a.sy[which][0] + hh * a.sy[which][1] + l * a.sy[which][2] + at.chunk * EPC;
+  }
+  ChunkTurn<DT> turn;
+  turn.load(a.rot, b * a.pos_b + (int64_t)l * a.rot.axes, (int)(at.chunk * EPC / 2), a.sign);
+#pragma unroll
+  for (int u = 0; u < HG; ++u) {
+    const int h = (int)(at.group + u * g.groups);
+    if (h >= all) break;
+    *(u32x4_t*)((typename Elem<DT>::storage*)a.y[h >= a.heads[0]] + to[u]) = turn.turned(w[u]);
+  }
+}
+
+template <int DT, int HG>
+__global__ __launch_bounds__(256) void afa_paged_append_chunk_kernel(const AppendArgs a, const ChunkGrid g) {
+  constexpr int EPC = RowChunk<DT>::EPC;
+  using S = typename Elem<DT>::storage;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= g.total) return;
+  const ChunkPlace at = chunk_place(g, i);
+  const int64_t t = at.token;
+  const int d = (int)(at.chunk * EPC), H = a.heads, K = a.kv_heads, all = H + 2 * K;
+  const int64_t slot = a.slots[t];
+  u32x4_t w[HG];
+#pragma unroll
+  for (int u = 0; u < HG; ++u) {
+    const int h = (int)(at.group + u * g.groups);
+    if (h >= all) break;
+    const S* x = h < H ? (const S*)a.q + t * a.q_t + h * a.q_h
+                 : h < H + K ? (const S*)a.k + t * a.k_t + (h - H) * a.k_h
+                             : (const S*)a.v + t * a.v_t + (h - H - K) * a.v_h;
+    w[u] = *(const u32x4_t*)(x + d);
+  }
+  ChunkTurn<DT> turn;
+  if (a.rot.rc != nullptr) turn.load(a.rot, t * a.rot.axes, d / 2, 1.0f);
+  const bool stored = slot >= 0 && slot < a.capacity;
+  const uint32_t page = stored ? (uint32_t)slot / (uint32_t)a.page_size : 0, place = (uint32_t)slot - page * a.page_size;
+#pragma unroll
+  for (int u = 0; u < HG; ++u) {
+    const int h = (int)(at.group + u * g.groups);
+    if (h >= all) break;
+    if (h < H ? a.q_out == nullptr : !stored) continue;
+    S* y = h < H ? (S*)a.q_out + (t * H + h) * a.dim
+           : h < H + K ? (S*)a.k_pages + page * a.ps.k_page + (h - H) * a.ps.k_head + place * a.ps.k_slot
+                       : (S*)a.v_pages + page * a.ps.v_page + (h - H - K) * a.ps.v_head + place * a.ps.v_slot;
+    *(u32x4_t*)(y + d) = a.rot.rc != nullptr && h < H + K ? turn.turned(w[u]) : w[u];
+  }
+}
+
+// Four heads a thread where that leaves threads enough to fill the device (about 2^17), else one.
+constexpr int HEADS = 4;
+inline ChunkGrid chunk_grid(int64_t tokens, int64_t heads, int64_t chunks, bool heads_inner, bool& four) {
+  four = tokens * chunks * heads >= (int64_t(1) << 19);
+  ChunkGrid g;
+  g.chunks = (uint32_t)chunks;
+  g.tokens = (uint32_t)tokens;
+  g.groups = (uint32_t)(four ? (heads + HEADS - 1) / HEADS : heads);
+  g.total = g.chunks * g.tokens * g.groups;
+  g.heads_inner = heads_inner;
+  return g;
+}
+
+// The cache write, as ago_axes_kernel: one thread a pair (or the last element of an odd head_dim) of a token's q, k and v
 // heads, in this order.
 template <int DT>
 __global__ __launch_bounds__(256) void afa_paged_append_kernel(const AppendArgs a, int64_t total) {
@@ -117,6 +263,23 @@ __global__ __launch_bounds__(256) void afa_paged_append_kernel(const AppendArgs 
 
 template <int DT>
 hipError_t rotate_axes_go(const RotateAxesArgs& a, hipStream_t st) {
+  if constexpr (DT != AFA_F64) {
+    constexpr int EPC = RowChunk<DT>::EPC;
+    bool whole = a.dim % EPC == 0;
+    for (int i = 0; i < 2 && whole; ++i) {
+      if (a.heads[i] == 0) continue;
+      whole = (((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) & 15u) == 0;
+      for (int j = 0; j < 3; ++j) whole = whole && a.sx[i][j] % EPC == 0 && a.sy[i][j] % EPC == 0;
+    }
+    if (whole) {
+      bool four;
+      const ChunkGrid g = chunk_grid(a.batch * a.seq, a.heads[0] + a.heads[1], a.dim / EPC, a.sx[0][1] < a.sx[0][2], four);
+      const dim3 grid((g.total + 255) / 256);
+      if (four) hipLaunchKernelGGL((ago_axes_chunk_kernel<DT, HEADS>), grid, dim3(256), 0, st, a, g);
+      else hipLaunchKernelGGL((ago_axes_chunk_kernel<DT, 1>), grid, dim3(256), 0, st, a, g);
+      return hipGetLastError();
+    }
+  }
   const int64_t n = a.batch * a.seq * (a.heads[0] + a.heads[1]) * (a.dim / 2);
   hipLaunchKernelGGL((ago_axes_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, n);
   return hipGetLastError();
@@ -124,6 +287,23 @@ hipError_t rotate_axes_go(const RotateAxesArgs& a, hipStream_t st) {
 
 template <int DT>
 hipError_t append_go(const AppendArgs& a, hipStream_t st) {
+  if constexpr (DT != AFA_F64) {
+    constexpr int EPC = RowChunk<DT>::EPC;
+    const uintptr_t bases = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_pages |
+                            (uintptr_t)a.v_pages;
+    bool whole = a.dim % EPC == 0 && (bases & 15u) == 0;
+    for (int64_t v : {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.ps.k_page, a.ps.k_head, a.ps.k_slot, a.ps.v_page,
+                      a.ps.v_head, a.ps.v_slot})
+      whole = whole && v % EPC == 0;
+    if (whole) {
+      bool four;
+      const ChunkGrid g = chunk_grid(a.tokens, a.heads + 2 * a.kv_heads, a.dim / EPC, true, four);
+      const dim3 grid((g.total + 255) / 256);
+      if (four) hipLaunchKernelGGL((afa_paged_append_chunk_kernel<DT, HEADS>), grid, dim3(256), 0, st, a, g);
+      else hipLaunchKernelGGL((afa_paged_append_chunk_kernel<DT, 1>), grid, dim3(256), 0, st, a, g);
+      return hipGetLastError();
+    }
+  }
   const int64_t n = (int64_t)a.tokens * (a.heads + 2 * a.kv_heads) * ((a.dim + 1) / 2);
   hipLaunchKernelGGL((afa_paged_append_kernel<DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, n);
   return hipGetLastError();
