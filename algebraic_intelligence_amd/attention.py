@@ -8,6 +8,7 @@ Every computation runs in the gfx950 kernels of libafa_hip.so (include/afa.h).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -372,8 +373,8 @@ def _axis_tables(rotary_params, head_dim, dtype, dev):
     c, s = _extract_cs(rotary_params)
     want = torch.float64 if dtype == torch.float64 else torch.float32
     if (isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype == want and s.dtype == want and c.ndim == 2
-            and head_dim % 2 == 0 and c.shape[1] == head_dim // 2 and c.shape == s.shape and c.device == dev
-            and s.device == dev and c.is_contiguous() and s.is_contiguous()):
+            and 2 * c.shape[1] == head_dim and c.shape == s.shape and c.device == dev and s.device == dev
+            and c.is_contiguous() and s.is_contiguous()):
         return c, s  # as the kernel takes them
     c, s = (_lib.table_2d(torch.as_tensor(t, device=dev), head_dim) for t in (c, s))
     if c.shape != s.shape:
@@ -389,39 +390,49 @@ def _axis_sections(sections, axes, pairs):
         if axes != 1:
             raise ValueError("positions of several axes need sections, the feature pairs of each axis")
         return None
-    sections = tuple(sections)
+    return _sections_array(tuple(sections), axes, pairs)
+
+
+@functools.lru_cache(maxsize=64)
+def _sections_array(sections, axes, pairs):
     if len(sections) != axes or any(int(n) != n or n < 0 for n in sections) or sum(sections) > pairs:
         raise ValueError(f"sections must be {axes} nonnegative integers with a sum of at most {pairs}, got {sections}")
     return (ctypes.c_int32 * axes)(*(int(n) for n in sections))
 
 
+_Strides12 = ctypes.c_int64 * 12
+
+
+def _axes_launch(q, k, c, s, positions, cuts, axes, transpose):
+    """q, and k unless None, (B, H, L, D) of one dtype, batch and length, rotated, or back; the results lie in
+    memory in their inputs' axis order."""
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    B, H, L, D = q.shape
+    y = _dense_like(q)
+    sq, sy = q.stride(), y.stride()
+    K, kp, zp, z = 0, None, None, None
+    sk = sz = (0, 0, 0)
+    if k is not None:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        z = _dense_like(k)
+        K, kp, zp, sk, sz = k.shape[1], k.data_ptr(), z.data_ptr(), k.stride(), z.stride()
+    dev = q.device
+    with _lib.on_device(dev):
+        rc = _lib.lib().ago_rotate_axes(
+            _lib.dtype_code(q.dtype), B, H, K, L, D, q.data_ptr(), kp, y.data_ptr(), zp,
+            _Strides12(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sy[0], sy[1], sy[2], sz[0], sz[1], sz[2]), c.data_ptr(),
+            s.data_ptr(), c.shape[0], positions.data_ptr(), positions.element_size(),
+            0 if positions.ndim == 2 else positions.stride(0), axes, cuts, transpose, _lib.stream_ptr(dev))
+    _lib.check(rc, "ago_rotate_axes")
+    return y, z
+
+
 def _dense_like(x):
     """An empty tensor of x's shape whose axes lie in memory in x's order, without gaps."""
     y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 or y.shape[-1] == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
-
-
-def _axes_launch(xs, c, s, positions, cuts, axes, transpose):
-    """Each (B, H, L, D) tensor of xs (one or two of one dtype, batch and length) rotated, or back."""
-    dev = xs[0].device
-    xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
-    ys = [_dense_like(x) for x in xs]
-    B, H, L, D = xs[0].shape
-    k = xs[1] if len(xs) == 2 else None
-    strides = []
-    for pair in (xs, ys):
-        for t in pair:
-            strides.extend(t.stride()[:3])
-        if k is None:
-            strides.extend((0, 0, 0))
-    with _lib.on_device(dev):
-        rc = _lib.lib().ago_rotate_axes(
-            _lib.dtype_code(xs[0].dtype), B, H, 0 if k is None else k.shape[1], L, D, xs[0].data_ptr(), _lib.ptr(k),
-            ys[0].data_ptr(), None if k is None else ys[1].data_ptr(), (ctypes.c_int64 * 12)(*strides), c.data_ptr(),
-            s.data_ptr(), c.shape[0], positions.data_ptr(), positions.element_size(),
-            0 if positions.ndim == 2 else positions.stride(0), axes, cuts, int(transpose), _lib.stream_ptr(dev))
-    _lib.check(rc, "ago_rotate_axes")
-    return ys
+    return y if y.stride(3) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 class _RotateAxes(torch.autograd.Function):
@@ -429,28 +440,34 @@ class _RotateAxes(torch.autograd.Function):
     transposed rotation of the cotangents, in one launch where both are there."""
 
     @staticmethod
-    def forward(ctx, q, k, c, s, positions, cuts, axes, transpose):
+    def forward(ctx, q, k, c, s, positions, cfg):
         ctx.save_for_backward(c, s, positions)
-        ctx.cfg = (cuts, axes, transpose)
+        ctx.cfg = cfg
         ctx.set_materialize_grads(False)
+        y, z = _axes_launch(q, k, c, s, positions, *cfg)
         if k is None:
-            return _axes_launch([q], c, s, positions, cuts, axes, transpose)[0]
-        out = _axes_launch([q, k], c, s, positions, cuts, axes, transpose)
-        fixed = [y for y, need in zip(out, ctx.needs_input_grad) if not need]
-        if fixed:
-            ctx.mark_non_differentiable(*fixed)
-        return tuple(out)
+            return y
+        if not (ctx.needs_input_grad[0] and ctx.needs_input_grad[1]):
+            ctx.mark_non_differentiable(z if ctx.needs_input_grad[0] else y)
+        return y, z
 
     @staticmethod
     def backward(ctx, gq, gk=None):
         c, s, positions = ctx.saved_tensors
         cuts, axes, transpose = ctx.cfg
-        args = (c, s, positions, cuts, axes, not transpose)
+        cfg = (cuts, axes, 1 - transpose)
         if gq is not None and gk is not None:
-            gq, gk = _RotateAxes.apply(gq, gk, *args)
+            gq, gk = _rotate_axes(gq, gk, c, s, positions, cfg)
         else:
-            gq, gk = (None if g is None else _RotateAxes.apply(g, None, *args) for g in (gq, gk))
-        return gq, gk, None, None, None, None, None, None
+            gq, gk = (None if g is None else _rotate_axes(g, None, c, s, positions, cfg) for g in (gq, gk))
+        return gq, gk, None, None, None, None
+
+
+def _rotate_axes(q, k, c, s, positions, cfg):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotateAxes.apply(q, k, c, s, positions, cfg)
+    y, z = _axes_launch(q, k, c, s, positions, *cfg)
+    return y if k is None else (y, z)
 
 
 def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
@@ -467,28 +484,31 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
     (fp64) from the tables as they are, with one rounding; a position outside the tables gives NaN.
     Differentiable with respect to q and k, twice too."""
     q = _float_input(q)
-    if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+    shape = q.shape
+    if len(shape) != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != shape[0] or k.shape[2:] != shape[2:])):
         raise ValueError("q and k must have shapes (batch, heads, sequence, dimension), alike but for the heads, got "
-                         f"{tuple(q.shape)} and {None if k is None else tuple(k.shape)}")
+                         f"{tuple(shape)} and {None if k is None else tuple(k.shape)}")
     if k is not None and k.dtype != q.dtype:
         raise TypeError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
-    B, _, L, D = q.shape
+    B, _, L, D = shape
     if D % 2 != 0:
         raise ValueError(f"Feature dimension must be even, got {D}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if positions.ndim not in (2, 3) or positions.shape[-2] != L or (positions.ndim == 3 and positions.shape[0] not in (1, B)):
-        raise ValueError(f"positions must have shape ({B}, {L}, axes) or ({L}, axes), got {tuple(positions.shape)}")
-    axes = positions.shape[-1]
+    at = positions.shape
+    if len(at) not in (2, 3) or at[-2] != L or (len(at) == 3 and at[0] not in (1, B)):
+        raise ValueError(f"positions must have shape ({B}, {L}, axes) or ({L}, axes), got {tuple(at)}")
+    axes = at[-1]
     cuts = _axis_sections(sections, axes, D // 2)
     _lib.dtype_code(q.dtype)
     dev = _lib.require_device(q, k, positions)
     c, s = _axis_tables(rotary_params, D, q.dtype, dev)
-    if positions.ndim == 3 and positions.shape[0] == 1:
+    if len(at) == 3 and at[0] == 1:
         positions = positions[0]
     positions = positions.contiguous()
-    if q.numel() == 0 or (k is not None and k.numel() == 0):
-        if q.numel() == 0:
-            return q.clone() if k is None else (q.clone(), k.clone())
-        return _RotateAxes.apply(q, None, c, s, positions, cuts, axes, False), k.clone()
-    return _RotateAxes.apply(q, k, c, s, positions, cuts, axes, False)
+    cfg = (cuts, axes, 0)
+    if q.numel() == 0:
+        return q.clone() if k is None else (q.clone(), k.clone() if k.numel() == 0 else _rotate_axes(k, None, c, s, positions, cfg))
+    if k is not None and k.numel() == 0:
+        return _rotate_axes(q, None, c, s, positions, cfg), k.clone()
+    return _rotate_axes(q, k, c, s, positions, cfg)

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64), lp = f.log_page, in_page = (1 << lp) - 1;
   const float scale = (float)a.scale;
   const int items = a.sched.header[PS_ITEMS];
-  const int64_t total = (int64_t)items * p.kv_heads;
+  const int64_t total = (int64_t)items * p.kv_heads;  // below 2^31
   // a row's four features d.. from its sums
   auto store4 = [&](int64_t at, int d, f32x4_t x, float sum) {
     const float all = sum + (float)a.omega;
@@ -195,8 +195,10 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   };
 
   for (int64_t w0 = blockIdx.x; w0 < total; w0 += gridDim.x) {
-    const int hk = (int)(w0 / items);
-    const PagedItem it = a.sched.items[w0 - (int64_t)hk * items];
+    // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
+    const unsigned which = (unsigned)w0 / (unsigned)p.kv_heads;
+    const int hk = (int)((unsigned)w0 - which * (unsigned)p.kv_heads);
+    const PagedItem it = a.sched.items[which];
     if (it.tile0 >= it.tile1) continue;
     const int c = it.cached, n = it.fresh, keys = c + n, nrows = n * G;
     const bool tree = a.masks != nullptr && n <= p.max_tree;
@@ -365,9 +367,23 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       for (int b = 0; b < QB; ++b) {
         float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float s = s4[b][e >> 2][e & 3] * scale;
-          w[e] = F32 ? rho8_refined(s) : rho8_exact(s);
+        for (int e = 0; e < 8; ++e) w[e] = s4[b][e >> 2][e & 3] * scale;
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = rho8_refined(w[e]);
+        } else {
+          // the branch-free form costs half of the other and loses nothing above 0, and below it
+          // 16 s^2 times the error of the hardware's rsqrt, 2.2e-4 at -8
+          float low = w[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) low = __builtin_fminf(low, w[e]);
+          if (__ballot(!(low > -8.0f)) == 0) {  // a NaN stays one in either form
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = rho8_fast(w[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = rho8_exact(w[e]);
+          }
         }
         if (masked) {
           const int64_t* words = tree ? a.masks + (int64_t)(it.start + token[b]) * W : nullptr;

@@ -114,7 +114,11 @@ class DraftPlan:
         self.pool, self.dtype = pool, dtype
         self.max_tokens, self.heads, self.kv_heads, self.head_dim = int(max_tokens), int(heads), int(kv_heads), int(head_dim)
         self.max_tree = int(max_tree)
-        dev = pool.device
+        dev = self.device = pool.device
+        self._q_shape = (self.max_tokens, self.heads, self.head_dim)
+        self._kv_shape = (self.max_tokens, self.kv_heads, self.head_dim)
+        self._page_shape = (pool.num_pages, self.kv_heads, pool.page_size, self.head_dim)
+        self._len_shape = (pool.max_requests,)
         c = self._c = _Plan(num_pages=pool.num_pages, page_size=pool.page_size, requests=pool.max_requests,
                             table_width=pool.block_tables.shape[1], max_tokens=max_tokens, max_new=max_new,
                             max_tree=max_tree, heads=heads, kv_heads=kv_heads, head_dim=head_dim, dtype=_lib.dtype_code(dtype))
@@ -147,7 +151,7 @@ class DraftPlan:
 def _lengths(name, t, dev, shape):
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     if t.device != dev:
         _lib.require_device(t)
@@ -168,8 +172,8 @@ def build_block_tables(plan: DraftPlan, cached_lens: torch.Tensor, new_lens: tor
     before it.  Returns the plan; nothing is read back to the host."""
     pool = plan.pool
     dev = pool.device
-    cached_lens = _lengths("cached_lens", cached_lens, dev, (pool.max_requests,))
-    new_lens = _lengths("new_lens", new_lens, dev, (pool.max_requests,))
+    cached_lens = _lengths("cached_lens", cached_lens, dev, plan._len_shape)
+    new_lens = _lengths("new_lens", new_lens, dev, plan._len_shape)
     if parents is not None:
         if plan.max_tree == 0:
             raise ValueError("parents need a plan with max_tree")
@@ -181,35 +185,36 @@ def build_block_tables(plan: DraftPlan, cached_lens: torch.Tensor, new_lens: tor
     return plan
 
 
+_Strides6, _Strides2 = ctypes.c_int64 * 6, ctypes.c_int64 * 2
+
+
 def _pages(plan, k_pages, v_pages):
     """Strides of the pages (page, head, slot of k, then of v), None where both are contiguous."""
-    pool = plan.pool
-    shape = (pool.num_pages, plan.kv_heads, pool.page_size, plan.head_dim)
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != plan.dtype:
-            raise TypeError(f"{name} must be {plan.dtype}, got {t.dtype}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-        if t.device != pool.device:
-            _lib.require_device(t)
-            raise ValueError(f"{name} must be on the plan's device {pool.device}, got {t.device}")
-        if t.stride(-1) != 1 and plan.head_dim != 1:
-            raise ValueError(f"{name} needs a contiguous head dimension")
+        if t.dtype != plan.dtype or t.shape != plan._page_shape or t.device != plan.device:
+            _refuse(plan, name, t, plan._page_shape)
     if k_pages.is_contiguous() and v_pages.is_contiguous():
         return None
-    return (ctypes.c_int64 * 6)(*k_pages.stride()[:3], *v_pages.stride()[:3])
+    k, v = k_pages.stride(), v_pages.stride()
+    if (k[3] != 1 or v[3] != 1) and plan.head_dim != 1:
+        raise ValueError("k_pages and v_pages need a contiguous head dimension")
+    return _Strides6(k[0], k[1], k[2], v[0], v[1], v[2])
 
 
-def _rows(plan, name, t, heads):
-    """t (max_tokens, heads, head_dim) with a contiguous head dimension."""
+def _rows(plan, name, t, shape):
+    """t of the plan's dtype and device, of shape (max_tokens, heads, head_dim), with a contiguous head dimension."""
+    if t.dtype != plan.dtype or t.shape != shape or t.device != plan.device:
+        _refuse(plan, name, t, shape)
+    return t if t.stride(2) == 1 or plan.head_dim == 1 else t.contiguous()
+
+
+def _refuse(plan, name, t, shape):
     if t.dtype != plan.dtype:
         raise TypeError(f"{name} must be {plan.dtype}, got {t.dtype}")
-    if tuple(t.shape) != (plan.max_tokens, heads, plan.head_dim):
-        raise ValueError(f"{name} must have shape {(plan.max_tokens, heads, plan.head_dim)}, got {tuple(t.shape)}")
-    if t.device != plan.pool.device:
-        _lib.require_device(t)
-        raise ValueError(f"{name} must be on the plan's device {plan.pool.device}, got {t.device}")
-    return t if t.stride(-1) == 1 or plan.head_dim == 1 else t.contiguous()
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    _lib.require_device(t)
+    raise ValueError(f"{name} must be on the plan's device {plan.device}, got {t.device}")
 
 
 def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -222,9 +227,9 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     cast); None: k is stored and q returned as they are.  ``positions`` (max_tokens, A) int32 with
     ``sections`` gives positions of A axes as in ``apply_ago_axis_rotations``; (max_tokens,) or None, the
     plan's positions, is one axis.  Tokens without a slot are not stored."""
-    q, k, v = _rows(plan, "q", q, plan.heads), _rows(plan, "k", k, plan.kv_heads), _rows(plan, "v", v, plan.kv_heads)
+    q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
     page_strides = _pages(plan, k_pages, v_pages)
-    dev = plan.pool.device
+    dev = plan.device
     c = s = None
     axes, cuts = 1, None
     q_out = q
@@ -235,12 +240,12 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
             shape = (plan.max_tokens,) if positions.ndim == 1 else (plan.max_tokens, axes)
             positions = _lengths("positions", positions, dev, shape)
         cuts = _axis_sections(sections, axes, plan.head_dim // 2)
-        q_out = torch.empty((plan.max_tokens, plan.heads, plan.head_dim), dtype=plan.dtype, device=dev)
+        q_out = torch.empty(plan._q_shape, dtype=plan.dtype, device=dev)
     elif positions is not None or sections is not None:
         raise ValueError("positions and sections need rotary_params")
     strides = None
     if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
-        strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+        strides = _Strides6(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_append(
             plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, None if c is None else q_out.data_ptr(),
@@ -263,9 +268,9 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     inference: not differentiable."""
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
-    q = _rows(plan, "q", q, plan.heads)
+    q = _rows(plan, "q", q, plan._q_shape)
     page_strides = _pages(plan, k_pages, v_pages)
-    dev = plan.pool.device
+    dev = plan.device
     if masks is not None:
         if plan.max_tree == 0:
             raise ValueError("masks need a plan with max_tree")
@@ -274,7 +279,7 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         masks = masks.contiguous()
     flags = 0
     if out is None:
-        out = torch.empty((plan.max_tokens, plan.heads, plan.head_dim), dtype=plan.dtype, device=dev)
+        out = torch.empty(plan._q_shape, dtype=plan.dtype, device=dev)
         flags = _lib.FLAG_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
@@ -284,7 +289,7 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if return_denominator:
         new = torch.empty if flags else torch.zeros
         den = new((plan.max_tokens, plan.heads), dtype=_lib.accum_dtype(q.dtype), device=dev)
-    strides = None if q.is_contiguous() else (ctypes.c_int64 * 2)(*q.stride()[:2])
+    strides = None if q.is_contiguous() else _Strides2(q.stride(0), q.stride(1))
     with _lib.on_device(dev):
         # the workspace comes from torch's caching allocator, so the library allocates nothing
         ws_bytes = plan._ws_bytes
