@@ -12,53 +12,75 @@ constexpr int kPagedTile = 32;   // keys of a tile, the unit in which a request'
 constexpr int kMaxTree = 256;    // nodes of a drafted tree
 constexpr int kMaxAxes = 4;
 
-// A part of one request's attention for one key/value head: query rows [row0, row0 + rows per item) of its
-// new * group rows, key tiles [tile0, tile1).  part: the slot of its partial sums, -1 where the part is whole.
-struct PagedItem {
-  int request, row0, tile0, tile1, part, cached, fresh, start;
+// How the attention of a plan is cut, a function of its sizes and the device alone.
+//
+// A segment is one request's query rows of one block (up to `rows` of its new tokens * group) over all of its
+// keys.  Laid end to end, a segment taking kPagedLead units and one for each of its key tiles, the segments
+// of a key/value head form a line that is cut into `slots` even stretches, one for each workgroup.  Every
+// workgroup so has the same work whatever the lengths; a segment that a cut crosses ends as partial sums,
+// at most two of a slot: of a segment that began earlier and of one that goes on.
+struct PagedCut {
+  int rows;
+  int64_t slots;  // per key/value head
 };
+constexpr int kPagedLead = 4;  // what a segment costs beside its tiles, in tiles
+constexpr int kPagedMin = 4;   // shortest stretch: a tile for each wave
+
+// A request with attention to do: its place on the line, and `cost` units for each of `blocks` row blocks.
+struct PagedLive {
+  int request, cached, fresh, start;
+  int64_t flat;
+  int blocks, cost;
+};
+// Where slot s begins: unit `at` of row block `block` of live request `live`.
+struct PagedSlot {
+  int live, block, at, unused;
+};
+
+// plan->schedule.  The ticket and the counters are 0 between calls.
+struct PagedHeader {
+  int ticket, slots;
+  int64_t stretch, end;  // of a slot, and of the line
+};
+struct PagedSchedule {
+  PagedHeader* header;
+  PagedLive* live;
+  PagedSlot* slot;
+  int* count;                        // (kv_heads, 2, 2 slots): parts that have arrived, and groups of them
+  int *pop, *push, *held, *cached;   // per request
+  int64_t* flat;                     // per request, then its place among the live ones
+  int* place;
+};
+
+PagedCut paged_cut(const afa_paged_plan& p, int cus);
+size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c);
+
+__host__ __device__ inline PagedSchedule paged_schedule(const afa_paged_plan& p, int64_t slots) {
+  PagedSchedule s;
+  char* at = (char*)p.schedule;
+  const int64_t R = p.requests;
+  s.header = (PagedHeader*)at;
+  at += 64;
+  s.live = (PagedLive*)at;
+  at += R * sizeof(PagedLive);
+  s.slot = (PagedSlot*)at;
+  at += slots * sizeof(PagedSlot);
+  s.flat = (int64_t*)at;
+  at += R * 8;
+  s.count = (int*)at;
+  s.pop = s.count + p.kv_heads * 4 * slots;
+  s.push = s.pop + R;
+  s.held = s.push + R;
+  s.cached = s.held + R;
+  s.place = s.cached + R;
+  return s;
+}
 
 // Key tiles that row block `block` of a request's n new tokens sees: all, or in a chain those up to the
 // block's last token.
 __host__ __device__ inline int paged_block_tiles(int c, int n, bool tree, int block, int rows, int group) {
   const unsigned last = (unsigned)(block * rows + rows - 1) / (unsigned)group;
   return (int)((unsigned)(c + (tree || last >= (unsigned)n ? n - 1 : (int)last) + kPagedTile) / kPagedTile);
-}
-
-// plan->schedule: a header, six ints per request, the items, then a counter for each part of each key/value head.
-// The ticket and the counters are 0 between calls.
-enum { PS_ITEMS = 0, PS_CHUNK = 1, PS_TICKET = 2, PS_INTS = 16 };
-struct PagedSchedule {
-  int* header;
-  int *pop, *push, *held, *chunks, *part, *item;  // per request
-  PagedItem* items;
-};
-
-// How the attention of a plan is cut, a function of its sizes and the device alone.
-struct PagedCut {
-  int rows;            // query rows of an item
-  int64_t target;      // items per head that fill the device
-  int64_t max_items;   // per head
-  int64_t max_parts;   // partial sums per head
-};
-
-PagedCut paged_cut(const afa_paged_plan& p, int cus);
-size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c);
-
-__host__ __device__ inline PagedSchedule paged_schedule(const afa_paged_plan& p) {
-  PagedSchedule s;
-  const int64_t R = p.requests;
-  s.header = p.schedule;
-  int* at = p.schedule + PS_INTS;
-  s.pop = at;
-  s.push = at + R;
-  s.held = at + 2 * R;
-  s.chunks = at + 3 * R;
-  s.part = at + 4 * R;
-  s.item = at + 5 * R;
-  // the items, two 16-byte words each, start at a multiple of 16 bytes
-  s.items = (PagedItem*)(p.schedule + ((PS_INTS + 6 * R + 3) & ~(int64_t)3));
-  return s;
 }
 
 hipError_t paged_build_launch(const afa_paged_plan& p, const PagedCut& c, const int32_t* cached, const int32_t* fresh,
@@ -108,7 +130,7 @@ hipError_t paged_fwd_generic_launch(const PagedFwdArgs& a, hipStream_t st);
 // Matrix-core path (afa_paged_mfma.hip): 16-byte aligned rows of q, pages and out.  ws: paged_fast_workspace bytes.
 bool paged_fast_supported(const afa_paged_plan& p);
 size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c);
-hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int cus, void* ws, hipStream_t st);
+hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, void* ws, hipStream_t st);
 
 struct RotateAxesArgs {
   const void *x[2];

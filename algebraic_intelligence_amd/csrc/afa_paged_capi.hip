@@ -151,7 +151,9 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
   if (p.max_tokens > (kLaunchThreads - 1) / 256 / p.heads) return AFA_ERR_SHAPE;
   afa::PagedFwdArgs a = {};
   a.plan = p;
-  a.sched = afa::paged_schedule(p);
+  const int cus = afa::device_cus();
+  const afa::PagedCut cut = afa::paged_cut(p, cus);
+  a.sched = afa::paged_schedule(p, cut.slots);
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages;
   a.masks = masks != nullptr ? masks : p.max_tree > 0 ? p.masks : nullptr;
   a.q_t = q_strides != nullptr ? q_strides[0] : p.heads * p.head_dim;
@@ -176,8 +178,6 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
     const hipError_t e = afa::paged_fwd_generic_launch(a, s);
     return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
   }
-  const int cus = afa::device_cus();
-  const afa::PagedCut cut = afa::paged_cut(p, cus);
   const size_t need = afa::paged_fast_workspace(p, cut);
   void* ws = workspace;
   if (ws == nullptr) {
@@ -188,7 +188,7 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
   } else if (!aligned16(ws)) {
     return AFA_ERR_ALIGN;
   }
-  hipError_t e = afa::paged_fwd_fast_launch(a, cut, cus, ws, s);
+  hipError_t e = afa::paged_fwd_fast_launch(a, cut, ws, s);
   if (workspace == nullptr) {
     const hipError_t e2 = hipFreeAsync(ws, s);
     if (e == hipSuccess) e = e2;

@@ -34,8 +34,7 @@ __global__ __launch_bounds__(ROW_KEYS) void afa_paged_row_kernel(const PagedFwdA
   if (r < 0 && !a.zero_tail) return;
   const bool live = r >= 0 && p.status[r] == AFA_PAGED_OK;
   const int start = live ? p.starts[r] : 0, n = live ? p.starts[r + 1] - start : 0, i = (int)t - start;
-  // cached tokens, from the first item of the request's schedule
-  const int c = live ? a.sched.items[a.sched.item[r]].cached : 0, keys = live ? c + n : 0;
+  const int c = live ? a.sched.cached[r] : 0, keys = live ? c + n : 0;
   const int W = (int)(p.max_tree / 64);
   const bool tree = a.masks != nullptr && n <= p.max_tree;
   for (int d = tid; d < D; d += ROW_KEYS) q_row[d] = elem<DT, A>(a.q, t * a.q_t + h * a.q_h + d);

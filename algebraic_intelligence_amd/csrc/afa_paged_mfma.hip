@@ -4,9 +4,9 @@
 //   out_i = sum_j w_ij v_j / (sum_j w_ij + Omega),  w_ij = rho(q_i.k_j / sqrt(D))^8
 //
 // The few query rows of a request that share a key/value head (its new tokens times the heads of the
-// group) meet every cached key once: the bytes of K and V bound the work.  A workgroup takes an item of
-// the plan, 16 QB rows and a run of 32-key tiles of one head, and its four waves a quarter of the run
-// each.  A wave needs no other until its end:
+// group) meet every cached key once: the bytes of K and V bound the work.  A workgroup takes a slot of the
+// plan (afa_paged.h): stretches of 32-key tiles of one head, of one segment after the other.  A wave needs no
+// other until a segment's end:
 //
 //   S^T = K Q^T    A = 16 keys, B = 16 rows; a lane ends with 8 keys' scores of row lane % 16
 //   w = rho^8      in place; they are the B operand of
@@ -90,10 +90,9 @@ __device__ __forceinline__ bool nonfinite(unsigned w) {
 
 struct PagedFast {
   PagedFwdArgs a;
-  float* part;       // (kv_heads, max_parts, rows, D) numerators
-  float *part_den, *part_sum;  // (kv_heads, max_parts, rows) row sums of the parts, and of their groups
-  int* count;        // (kv_heads, max_parts), 0 between calls
-  int64_t max_parts;
+  float* part;                 // (kv_heads, 2 slots, rows, D) numerators
+  float *part_den, *part_sum;  // (kv_heads, 2 slots, rows) row sums of the parts, and of their groups
+  int64_t slots;
   int log_page, dim;
   uint32_t k_page, k_slot, v_page, v_slot;  // strides in bytes
 };
@@ -134,14 +133,27 @@ __device__ __forceinline__ bool arrived(int* count, int n, int* flag) {
   return *flag != 0;
 }
 
-// Sum of four features and of the row sums over `n` parts, `stride` rows apart, in their order.
-__device__ __forceinline__ f32x4_t sum_parts(const float* part, const float* den, int n, int64_t stride, int D, float& sum) {
+// Sum of four features and of the row sums over `n` parts in their order, which lie at rows at(0), at(1), ...
+template <typename F>
+__device__ __forceinline__ f32x4_t sum_parts(const float* part, const float* den, int n, int D, float& sum, const F& at) {
   f32x4_t x = {0, 0, 0, 0};
   sum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    x += get4(part + i * stride * D);
-    sum += get1(den + i * stride);
+  for (int i = 0; i < n; i += 8) {
+    // up to eight parts in flight
+    f32x4_t y[8];
+    float s[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (i + u >= n) break;
+      y[u] = get4(part + at(i + u) * D);
+      s[u] = get1(den + at(i + u));
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (i + u >= n) break;
+      x += y[u];
+      sum += s[u];
+    }
   }
   return x;
 }
@@ -154,12 +166,13 @@ __device__ __forceinline__ int group_size(int parts) {
   return s * s < parts ? s + 1 : s;
 }
 
-// Waves for each SIMD that the registers are kept to: two where Q, the sums and a tile of K and V leave
-// room for them, one wave's loads then run under another's arithmetic.
-constexpr int paged_waves(bool f32, int dp, int qb) { return dp < 256 && dp * (f32 ? 2 : 1) * qb <= 256 ? 2 : 1; }
+// Four waves: QB row blocks of 16 each, RW of them side by side that meet the same keys (the later ones from
+// L1 or L2), KW along the keys.
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
 
-template <int DT, int DP, bool FULL, int QB>
-__global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_paged_tile_kernel(const PagedFast f) {
+template <int DT, int DP, bool FULL, int QB, int RW>
+__global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_kernel(const PagedFast f) {
+  constexpr int KW = WAVES / RW, NBUF = KW > 1 ? KW / 2 : 1;
   constexpr bool F32 = DT == AFA_F32;
   constexpr int ESZ = F32 ? 4 : 2;
   constexpr int EPL = DP / 16;            // features of V a lane, and products of O
@@ -167,19 +180,19 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   constexpr int KS = F32 ? DP / 16 : DP / 32;  // 16-byte chunks of a K row a lane
   constexpr int KB = F32 ? 16 : 32;       // features of a chunk over the four lane groups
   constexpr int GR = F32 ? 2 : 1;         // groups of 8 keys that a lane reads of K, and of V
-  constexpr int ROWS = 16 * QB, LD = DP + 4;
-  __shared__ float red[2][ROWS][LD];
-  __shared__ float red_den[4][ROWS];
-  __shared__ int red_odd[4], flag;
+  constexpr int ROWS = 16 * QB * RW, LD = DP + 4;
+  __shared__ float red[NBUF][ROWS][LD];
+  __shared__ float red_den[KW][ROWS];
+  __shared__ int red_odd[WAVES], flag;
   const PagedFwdArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
   const int D = FULL ? DP : f.dim;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, mine0 = 16 * QB * (wave % RW);
   const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64), lp = f.log_page, in_page = (1 << lp) - 1;
   const float scale = (float)a.scale;
-  const int items = a.sched.header[PS_ITEMS];
-  const int64_t total = (int64_t)items * p.kv_heads;  // below 2^31
+  // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
+  const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads), hk = (int)(blockIdx.x - (unsigned)slot * (unsigned)p.kv_heads);
   // a row's four features d.. from its sums
   auto store4 = [&](int64_t at, int d, f32x4_t x, float sum) {
     const float all = sum + (float)a.omega;
@@ -194,19 +207,38 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
     if (d == 0 && a.denom != nullptr) ((float*)a.denom)[at] = all;
   };
 
-  for (int64_t w0 = blockIdx.x; w0 < total; w0 += gridDim.x) {
-    // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
-    const unsigned which = (unsigned)w0 / (unsigned)p.kv_heads;
-    const int hk = (int)((unsigned)w0 - which * (unsigned)p.kv_heads);
-    const PagedItem it = a.sched.items[which];
-    if (it.tile0 >= it.tile1) continue;
-    const int c = it.cached, n = it.fresh, keys = c + n, nrows = n * G;
+  const bool busy = slot < a.sched.header->slots;
+  const PagedSlot begin = a.sched.slot[busy ? slot : 0];
+  const int64_t stretch = a.sched.header->stretch;
+  int64_t pos = slot * stretch;
+  const int64_t stop = busy ? min(pos + stretch, a.sched.header->end) : pos;
+  int live = begin.live, block = begin.block, unit = begin.at;
+  while (pos < stop) {
+    const PagedLive q = a.sched.live[live];
+    const int c = q.cached, n = q.fresh, keys = c + n, nrows = n * G, row0 = block * ROWS;
     const bool tree = a.masks != nullptr && n <= p.max_tree;
-    const int32_t* table = p.block_tables + (int64_t)it.request * p.table_width;
+    const int take = (int)min((int64_t)(q.cost - unit), stop - pos);
+    const int tiles = paged_block_tiles(c, n, tree, block, ROWS, G);
+    const int tile0 = max(unit - kPagedLead, 0), tile1 = min(unit + take - kPagedLead, tiles);
+    // the slots that hold keys of this segment
+    const int64_t key0 = pos - unit + kPagedLead;
+    const int from_slot = (int)(key0 / stretch), parts = (int)((key0 + tiles - 1) / stretch) - from_slot + 1;
+    pos += take;
+    unit += take;
+    if (unit == q.cost) {
+      unit = 0;
+      if (++block == q.blocks) {
+        block = 0;
+        ++live;
+      }
+    }
+    if (tile0 >= tile1) continue;
+    const int32_t* table = p.block_tables + (int64_t)q.request * p.table_width;
     const char* k_base = (const char*)a.k_pages + hk * a.ps.k_head * ESZ;
     const char* v_base = (const char*)a.v_pages + hk * a.ps.v_head * ESZ;
-    const int per = (it.tile1 - it.tile0 + 3) / 4;
-    const int t0 = it.tile0 + wave * per, t1 = min(t0 + per, it.tile1);
+    const int per = (tile1 - tile0 + KW - 1) / KW;
+    // a wave without rows has no keys
+    const int t0 = tile0 + kw * per, t1 = row0 + mine0 < nrows ? min(t0 + per, tile1) : t0;
 
     // 64 entries of the table, one a lane, from the page of the wave's first tile on
     int entry0 = 0, entry = 0;
@@ -276,13 +308,13 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
     int token[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-      const int row = min(it.row0 + 16 * b + m, nrows - 1);
+      const int row = min(row0 + mine0 + 16 * b + m, nrows - 1);
       token[b] = row / G;
-      const char* q = (const char*)a.q + ((int64_t)(it.start + token[b]) * a.q_t + (hk * G + row - token[b] * G) * a.q_h) * ESZ;
+      const char* x = (const char*)a.q + ((int64_t)(q.start + token[b]) * a.q_t + (hk * G + row - token[b] * G) * a.q_h) * ESZ;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = KB * ks + 16 / ESZ * g;
-        qf[b][ks] = FULL || d < D ? *(const u32x4_t*)(q + d * ESZ) : u32x4_t{0, 0, 0, 0};
+        qf[b][ks] = FULL || d < D ? *(const u32x4_t*)(x + d * ESZ) : u32x4_t{0, 0, 0, 0};
       }
     }
 
@@ -386,7 +418,7 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
           }
         }
         if (masked) {
-          const int64_t* words = tree ? a.masks + (int64_t)(it.start + token[b]) * W : nullptr;
+          const int64_t* words = tree ? a.masks + (int64_t)(q.start + token[b]) * W : nullptr;
           unsigned sees;
           if constexpr (F32) {
             sees = sees_bits(kb - c + 4 * g, 4, n, token[b], words, W) |
@@ -457,14 +489,14 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       if (more) load_v();
     }
 
-    // join the waves: 0 and 1 store, 2 and 3 add to theirs
+    // join the waves along the keys: the first half stores, the second adds to theirs
     __syncthreads();  // red is free of the item before
     if (lane == 0) red_odd[wave] = any_odd;
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
       den[b] += __shfl_xor(den[b], 16);
       den[b] += __shfl_xor(den[b], 32);
-      if (g == 0) red_den[wave][16 * b + m] = den[b];
+      if (g == 0) red_den[kw][mine0 + 16 * b + m] = den[b];
       if constexpr (DT == AFA_F16) {
         const float back = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc[b]));
 #pragma unroll
@@ -472,15 +504,15 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       }
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if ((wave >> 1) == half) {
+    for (int half = 0; half < KW / NBUF; ++half) {
+      if (kw / NBUF == half) {
 #pragma unroll
         for (int b = 0; b < QB; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < EPL; j += 4) {
-              f32x4_t* to = (f32x4_t*)&red[wave & 1][16 * b + m][EPL * (4 * g + i) + j];
+              f32x4_t* to = (f32x4_t*)&red[kw % NBUF][mine0 + 16 * b + m][EPL * (4 * g + i) + j];
               f32x4_t x = {acc[b][j][i], acc[b][j + 1][i], acc[b][j + 2][i], acc[b][j + 3][i]};
               *to = half ? *to + x : x;
             }
@@ -488,20 +520,30 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
       __syncthreads();
     }
     auto out_row = [&](int row) {
-      const int who = (it.row0 + row) / G;
-      return (int64_t)(it.start + who) * H + hk * G + (it.row0 + row - who * G);
+      const int who = (row0 + row) / G;
+      return (int64_t)(q.start + who) * H + hk * G + (row0 + row - who * G);
     };
-    const bool odd = (red_odd[0] | red_odd[1] | red_odd[2] | red_odd[3]) != 0;
-    const int mine = min(ROWS, nrows - it.row0), quads = D / 4;
-    for (int e = tid; e < mine * quads; e += 256) {
+    bool odd = false;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) odd = odd || red_odd[w] != 0;
+    const int mine = min(ROWS, nrows - row0), quads = D / 4;
+    // part i of this segment: a slot's second where it begins there, else its first
+    const int64_t head0 = (int64_t)hk * 2 * f.slots;
+    auto part_of = [&](int i) { return head0 + 2 * (from_slot + i) + (i == 0); };
+    const int64_t my_part = part_of(slot - from_slot);
+    for (int e = tid; e < mine * quads; e += THREADS) {
       const int row = e / quads, d = 4 * (e - row * quads);
-      f32x4_t x = *(const f32x4_t*)&red[0][row][d] + *(const f32x4_t*)&red[1][row][d];
-      const float sum = (red_den[0][row] + red_den[1][row]) + (red_den[2][row] + red_den[3][row]);
+      f32x4_t x = *(const f32x4_t*)&red[0][row][d];
+      float sum = red_den[0][row];
+#pragma unroll
+      for (int w = 1; w < NBUF; ++w) x += *(const f32x4_t*)&red[w][row][d];
+#pragma unroll
+      for (int w = 1; w < KW; ++w) sum += red_den[w][row];
       if (odd) {
         // drafted values that are not finite, of weights above 0: the value itself
-        const int who = (it.row0 + row) / G;
-        const int64_t* words = a.masks + (int64_t)(it.start + who) * W;
-        for (int pos = max(it.tile0 * kPagedTile, c); pos < min(it.tile1 * kPagedTile, keys); ++pos) {
+        const int who = (row0 + row) / G;
+        const int64_t* words = a.masks + (int64_t)(q.start + who) * W;
+        for (int pos = max(tile0 * kPagedTile, c); pos < min(tile1 * kPagedTile, keys); ++pos) {
           const bool sees = tree ? words[(pos - c) >> 6] >> ((pos - c) & 63) & 1 : pos - c <= who;
           const int page = table[pos >> lp];
           if (!sees || (unsigned)page >= (unsigned)p.num_pages) continue;
@@ -513,49 +555,45 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
           }
         }
       }
-      if (it.part >= 0) {
-        const int64_t to = ((int64_t)hk * f.max_parts + it.part) * ROWS + row;
+      if (parts > 1) {
+        const int64_t to = my_part * ROWS + row;
         put4(f.part + to * D + d, x);
         if (d == 0) put1(f.part_den + to, sum);
       } else {
         store4(out_row(row), d, x, sum);
       }
     }
-    if (it.part < 0) continue;
+    if (parts == 1) continue;
 
-    const int chunk = a.sched.header[PS_CHUNK], ch = it.tile0 / chunk;
-    const int parts = (paged_block_tiles(c, n, tree, it.row0 / ROWS, ROWS, G) + chunk - 1) / chunk;
-    const int size = group_size(parts), groups = (parts + size - 1) / size, group = ch / size;
-    const int64_t base = (int64_t)hk * f.max_parts + it.part - ch, from = base + group * size;
-    const int here = min(size, parts - group * size);
-    if (!arrived(f.count + base + group, here, &flag)) continue;
-    for (int e = tid; e < mine * quads; e += 256) {
+    const int size = group_size(parts), groups = (parts + size - 1) / size, g0 = (slot - from_slot) / size * size;
+    const int here = min(size, parts - g0);
+    int* count = a.sched.count + (int64_t)hk * 4 * f.slots;
+    if (!arrived(count + (part_of(g0) - head0), here, &flag)) continue;
+    for (int e = tid; e < mine * quads; e += THREADS) {
       const int row = e / quads, d = 4 * (e - row * quads);
-      const int64_t at = from * ROWS + row;
       float sum;
-      const f32x4_t x = sum_parts(f.part + at * D + d, f.part_den + at, here, ROWS, D, sum);
+      const f32x4_t x = sum_parts(f.part + d, f.part_den, here, D, sum, [&](int i) { return part_of(g0 + i) * ROWS + row; });
       if (groups == 1) {
         store4(out_row(row), d, x, sum);
       } else {
         // over the group's first part, of which this thread alone reads these features
-        put4(f.part + at * D + d, x);
-        if (d == 0) put1(f.part_sum + at, sum);
+        const int64_t to = part_of(g0) * ROWS + row;
+        put4(f.part + to * D + d, x);
+        if (d == 0) put1(f.part_sum + to, sum);
       }
     }
-    // 9 parts or more: fewer groups than parts - 1, so that this counter is none of theirs
-    if (groups == 1 || !arrived(f.count + base + parts - 1, groups, &flag)) continue;
-    for (int e = tid; e < mine * quads; e += 256) {
+    if (groups == 1 || !arrived(count + 2 * f.slots + (part_of(0) - head0), groups, &flag)) continue;
+    for (int e = tid; e < mine * quads; e += THREADS) {
       const int row = e / quads, d = 4 * (e - row * quads);
-      const int64_t at = base * ROWS + row;
       float sum;
-      const f32x4_t x = sum_parts(f.part + at * D + d, f.part_sum + at, groups, (int64_t)size * ROWS, D, sum);
+      const f32x4_t x = sum_parts(f.part + d, f.part_sum, groups, D, sum, [&](int i) { return part_of(i * size) * ROWS + row; });
       store4(out_row(row), d, x, sum);
     }
   }
 
-  // The rows that no item has: those of requests that were not served, and those behind the last
+  // The rows that no segment has: those of requests that were not served, and those behind the last
   // request's where they are asked for.  A lane looks at a token, its wave writes the row.
-  const int64_t waves = (int64_t)gridDim.x * 4, me = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t waves = (int64_t)gridDim.x * WAVES, me = (int64_t)blockIdx.x * WAVES + wave;
   for (int64_t t0 = me; t0 < p.max_tokens; t0 += 64 * waves) {
     const int64_t t = t0 + lane * waves;
     int r = -1;
@@ -575,30 +613,34 @@ __global__ __launch_bounds__(256, paged_waves(DT == AFA_F32, DP, QB)) void afa_p
   }
 }
 
-template <int DT, int DP, bool FULL>
-hipError_t tile_go(const PagedFast& f, int rows, unsigned grid, hipStream_t st) {
-  if (rows == 16) hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 1>), dim3(grid), dim3(256), 0, st, f);
-  else if (rows == 32) {
-    if constexpr (DT != AFA_F32 || DP < 256)
-      hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 2>), dim3(grid), dim3(256), 0, st, f);
-  } else {
-    if constexpr (DP <= (DT == AFA_F32 ? 64 : 128))
-      hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, 4>), dim3(grid), dim3(256), 0, st, f);
-  }
+template <int DT, int DP, bool FULL, int QB, int RW>
+hipError_t tile_launch(const PagedFast& f, hipStream_t st) {
+  hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, QB, RW>), dim3((unsigned)(f.slots * f.a.plan.kv_heads)),
+                     dim3(THREADS), 0, st, f);
   return hipGetLastError();
 }
 
-template <int DT>
-hipError_t fast_go(const PagedFast& f, int rows, unsigned grid, hipStream_t st) {
-  hipError_t e;
-  switch (f.dim) {
-    case 64: e = tile_go<DT, 64, true>(f, rows, grid, st); break;
-    case 128: e = tile_go<DT, 128, true>(f, rows, grid, st); break;
-    case 256: e = tile_go<DT, 256, true>(f, rows, grid, st); break;
-    case 96: e = tile_go<DT, 128, false>(f, rows, grid, st); break;
-    default: e = tile_go<DT, 64, false>(f, rows, grid, st); break;
+template <int DT, int DP, bool FULL>
+hipError_t tile_go(const PagedFast& f, int rows, hipStream_t st) {
+  if (rows == 16) return tile_launch<DT, DP, FULL, 1, 1>(f, st);
+  if constexpr (DP * (DT == AFA_F32 ? 2 : 1) > 128) {
+    return rows == 32 ? tile_launch<DT, DP, FULL, 1, 2>(f, st) : tile_launch<DT, DP, FULL, 1, 4>(f, st);
+  } else {
+    return rows == 32   ? tile_launch<DT, DP, FULL, 2, 1>(f, st)
+           : rows == 64 ? tile_launch<DT, DP, FULL, 2, 2>(f, st)
+                        : tile_launch<DT, DP, FULL, 2, 4>(f, st);
   }
-  return e;
+}
+
+template <int DT>
+hipError_t fast_go(const PagedFast& f, int rows, hipStream_t st) {
+  switch (f.dim) {
+    case 64: return tile_go<DT, 64, true>(f, rows, st);
+    case 128: return tile_go<DT, 128, true>(f, rows, st);
+    case 256: return tile_go<DT, 256, true>(f, rows, st);
+    case 96: return tile_go<DT, 128, false>(f, rows, st);
+    default: return tile_go<DT, 64, false>(f, rows, st);
+  }
 }
 
 }  // namespace
@@ -610,17 +652,16 @@ bool paged_fast_supported(const afa_paged_plan& p) {
 }
 
 size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c) {
-  return (size_t)(p.kv_heads * c.max_parts * c.rows) * (size_t)(p.head_dim + 2) * 4;
+  return (size_t)(p.kv_heads * 2 * c.slots * c.rows) * (size_t)(p.head_dim + 2) * 4;
 }
 
-hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int cus, void* ws, hipStream_t st) {
+hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, void* ws, hipStream_t st) {
   PagedFast f;
   f.a = a;
   f.part = (float*)ws;
-  f.part_den = f.part + a.plan.kv_heads * c.max_parts * c.rows * a.plan.head_dim;
-  f.part_sum = f.part_den + a.plan.kv_heads * c.max_parts * c.rows;
-  f.count = (int*)(a.sched.items + c.max_items);
-  f.max_parts = c.max_parts;
+  f.part_den = f.part + a.plan.kv_heads * 2 * c.slots * c.rows * a.plan.head_dim;
+  f.part_sum = f.part_den + a.plan.kv_heads * 2 * c.slots * c.rows;
+  f.slots = c.slots;
   f.dim = (int)a.plan.head_dim;
   const uint32_t esz = a.plan.dtype == AFA_F32 ? 4 : 2;
   f.k_page = (uint32_t)a.ps.k_page * esz;
@@ -628,12 +669,10 @@ hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, int c
   f.v_page = (uint32_t)a.ps.v_page * esz;
   f.v_slot = (uint32_t)a.ps.v_slot * esz;
   f.log_page = __builtin_ctzll((unsigned long long)a.plan.page_size);
-  const int64_t most = c.max_items * a.plan.kv_heads, fill = 4 * (int64_t)cus;
-  const unsigned grid = (unsigned)(most < fill ? most : fill);
   switch ((int)a.plan.dtype) {
-    case AFA_F32: return fast_go<AFA_F32>(f, c.rows, grid, st);
-    case AFA_BF16: return fast_go<AFA_BF16>(f, c.rows, grid, st);
-    default: return fast_go<AFA_F16>(f, c.rows, grid, st);
+    case AFA_F32: return fast_go<AFA_F32>(f, c.rows, st);
+    case AFA_BF16: return fast_go<AFA_BF16>(f, c.rows, st);
+    default: return fast_go<AFA_F16>(f, c.rows, st);
   }
 }
 

@@ -1,5 +1,5 @@
 // A serving step's plan from request lengths: pages taken and given back, block tables, the new tokens'
-// slots, positions and tree masks, and the items that the attention's workgroups take.
+// slots, positions and tree masks, and how the attention's workgroups share the work.
 //
 // With c cached and n new tokens of request r and pages of P tokens:
 //   need = ceil((c + n) / P);  pages popped from the ring: max(need - held, 0), at the sum of the same
@@ -19,34 +19,30 @@ namespace afa {
 PagedCut paged_cut(const afa_paged_plan& p, int cus) {
   PagedCut c;
   const int64_t group = p.heads / p.kv_heads, most = p.max_new * group;
-  // as many rows as a wave's registers hold beside a tile of K and V
-  const int64_t bytes = p.head_dim * (p.dtype == AFA_F32 ? 4 : 2), limit = bytes <= 256 ? 64 : bytes <= 512 ? 32 : 16;
-  c.rows = most <= 16 || limit == 16 ? 16 : most <= 32 || limit == 32 ? 32 : 64;
-  const int64_t want = 2 * (int64_t)cus;
-  c.target = (want + p.kv_heads - 1) / p.kv_heads;
-  // Keys are cut into chunks of at least total / target tiles, total the sum of tiles over the row blocks.
-  // A block cut in two or more has at most 2 tiles / chunk parts, all blocks together 2 target.
-  c.max_parts = 2 * c.target;
-  c.max_items = c.max_parts + (p.max_tokens * group + c.rows - 1) / c.rows + p.requests;
+  // rows of a segment: 16, or up to 128 (64 where a row takes 512 bytes and more) as its workgroup has waves
+  const int64_t bytes = p.head_dim * (p.dtype == AFA_F32 ? 4 : 2), limit = bytes <= 256 ? 128 : 64;
+  c.rows = 16;
+  while (c.rows < most && c.rows < limit) c.rows *= 2;
+  // workgroups that fit the device's registers at once
+  const int64_t want = (bytes >= 512 ? 1 : 2) * (int64_t)cus;
+  c.slots = want > p.kv_heads ? want / p.kv_heads : 1;
   return c;
 }
 
 size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c) {
-  const int64_t ints = (PS_INTS + 6 * p.requests + 3) & ~(int64_t)3;
-  return (size_t)ints * 4 + (size_t)c.max_items * sizeof(PagedItem) + (size_t)(p.kv_heads * c.max_parts) * 4;
+  return (size_t)(64 + p.requests * (int64_t)(sizeof(PagedLive) + 8 + 20) + c.slots * (int64_t)sizeof(PagedSlot) +
+                  p.kv_heads * c.slots * 16);
 }
 
 namespace {
 
-// Fewest tiles of a chunk: one for each wave of the attention's workgroups.
-constexpr int kMinChunk = 4;
 // Most requests whose sums every workgroup forms for itself, four a thread at most.
 constexpr int kOwnSums = 4 * kMaxTree;
 
-// The attention's cut as the kernels take it: rows of an item (a power of two), query heads a key head, and
-// items per head that fill the device.
+// The attention's cut as the kernels take it: rows of a segment (a power of two), query heads of a key head, and
+// slots.
 struct Cut {
-  int log_rows, group, target;
+  int log_rows, group, slots;
   __device__ int blocks(int n) const { return (n * group + (1 << log_rows) - 1) >> log_rows; }
 };
 
@@ -111,7 +107,8 @@ __device__ __forceinline__ int ring_place(int64_t i, int pages) {
 // What request r's workgroup has to know.
 struct Mine {
   Request q;
-  int start, pop, push, chunk, chunks, part, item;  // chunks 0: no attention
+  int start, pop, push, place;
+  int64_t flat, stretch;
 };
 
 // The sums over all requests, formed by a whole workgroup; thread i has requests [i k, i k + k).  `mine` is that
@@ -194,50 +191,41 @@ struct PlanSums {
     first.v[2] = pg.v[1];
   }
 
-  static __device__ int tiles(const Request& q) { return (q.c + q.n + kPagedTile - 1) / kPagedTile; }
+  static __device__ bool live(const Request& q) { return q.status == AFA_PAGED_OK && q.n > 0; }
+  static __device__ int cost(const Request& q) { return kPagedLead + (q.c + q.n + kPagedTile - 1) / kPagedTile; }
 
   __device__ Mine run(int which, bool store, Mine* shared) {
-    const PagedSchedule s = paged_schedule(p);
+    const PagedSchedule s = paged_schedule(p, cut.slots);
     prepare();
     Sums work = {{0, 0, 0}}, total;
     each(first, count, [&](int, const Request& q, const Sums&) {
-      if (q.status != AFA_PAGED_OK) return;
-      work.v[0] += (int64_t)cut.blocks(q.n) * tiles(q);
-      work.v[1] += max(q.need - q.held, 0);
+      if (live(q)) {
+        work.v[0] += (int64_t)cut.blocks(q.n) * cost(q);
+        work.v[1] += 1;
+      }
+      if (q.status == AFA_PAGED_OK) work.v[2] += max(q.need - q.held, 0);
     });
-    block_before<THREADS, 2>(work, lds, total);
-    taken = total.v[1];
-    // at least an equal share, and no longer than any request
-    const double share = (double)total.v[0] / (double)cut.target;
-    const int chunk = max((int)(share < 0x1p26 ? share : 0x1p26) + 1, kMinChunk);
-    auto chunks_of = [&](const Request& q) {
-      return q.status == AFA_PAGED_OK && q.n > 0 ? (int)((unsigned)(tiles(q) + chunk - 1) / (unsigned)chunk) : 0;
-    };
-    Sums cuts = {{0, 0, 0}};
-    each(first, count, [&](int, const Request& q, const Sums&) {
-      const int chunks = chunks_of(q), items = chunks > 0 ? cut.blocks(q.n) * chunks : 0;
-      cuts.v[0] += items;
-      if (chunks > 1) cuts.v[1] += items;
-    });
-    Sums at = block_before<THREADS, 2>(cuts, lds, total);
+    Sums at = block_before<THREADS, 3>(work, lds, total);
+    taken = total.v[2];
+    end = (int)min(all.v[0], p.max_tokens);
+    // an equal share, by a division that may be one too long; slots behind the line's end stay empty
+    const int64_t share = (int64_t)((double)total.v[0] / (double)cut.slots) + 1, stretch = max(share, (int64_t)kPagedMin);
     each(first, count, [&](int r, const Request& q, const Sums& b) {
-      const int chunks = chunks_of(q), items = chunks > 0 ? cut.blocks(q.n) * chunks : 0;
       Mine m;
       m.q = q;
       m.start = (int)min(b.v[0], p.max_tokens);
       m.pop = ring_place(head + b.v[1], pages);
       m.push = ring_place(head + count + b.v[2], pages);
-      m.chunk = chunk;
-      m.chunks = chunks;
-      m.item = (int)at.v[0];
-      m.part = (int)at.v[1];
-      at.v[0] += items;
-      if (chunks > 1) at.v[1] += items;
+      m.flat = at.v[0];
+      m.place = (int)at.v[1];
+      m.stretch = stretch;
+      if (live(q)) {
+        at.v[0] += (int64_t)cut.blocks(q.n) * cost(q);
+        at.v[1] += 1;
+      }
       if (r == which) *shared = m;
       if (store || r == which) {
-        s.item[r] = m.item;
-        s.part[r] = m.part;
-        s.chunks[r] = m.chunks;
+        s.cached[r] = q.c;
         p.status[r] = q.status;
         p.starts[r + 1] = (int)min(b.v[0] + max(q.n, 0), p.max_tokens);
       }
@@ -245,12 +233,14 @@ struct PlanSums {
         s.pop[r] = m.pop;
         s.push[r] = m.push;
         s.held[r] = q.held;
+        s.flat[r] = m.flat;
+        s.place[r] = m.place;
       }
     });
-    end = (int)min(all.v[0], p.max_tokens);
     if (threadIdx.x == 0 && (store || which == 0)) {
-      s.header[PS_ITEMS] = (int)total.v[0];
-      s.header[PS_CHUNK] = chunk;
+      s.header->slots = (int)((total.v[0] + stretch - 1) / stretch);
+      s.header->stretch = stretch;
+      s.header->end = total.v[0];
       p.starts[0] = 0;
     }
     __syncthreads();
@@ -267,11 +257,11 @@ struct PlanSums {
   }
 };
 
-// Request r's tokens, pages and items by one or more workgroups (gridDim.y); r = requests: the rows behind
+// Request r's tokens, pages and stretches by one or more workgroups (gridDim.y); r = requests: the rows behind
 // the last request's, from row `end` on.
 __device__ void fill(const afa_paged_plan& p, const Cut& cut, const int32_t* parents, const int r, const Mine& mine,
                      const int end) {
-  const PagedSchedule s = paged_schedule(p);
+  const PagedSchedule s = paged_schedule(p, cut.slots);
   const int P = (int)p.page_size, words = (int)(p.max_tree / 64), pages = (int)p.num_pages;
   const int tid = threadIdx.x, step = gridDim.y * kMaxTree, first = blockIdx.y * kMaxTree + tid;
   const int c = mine.q.c, n = mine.q.n, held = mine.q.held, need = mine.q.need, start = mine.start;
@@ -341,20 +331,13 @@ __device__ void fill(const afa_paged_plan& p, const Cut& cut, const int32_t* par
     }
   }
   if (n == 0) return;
-  const int chunk = mine.chunk, chunks = mine.chunks, blocks = cut.blocks(n), rows = 1 << cut.log_rows;
-  for (int j = first; j < blocks * chunks; j += step) {
-    // row blocks run fastest: those that read the same keys follow one another
-    const int ch = (int)((unsigned)j / (unsigned)blocks), block = j - ch * blocks;
-    PagedItem it;
-    it.request = r;
-    it.row0 = block * rows;
-    it.tile0 = ch * chunk;
-    it.tile1 = min(it.tile0 + chunk, paged_block_tiles(c, n, n <= p.max_tree, block, rows, cut.group));
-    it.part = chunks > 1 ? mine.part + block * chunks + ch : -1;
-    it.cached = c;
-    it.fresh = n;
-    it.start = start;
-    s.items[mine.item + j] = it;
+  const int blocks = cut.blocks(n), cost = kPagedLead + (c + n + kPagedTile - 1) / kPagedTile;
+  if (first == 0) s.live[mine.place] = PagedLive{r, c, n, start, mine.flat, blocks, cost};
+  const int64_t stop = mine.flat + (int64_t)blocks * cost;
+  for (int64_t i = (mine.flat + mine.stretch - 1) / mine.stretch + first; i * mine.stretch < stop; i += step) {
+    const int64_t at = i * mine.stretch - mine.flat;
+    const int block = (int)(at / cost);
+    s.slot[i] = PagedSlot{mine.place, block, (int)(at - (int64_t)block * cost), 0};
   }
 }
 
@@ -369,7 +352,7 @@ __global__ __launch_bounds__(kMaxTree) void afa_paged_plan_kernel(const afa_page
   PlanSums<kMaxTree, K> sums{p, cut, cached, fresh, lds};
   const Mine mine = sums.run(blockIdx.x, false, &shared);
   if (threadIdx.x == 0) {
-    int* ticket = paged_schedule(p).header + PS_TICKET;
+    int* ticket = &paged_schedule(p, cut.slots).header->ticket;
     last = atomicAdd(ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
     if (last) *ticket = 0;
   }
@@ -391,17 +374,16 @@ __global__ __launch_bounds__(SCAN) void afa_paged_scan_kernel(const afa_paged_pl
 
 __global__ __launch_bounds__(kMaxTree) void afa_paged_fill_kernel(const afa_paged_plan p, const Cut cut, const int32_t* cached,
                                                                   const int32_t* fresh, const int32_t* parents) {
-  const PagedSchedule s = paged_schedule(p);
+  const PagedSchedule s = paged_schedule(p, cut.slots);
   const int r = blockIdx.x, R = (int)p.requests;
   Mine m = {};
   if (r < R) {
     m.start = p.starts[r];
     m.pop = s.pop[r];
     m.push = s.push[r];
-    m.chunk = s.header[PS_CHUNK];
-    m.chunks = s.chunks[r];
-    m.part = s.part[r];
-    m.item = s.item[r];
+    m.flat = s.flat[r];
+    m.place = s.place[r];
+    m.stretch = s.header->stretch;
     m.q = Request{cached[r], fresh[r], s.held[r], p.held[r], p.status[r]};
   }
   fill(p, cut, parents, r, m, p.starts[R]);
@@ -414,7 +396,7 @@ hipError_t paged_build_launch(const afa_paged_plan& p, const PagedCut& c, const 
   // a workgroup of long prompts takes about 1024 of their tokens
   const int64_t y = (p.max_new + 1023) / 1024;
   const dim3 grid((unsigned)(p.requests + 1), (unsigned)(y < 64 ? y : 64));
-  const Cut cut{c.rows == 16 ? 4 : c.rows == 32 ? 5 : 6, (int)(p.heads / p.kv_heads), (int)c.target};
+  const Cut cut{__builtin_ctz((unsigned)c.rows), (int)(p.heads / p.kv_heads), (int)c.slots};
   if (p.requests <= kOwnSums) {
     if (p.requests <= kMaxTree)
       hipLaunchKernelGGL((afa_paged_plan_kernel<1>), grid, dim3(kMaxTree), 0, st, p, cut, cached, fresh, parents);
