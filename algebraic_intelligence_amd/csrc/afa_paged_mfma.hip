@@ -166,9 +166,17 @@ __device__ __forceinline__ int group_size(int parts) {
   return s * s < parts ? s + 1 : s;
 }
 
-// Four waves: QB row blocks of 16 each, RW of them side by side that meet the same keys (the later ones from
-// L1 or L2), KW along the keys.
+// Four waves of QB row blocks of 16 each: all along the keys, each with tiles of its own (RW = 1), two by two, or
+// side by side (RW = 4).  Waves side by side meet the same keys; four of them share a ring of tiles in LDS,
+// which direct loads fill ahead of them, two read the tile once each.
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
+
+// Tiles of the ring: as many as leave room for the workgroups that the registers hold.
+template <int DT, int DP>
+constexpr int ring_tiles() {
+  constexpr int bytes = 2 * kPagedTile * DP * (DT == AFA_F32 ? 4 : 2);
+  return bytes <= 16384 || (DP == 256 && bytes <= 32768) ? 4 : 2;
+}
 
 template <int DT, int DP, bool FULL, int QB, int RW>
 __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_kernel(const PagedFast f) {
@@ -181,7 +189,13 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
   constexpr int KB = F32 ? 16 : 32;       // features of a chunk over the four lane groups
   constexpr int GR = F32 ? 2 : 1;         // groups of 8 keys that a lane reads of K, and of V
   constexpr int ROWS = 16 * QB * RW, LD = DP + 4;
-  __shared__ float red[NBUF][ROWS][LD];
+  // the ring, in rows of PITCH bytes whose 16-byte chunks are swizzled by swizzle(row), and the joined rows after it
+  constexpr bool SHARED = RW == 4;
+  constexpr int NST = SHARED ? ring_tiles<DT, DP>() : 1, PITCH = DP * ESZ, HALF = kPagedTile * PITCH, TILE = 2 * HALF;
+  constexpr int NI = HALF / 1024 / WAVES;  // direct loads of a wave for K of a tile, and for V
+  constexpr int RED = NBUF * ROWS * LD * 4, RING = SHARED ? NST * TILE : 0;
+  __shared__ __attribute__((aligned(1024))) char smem[RED > RING ? RED : RING];
+  float (*red)[ROWS][LD] = (float (*)[ROWS][LD])smem;
   __shared__ float red_den[KW][ROWS];
   __shared__ int red_odd[WAVES], flag;
   const PagedFwdArgs& a = f.a;
@@ -238,7 +252,8 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     const char* v_base = (const char*)a.v_pages + hk * a.ps.v_head * ESZ;
     const int per = (tile1 - tile0 + KW - 1) / KW;
     // a wave without rows has no keys
-    const int t0 = tile0 + kw * per, t1 = row0 + mine0 < nrows ? min(t0 + per, tile1) : t0;
+    const bool rows_here = row0 + mine0 < nrows;
+    const int t0 = tile0 + kw * per, t1 = rows_here || SHARED ? min(t0 + per, tile1) : t0;
 
     // 64 entries of the table, one a lane, from the page of the wave's first tile on
     int entry0 = 0, entry = 0;
@@ -265,8 +280,66 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
                 ((uint32_t)(vpos & in_page) * f.v_slot + EPL * ESZ * m);
       }
     };
+    // eight rows that a ds_read_b128 touches at once take eight different chunks of a bank cycle
+    auto swizzle = [](int row) { return F32 ? row & 7 : (row & 3) | (row >> 1 & 4); };
+    unsigned lost_ring = 0;
+    // a wave's share of a tile into the ring: its rows' chunks, lane by lane
+    auto stage = [&](int t) {
+      const int kb = t * kPagedTile, st = t & (NST - 1);
+      if (((kb + kPagedTile - 1) >> lp) - entry0 > 63) load_entries(t);
+      char* to = smem + st * TILE;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int at = (wave * NI + i) * 1024, row = (at + 16 * lane) / PITCH;
+        const int chunk = ((at + 16 * lane) % PITCH / 16) ^ swizzle(row);
+        const int page = max(__shfl(entry, (min(kb + row, keys - 1) >> lp) - entry0), 0);
+        const uint32_t in = (uint32_t)((kb + row) & in_page);
+        if (FULL || chunk * 16 < D * ESZ) {
+          lds_dma16(k_base + (uint64_t)(uint32_t)page * f.k_page + (in * f.k_slot + 16 * chunk), to + at);
+          lds_dma16(v_base + (uint64_t)(uint32_t)page * f.v_page + (in * f.v_slot + 16 * chunk), to + HALF + at);
+        }
+      }
+      unsigned gone = 0;
+#pragma unroll
+      for (int u = 0; u < GR; ++u) {
+        const int vpos = kb + (F32 ? 16 * u + 4 * g : 8 * g);
+        gone |= (__shfl(entry, (min(vpos, keys - 1) >> lp) - entry0) < 0 ? 1u : 0u) << u;
+      }
+      lost_ring = (lost_ring & ~(3u << 2 * st)) | gone << 2 * st;
+    };
     u32x4_t kf[2][KS];
     unsigned vf[8][VW];
+    auto read_k = [&](int st) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3) + 4 * u;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int chunk = 4 * ks + g;
+          kf[u][ks] = *(const u32x4_t*)(smem + st * TILE + row * PITCH + (chunk ^ swizzle(row)) * 16);
+          if (!FULL && KB * ks + 16 / ESZ * g >= D) kf[u][ks] = u32x4_t{0, 0, 0, 0};
+        }
+      }
+    };
+    auto read_v = [&](int st) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i;
+        const char* r = smem + st * TILE + HALF + row * PITCH;
+        if constexpr (VW == 2) {
+          const u32x2_t x = *(const u32x2_t*)(r + ((m >> 1) ^ swizzle(row)) * 16 + 8 * (m & 1));
+          vf[i][0] = x[0];
+          vf[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int q4 = 0; q4 < VW / 4; ++q4) {
+            const u32x4_t x = *(const u32x4_t*)(r + ((VW / 4 * m + q4) ^ swizzle(row)) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = x[e];
+          }
+        }
+      }
+    };
     auto load_k = [&]() {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -296,7 +369,13 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
         }
       }
     };
-    if (t0 < t1) {
+    if constexpr (SHARED) {
+      __syncthreads();  // smem is free of the segment before
+      load_entries(t0);
+#pragma unroll
+      for (int i = 0; i < NST - 1; ++i)
+        if (t0 + i < t1) stage(t0 + i);
+    } else if (t0 < t1) {
       load_entries(t0);
       locate(t0);
       load_k();
@@ -331,8 +410,27 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
 
     for (int t = t0; t < t1; ++t) {
       const int kb = t * kPagedTile;
+      if constexpr (SHARED) {
+        // this wave's loads of tile t are done, those of up to NST - 2 later ones may go on; then every wave's,
+        // and every wave has read tile t - 1, whose place the next one takes
+        const int later = min(NST - 2, t1 - 1 - t);
+        if (later == 2) __builtin_amdgcn_s_waitcnt(vmcnt_only(4 * NI));
+        else if (later == 1) __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * NI));
+        else __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + NST - 1 < t1) stage(t + NST - 1);
+        if (!rows_here) continue;
+        const int st = t & (NST - 1);
 #pragma unroll
-      for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
+        for (int u = 0; u < GR; ++u) lost[u] = lost_ring >> (2 * st + u) & 1;
+        read_k(st);
+        read_v(st);
+      } else {
+#pragma unroll
+        for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
+      }
       // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
       f32x4_t s4[QB][2];
 #pragma unroll
@@ -356,12 +454,14 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
         }
       // K of the next tile comes while this one's weights are formed, V while the next one's scores are
       const bool more = t + 1 < t1;
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) {
-        locate(t + 1);
-        load_k();
+      if constexpr (!SHARED) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+          locate(t + 1);
+          load_k();
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
 
       // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
       // drafted values that are not finite are taken out of the product, in which a weight of 0 would
@@ -485,8 +585,10 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
           for (int b = 0; b < QB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) load_v();
+      if constexpr (!SHARED) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_v();
+      }
     }
 
     // join the waves along the keys: the first half stores, the second adds to theirs
@@ -627,7 +729,7 @@ hipError_t tile_go(const PagedFast& f, int rows, hipStream_t st) {
     return rows == 32 ? tile_launch<DT, DP, FULL, 1, 2>(f, st) : tile_launch<DT, DP, FULL, 1, 4>(f, st);
   } else {
     return rows == 32   ? tile_launch<DT, DP, FULL, 2, 1>(f, st)
-           : rows == 64 ? tile_launch<DT, DP, FULL, 2, 2>(f, st)
+           : rows == 64 ? tile_launch<DT, DP, FULL, 1, 4>(f, st)
                         : tile_launch<DT, DP, FULL, 2, 4>(f, st);
   }
 }
