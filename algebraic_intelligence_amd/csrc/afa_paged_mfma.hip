@@ -25,6 +25,8 @@
 // Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
 // the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
 // a row's weights are scaled by a power of two, lowered when a larger weight comes.
+#include <type_traits>
+
 #include "afa_common.h"
 #include "afa_paged.h"
 
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
   const afa_paged_plan& p = a.plan;
   const int D = FULL ? DP : f.dim;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, mine0 = 16 * QB * (wave % RW);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
   const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64), lp = f.log_page, in_page = (1 << lp) - 1;
   const float scale = (float)a.scale;
   // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     const char* v_base = (const char*)a.v_pages + hk * a.ps.v_head * ESZ;
     const int per = (tile1 - tile0 + KW - 1) / KW;
     // a wave without rows has no keys
-    const bool rows_here = row0 + mine0 < nrows;
+    const bool rows_here = row0 + 16 * rw < nrows, both = QB == 2 && row0 + 16 * (RW + rw) < nrows;
     const int t0 = tile0 + kw * per, t1 = rows_here || SHARED ? min(t0 + per, tile1) : t0;
 
     // 64 entries of the table, one a lane, from the page of the wave's first tile on
@@ -269,6 +271,18 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     auto locate = [&](int t) {
       const int kb = t * kPagedTile;
       if (((kb + kPagedTile - 1) >> lp) - entry0 > 63) load_entries(t);
+      if (lp >= 5) {  // the tile lies within one page
+        const int page = __builtin_amdgcn_readlane(entry, (kb >> lp) - entry0), at = max(page, 0);
+        const char* k = k_base + ((uint64_t)(uint32_t)at * f.k_page + (uint32_t)(kb & in_page) * f.k_slot);
+        const char* v = v_base + ((uint64_t)(uint32_t)at * f.v_page + (uint32_t)(kb & in_page) * f.v_slot);
+#pragma unroll
+        for (int u = 0; u < GR; ++u) {
+          lost_next[u] = page < 0;
+          kp[u] = k + ((F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3)) * f.k_slot + 16 * g);
+          vp[u] = v + ((F32 ? 16 * u + 4 * g : 8 * g) * f.v_slot + EPL * ESZ * m);
+        }
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < GR; ++u) {
         const int kpos = kb + (F32 ? 16 * u + m : 8 * (m >> 2) + (m & 3)), vpos = kb + (F32 ? 16 * u + 4 * g : 8 * g);
@@ -288,6 +302,22 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
       const int kb = t * kPagedTile, st = t & (NST - 1);
       if (((kb + kPagedTile - 1) >> lp) - entry0 > 63) load_entries(t);
       char* to = smem + st * TILE;
+      if (lp >= 5) {
+        const int page = __builtin_amdgcn_readlane(entry, (kb >> lp) - entry0), from = max(page, 0);
+        const char* k = k_base + ((uint64_t)(uint32_t)from * f.k_page + (uint32_t)(kb & in_page) * f.k_slot);
+        const char* v = v_base + ((uint64_t)(uint32_t)from * f.v_page + (uint32_t)(kb & in_page) * f.v_slot);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int at = (wave * NI + i) * 1024, row = (at + 16 * lane) / PITCH;
+          const int chunk = ((at + 16 * lane) % PITCH / 16) ^ swizzle(row);
+          if (FULL || chunk * 16 < D * ESZ) {
+            lds_dma16(k, row * f.k_slot + 16 * chunk, to + at);
+            lds_dma16(v, row * f.v_slot + 16 * chunk, to + HALF + at);
+          }
+        }
+        lost_ring = (lost_ring & ~(3u << 2 * st)) | (page < 0 ? 3u : 0u) << 2 * st;
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int at = (wave * NI + i) * 1024, row = (at + 16 * lane) / PITCH;
@@ -387,7 +417,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     int token[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-      const int row = min(row0 + mine0 + 16 * b + m, nrows - 1);
+      const int row = min(row0 + 16 * (b * RW + rw) + m, nrows - 1);
       token[b] = row / G;
       const char* x = (const char*)a.q + ((int64_t)(q.start + token[b]) * a.q_t + (hk * G + row - token[b] * G) * a.q_h) * ESZ;
 #pragma unroll
@@ -408,8 +438,10 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     }
     bool any_odd = false;
 
+    // the wave's tiles for its first NB row blocks
+    auto meet = [&](auto blocks) {
+      constexpr int NB = decltype(blocks)::value;
     for (int t = t0; t < t1; ++t) {
-      const int kb = t * kPagedTile;
       if constexpr (SHARED) {
         // this wave's loads of tile t are done, those of up to NST - 2 later ones may go on; then every wave's,
         // and every wave has read tile t - 1, whose place the next one takes
@@ -431,10 +463,11 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
 #pragma unroll
         for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
       }
+      const int kb = t * kPagedTile;
       // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
-      f32x4_t s4[QB][2];
+      f32x4_t s4[NB][2];
 #pragma unroll
-      for (int b = 0; b < QB; ++b)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           s4[b][u] = f32x4_t{0, 0, 0, 0};
@@ -494,9 +527,9 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
       }
 
       // Weights, in place of the scores in fp32, as planes otherwise.
-      u32x4_t hi[F32 ? 1 : QB], lo[F32 ? 1 : QB];
+      u32x4_t hi[F32 ? 1 : NB], lo[F32 ? 1 : NB];
 #pragma unroll
-      for (int b = 0; b < QB; ++b) {
+      for (int b = 0; b < NB; ++b) {
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = s4[b][e >> 2][e & 3] * scale;
@@ -571,7 +604,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int b = 0; b < QB; ++b)
+            for (int b = 0; b < NB; ++b)
               acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[e][j]), s4[b][e >> 2][e & 3],
                                                                acc[b][j], 0, 0, 0);
         } else {
@@ -580,16 +613,19 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
           for (int e = 0; e < 4; ++e)
             v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-          for (int b = 0; b < QB; ++b) acc[b][j] = mma16<DT>(v, hi[b], acc[b][j]);
+          for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, hi[b], acc[b][j]);
 #pragma unroll
-          for (int b = 0; b < QB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
+          for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
         }
       }
       if constexpr (!SHARED) {
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_v();
       }
-    }
+      }
+    };
+    if (both) meet(std::integral_constant<int, QB>());
+    else meet(std::integral_constant<int, 1>());
 
     // join the waves along the keys: the first half stores, the second adds to theirs
     __syncthreads();  // red is free of the item before
@@ -598,7 +634,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     for (int b = 0; b < QB; ++b) {
       den[b] += __shfl_xor(den[b], 16);
       den[b] += __shfl_xor(den[b], 32);
-      if (g == 0) red_den[kw][mine0 + 16 * b + m] = den[b];
+      if (g == 0) red_den[kw][16 * (b * RW + rw) + m] = den[b];
       if constexpr (DT == AFA_F16) {
         const float back = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc[b]));
 #pragma unroll
@@ -614,7 +650,7 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < EPL; j += 4) {
-              f32x4_t* to = (f32x4_t*)&red[kw % NBUF][mine0 + 16 * b + m][EPL * (4 * g + i) + j];
+              f32x4_t* to = (f32x4_t*)&red[kw % NBUF][16 * (b * RW + rw) + m][EPL * (4 * g + i) + j];
               f32x4_t x = {acc[b][j][i], acc[b][j + 1][i], acc[b][j + 2][i], acc[b][j + 3][i]};
               *to = half ? *to + x : x;
             }
