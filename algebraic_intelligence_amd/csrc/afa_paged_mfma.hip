@@ -34,8 +34,6 @@ namespace afa {
 
 namespace {
 
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-
 template <int DT>
 __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   if constexpr (DT == AFA_BF16)
@@ -110,16 +108,13 @@ __device__ __forceinline__ void put1(float* p, float x) {
 __device__ __forceinline__ float get1(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void put4(float* p, f32x4_t x) {
-  const f32x2_t a = {x[0], x[1]}, b = {x[2], x[3]};
-  __hip_atomic_store((u64*)p, __builtin_bit_cast(u64, a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __hip_atomic_store((u64*)p + 1, __builtin_bit_cast(u64, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// 16 bytes at byte `at` of a head's parts, of the same scope (sc1).
+constexpr int kDeviceScope = 16;
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t parts, uint32_t at, f32x4_t x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), parts, at, 0, kDeviceScope);
 }
-__device__ __forceinline__ f32x4_t get4(const float* p) {
-  const u64 x = __hip_atomic_load((const u64*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const u64 y = __hip_atomic_load((const u64*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const f32x2_t a = __builtin_bit_cast(f32x2_t, x), b = __builtin_bit_cast(f32x2_t, y);
-  return f32x4_t{a[0], a[1], b[0], b[1]};
+__device__ __forceinline__ f32x4_t get4(__amdgpu_buffer_rsrc_t parts, uint32_t at) {
+  return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(parts, at, 0, kDeviceScope));
 }
 
 // Whether this workgroup is the last of `n` to get here; its stores are complete before it counts.  The last
@@ -135,29 +130,51 @@ __device__ __forceinline__ bool arrived(int* count, int n, int* flag) {
   return *flag != 0;
 }
 
-// Sum of four features and of the row sums over `n` parts in their order, which lie at rows at(0), at(1), ...
-template <typename F>
-__device__ __forceinline__ f32x4_t sum_parts(const float* part, const float* den, int n, int D, float& sum, const F& at) {
-  f32x4_t x = {0, 0, 0, 0};
-  sum = 0.0f;
-  for (int i = 0; i < n; i += 8) {
-    // up to eight parts in flight
-    f32x4_t y[8];
-    float s[8];
+// Sums of `n` parts in their order, part i at row base(i): of every row into `sums` (LDS), and of four features at a
+// time, handed to put(row, feature, sums).  Up to 24 reads of a thread are in flight: they come from memory
+// that all XCDs see, and one workgroup has several hundred KB to read where rows are many.
+template <int THREADS, typename B, typename P>
+__device__ __forceinline__ void sum_parts(__amdgpu_buffer_rsrc_t parts, const float* den, int n, int rows, int D, float* sums,
+                                          const B& base, const P& put) {
+  for (int row = threadIdx.x; row < rows; row += THREADS) {
+    float x = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float y[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (i + u >= n) break;
-      y[u] = get4(part + at(i + u) * D);
-      s[u] = get1(den + at(i + u));
+      for (int i = 0; i < 8; ++i) y[i] = get1(den + base(min(i0 + i, n - 1)) + row);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x += i0 + i < n ? y[i] : 0.0f;
+    }
+    sums[row] = x;
+  }
+  __syncthreads();
+  const int quads = D / 4, all = rows * quads;
+  constexpr int U = 3, N = 8;
+  for (int e0 = threadIdx.x; e0 < all; e0 += U * THREADS) {
+    f32x4_t x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = f32x4_t{0, 0, 0, 0};
+    for (int i0 = 0; i0 < n; i0 += N) {
+      f32x4_t y[N][U];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          // past the last part or row: outside the resource, 0
+          y[i][u] = get4(parts, i0 + i < n && e0 + u * THREADS < all
+                                    ? (uint32_t)(base(i0 + i) * D * 4 + (int64_t)(e0 + u * THREADS) * 16)
+                                    : 0xfffffff0u);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] += y[i][u];
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (i + u >= n) break;
-      x += y[u];
-      sum += s[u];
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * THREADS, row = e / quads;
+      if (e < all) put(row, 4 * (e - row * quads), x[u]);
     }
   }
-  return x;
 }
 
 // Parts are summed in groups, these by the last of each, and the groups by the last of them: one
@@ -666,8 +683,11 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     for (int w = 0; w < WAVES; ++w) odd = odd || red_odd[w] != 0;
     const int mine = min(ROWS, nrows - row0), quads = D / 4;
     // part i of this segment: a slot's second where it begins there, else its first
-    const int64_t head0 = (int64_t)hk * 2 * f.slots;
-    auto part_of = [&](int i) { return head0 + 2 * (from_slot + i) + (i == 0); };
+    auto part_of = [&](int i) { return (int64_t)2 * (from_slot + i) + (i == 0); };
+    const int64_t head0 = (int64_t)hk * 2 * f.slots * ROWS;
+    float *part_den = f.part_den + head0, *part_sum = f.part_sum + head0;
+    const __amdgpu_buffer_rsrc_t buffer =
+        __builtin_amdgcn_make_buffer_rsrc(f.part + head0 * D, 0, (int)(2 * f.slots * ROWS * D * 4), 0x00020000);
     const int64_t my_part = part_of(slot - from_slot);
     for (int e = tid; e < mine * quads; e += THREADS) {
       const int row = e / quads, d = 4 * (e - row * quads);
@@ -694,9 +714,8 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
         }
       }
       if (parts > 1) {
-        const int64_t to = my_part * ROWS + row;
-        put4(f.part + to * D + d, x);
-        if (d == 0) put1(f.part_den + to, sum);
+        put4(buffer, (uint32_t)((my_part * ROWS + row) * D + d) * 4, x);
+        if (d == 0) put1(part_den + my_part * ROWS + row, sum);
       } else {
         store4(out_row(row), d, x, sum);
       }
@@ -706,27 +725,21 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
     const int size = group_size(parts), groups = (parts + size - 1) / size, g0 = (slot - from_slot) / size * size;
     const int here = min(size, parts - g0);
     int* count = a.sched.count + (int64_t)hk * 4 * f.slots;
-    if (!arrived(count + (part_of(g0) - head0), here, &flag)) continue;
-    for (int e = tid; e < mine * quads; e += THREADS) {
-      const int row = e / quads, d = 4 * (e - row * quads);
-      float sum;
-      const f32x4_t x = sum_parts(f.part + d, f.part_den, here, D, sum, [&](int i) { return part_of(g0 + i) * ROWS + row; });
-      if (groups == 1) {
-        store4(out_row(row), d, x, sum);
-      } else {
-        // over the group's first part, of which this thread alone reads these features
-        const int64_t to = part_of(g0) * ROWS + row;
-        put4(f.part + to * D + d, x);
-        if (d == 0) put1(f.part_sum + to, sum);
-      }
-    }
-    if (groups == 1 || !arrived(count + 2 * f.slots + (part_of(0) - head0), groups, &flag)) continue;
-    for (int e = tid; e < mine * quads; e += THREADS) {
-      const int row = e / quads, d = 4 * (e - row * quads);
-      float sum;
-      const f32x4_t x = sum_parts(f.part + d, f.part_sum, groups, D, sum, [&](int i) { return part_of(i * size) * ROWS + row; });
-      store4(out_row(row), d, x, sum);
-    }
+    if (!arrived(count + part_of(g0), here, &flag)) continue;
+    const int64_t to = part_of(g0) * ROWS;
+    sum_parts<THREADS>(buffer, part_den, here, mine, D, red_den[0], [&](int i) { return part_of(g0 + i) * ROWS; },
+                       [&](int row, int d, f32x4_t x) {
+                         if (groups == 1) {
+                           store4(out_row(row), d, x, red_den[0][row]);
+                         } else {
+                           // over the group's first part, of which this thread alone reads these features
+                           put4(buffer, (uint32_t)((to + row) * D + d) * 4, x);
+                           if (d == 0) put1(part_sum + to + row, red_den[0][row]);
+                         }
+                       });
+    if (groups == 1 || !arrived(count + 2 * f.slots + part_of(0), groups, &flag)) continue;
+    sum_parts<THREADS>(buffer, part_sum, groups, mine, D, red_den[0], [&](int i) { return part_of(i * size) * ROWS; },
+                       [&](int row, int d, f32x4_t x) { store4(out_row(row), d, x, red_den[0][row]); });
   }
 
   // The rows that no segment has: those of requests that were not served, and those behind the last
@@ -760,14 +773,13 @@ hipError_t tile_launch(const PagedFast& f, hipStream_t st) {
 
 template <int DT, int DP, bool FULL>
 hipError_t tile_go(const PagedFast& f, int rows, hipStream_t st) {
+  constexpr int ROW = DP * (DT == AFA_F32 ? 4 : 2);
   if (rows == 16) return tile_launch<DT, DP, FULL, 1, 1>(f, st);
-  if constexpr (DP * (DT == AFA_F32 ? 2 : 1) > 128) {
-    return rows == 32 ? tile_launch<DT, DP, FULL, 1, 2>(f, st) : tile_launch<DT, DP, FULL, 1, 4>(f, st);
-  } else {
-    return rows == 32   ? tile_launch<DT, DP, FULL, 2, 1>(f, st)
-           : rows == 64 ? tile_launch<DT, DP, FULL, 1, 4>(f, st)
-                        : tile_launch<DT, DP, FULL, 2, 4>(f, st);
-  }
+  // 32 rows: a wave's own where two row blocks fit its registers, else two waves that meet the same keys
+  if (rows == 32) return tile_launch<DT, DP, FULL, ROW <= 128 ? 2 : 1, ROW <= 128 ? 1 : 2>(f, st);
+  if (rows == 64) return tile_launch<DT, DP, FULL, 1, 4>(f, st);
+  if constexpr (ROW <= 256) return tile_launch<DT, DP, FULL, 2, 4>(f, st);
+  return hipErrorInvalidValue;  // no plan has more than 64 rows of these
 }
 
 template <int DT>
