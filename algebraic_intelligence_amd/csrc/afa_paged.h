@@ -37,10 +37,12 @@ struct PagedSlot {
   int live, block, at, unused;
 };
 
-// plan->schedule.  The ticket and the counters are 0 between calls.
+// plan->schedule.  The tickets and the counters are 0 between calls.
+constexpr int kTickets = 32;  // of groups of workgroups, each on a cache line of its own, then one of the groups
 struct PagedHeader {
-  int ticket, slots;
   int64_t stretch, end;  // of a slot, and of the line
+  int slots, unused[11];
+  int ticket[kTickets + 1][16];
 };
 struct PagedSchedule {
   PagedHeader* header;
@@ -60,7 +62,7 @@ __host__ __device__ inline PagedSchedule paged_schedule(const afa_paged_plan& p,
   char* at = (char*)p.schedule;
   const int64_t R = p.requests;
   s.header = (PagedHeader*)at;
-  at += 64;
+  at += sizeof(PagedHeader);
   s.live = (PagedLive*)at;
   at += R * sizeof(PagedLive);
   s.slot = (PagedSlot*)at;

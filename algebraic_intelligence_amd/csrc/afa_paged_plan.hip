@@ -30,7 +30,7 @@ PagedCut paged_cut(const afa_paged_plan& p, int cus) {
 }
 
 size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c) {
-  return (size_t)(64 + p.requests * (int64_t)(sizeof(PagedLive) + 8 + 20) + c.slots * (int64_t)sizeof(PagedSlot) +
+  return (size_t)((int64_t)sizeof(PagedHeader) + p.requests * (int64_t)(sizeof(PagedLive) + 8 + 20) + c.slots * (int64_t)sizeof(PagedSlot) +
                   p.kv_heads * c.slots * 16);
 }
 
@@ -352,9 +352,18 @@ __global__ __launch_bounds__(kMaxTree) void afa_paged_plan_kernel(const afa_page
   PlanSums<kMaxTree, K> sums{p, cut, cached, fresh, lds};
   const Mine mine = sums.run(blockIdx.x, false, &shared);
   if (threadIdx.x == 0) {
-    int* ticket = &paged_schedule(p, cut.slots).header->ticket;
-    last = atomicAdd(ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
-    if (last) *ticket = 0;
+    // the last of all by two steps: several hundred counts of one address would take longer than the rest
+    int (*ticket)[16] = paged_schedule(p, cut.slots).header->ticket;
+    const int all = (int)(gridDim.x * gridDim.y), id = (int)(blockIdx.y * gridDim.x + blockIdx.x), set = id % kTickets;
+    last = true;
+    if (all > kTickets) {
+      last = atomicAdd(ticket[set], 1) == (all - set + kTickets - 1) / kTickets - 1;
+      if (last) *ticket[set] = 0;
+    }
+    if (last) {
+      last = atomicAdd(ticket[kTickets], 1) == min(all, kTickets) - 1;
+      if (last) *ticket[kTickets] = 0;
+    }
   }
   fill(p, cut, parents, blockIdx.x, mine, sums.end);
   __syncthreads();
