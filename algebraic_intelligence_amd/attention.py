@@ -403,36 +403,52 @@ def _sections_array(sections, axes, pairs):
 _Strides12 = ctypes.c_int64 * 12
 
 
-def _axes_launch(q, k, c, s, positions, cuts, axes, transpose):
+class _AxesConfig(NamedTuple):
+    """What a rotation by several axes and its VJP share beside their tensors."""
+
+    dtype: int
+    pos_bytes: int
+    pos_b: int
+    axes: int
+    cuts: object
+
+
+def _axes_launch(q, k, c, s, positions, cfg, transpose):
     """q, and k unless None, (B, H, L, D) of one dtype, batch and length, rotated, or back; the results lie in
     memory in their inputs' axis order."""
-    if q.stride(3) != 1:
+    sq = q.stride()
+    if sq[3] != 1:
         q = q.contiguous()
+        sq = q.stride()
+    y = torch.empty_like(q)
+    sy = y.stride()
+    if sy[3] != 1:
+        y = torch.empty_like(q, memory_format=torch.contiguous_format)
+        sy = y.stride()
     B, H, L, D = q.shape
-    y = _dense_like(q)
-    sq, sy = q.stride(), y.stride()
-    K, kp, zp, z = 0, None, None, None
-    sk = sz = (0, 0, 0)
-    if k is not None:
-        if k.stride(3) != 1:
+    if k is None:
+        z = kp = zp = None
+        K, sk, sz = 0, sq, sy
+    else:
+        sk = k.stride()
+        if sk[3] != 1:
             k = k.contiguous()
-        z = _dense_like(k)
-        K, kp, zp, sk, sz = k.shape[1], k.data_ptr(), z.data_ptr(), k.stride(), z.stride()
+            sk = k.stride()
+        z = torch.empty_like(k)
+        sz = z.stride()
+        if sz[3] != 1:
+            z = torch.empty_like(k, memory_format=torch.contiguous_format)
+            sz = z.stride()
+        K, kp, zp = k.shape[1], k.data_ptr(), z.data_ptr()
     dev = q.device
     with _lib.on_device(dev):
         rc = _lib.lib().ago_rotate_axes(
-            _lib.dtype_code(q.dtype), B, H, K, L, D, q.data_ptr(), kp, y.data_ptr(), zp,
+            cfg.dtype, B, H, K, L, D, q.data_ptr(), kp, y.data_ptr(), zp,
             _Strides12(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sy[0], sy[1], sy[2], sz[0], sz[1], sz[2]), c.data_ptr(),
-            s.data_ptr(), c.shape[0], positions.data_ptr(), positions.element_size(),
-            0 if positions.ndim == 2 else positions.stride(0), axes, cuts, transpose, _lib.stream_ptr(dev))
+            s.data_ptr(), c.shape[0], positions.data_ptr(), cfg.pos_bytes, cfg.pos_b, cfg.axes, cfg.cuts, transpose,
+            _lib.stream_ptr(dev))
     _lib.check(rc, "ago_rotate_axes")
     return y, z
-
-
-def _dense_like(x):
-    """An empty tensor of x's shape whose axes lie in memory in x's order, without gaps."""
-    y = torch.empty_like(x)
-    return y if y.stride(3) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 class _RotateAxes(torch.autograd.Function):
@@ -440,11 +456,11 @@ class _RotateAxes(torch.autograd.Function):
     transposed rotation of the cotangents, in one launch where both are there."""
 
     @staticmethod
-    def forward(ctx, q, k, c, s, positions, cfg):
+    def forward(ctx, q, k, c, s, positions, cfg, transpose):
         ctx.save_for_backward(c, s, positions)
-        ctx.cfg = cfg
+        ctx.cfg = cfg, 1 - transpose
         ctx.set_materialize_grads(False)
-        y, z = _axes_launch(q, k, c, s, positions, *cfg)
+        y, z = _axes_launch(q, k, c, s, positions, cfg, transpose)
         if k is None:
             return y
         if not (ctx.needs_input_grad[0] and ctx.needs_input_grad[1]):
@@ -454,19 +470,18 @@ class _RotateAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk=None):
         c, s, positions = ctx.saved_tensors
-        cuts, axes, transpose = ctx.cfg
-        cfg = (cuts, axes, 1 - transpose)
+        cfg, back = ctx.cfg
         if gq is not None and gk is not None:
-            gq, gk = _rotate_axes(gq, gk, c, s, positions, cfg)
+            gq, gk = _rotate_axes(gq, gk, c, s, positions, cfg, back)
         else:
-            gq, gk = (None if g is None else _rotate_axes(g, None, c, s, positions, cfg) for g in (gq, gk))
-        return gq, gk, None, None, None, None
+            gq, gk = (None if g is None else _rotate_axes(g, None, c, s, positions, cfg, back) for g in (gq, gk))
+        return gq, gk, None, None, None, None, None
 
 
-def _rotate_axes(q, k, c, s, positions, cfg):
+def _rotate_axes(q, k, c, s, positions, cfg, transpose):
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotateAxes.apply(q, k, c, s, positions, cfg)
-    y, z = _axes_launch(q, k, c, s, positions, *cfg)
+        return _RotateAxes.apply(q, k, c, s, positions, cfg, transpose)
+    y, z = _axes_launch(q, k, c, s, positions, cfg, transpose)
     return y if k is None else (y, z)
 
 
@@ -500,15 +515,14 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
         raise ValueError(f"positions must have shape ({B}, {L}, axes) or ({L}, axes), got {tuple(at)}")
     axes = at[-1]
     cuts = _axis_sections(sections, axes, D // 2)
-    _lib.dtype_code(q.dtype)
+    dt = _lib.dtype_code(q.dtype)
     dev = _lib.require_device(q, k, positions)
     c, s = _axis_tables(rotary_params, D, q.dtype, dev)
-    if len(at) == 3 and at[0] == 1:
-        positions = positions[0]
     positions = positions.contiguous()
-    cfg = (cuts, axes, 0)
+    cfg = _AxesConfig(dt, positions.element_size(), L * axes if len(at) == 3 and at[0] > 1 else 0, axes, cuts)
     if q.numel() == 0:
-        return q.clone() if k is None else (q.clone(), k.clone() if k.numel() == 0 else _rotate_axes(k, None, c, s, positions, cfg))
+        return q.clone() if k is None else (
+            q.clone(), k.clone() if k.numel() == 0 else _rotate_axes(k, None, c, s, positions, cfg, 0))
     if k is not None and k.numel() == 0:
-        return _rotate_axes(q, None, c, s, positions, cfg), k.clone()
-    return _rotate_axes(q, k, c, s, positions, cfg)
+        return _rotate_axes(q, None, c, s, positions, cfg, 0), k.clone()
+    return _rotate_axes(q, k, c, s, positions, cfg, 0)
