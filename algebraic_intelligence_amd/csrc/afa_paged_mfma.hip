@@ -197,15 +197,20 @@ constexpr int ring_tiles() {
   return bytes <= 16384 || (DP == 256 && bytes <= 32768) ? 4 : 2;
 }
 
-template <int DT, int DP, bool FULL, int QB, int RW>
-__global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_kernel(const PagedFast f) {
+// D features in products of 16 of 64, 128 or 256.
+constexpr int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+template <int DT, int D, int QB, int RW>
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kernel(const PagedFast f) {
+  constexpr int DP = padded(D);
+  constexpr bool FULL = D == DP;
   constexpr int KW = WAVES / RW, NBUF = KW > 1 ? KW / 2 : 1;
   constexpr bool F32 = DT == AFA_F32;
   constexpr int ESZ = F32 ? 4 : 2;
   constexpr int EPL = DP / 16;            // features of V a lane, and products of O
   constexpr int VW = EPL * ESZ / 4;       // their 32-bit words
-  constexpr int KS = F32 ? DP / 16 : DP / 32;  // 16-byte chunks of a K row a lane
-  constexpr int KB = F32 ? 16 : 32;       // features of a chunk over the four lane groups
+  constexpr int KB = F32 ? 16 : 32;       // features of a 16-byte chunk over the four lane groups
+  constexpr int KS = (D + KB - 1) / KB;   // chunks of a K row a lane
   constexpr int GR = F32 ? 2 : 1;         // groups of 8 keys that a lane reads of K, and of V
   constexpr int ROWS = 16 * QB * RW, LD = DP + 4;
   // the ring, in rows of PITCH bytes whose 16-byte chunks are swizzled by swizzle(row), and the joined rows after it
@@ -219,7 +224,6 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
   __shared__ int red_odd[WAVES], flag;
   const PagedFwdArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
-  const int D = FULL ? DP : f.dim;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
   const int H = (int)p.heads, G = a.group, W = (int)(p.max_tree / 64), lp = f.log_page, in_page = (1 << lp) - 1;
@@ -764,32 +768,33 @@ __global__ __launch_bounds__(THREADS, DP == 256 ? 1 : 2) void afa_paged_tile_ker
   }
 }
 
-template <int DT, int DP, bool FULL, int QB, int RW>
+template <int DT, int D, int QB, int RW>
 hipError_t tile_launch(const PagedFast& f, hipStream_t st) {
-  hipLaunchKernelGGL((afa_paged_tile_kernel<DT, DP, FULL, QB, RW>), dim3((unsigned)(f.slots * f.a.plan.kv_heads)),
-                     dim3(THREADS), 0, st, f);
+  hipLaunchKernelGGL((afa_paged_tile_kernel<DT, D, QB, RW>), dim3((unsigned)(f.slots * f.a.plan.kv_heads)), dim3(THREADS), 0,
+                     st, f);
   return hipGetLastError();
 }
 
-template <int DT, int DP, bool FULL>
+template <int DT, int D>
 hipError_t tile_go(const PagedFast& f, int rows, hipStream_t st) {
-  constexpr int ROW = DP * (DT == AFA_F32 ? 4 : 2);
-  if (rows == 16) return tile_launch<DT, DP, FULL, 1, 1>(f, st);
+  constexpr int ROW = D * (DT == AFA_F32 ? 4 : 2);
+  if (rows == 16) return tile_launch<DT, D, 1, 1>(f, st);
   // 32 rows: a wave's own where two row blocks fit its registers, else two waves that meet the same keys
-  if (rows == 32) return tile_launch<DT, DP, FULL, ROW <= 128 ? 2 : 1, ROW <= 128 ? 1 : 2>(f, st);
-  if (rows == 64) return tile_launch<DT, DP, FULL, 1, 4>(f, st);
-  if constexpr (ROW <= 256) return tile_launch<DT, DP, FULL, 2, 4>(f, st);
+  if (rows == 32) return tile_launch<DT, D, ROW <= 128 ? 2 : 1, ROW <= 128 ? 1 : 2>(f, st);
+  if (rows == 64) return tile_launch<DT, D, 1, 4>(f, st);
+  if constexpr (ROW <= 256) return tile_launch<DT, D, 2, 4>(f, st);
   return hipErrorInvalidValue;  // no plan has more than 64 rows of these
 }
 
 template <int DT>
 hipError_t fast_go(const PagedFast& f, int rows, hipStream_t st) {
   switch (f.dim) {
-    case 64: return tile_go<DT, 64, true>(f, rows, st);
-    case 128: return tile_go<DT, 128, true>(f, rows, st);
-    case 256: return tile_go<DT, 256, true>(f, rows, st);
-    case 96: return tile_go<DT, 128, false>(f, rows, st);
-    default: return tile_go<DT, 64, false>(f, rows, st);
+    case 32: return tile_go<DT, 32>(f, rows, st);
+    case 48: return tile_go<DT, 48>(f, rows, st);
+    case 64: return tile_go<DT, 64>(f, rows, st);
+    case 96: return tile_go<DT, 96>(f, rows, st);
+    case 128: return tile_go<DT, 128>(f, rows, st);
+    default: return tile_go<DT, 256>(f, rows, st);
   }
 }
 

@@ -6,9 +6,10 @@ needs the lengths on the host, so a step of fixed sizes can be captured into a H
 with other lengths, parents and activations in the same tensors.  The reference trains only and has
 no counterpart; the attention is its AFA (src/kernels/pallas_afa.py:104-151) over other keys.
 
-``PagePool`` holds which pages belong to which request; ``DraftPlan`` the buffers of one step.  Steps
-that run at the same time on different streams need a plan each, and the pool is brought up to date by
-one step at a time.
+``PagePool`` holds which pages belong to which request; ``DraftPlan`` the buffers of one step, the
+attention's partial sums among them.  Calls that share a plan must be ordered on one stream (or by
+events); steps that run at the same time need a plan each, and the pool is brought up to date by one
+``build_block_tables`` at a time.
 """
 from __future__ import annotations
 
@@ -137,6 +138,8 @@ class DraftPlan:
         self.masks = torch.zeros((self.max_tokens, max_tree // 64), dtype=torch.int64, device=dev) if max_tree else None
         # zeros: a plan without a step has no items
         self._schedule = torch.zeros(schedule // 4, **ints)
+        # the attention's partial sums; calls that share a plan are ordered, so they share these too
+        self._ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev) if self._ws_bytes else None
         for name, t in (("block_tables", pool.block_tables), ("held", pool.held), ("ring", pool.ring),
                         ("ring_state", pool.ring_state), ("slots", self.slots), ("positions", self.positions),
                         ("token_request", self.requests), ("starts", self.starts), ("status", self.status),
@@ -291,11 +294,8 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         den = new((plan.max_tokens, plan.heads), dtype=_lib.accum_dtype(q.dtype), device=dev)
     strides = None if q.is_contiguous() else _Strides2(q.stride(0), q.stride(1))
     with _lib.on_device(dev):
-        # the workspace comes from torch's caching allocator, so the library allocates nothing
-        ws_bytes = plan._ws_bytes
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = _lib.lib().afa_paged_fwd(
             plan._ref, q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(masks),
-            out.data_ptr(), _lib.ptr(den), float(sink_omega), flags, _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+            out.data_ptr(), _lib.ptr(den), sink_omega, flags, _lib.ptr(plan._ws), plan._ws_bytes, _lib.stream_ptr(dev))
     _lib.check(rc, "afa_paged_fwd")
     return (out, den) if return_denominator else out
