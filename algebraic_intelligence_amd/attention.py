@@ -8,7 +8,6 @@ Every computation runs in the gfx950 kernels of libafa_hip.so (include/afa.h).
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import NamedTuple
 
@@ -390,14 +389,10 @@ def _axis_sections(sections, axes, pairs):
         if axes != 1:
             raise ValueError("positions of several axes need sections, the feature pairs of each axis")
         return None
-    return _sections_array(tuple(sections), axes, pairs)
-
-
-@functools.lru_cache(maxsize=64)
-def _sections_array(sections, axes, pairs):
-    if len(sections) != axes or any(int(n) != n or n < 0 for n in sections) or sum(sections) > pairs:
+    whole = tuple(int(n) for n in sections)
+    if len(whole) != axes or min(whole) < 0 or sum(whole) > pairs or any(a != b for a, b in zip(whole, sections)):
         raise ValueError(f"sections must be {axes} nonnegative integers with a sum of at most {pairs}, got {sections}")
-    return (ctypes.c_int32 * axes)(*(int(n) for n in sections))
+    return (ctypes.c_int32 * axes)(*whole)
 
 
 _Strides12 = ctypes.c_int64 * 12

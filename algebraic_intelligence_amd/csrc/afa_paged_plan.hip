@@ -36,8 +36,10 @@ size_t paged_schedule_bytes(const afa_paged_plan& p, const PagedCut& c) {
 
 namespace {
 
-// Most requests whose sums every workgroup forms for itself, four a thread at most.
-constexpr int kOwnSums = 4 * kMaxTree;
+// Most requests whose sums every workgroup forms for itself, four a thread at most, and most workgroups that
+// do: as many as the device holds at once.  512 requests with trees take 8.8 us this way, and two launches,
+// of which the first has one workgroup, about 11.
+constexpr int kOwnSums = 4 * kMaxTree, kOwnGroups = 2048;
 
 // The attention's cut as the kernels take it: rows of a segment (a power of two), query heads of a key head, and
 // slots.
@@ -406,7 +408,7 @@ hipError_t paged_build_launch(const afa_paged_plan& p, const PagedCut& c, const 
   const int64_t y = (p.max_new + 1023) / 1024;
   const dim3 grid((unsigned)(p.requests + 1), (unsigned)(y < 64 ? y : 64));
   const Cut cut{__builtin_ctz((unsigned)c.rows), (int)(p.heads / p.kv_heads), (int)c.slots};
-  if (p.requests <= kOwnSums) {
+  if (p.requests <= kOwnSums && (int64_t)grid.x * grid.y <= kOwnGroups) {
     if (p.requests <= kMaxTree)
       hipLaunchKernelGGL((afa_paged_plan_kernel<1>), grid, dim3(kMaxTree), 0, st, p, cut, cached, fresh, parents);
     else

@@ -274,7 +274,8 @@ int oace_softmax_loss_bwd(int dtype, int64_t rows, int64_t vocab, const void* lo
  *
  * afa_paged_plan describes the pool and one step's plan: sizes and device pointers, all owned by the
  * caller.  afa_paged_build fills the plan's arrays for a step; afa_paged_append and afa_paged_fwd
- * read them, for any number of layers.  Calls that share a plan must be ordered on one stream.
+ * read them, and the pool's block tables, for any number of layers, until another plan is built on the
+ * pool.  Calls that share a plan must be ordered on one stream.
  */
 typedef struct afa_paged_plan {
   int64_t num_pages, page_size;      /* num_pages * page_size < 2^31; page_size any positive size */

@@ -87,7 +87,7 @@ def _same_pool(pool, oracle):
 @pytest.mark.parametrize("pages,page,R,max_len,T,max_new,max_tree,tree", [
     (64, 16, 5, 300, 90, 40, 64, True), (30, 1, 3, 40, 30, 20, 64, True), (200, 3, 40, 50, 300, 12, 0, False),
     (4000, 8, 1500, 60, 5000, 9, 128, True), (2500, 4, 1024, 30, 2000, 4, 64, False),
-    (300, 64, 2, 12000, 9000, 5000, 256, True), (1, 7, 1, 7, 7, 7, 64, True), (60, 32, 33, 100, 64, 64, 192, True),
+    (300, 64, 2, 12000, 9000, 5000, 256, True), (400, 512, 40, 100000, 150000, 100000, 64, True), (1, 7, 1, 7, 7, 7, 64, True), (60, 32, 33, 100, 64, 64, 192, True),
 ])
 def test_plans_over_a_pools_life(pages, page, R, max_len, T, max_new, max_tree, tree):
     """Random steps, among them ones that no request, some or all can be served in: lengths and
@@ -96,7 +96,7 @@ def test_plans_over_a_pools_life(pages, page, R, max_len, T, max_new, max_tree, 
     pool, oracle = A.PagePool(pages, page, R, max_len), P.Pool(pages, page, R, max_len)
     plan = _plan(pool, T, max_new, max_tree)
     for step in range(8):
-        most = max(1, min(max_new, 2 * T // R))
+        most = max(1, min(max_new, 2 * T // R, 5000))
         cached, new = rng.integers(0, max_len, R), rng.integers(0, most + 1, R)
         if step % 2:
             cached = np.minimum(cached, 2 * pages * page // R // (step + 1))
