@@ -379,14 +379,16 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
         const char* r = smem + st * TILE + HALF + row * PITCH;
         if constexpr (VW == 2) {
           const u32x2_t x = *(const u32x2_t*)(r + ((m >> 1) ^ swizzle(row)) * 16 + 8 * (m & 1));
-          vf[i][0] = x[0];
-          vf[i][1] = x[1];
+          const bool in = FULL || EPL * m < D;  // nothing is staged behind the row
+          vf[i][0] = in ? x[0] : 0;
+          vf[i][1] = in ? x[1] : 0;
         } else {
 #pragma unroll
           for (int q4 = 0; q4 < VW / 4; ++q4) {
             const u32x4_t x = *(const u32x4_t*)(r + ((VW / 4 * m + q4) ^ swizzle(row)) * 16);
+            const bool in = FULL || EPL * m + 16 / ESZ * q4 < D;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = x[e];
+            for (int e = 0; e < 4; ++e) vf[i][4 * q4 + e] = in ? x[e] : 0;
           }
         }
       }
