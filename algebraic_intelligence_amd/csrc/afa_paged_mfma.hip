@@ -16,7 +16,10 @@
 // of a lane belong to the 8 consecutive keys that it holds of V (16-bit types: keys 8g..8g+7 for lane
 // group g = lane / 16).  Likewise feature d = EPL * row + j is row `row` of product j: a lane reads EPL
 // consecutive features of 8 V rows, 16 lanes a whole row, and forms the columns by 4 byte permutes each.
-// No LDS, no barrier and no cross-lane step in the loop.
+// No cross-lane step is in the loop, and with up to 32 rows no LDS and no barrier: K of the next tile comes
+// while a tile's weights are formed, V while the next scores are.  With 64 and 128 rows the four waves have 16
+// or 32 rows each and share a ring of tiles in LDS, which direct loads fill up to three tiles ahead: a tile is
+// loaded once for all, and the loads in flight cost no registers.
 //
 // The sums are additive: rows split over waves, and over workgroups where the plan cut the keys, are
 // joined by adding numerators and denominators in a fixed order (LDS; fp32 parts that the last workgroup of a
@@ -25,6 +28,13 @@
 // Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
 // the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
 // a row's weights are scaled by a power of two, lowered when a larger weight comes.
+//
+// HBM bound where requests are many or long.  96 requests of one token over up to 4096 cached, 16 heads of 64,
+// bf16: 160 us, 5.7 TB/s.  4 requests of 6 tokens over up to 131072, 16 query on 4 key heads of 128, fp16: 119 us,
+// 4.7 TB/s, of which the parts take 5.  32 requests of up to 32 drafted tokens over up to 8192, 16 on 4 heads of
+// 128, bf16 (128 rows): 105 us, 3.0 TB/s; its loads alone take 76, the parts 12, the rest is arithmetic that
+// they do not hide.  40 requests of up to 13 over 3001, 6 heads of 48, fp32: 38 us, 3.8 TB/s, the parts 7.  One token
+// over 700, 12 heads of 64: 8 us, a chain of dependent reads (plan, table, keys, parts).
 #include <type_traits>
 
 #include "afa_common.h"
@@ -625,11 +635,13 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
       for (int j = 0; j < EPL; ++j) {
         if constexpr (F32) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
+          for (int e = 0; e < 8; ++e) {
+            const unsigned x = vf[e][j];
+            const float v = __builtin_bit_cast(float, x);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vf[e][j]), s4[b][e >> 2][e & 3],
-                                                               acc[b][j], 0, 0, 0);
+              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s4[b][e >> 2][e & 3], acc[b][j], 0, 0, 0);
+          }
         } else {
           u32x4_t v;
 #pragma unroll
