@@ -671,7 +671,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
       den[b] += __shfl_xor(den[b], 32);
       if (g == 0) red_den[kw][16 * (b * RW + rw) + m] = den[b];
       if constexpr (DT == AFA_F16) {
-        const float back = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc[b]));
+        const float by = sc[b];  // a power of two
+        const float back = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, by));
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[b][j] *= back;
       }
