@@ -474,189 +474,189 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
     // the wave's tiles for its first NB row blocks
     auto meet = [&](auto blocks) {
       constexpr int NB = decltype(blocks)::value;
-    for (int t = t0; t < t1; ++t) {
-      if constexpr (SHARED) {
-        // this wave's loads of tile t are done, those of up to NST - 2 later ones may go on; then every wave's,
-        // and every wave has read tile t - 1, whose place the next one takes
-        const int later = min(NST - 2, t1 - 1 - t);
-        if (later == 2) __builtin_amdgcn_s_waitcnt(vmcnt_only(4 * NI));
-        else if (later == 1) __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * NI));
-        else __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + NST - 1 < t1) stage(t + NST - 1);
-        if (!rows_here) continue;
-        const int st = t & (NST - 1);
+      for (int t = t0; t < t1; ++t) {
+        if constexpr (SHARED) {
+          // this wave's loads of tile t are done, those of up to NST - 2 later ones may go on; then every wave's,
+          // and every wave has read tile t - 1, whose place the next one takes
+          const int later = min(NST - 2, t1 - 1 - t);
+          if (later == 2) __builtin_amdgcn_s_waitcnt(vmcnt_only(4 * NI));
+          else if (later == 1) __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * NI));
+          else __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (t + NST - 1 < t1) stage(t + NST - 1);
+          if (!rows_here) continue;
+          const int st = t & (NST - 1);
 #pragma unroll
-        for (int u = 0; u < GR; ++u) lost[u] = lost_ring >> (2 * st + u) & 1;
-        read_k(st);
-        read_v(st);
-      } else {
+          for (int u = 0; u < GR; ++u) lost[u] = lost_ring >> (2 * st + u) & 1;
+          read_k(st);
+          read_v(st);
+        } else {
 #pragma unroll
-        for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
-      }
-      const int kb = t * kPagedTile;
-      // scores of row 16 b + m: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
-      f32x4_t s4[NB][2];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          s4[b][u] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (F32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const unsigned x = kf[u][ks][e], y = qf[b][ks][e];
-                s4[b][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y),
-                                                                s4[b][u], 0, 0, 0);
-              }
-            } else {
-              s4[b][u] = mma16<DT>(kf[u][ks], qf[b][ks], s4[b][u]);
-            }
-          }
+          for (int u = 0; u < GR; ++u) lost[u] = lost_next[u];
         }
-      // K of the next tile comes while this one's weights are formed, V while the next one's scores are
-      const bool more = t + 1 < t1;
-      if constexpr (!SHARED) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) {
-          locate(t + 1);
-          load_k();
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-
-      // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
-      // drafted values that are not finite are taken out of the product, in which a weight of 0 would
-      // not hide them; the rows that see them get them at the end.
-      bool any_lost = lost[0];
-      if constexpr (F32) any_lost = any_lost || lost[GR - 1];
-      const bool masked = kb + kPagedTile > c || __ballot(any_lost) != 0;
-      if (masked) {
-        bool odd = false;
+        const int kb = t * kPagedTile;
+        // scores of row m of row block b: element e is key 8 g + e (fp32: 16 (e / 4) + 4 g + e % 4)
+        f32x4_t s4[NB][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int pos = kb + (F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i);
-          const bool gone = pos >= keys || lost[F32 ? i >> 2 : 0];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            unsigned x = gone ? 0u : vf[i][e];
-            if (pos >= c && nonfinite<DT>(x)) {
-              odd = true;
+          for (int u = 0; u < 2; ++u) {
+            s4[b][u] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
               if constexpr (F32) {
-                x = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const unsigned x = kf[u][ks][e], y = qf[b][ks][e];
+                  s4[b][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y),
+                                                                  s4[b][u], 0, 0, 0);
+                }
               } else {
-                constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
-                x &= ((x & E) == E ? 0xffff0000u : ~0u) & ((x >> 16 & E) == E ? 0xffffu : ~0u);
+                s4[b][u] = mma16<DT>(kf[u][ks], qf[b][ks], s4[b][u]);
               }
             }
-            vf[i][e] = x;
           }
+        // K of the next tile comes while this one's weights are formed, V while the next one's scores are
+        const bool more = t + 1 < t1;
+        if constexpr (!SHARED) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (more) {
+            locate(t + 1);
+            load_k();
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        any_odd = any_odd || __ballot(odd) != 0;
-      }
 
-      // Weights, in place of the scores in fp32, as planes otherwise.
-      u32x4_t hi[F32 ? 1 : NB], lo[F32 ? 1 : NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = s4[b][e >> 2][e & 3] * scale;
-        if constexpr (F32) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = rho8_refined(w[e]);
-        } else {
-          // the branch-free form costs half of the other and loses nothing above 0, and below it
-          // 16 s^2 times the error of the hardware's rsqrt, 2.2e-4 at -8
-          float low = w[0];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) low = __builtin_fminf(low, w[e]);
-          if (__ballot(!(low > -8.0f)) == 0) {  // a NaN stays one in either form
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = rho8_fast(w[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = rho8_exact(w[e]);
-          }
-        }
+        // Tiles with drafted keys, keys behind the last or lost pages: rows past the end are cleared, and
+        // drafted values that are not finite are taken out of the product, in which a weight of 0 would
+        // not hide them; the rows that see them get them at the end.
+        bool any_lost = lost[0];
+        if constexpr (F32) any_lost = any_lost || lost[GR - 1];
+        const bool masked = kb + kPagedTile > c || __ballot(any_lost) != 0;
         if (masked) {
-          const int64_t* words = tree ? a.masks + (int64_t)(q.start + token[b]) * W : nullptr;
-          unsigned sees;
-          if constexpr (F32) {
-            sees = sees_bits(kb - c + 4 * g, 4, n, token[b], words, W) |
-                   sees_bits(kb - c + 16 + 4 * g, 4, n, token[b], words, W) << 4;
-            if (lost[0]) sees &= 0xf0;
-            if (lost[GR - 1]) sees &= 0x0f;
-          } else {
-            sees = lost[0] ? 0 : sees_bits(kb - c + 8 * g, 8, n, token[b], words, W);
-          }
+          bool odd = false;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = sees >> e & 1 ? w[e] : 0.0f;
-        }
-        den[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-        if constexpr (F32) {
+          for (int i = 0; i < 8; ++i) {
+            const int pos = kb + (F32 ? 16 * (i >> 2) + 4 * g + (i & 3) : 8 * g + i);
+            const bool gone = pos >= keys || lost[F32 ? i >> 2 : 0];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s4[b][e >> 2][e & 3] = w[e];
-        } else {
-          if constexpr (DT == AFA_F16) {
-            float top = w[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, w[e]);
-            if (__ballot(!(top * sc[b] <= 32768.0f)) != 0) {
-              // a row's largest weight so far now lies in [16, 32)
-              top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-              top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-              if (top * sc[b] > 32768.0f && top < __builtin_inff()) {
-                const int e = (__builtin_bit_cast(int, top) >> 23) - 127;
-                const float to = __builtin_bit_cast(float, (127 + 4 - e) << 23);
-                const float ratio = to / sc[b];
-                sc[b] = to;
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) acc[b][j] *= ratio;
+            for (int e = 0; e < VW; ++e) {
+              unsigned x = gone ? 0u : vf[i][e];
+              if (pos >= c && nonfinite<DT>(x)) {
+                odd = true;
+                if constexpr (F32) {
+                  x = 0;
+                } else {
+                  constexpr unsigned E = DT == AFA_BF16 ? 0x7f80u : 0x7c00u;
+                  x &= ((x & E) == E ? 0xffff0000u : ~0u) & ((x >> 16 & E) == E ? 0xffffu : ~0u);
+                }
               }
+              vf[i][e] = x;
+            }
+          }
+          any_odd = any_odd || __ballot(odd) != 0;
+        }
+
+        // Weights, in place of the scores in fp32, as planes otherwise.
+        u32x4_t hi[F32 ? 1 : NB], lo[F32 ? 1 : NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = s4[b][e >> 2][e & 3] * scale;
+          if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = rho8_refined(w[e]);
+          } else {
+            // the branch-free form costs half of the other and loses nothing above 0, and below it
+            // 16 s^2 times the error of the hardware's rsqrt, 2.2e-4 at -8
+            float low = w[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) low = __builtin_fminf(low, w[e]);
+            if (__ballot(!(low > -8.0f)) == 0) {  // a NaN stays one in either form
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = rho8_fast(w[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = rho8_exact(w[e]);
+            }
+          }
+          if (masked) {
+            const int64_t* words = tree ? a.masks + (int64_t)(q.start + token[b]) * W : nullptr;
+            unsigned sees;
+            if constexpr (F32) {
+              sees = sees_bits(kb - c + 4 * g, 4, n, token[b], words, W) |
+                     sees_bits(kb - c + 16 + 4 * g, 4, n, token[b], words, W) << 4;
+              if (lost[0]) sees &= 0xf0;
+              if (lost[GR - 1]) sees &= 0x0f;
+            } else {
+              sees = lost[0] ? 0 : sees_bits(kb - c + 8 * g, 8, n, token[b], words, W);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] *= sc[b];
+            for (int e = 0; e < 8; ++e) w[e] = sees >> e & 1 ? w[e] : 0.0f;
           }
+          den[b] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+          if constexpr (F32) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned x = Elem<DT>::pack(w[2 * e], w[2 * e + 1]);
-            hi[b][e] = x;
-            lo[b][e] = Elem<DT>::pack(w[2 * e] - Elem<DT>::lo(x), w[2 * e + 1] - Elem<DT>::hi(x));
+            for (int e = 0; e < 8; ++e) s4[b][e >> 2][e & 3] = w[e];
+          } else {
+            if constexpr (DT == AFA_F16) {
+              float top = w[0];
+#pragma unroll
+              for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, w[e]);
+              if (__ballot(!(top * sc[b] <= 32768.0f)) != 0) {
+                // a row's largest weight so far now lies in [16, 32)
+                top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+                top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                if (top * sc[b] > 32768.0f && top < __builtin_inff()) {
+                  const int e = (__builtin_bit_cast(int, top) >> 23) - 127;
+                  const float to = __builtin_bit_cast(float, (127 + 4 - e) << 23);
+                  const float ratio = to / sc[b];
+                  sc[b] = to;
+#pragma unroll
+                  for (int j = 0; j < EPL; ++j) acc[b][j] *= ratio;
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] *= sc[b];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned x = Elem<DT>::pack(w[2 * e], w[2 * e + 1]);
+              hi[b][e] = x;
+              lo[b][e] = Elem<DT>::pack(w[2 * e] - Elem<DT>::lo(x), w[2 * e + 1] - Elem<DT>::hi(x));
+            }
           }
         }
-      }
 
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        if constexpr (F32) {
+        for (int j = 0; j < EPL; ++j) {
+          if constexpr (F32) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const unsigned x = vf[e][j];
-            const float v = __builtin_bit_cast(float, x);
+            for (int e = 0; e < 8; ++e) {
+              const unsigned x = vf[e][j];
+              const float v = __builtin_bit_cast(float, x);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-              acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s4[b][e >> 2][e & 3], acc[b][j], 0, 0, 0);
+              for (int b = 0; b < NB; ++b)
+                acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s4[b][e >> 2][e & 3], acc[b][j], 0, 0, 0);
+            }
+          } else {
+            u32x4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, hi[b], acc[b][j]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
           }
-        } else {
-          u32x4_t v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = __builtin_amdgcn_perm(vf[2 * e + 1][j >> 1], vf[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, hi[b], acc[b][j]);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
         }
-      }
-      if constexpr (!SHARED) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) load_v();
-      }
+        if constexpr (!SHARED) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (more) load_v();
+        }
       }
     };
     if (both) meet(std::integral_constant<int, QB>());

@@ -228,9 +228,10 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     at the tokens' slots of ``k_pages`` and ``v_pages``, and return the rotated q.
 
     ``rotary_params``: Cayley tables (positions, head_dim / 2), in fp32 (fp64 for fp64 inputs; others are
-    cast); a position outside them gives NaN.  None: k is stored and q returned as they are.  ``positions`` (max_tokens, A) int32 with
-    ``sections`` gives positions of A axes as in ``apply_ago_axis_rotations``; (max_tokens,) or None, the
-    plan's positions, is one axis.  Tokens without a slot are not stored."""
+    cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
+    ``positions`` (max_tokens, A) int32 with ``sections`` gives positions of A axes as in
+    ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
+    without a slot are not stored."""
     q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
     page_strides = _pages(plan, k_pages, v_pages)
     dev = plan.device
@@ -267,10 +268,10 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     Returns out (max_tokens, heads, head_dim), or (out, d) with d = sum_j rho(s_ij)^8 + sink_omega of shape
     (max_tokens, heads) in fp32 (fp64 for fp64 inputs).  heads / kv_heads query heads share a key/value
-    head.  ``masks`` replaces the plan's (max_tokens, max_tree / 64) int64 masks: they hide drafted tokens only, and
-    none in requests of more than max_tree new tokens.  A row that sees no key is 0, and a key that a row does
-    not see, whatever its page holds, does not touch it.  Rows behind the last request's are 0, or left as they were where ``out`` is given.  For
-    inference: not differentiable."""
+    head.  ``masks`` replaces the plan's (max_tokens, max_tree / 64) int64 masks: they hide drafted tokens
+    only, and none in requests of more than max_tree new tokens.  A row that sees no key is 0, and a key
+    that a row does not see, whatever its page holds, does not touch it.  Rows behind the last request's
+    are 0, or left as they were where ``out`` is given.  For inference: not differentiable."""
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
     q = _rows(plan, "q", q, plan._q_shape)
