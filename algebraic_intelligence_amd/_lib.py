@@ -9,6 +9,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import struct
 import threading
 
 import torch
@@ -133,12 +134,14 @@ def stream_ptr(device: torch.device) -> int:
 
 
 _HERE = contextlib.nullcontext()
+# the C call behind torch.cuda.current_device(), whose tensors exist once a device is asked for here
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(device: torch.device):
     """A context in which `device` is the current one: torch.cuda.device(device), or nothing to do
     where it already is."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -150,6 +153,10 @@ def workspace_size(name: str, device: torch.device, *sizes) -> int:
     """A workspace query, a function of the sizes and the device it runs on; called with that device
     current.  Kept for the sizes a program repeats."""
     return _workspace(name, device.index, *sizes)
+
+
+# int64 values, such as strides, as the bytes a C array of them has
+pack2, pack6, pack12 = (struct.Struct(f"{n}q").pack for n in (2, 6, 12))
 
 
 def ptr(t):

@@ -8,6 +8,7 @@ Every computation runs in the gfx950 kernels of libafa_hip.so (include/afa.h).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -369,12 +370,13 @@ def apply_ago_rotations(q, k, rotary_params=None, seq_axis=None):
 # ------------------------------------------------------------------- AGO by positions of several axes
 def _axis_tables(rotary_params, head_dim, dtype, dev):
     """(c, s) device tables in fp32 (fp64 for fp64 inputs), contiguous, of one shape."""
-    c, s = _extract_cs(rotary_params)
-    want = torch.float64 if dtype == torch.float64 else torch.float32
-    if (isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype == want and s.dtype == want and c.ndim == 2
-            and 2 * c.shape[1] == head_dim and c.shape == s.shape and c.device == dev and s.device == dev
-            and c.is_contiguous() and s.is_contiguous()):
-        return c, s  # as the kernel takes them
+    c, s = rotary_params if type(rotary_params) is tuple and len(rotary_params) == 2 else _extract_cs(rotary_params)
+    want = torch.float64 if dtype is torch.float64 else torch.float32
+    if isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype is want and s.dtype is want:
+        shape = c.shape
+        if (len(shape) == 2 and 2 * shape[1] == head_dim and shape == s.shape and c.device == dev and s.device == dev
+                and c.is_contiguous() and s.is_contiguous()):
+            return c, s  # as the kernel takes them
     c, s = (_lib.table_2d(torch.as_tensor(t, device=dev), head_dim) for t in (c, s))
     if c.shape != s.shape:
         raise ValueError(f"rotary tables must match, got {tuple(c.shape)} and {tuple(s.shape)}")
@@ -389,13 +391,24 @@ def _axis_sections(sections, axes, pairs):
         if axes != 1:
             raise ValueError("positions of several axes need sections, the feature pairs of each axis")
         return None
+    if type(sections) is tuple:
+        for n in sections:
+            if type(n) is not int:
+                break
+        else:
+            return _sections_array(sections, axes, pairs)
     whole = tuple(int(n) for n in sections)
-    if len(whole) != axes or min(whole) < 0 or sum(whole) > pairs or any(a != b for a, b in zip(whole, sections)):
+    if any(a != b for a, b in zip(whole, sections)):
         raise ValueError(f"sections must be {axes} nonnegative integers with a sum of at most {pairs}, got {sections}")
-    return (ctypes.c_int32 * axes)(*whole)
+    return _sections_array(whole, axes, pairs)
 
 
-_Strides12 = ctypes.c_int64 * 12
+@functools.lru_cache(maxsize=64)
+def _sections_array(sections, axes, pairs):
+    """sections, a tuple of int, as a C array; kept, as a program has few."""
+    if len(sections) != axes or min(sections) < 0 or sum(sections) > pairs:
+        raise ValueError(f"sections must be {axes} nonnegative integers with a sum of at most {pairs}, got {sections}")
+    return (ctypes.c_int32 * axes)(*sections)
 
 
 class _AxesConfig(NamedTuple):
@@ -439,7 +452,7 @@ def _axes_launch(q, k, c, s, positions, cfg, transpose):
     with _lib.on_device(dev):
         rc = _lib.lib().ago_rotate_axes(
             cfg.dtype, B, H, K, L, D, q.data_ptr(), kp, y.data_ptr(), zp,
-            _Strides12(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sy[0], sy[1], sy[2], sz[0], sz[1], sz[2]), c.data_ptr(),
+            _lib.pack12(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sy[0], sy[1], sy[2], sz[0], sz[1], sz[2]), c.data_ptr(),
             s.data_ptr(), c.shape[0], positions.data_ptr(), cfg.pos_bytes, cfg.pos_b, cfg.axes, cfg.cuts, transpose,
             _lib.stream_ptr(dev))
     _lib.check(rc, "ago_rotate_axes")

@@ -189,9 +189,6 @@ def build_block_tables(plan: DraftPlan, cached_lens: torch.Tensor, new_lens: tor
     return plan
 
 
-_Strides6, _Strides2 = ctypes.c_int64 * 6, ctypes.c_int64 * 2
-
-
 def _pages(plan, k_pages, v_pages):
     """Strides of the pages (page, head, slot of k, then of v), None where both are contiguous."""
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
@@ -202,7 +199,7 @@ def _pages(plan, k_pages, v_pages):
     k, v = k_pages.stride(), v_pages.stride()
     if (k[3] != 1 or v[3] != 1) and plan.head_dim != 1:
         raise ValueError("k_pages and v_pages need a contiguous head dimension")
-    return _Strides6(k[0], k[1], k[2], v[0], v[1], v[2])
+    return _lib.pack6(k[0], k[1], k[2], v[0], v[1], v[2])
 
 
 def _rows(plan, name, t, shape):
@@ -210,6 +207,12 @@ def _rows(plan, name, t, shape):
     if t.dtype != plan.dtype or t.shape != shape or t.device != plan.device:
         _refuse(plan, name, t, shape)
     return t if t.stride(2) == 1 or plan.head_dim == 1 else t.contiguous()
+
+
+def _like_rows(q):
+    """An empty contiguous tensor like q."""
+    y = torch.empty_like(q)  # half the time of torch.empty
+    return y if y.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
 def _refuse(plan, name, t, shape):
@@ -245,12 +248,12 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
             shape = (plan.max_tokens,) if positions.ndim == 1 else (plan.max_tokens, axes)
             positions = _lengths("positions", positions, dev, shape)
         cuts = _axis_sections(sections, axes, plan.head_dim // 2)
-        q_out = torch.empty(plan._q_shape, dtype=plan.dtype, device=dev)
+        q_out = _like_rows(q)
     elif positions is not None or sections is not None:
         raise ValueError("positions and sections need rotary_params")
     strides = None
     if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
-        strides = _Strides6(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        strides = _lib.pack6(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_append(
             plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, None if c is None else q_out.data_ptr(),
@@ -285,7 +288,7 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         masks = masks.contiguous()
     flags = 0
     if out is None:
-        out = torch.empty(plan._q_shape, dtype=plan.dtype, device=dev)
+        out = _like_rows(q)
         flags = _lib.FLAG_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
@@ -295,7 +298,7 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if return_denominator:
         new = torch.empty if flags else torch.zeros
         den = new((plan.max_tokens, plan.heads), dtype=_lib.accum_dtype(q.dtype), device=dev)
-    strides = None if q.is_contiguous() else _Strides2(q.stride(0), q.stride(1))
+    strides = None if q.is_contiguous() else _lib.pack2(q.stride(0), q.stride(1))
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_fwd(
             plan._ref, q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(masks),
