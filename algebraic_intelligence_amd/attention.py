@@ -505,7 +505,8 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
 
     Returns (q_rot, k_rot) (q_rot alone without k) in the inputs' dtype and axis order, formed in fp32
     (fp64) from the tables as they are, with one rounding; a position outside the tables gives NaN.
-    Differentiable with respect to q and k, twice too."""
+    Differentiable with respect to q and k, twice too.  As for every torch function, a backward pass is
+    captured into a HIP graph only while no eager graph of the same leaves lives."""
     q = _float_input(q)
     shape = q.shape
     if len(shape) != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != shape[0] or k.shape[2:] != shape[2:])):

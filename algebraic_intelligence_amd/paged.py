@@ -215,6 +215,13 @@ def _like_rows(q):
     return y if y.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
+def _overlap(a, b):
+    """Whether the address ranges of a and b meet."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
+        1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def _refuse(plan, name, t, shape):
     if t.dtype != plan.dtype:
         raise TypeError(f"{name} must be {plan.dtype}, got {t.dtype}")
@@ -234,7 +241,7 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
     ``positions`` (max_tokens, A) int32 with ``sections`` gives positions of A axes as in
     ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
-    without a slot are not stored."""
+    without a slot are not stored.  For inference: not differentiable."""
     q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
     page_strides = _pages(plan, k_pages, v_pages)
     dev = plan.device
@@ -292,8 +299,8 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         flags = _lib.FLAG_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
-    elif out.data_ptr() == q.data_ptr():
-        raise ValueError("out must not be q")
+    elif _overlap(out, q):
+        raise ValueError("out must not overlap q")
     den = None
     if return_denominator:
         new = torch.empty if flags else torch.zeros

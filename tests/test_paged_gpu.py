@@ -257,6 +257,37 @@ def test_axis_rotation_on_a_stream():
     assert torch.equal(got, want)
 
 
+def test_captured_axis_rotation_and_gradient():
+    """Forward and backward in one graph, replayed with other activations, positions and cotangents;
+    the eager calls use leaves of their own, so that no eager graph of the captured ones lives."""
+    tab, cuts = _tables(40, 64), (8, 12, 12)
+    new = lambda: [torch.randn(2, n, 77, 64, device="cuda", dtype=BF16) for n in (6, 2)]  # noqa: E731
+    x, g, pos = new(), new(), torch.randint(0, 40, (2, 77, 3), device="cuda")
+
+    def run(x):
+        leaves = [t.requires_grad_(True) for t in x]
+        y = A.apply_ago_axis_rotations(*leaves, tab, pos, cuts)
+        return [t.detach() for t in y], torch.autograd.grad(y, leaves, g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run([t.clone() for t in x])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, d = run([t.view_as(t) for t in x])
+    for _ in range(5):
+        for t, n in zip(x + g, new() + new()):
+            t.copy_(n)
+        pos.random_(0, 40)
+        graph.replay()
+        ey, ed = run([t.clone() for t in x])
+        torch.cuda.synchronize()
+        for got, want in zip([*y, *d], [*ey, *ed]):
+            assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------------------- cache write
 def _pages(pool, K, D, dt, fill=0.0):
     return tuple(torch.full_like(t, fill) for t in pool.new_pages(K, D, dt))
@@ -554,6 +585,9 @@ def test_attention_refusals():
         call(out=torch.empty_like(x.q, dtype=F32))
     with pytest.raises(ValueError, match="out"):
         call(out=x.q)
+    both = torch.zeros((x.q.shape[0] + 1, *x.q.shape[1:]), device="cuda", dtype=x.q.dtype)
+    with pytest.raises(ValueError, match="overlap"):
+        call(q=both[1:], out=both[:-1])
     with pytest.raises(ValueError, match="max_tree"):
         p = _plan(x.pool, 3, max_tree=0, heads=4, kv_heads=2)
         A.paged_tree_afa(x.q, x.kp, x.vp, p, masks=x.plan.masks)
