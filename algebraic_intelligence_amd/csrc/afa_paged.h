@@ -23,8 +23,8 @@ struct PagedCut {
   int rows;
   int64_t slots;  // per key/value head
 };
-// What a segment costs beside its tiles, in tiles (its start, the join of its waves).  2, 4, 8 and 16 take 107, 105,
-// 105 and 109 us for 32 requests of up to 32 drafted tokens over up to 8192, and 43, 41, 40 and 43 for 40 of up to
+// What a segment costs beside its tiles, in tiles (its start, the join of its waves).  2, 4, 8 and 16 take 98, 96,
+// 96 and 100 us for 32 requests of up to 32 drafted tokens over up to 8192, and 40, 38, 38 and 40 for 40 of up to
 // 13 over up to 3001 in fp32.
 constexpr int kPagedLead = 4;
 constexpr int kPagedMin = 4;  // shortest stretch: a tile for each wave
