@@ -32,8 +32,8 @@
 // HBM bound where requests are many or long.  96 requests of one token over up to 4096 cached, 16 heads of 64,
 // bf16: 160 us, 5.7 TB/s.  4 requests of 6 tokens over up to 131072, 16 query on 4 key heads of 128, fp16: 119 us,
 // 4.7 TB/s, of which the parts take 5.  32 requests of up to 32 drafted tokens over up to 8192, 16 on 4 heads of
-// 128, bf16 (128 rows): 105 us, 3.0 TB/s; its loads alone take 76, the parts 12, the rest is arithmetic that
-// they do not hide.  40 requests of up to 13 over 3001, 6 heads of 48, fp32: 38 us, 3.8 TB/s, the parts 7.  One token
+// 128, bf16 (128 rows): 94 us, 3.3 TB/s: MFMA and vector instructions one after the other (about 73), and the
+// parts (about 10).  40 requests of up to 13 over 3001, 6 heads of 48, fp32: 38 us, 3.8 TB/s, the parts 7.  One token
 // over 700, 12 heads of 64: 8 us, a chain of dependent reads (plan, table, keys, parts).
 #include <type_traits>
 
@@ -641,6 +641,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
           }
         }
 
+        // a wave with products ready goes before one that forms weights (trees: 94 us for 96)
+        if constexpr (SHARED) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
           if constexpr (F32) {
@@ -663,6 +665,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
             for (int b = 0; b < NB; ++b) acc[b][j] = mma16<DT>(v, lo[b], acc[b][j]);
           }
         }
+        if constexpr (SHARED) __builtin_amdgcn_s_setprio(0);
         if constexpr (!SHARED) {
           __builtin_amdgcn_sched_barrier(0);
           if (more) load_v();
