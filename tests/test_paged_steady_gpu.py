@@ -1,6 +1,7 @@
 """The serving operators at the sizes at which they spend their time: attention whose workgroups run through tens of
 key tiles, several requests and more pages than they hold entries of, in every instance of the kernel; pages of
-other stride orders; rotations and cache writes of several heads a thread, and past the caches.
+other stride orders; rotations and cache writes of several heads a thread, and past the caches; a decoded
+sequence row by row.
 
 Bounds count roundings as tests/test_paged_gpu.py does.
 """
@@ -245,3 +246,61 @@ def test_append_of_many_tokens(dt, H, K, D, page, tokens):
     want_k[slots // page, :, slots % page] = turn(k)[:tokens]
     want_v[slots // page, :, slots % page] = v[:tokens]
     assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+# ------------------------------------------------------------------------------------ whole steps
+@pytest.mark.parametrize("dt,H,K,D,page", [(F32, 4, 2, 64, 16), (BF16, 4, 4, 128, 32), (F16, 6, 2, 48, 8), (BF16, 8, 1, 64, 64)])
+def test_decoded_rows_are_the_sequences(dt, H, K, D, page):
+    """Three sequences decoded through a prompt, drafted trees of which a path is accepted, and single
+    tokens.  The rows on the accepted path against 64-bit attention over the sequence's own keys, rotated
+    and rounded apart from the cache: each within its own bound, which is far below the row."""
+    rng = np.random.default_rng(D)
+    R, L, G = 3, 90, H // K
+    rot = A.build_cayley_rotary_matrix(D, 128)
+    at = torch.arange(L, device="cuda")[:, None]
+    seq, turned = [], []
+    for _ in range(R):
+        q, k, v = (torch.tensor(rng.standard_normal((L, n, D)), device="cuda").to(dt) for n in (H, K, K))
+        seq.append((q, k, v))
+        yq, yk = A.apply_ago_axis_rotations(q.transpose(0, 1)[None], k.transpose(0, 1)[None], rot, at)
+        turned.append((yq[0].transpose(0, 1), _f64(yk[0]), _f64(v.transpose(0, 1))))
+    pool = A.PagePool(100, page, R, L + 20)
+    kp, vp = (torch.full_like(p, float("nan")) for p in pool.new_pages(K, D, dt))
+    done = np.zeros(R, int)
+    for accept, others in [(40, 0), (17, 0), (1, 0), (1, 6), (3, 9), (1, 0), (5, 2), (1, 30)]:
+        new = np.array([accept + others, accept, accept + others])
+        T = int(new.sum()) + 2
+        plan = _plan(pool, T, int(new.max()), 64, H, K, D, dt)
+        rows = [torch.randn(T, n, D, device="cuda").to(dt) for n in (H, K, K)]
+        parents, path, first = np.full(T, -1), [], 0
+        for r in range(R):
+            n = int(new[r])
+            on = np.sort(rng.choice(n, accept, replace=False))
+            for i in range(n):
+                before = [j for j in on if j < i]
+                parents[first + i] = (before[-1] if before else -1) if i in on else (rng.integers(-1, i) if i else -1)
+            for x, whole in zip(rows, seq[r]):
+                x[first + torch.tensor(on, device="cuda")] = whole[done[r]:done[r] + accept]
+            path.append(first + on)
+            first += n
+        A.build_block_tables(plan, _i32(done), _i32(new), _i32(parents) if others else None)
+        assert (plan.status == 0).all()
+        q = A.append_to_cache(*rows, kp, vp, plan, rot)
+        out = A.paged_tree_afa(q, kp, vp, plan)
+        for r in range(R):
+            yq, yk, yv = turned[r]
+            assert torch.equal(q[path[r]], yq[done[r]:done[r] + accept])
+            for i, row in enumerate(path[r]):
+                j = done[r] + i
+                for h in range(H):
+                    ref, _, size, S = P.attention_row(_f64(yq[j, h]), yk[h // G, :j + 1], yv[h // G, :j + 1], 0.5)
+                    e = _weight_error(dt, D, S, j + 1)
+                    bound = 2 * e * size + (_half(dt) + 4 * U) * np.abs(ref) + _tiny(dt)
+                    assert np.linalg.norm(bound) <= np.linalg.norm(ref) / 8
+                    _close(out[row, h], ref, bound, (accept, others, r, i, h))
+        # the accepted path is stored again where the next step expects it
+        keep = _plan(pool, R * accept, accept, 0, H, K, D, dt)
+        A.build_block_tables(keep, _i32(done), _i32([accept] * R))
+        chosen = torch.tensor(np.concatenate(path), device="cuda")
+        A.append_to_cache(*(x[chosen].contiguous() for x in rows), kp, vp, keep, rot)
+        done += accept
