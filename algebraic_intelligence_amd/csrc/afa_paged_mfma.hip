@@ -70,6 +70,22 @@ __device__ __forceinline__ float rho8_refined(float s) {
   return s < 0.0f ? inv : p8;
 }
 
+// rho(s)^8 in bf16 and fp16 calls: above kLowScore the branch-free form, which costs half of the other and loses
+// nothing above 0, and below it 16 s^2 times the error of the hardware's rsqrt, 2.2e-4 at -8; below kLowScore the
+// form without cancellation.  A weight goes by its own score alone, whatever scores a wave forms beside it, of
+// keys that the row does not see among them.
+constexpr float kLowScore = -8.0f;
+__device__ __forceinline__ float rho8_by_score(float s) {
+  const bool low = !(s > kLowScore);  // a NaN stays one in either form
+  const float t = __builtin_fmaf(s, s, 1.0f);
+  const float r = __builtin_amdgcn_rsqf(t);
+  const float rho = __builtin_fmaf(t, r, low ? __builtin_fabsf(s) : s);
+  const float p2 = rho * rho;
+  const float p4 = p2 * p2;
+  const float p8 = p4 * p4;
+  return low ? __builtin_amdgcn_rcpf(p8) : p8;
+}
+
 // Bits of `len` consecutive drafted tokens from index i0 on (negative: cached, seen) that the row sees.
 // words: the row's masks, nullptr for a chain whose row is token `self`; n: the request's new tokens.
 __device__ __forceinline__ unsigned sees_bits(int i0, int len, int n, int self, const int64_t* words, int W) {
@@ -580,17 +596,16 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = rho8_refined(w[e]);
           } else {
-            // the branch-free form costs half of the other and loses nothing above 0, and below it
-            // 16 s^2 times the error of the hardware's rsqrt, 2.2e-4 at -8
-            float low = w[0];
+            // where no score is low all lanes take the branch-free form, which gives such scores the same bits
+            float least = w[0];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) low = __builtin_fminf(low, w[e]);
-            if (__ballot(!(low > -8.0f)) == 0) {  // a NaN stays one in either form
+            for (int e = 1; e < 8; ++e) least = __builtin_fminf(least, w[e]);
+            if (__ballot(!(least > kLowScore)) == 0) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) w[e] = rho8_fast(w[e]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = rho8_exact(w[e]);
+              for (int e = 0; e < 8; ++e) w[e] = rho8_by_score(w[e]);
             }
           }
           if (masked) {
