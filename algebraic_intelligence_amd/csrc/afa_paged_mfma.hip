@@ -27,7 +27,7 @@
 //
 // Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
 // the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
-// a row's weights are scaled by a power of two, lowered when a larger weight comes.
+// a row's weights are scaled by a power of two, lowered when a larger weight comes (kFirstScale).
 //
 // HBM bound where requests are many or long.  96 requests of one token over up to 4096 cached, 16 heads of 64,
 // bf16: 160 us, 5.7 TB/s.  4 requests of 6 tokens over up to 131072, 16 query on 4 key heads of 128, fp16: 119 us,
@@ -85,6 +85,11 @@ __device__ __forceinline__ float rho8_by_score(float s) {
   const float p8 = p4 * p4;
   return low ? __builtin_amdgcn_rcpf(p8) : p8;
 }
+
+// The power of two by which a row's fp16 weights begin.  It is only ever lowered, so it decides how small weights may
+// be that have a row to themselves: 2^-120, a score of -16384, is 1 then.  A first weight of about 1 lowers it
+// at once, as any start does; its inverse and that of the lowest, 2^-123, are normal numbers.
+constexpr float kFirstScale = 0x1p120f;
 
 // Bits of `len` consecutive drafted tokens from index i0 on (negative: cached, seen) that the row sees.
 // words: the row's masks, nullptr for a chain whose row is token `self`; n: the request's new tokens.
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
       den[b] = 0.0f;
-      sc[b] = 0x1p60f;
+      sc[b] = kFirstScale;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) acc[b][j] = f32x4_t{0, 0, 0, 0};
     }

@@ -55,3 +55,41 @@ def test_weights_do_not_depend_on_hidden_keys(dt, H, K, n, D, page):
     assert 0 < hidden[:n].sum() < n
     for got, want in zip(_run(x), first):
         assert torch.equal(got[hidden], want[hidden])
+
+
+@pytest.mark.parametrize("dt,score", [(t, s) for t in (BF16, F16, F32) for s in (90, 300, 1000, 3000)]
+                         + [(F16, 15000), (F32, 15000)])
+@pytest.mark.parametrize("H,K,n", ROWS)
+def test_weights_far_below_one(dt, score, H, K, n):
+    """Every score is the same far negative one and there is no sink: the result is the mean of the visible
+    values.  The scores are exact (a^2 of 16 bits, 64 of them), so that a row's weights are equal and what
+    they lose to their planes is common to all: each product's planes h^2, for fp16 planes 2^-25 of a row's
+    largest weight, and N sums.  Each of the at most 2 N + 2 products, sums and scalings that falls below the smallest
+    normal number, 2^-126, is off by half a subnormal step, 2^-150, of the N w that it is divided by."""
+    a = {90: 3.375, 300: 6.125, 1000: 11.1875, 3000: 19.375, 15000: 43.25}[score]
+    x = _Cache(dt, [(150, n), (33, n), (0, 2)], H, K, 64, 16, seed=n)
+    x.q = torch.full_like(x.q, a)
+    _set_keys(x, 16, lambda k: torch.full_like(k, -a))
+    out, den = _run(x, sink_omega=0.0)
+    w = (np.sqrt(1 + (8 * a * a) ** 2) + 8 * a * a) ** -8.0
+    for r, (c, m) in enumerate(x.lens):
+        v = _f64(x.v[r])
+        for i in range(m):
+            t = x.starts[r] + i
+            see = np.concatenate((np.ones(c, bool), x.sees[t, :m]))
+            N = int(see.sum())
+            e = 105 * U + (0 if dt == F32 else 2.2e-4)
+            _close(den[t], np.full(H, N * w), np.full(H, (e + N * U) * N * w), (r, i))
+            mean, size = (np.repeat(y[see].mean(0), H // K, 0) for y in (v, np.abs(v)))
+            e = 2 * N * U + (0 if dt == F32 else _half(dt) ** 2) + (N * 2.0 ** -25 if dt == F16 else 0)
+            small = (2 * N + 2) * 2.0 ** -150 / (N * w)
+            _close(out[t], mean, e * size + (_half(dt) + 2 * U) * np.abs(mean) + small + _tiny(dt), (r, i))
+
+
+@pytest.mark.parametrize("scale", [45.0, 150.0])
+def test_fp16_negative_scores(scale):
+    """Random scores of about -230 and -770, no sink."""
+    x = _Cache(F16, [(150, 3), (40, 20)], 2, 2, 64, 16, seed=4)
+    x.q = ((x.q.abs() + 0.25) * scale).to(F16)
+    _set_keys(x, 16, lambda k: -k.abs())
+    x.check(sink=0.0)
