@@ -749,6 +749,27 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
       for (int w = 1; w < NBUF; ++w) x += *(const f32x4_t*)&red[w][row][d];
 #pragma unroll
       for (int w = 1; w < KW; ++w) sum += red_den[w][row];
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) finite = finite && __builtin_fabsf(x[i]) < __builtin_inff();
+      if (!finite && sum < __builtin_inff()) {
+        // Weights are finite, so a cached value may be what is not.  Such a value is the sum, whatever its
+        // products with a weight's planes gave (the second plane may be 0 or negative).
+        f32x4_t y = {0, 0, 0, 0};
+        for (int pos = tile0 * kPagedTile; pos < min(tile1 * kPagedTile, c); ++pos) {
+          const int page = table[pos >> lp];
+          if ((unsigned)page >= (unsigned)p.num_pages) continue;
+          const char* v = v_base + (uint64_t)(uint32_t)page * f.v_page + (uint32_t)(pos & in_page) * f.v_slot;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float z = Elem<DT>::load(v, d + i);
+            if (!(__builtin_fabsf(z) < __builtin_inff())) y[i] += z;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(__builtin_fabsf(y[i]) < __builtin_inff())) x[i] = y[i];
+      }
       if (odd) {
         // drafted values that are not finite, of weights above 0: the value itself
         const int who = (row0 + row) / G;

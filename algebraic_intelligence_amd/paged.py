@@ -280,8 +280,9 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     (max_tokens, heads) in fp32 (fp64 for fp64 inputs).  heads / kv_heads query heads share a key/value
     head.  ``masks`` replaces the plan's (max_tokens, max_tree / 64) int64 masks: they hide drafted tokens
     only, and none in requests of more than max_tree new tokens.  A row that sees no key is 0, and a key
-    that a row does not see, whatever its page holds, does not touch it.  Rows behind the last request's
-    are 0, or left as they were where ``out`` is given.  For inference: not differentiable."""
+    that a row does not see, whatever its page holds, does not touch it; an infinity or a NaN in a value
+    that it sees is its result in that feature.  Rows behind the last request's are 0, or left as they
+    were where ``out`` is given.  For inference: not differentiable."""
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
     q = _rows(plan, "q", q, plan._q_shape)

@@ -340,9 +340,10 @@ int afa_paged_append(const afa_paged_plan* plan, const void* q, const void* k, c
  * AFA of the step's tokens over the cache: out_i = sum_j w_ij v_j / (sum_j w_ij + sink), w = rho(s)^8,
  * over the cached tokens and the drafted ones that token i's mask shows.  q (max_tokens, heads, head_dim)
  * with strides {q_t, q_h} (NULL: contiguous); masks: nullable, the plan's; out and denom (nullable,
- * (max_tokens, heads), accumulation type) contiguous.  A row without a visible key is 0.  Rows behind the
- * last request's are left as they were, or with AFA_FLAG_ZERO_TAIL set to 0.  A page id outside the
- * pool holds no keys.  workspace: afa_paged_workspace_size() bytes, 16-byte aligned, or NULL.
+ * (max_tokens, heads), accumulation type) contiguous.  A row without a visible key is 0; an infinity or a
+ * NaN in a value that a row sees is its result in that feature.  Rows behind the last request's are left
+ * as they were, or with AFA_FLAG_ZERO_TAIL set to 0.  A page id outside the pool holds no keys.
+ * workspace: afa_paged_workspace_size() bytes, 16-byte aligned, or NULL.
  */
 #define AFA_FLAG_ZERO_TAIL 0x400u
 size_t afa_paged_workspace_size(const afa_paged_plan* plan);

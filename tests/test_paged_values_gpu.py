@@ -93,3 +93,33 @@ def test_fp16_negative_scores(scale):
     x.q = ((x.q.abs() + 0.25) * scale).to(F16)
     _set_keys(x, 16, lambda k: -k.abs())
     x.check(sink=0.0)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32, F64])
+@pytest.mark.parametrize("H,K,n", ROWS)
+@pytest.mark.parametrize("cached,D", [(40, 64), (700, 64), (60, 128), (60, 48)])
+def test_cached_values_that_are_not_finite(dt, H, K, n, cached, D):
+    """An infinity or NaN among the cached values is the result, in its feature, of every row of its request;
+    infinities of both signs are NaN; nothing else changes."""
+    x = _Cache(dt, [(cached, n), (33, n), (70, 1)], H, K, D, 16, seed=cached + n)
+    first, den = _run(x)
+
+    def put(key, feature, value):
+        x.vp[x.tables[0][key // 16], :, key % 16, feature] = float(value)
+
+    put(3, 5, "inf")
+    put(9, 1, "-inf")
+    put(11, 2, "nan")
+    put(2, D - 1, "inf")
+    put(cached - 1, D - 1, "-inf")
+    put(cached + 1, 5, "-inf")  # drafted: NaN with the cached one in the rows that see it
+    want = first.clone()
+    want[:n, :, 5], want[:n, :, 1], want[:n, :, 2], want[:n, :, D - 1] = (float(s) for s in ("inf", "-inf", "nan", "nan"))
+    sees = torch.tensor(x.sees[:n, 1], device="cuda")
+    assert 0 < sees.sum() < n
+    want[:n, :, 5][sees] = float("nan")
+    out, same = _run(x)
+    assert torch.equal(same, den)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(out), nan)
+    assert torch.equal(out[~nan], want[~nan])
