@@ -54,6 +54,10 @@ __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
                                                   0);
 }
 
+// Below this score a weight is under the smallest normal number, 2^-126, and counts as 0: further down its inverse
+// and then the square of the score no longer fit, and their products would be NaN.
+constexpr float kNoWeight = -28000.0f;
+
 // rho(s)^8 in fp32 with the square root and the reciprocal refined by one Newton step each: the
 // hardware's are off by 1 ulp, which three squarings make 8.
 __device__ __forceinline__ float rho8_refined(float s) {
@@ -67,7 +71,7 @@ __device__ __forceinline__ float rho8_refined(float s) {
   const float p8 = p4 * p4;
   const float i0 = __builtin_amdgcn_rcpf(p8);
   const float inv = __builtin_fmaf(i0, __builtin_fmaf(-p8, i0, 1.0f), i0);
-  return s < 0.0f ? inv : p8;
+  return s < kNoWeight ? 0.0f : s < 0.0f ? inv : p8;
 }
 
 // rho(s)^8 in bf16 and fp16 calls: above kLowScore the branch-free form, which costs half of the other and loses
@@ -83,7 +87,7 @@ __device__ __forceinline__ float rho8_by_score(float s) {
   const float p2 = rho * rho;
   const float p4 = p2 * p2;
   const float p8 = p4 * p4;
-  return low ? __builtin_amdgcn_rcpf(p8) : p8;
+  return s < kNoWeight ? 0.0f : low ? __builtin_amdgcn_rcpf(p8) : p8;
 }
 
 // The power of two by which a row's fp16 weights begin.  It is only ever lowered, so it decides how small weights may
