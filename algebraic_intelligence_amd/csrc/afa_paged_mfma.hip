@@ -54,9 +54,10 @@ __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
                                                   0);
 }
 
-// Below this score a weight is under the smallest normal number, 2^-126, and counts as 0: further down its inverse
-// and then the square of the score no longer fit, and their products would be NaN.
-constexpr float kNoWeight = -28000.0f;
+// Weights end at 2^-126, the smallest normal number (scores of -27554 and below): the eighth power is cut off there
+// before its inverse is formed.  Further down it no longer fits and then the square of the score does not, which
+// gives an infinity and a NaN, and the cut takes either.
+constexpr float kMostPower = 0x1p126f;
 
 // rho(s)^8 in fp32 with the square root and the reciprocal refined by one Newton step each: the
 // hardware's are off by 1 ulp, which three squarings make 8.
@@ -69,9 +70,10 @@ __device__ __forceinline__ float rho8_refined(float s) {
   const float p2 = rho * rho;
   const float p4 = p2 * p2;
   const float p8 = p4 * p4;
-  const float i0 = __builtin_amdgcn_rcpf(p8);
-  const float inv = __builtin_fmaf(i0, __builtin_fmaf(-p8, i0, 1.0f), i0);
-  return s < kNoWeight ? 0.0f : s < 0.0f ? inv : p8;
+  const float cut = __builtin_fminf(p8, kMostPower);
+  const float i0 = __builtin_amdgcn_rcpf(cut);
+  const float inv = __builtin_fmaf(i0, __builtin_fmaf(-cut, i0, 1.0f), i0);
+  return s < 0.0f ? inv : p8;  // a NaN stays one
 }
 
 // rho(s)^8 in bf16 and fp16 calls: above kLowScore the branch-free form, which costs half of the other and loses
@@ -80,14 +82,14 @@ __device__ __forceinline__ float rho8_refined(float s) {
 // keys that the row does not see among them.
 constexpr float kLowScore = -8.0f;
 __device__ __forceinline__ float rho8_by_score(float s) {
-  const bool low = !(s > kLowScore);  // a NaN stays one in either form
+  const bool low = s <= kLowScore;
   const float t = __builtin_fmaf(s, s, 1.0f);
   const float r = __builtin_amdgcn_rsqf(t);
   const float rho = __builtin_fmaf(t, r, low ? __builtin_fabsf(s) : s);
   const float p2 = rho * rho;
   const float p4 = p2 * p2;
   const float p8 = p4 * p4;
-  return s < kNoWeight ? 0.0f : low ? __builtin_amdgcn_rcpf(p8) : p8;
+  return low ? __builtin_amdgcn_rcpf(__builtin_fminf(p8, kMostPower)) : p8;  // a NaN stays one
 }
 
 // The power of two by which a row's fp16 weights begin.  It is only ever lowered, so it decides how small weights may
@@ -745,58 +747,51 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
     const __amdgpu_buffer_rsrc_t buffer =
         __builtin_amdgcn_make_buffer_rsrc(f.part + head0 * D, 0, (int)(2 * f.slots * ROWS * D * 4), 0x00020000);
     const int64_t my_part = part_of(slot - from_slot);
-    for (int e = tid; e < mine * quads; e += THREADS) {
-      const int row = e / quads, d = 4 * (e - row * quads);
-      f32x4_t x = *(const f32x4_t*)&red[0][row][d];
-      float sum = red_den[0][row];
+    f32x4_t zero = {0, 0, 0, 0};  // NaN where a sum is not finite
+    auto hand_on = [&](auto again) {
+      for (int e = tid; e < mine * quads; e += THREADS) {
+        const int row = e / quads, d = 4 * (e - row * quads);
+        f32x4_t x = *(const f32x4_t*)&red[0][row][d];
+        float sum = red_den[0][row];
 #pragma unroll
-      for (int w = 1; w < NBUF; ++w) x += *(const f32x4_t*)&red[w][row][d];
+        for (int w = 1; w < NBUF; ++w) x += *(const f32x4_t*)&red[w][row][d];
 #pragma unroll
-      for (int w = 1; w < KW; ++w) sum += red_den[w][row];
-      bool finite = true;
+        for (int w = 1; w < KW; ++w) sum += red_den[w][row];
+        if constexpr (decltype(again)::value) {
+          const int who = (row0 + row) / G;
+          const int64_t* words = a.masks + (int64_t)(q.start + who) * W;
+          f32x4_t y = {0, 0, 0, 0};
+          for (int pos = tile0 * kPagedTile; pos < min(tile1 * kPagedTile, keys); ++pos) {
+            const bool sees = pos < c || (tree ? words[(pos - c) >> 6] >> ((pos - c) & 63) & 1 : pos - c <= who);
+            const int page = table[pos >> lp];
+            if (!sees || (unsigned)page >= (unsigned)p.num_pages) continue;
+            const char* v = v_base + (uint64_t)(uint32_t)page * f.v_page + (uint32_t)(pos & in_page) * f.v_slot;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) finite = finite && __builtin_fabsf(x[i]) < __builtin_inff();
-      if (!finite && sum < __builtin_inff()) {
-        // Weights are finite, so a cached value may be what is not.  Such a value is the sum, whatever its
-        // products with a weight's planes gave (the second plane may be 0 or negative).
-        f32x4_t y = {0, 0, 0, 0};
-        for (int pos = tile0 * kPagedTile; pos < min(tile1 * kPagedTile, c); ++pos) {
-          const int page = table[pos >> lp];
-          if ((unsigned)page >= (unsigned)p.num_pages) continue;
-          const char* v = v_base + (uint64_t)(uint32_t)page * f.v_page + (uint32_t)(pos & in_page) * f.v_slot;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float z = Elem<DT>::load(v, d + i);
-            if (!(__builtin_fabsf(z) < __builtin_inff())) y[i] += z;
+            for (int i = 0; i < 4; ++i) {
+              const float z = Elem<DT>::load(v, d + i);
+              if (!(__builtin_fabsf(z) < __builtin_inff())) y[i] += z;
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(__builtin_fabsf(y[i]) < __builtin_inff())) x[i] = y[i];
+        } else if constexpr (!F32) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(x[i], 0.0f, zero[i]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(__builtin_fabsf(y[i]) < __builtin_inff())) x[i] = y[i];
-      }
-      if (odd) {
-        // drafted values that are not finite, of weights above 0: the value itself
-        const int who = (row0 + row) / G;
-        const int64_t* words = a.masks + (int64_t)(q.start + who) * W;
-        for (int pos = max(tile0 * kPagedTile, c); pos < min(tile1 * kPagedTile, keys); ++pos) {
-          const bool sees = tree ? words[(pos - c) >> 6] >> ((pos - c) & 63) & 1 : pos - c <= who;
-          const int page = table[pos >> lp];
-          if (!sees || (unsigned)page >= (unsigned)p.num_pages) continue;
-          const char* v = v_base + (uint64_t)(uint32_t)page * f.v_page + (uint32_t)(pos & in_page) * f.v_slot;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float y = Elem<DT>::load(v, d + i);
-            if (!(__builtin_fabsf(y) < __builtin_inff())) x[i] += y;
-          }
+        if (parts > 1) {
+          put4(buffer, (uint32_t)((my_part * ROWS + row) * D + d) * 4, x);
+          if (d == 0) put1(part_den + my_part * ROWS + row, sum);
+        } else {
+          store4(out_row(row), d, x, sum);
         }
       }
-      if (parts > 1) {
-        put4(buffer, (uint32_t)((my_part * ROWS + row) * D + d) * 4, x);
-        if (d == 0) put1(part_den + my_part * ROWS + row, sum);
-      } else {
-        store4(out_row(row), d, x, sum);
-      }
-    }
+    };
+    hand_on(std::false_type());
+    // A value that is not finite is the sum of every row that sees it, as weights are above 0.  Drafted ones were taken
+    // out of the products; a cached one may have become NaN there, since a weight's second plane may be 0 or
+    // negative.  Such sums are formed again, from these values alone.
+    if (odd || (zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.0f) hand_on(std::true_type());
     if (parts == 1) continue;
 
     const int size = group_size(parts), groups = (parts + size - 1) / size, g0 = (slot - from_slot) / size * size;
