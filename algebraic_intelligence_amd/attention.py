@@ -487,7 +487,7 @@ class _RotateAxes(torch.autograd.Function):
 
 
 def _rotate_axes(q, k, c, s, positions, cfg, transpose):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or _lib.in_forward_mode():
         return _RotateAxes.apply(q, k, c, s, positions, cfg, transpose)
     y, z = _axes_launch(q, k, c, s, positions, cfg, transpose)
     return y if k is None else (y, z)
@@ -505,8 +505,9 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
 
     Returns (q_rot, k_rot) (q_rot alone without k) in the inputs' dtype and axis order, formed in fp32
     (fp64) from the tables as they are, with one rounding; a position outside the tables gives NaN.
-    Differentiable with respect to q and k, twice too.  As for every torch function, a backward pass is
-    captured into a HIP graph only while no eager graph of the same leaves lives."""
+    Differentiable with respect to q and k, twice too, in reverse mode; a forward-mode tangent is refused, as
+    by the other rotations.  As for every torch function, a backward pass is captured into a HIP graph only
+    while no eager graph of the same leaves lives."""
     q = _float_input(q)
     shape = q.shape
     if len(shape) != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != shape[0] or k.shape[2:] != shape[2:])):

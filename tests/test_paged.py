@@ -176,3 +176,31 @@ def test_axis_rotation_refusals():
         call(p=torch.zeros(6, 5, dtype=torch.int64), s=(1,) * 5)
     with pytest.raises(ValueError, match="axes"):
         call(p=torch.zeros(6, 0, dtype=torch.int64), s=())
+
+
+def _stub_rotation(monkeypatch):
+    """The rotation's checks and autograd on the CPU, with the launch left out."""
+    from algebraic_intelligence_amd import attention
+
+    monkeypatch.setattr(_lib, "require_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(attention, "_axes_launch", lambda q, k, *rest: (torch.zeros(q.shape), None if k is None else
+                                                                        torch.zeros(k.shape)))
+
+
+def test_axis_rotation_refuses_tangents(monkeypatch):
+    """A dual q or k is refused, also where no gradient is recorded, and never comes back without its tangent."""
+    from torch.autograd import forward_ad
+
+    _stub_rotation(monkeypatch)
+    q, k = torch.ones(2, 4, 6, 8), torch.ones(2, 2, 6, 8)
+    tables, at = (torch.ones(10, 4), torch.zeros(10, 4)), torch.zeros(6, 2, dtype=torch.int64)
+    call = lambda q, k: A.apply_ago_axis_rotations(q, k, tables, at, (2, 2))  # noqa: E731
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(q), None), (dual(q), k), (q, dual(k))):
+            with pytest.raises(NotImplementedError):
+                call(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call(*args)
+        assert call(q, k)[1].shape == k.shape and call(q, None).shape == q.shape
+    assert call(q, k)[0].shape == q.shape
