@@ -18,6 +18,7 @@ import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import _axis_sections, _axis_tables
@@ -189,6 +190,18 @@ def build_block_tables(plan: DraftPlan, cached_lens: torch.Tensor, new_lens: tor
     return plan
 
 
+def _inference_only(name, *tensors):
+    """Refuses tensors that a derivative is asked of, which the call's result would not have."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
+    if _lib.in_forward_mode():
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no derivative, and a tensor carries a tangent")
+
+
 def _pages(plan, k_pages, v_pages):
     """Strides of the pages (page, head, slot of k, then of v), None where both are contiguous."""
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
@@ -241,7 +254,9 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
     ``positions`` (max_tokens, A) int32 with ``sections`` gives positions of A axes as in
     ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
-    without a slot are not stored.  For inference: not differentiable."""
+    without a slot are not stored.  For inference: inputs that require a gradient are refused where gradients are
+    recorded."""
+    _inference_only("append_to_cache", q, k, v, k_pages, v_pages)
     q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
     page_strides = _pages(plan, k_pages, v_pages)
     dev = plan.device
@@ -282,7 +297,9 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     only, and none in requests of more than max_tree new tokens.  A row that sees no key is 0, and a key
     that a row does not see, whatever its page holds, does not touch it; an infinity or a NaN in a value
     that it sees is its result in that feature.  Rows behind the last request's are 0, or left as they
-    were where ``out`` is given.  For inference: not differentiable."""
+    were where ``out`` is given.  For inference: tensors that require a gradient are refused where gradients
+    are recorded."""
+    _inference_only("paged_tree_afa", q, k_pages, v_pages)
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
     q = _rows(plan, "q", q, plan._q_shape)
@@ -302,6 +319,8 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
     elif _overlap(out, q):
         raise ValueError("out must not overlap q")
+    else:
+        _inference_only("paged_tree_afa", out)
     den = None
     if return_denominator:
         new = torch.empty if flags else torch.zeros

@@ -204,3 +204,62 @@ def test_axis_rotation_refuses_tangents(monkeypatch):
                 call(*args)
         assert call(q, k)[1].shape == k.shape and call(q, None).shape == q.shape
     assert call(q, k)[0].shape == q.shape
+
+
+class _StubPlan:
+    """What the serving calls look at before any device work, on the CPU."""
+
+    def __init__(self, dtype=torch.float32):
+        self.dtype, self.device, self.head_dim, self.max_tree, self.max_tokens, self.heads = dtype, torch.device("cpu"), 8, 64, 6, 4
+        self._q_shape, self._kv_shape, self._page_shape = (6, 4, 8), (6, 2, 8), (3, 2, 16, 8)
+        self.masks = torch.zeros(6, 1, dtype=torch.int64)
+
+    def tensors(self):
+        new = lambda shape: torch.zeros(shape, dtype=self.dtype)  # noqa: E731
+        return {"q": new(self._q_shape), "k": new(self._kv_shape), "v": new(self._kv_shape), "k_pages": new(self._page_shape),
+                "v_pages": new(self._page_shape)}
+
+
+def _serve(plan, t, **kw):
+    """(name, call) of the two serving calls on tensors t."""
+    rotary = torch.ones(9, 4), torch.zeros(9, 4)
+    return [("append_to_cache", lambda: A.append_to_cache(t["q"], t["k"], t["v"], t["k_pages"], t["v_pages"], plan, rotary)),
+            ("paged_tree_afa", lambda: A.paged_tree_afa(t["q"], t["k_pages"], t["v_pages"], plan, **kw))]
+
+
+def _reaches_the_device(call):
+    """Every check of the call passes: it ends only where it asks for the GPU."""
+    if not torch.cuda.is_available():
+        with pytest.raises((RuntimeError, AttributeError, ctypes.ArgumentError, AssertionError)) as e:
+            call()
+        assert "gradient" not in str(e.value) and "overlap" not in str(e.value) and "tangent" not in str(e.value)
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "k_pages", "v_pages"])
+def test_serving_refuses_what_needs_a_gradient(name):
+    """No input loses a gradient or a tangent without a word; under no_grad the same tensors are taken."""
+    from torch.autograd import forward_ad
+
+    plan = _StubPlan()
+    t = plan.tensors()
+    plain = t[name]
+    for what, call in _serve(plan, t):
+        if name in ("k", "v") and what == "paged_tree_afa":
+            continue
+        t[name] = plain.clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match=f"{what} has no gradient"):
+            call()
+        with torch.no_grad():
+            _reaches_the_device(call)
+        with forward_ad.dual_level():
+            t[name] = forward_ad.make_dual(plain, torch.ones_like(plain))
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+                call()
+            t[name] = plain
+            _reaches_the_device(call)
+    out = plain.clone().requires_grad_(True)
+    if name == "q":
+        with pytest.raises(RuntimeError, match="no gradient"):
+            A.paged_tree_afa(plain, t["k_pages"], t["v_pages"], plan, out=out)
