@@ -121,6 +121,7 @@ class DraftPlan:
         self._q_shape = (self.max_tokens, self.heads, self.head_dim)
         self._kv_shape = (self.max_tokens, self.kv_heads, self.head_dim)
         self._page_shape = (pool.num_pages, self.kv_heads, pool.page_size, self.head_dim)
+        self._page_bytes = pool.num_pages * self.kv_heads * pool.page_size * self.head_dim * dtype.itemsize
         self._len_shape = (pool.max_requests,)
         c = self._c = _Plan(num_pages=pool.num_pages, page_size=pool.page_size, requests=pool.max_requests,
                             table_width=pool.block_tables.shape[1], max_tokens=max_tokens, max_new=max_new,
@@ -228,11 +229,28 @@ def _like_rows(q):
     return y if y.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
+def _span(t):
+    """First byte of t and the one behind its last."""
+    n = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
 def _overlap(a, b):
     """Whether the address ranges of a and b meet."""
-    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
-        1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (a, b))
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
+
+
+def _own_places(plan, k_pages, v_pages, contiguous):
+    """Refuses pages in which two of a step's rows would be written to one place, as far as addresses and
+    strides tell."""
+    apart = abs(k_pages.data_ptr() - v_pages.data_ptr())
+    if apart < plan._page_bytes if contiguous else apart == 0:
+        raise ValueError("k_pages and v_pages must not overlap")
+    if not contiguous:
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
+                raise ValueError(f"{name} must not be an expanded tensor")
 
 
 def _refuse(plan, name, t, shape):
@@ -254,11 +272,12 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
     ``positions`` (max_tokens, A) int32 with ``sections`` gives positions of A axes as in
     ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
-    without a slot are not stored.  For inference: inputs that require a gradient are refused where gradients are
-    recorded."""
+    without a slot are not stored.  The pages hold k and v in places of their own, apart from q, k and v.
+    For inference: inputs that require a gradient are refused where gradients are recorded."""
     _inference_only("append_to_cache", q, k, v, k_pages, v_pages)
     q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
     page_strides = _pages(plan, k_pages, v_pages)
+    _own_places(plan, k_pages, v_pages, page_strides is None)
     dev = plan.device
     c = s = None
     axes, cuts = 1, None
@@ -317,8 +336,8 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         flags = _lib.FLAG_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
-    elif _overlap(out, q):
-        raise ValueError("out must not overlap q")
+    elif _overlap(out, q) or _overlap(out, k_pages) or _overlap(out, v_pages):
+        raise ValueError("out must not overlap q, k_pages or v_pages")
     else:
         _inference_only("paged_tree_afa", out)
     den = None

@@ -212,7 +212,7 @@ class _StubPlan:
     def __init__(self, dtype=torch.float32):
         self.dtype, self.device, self.head_dim, self.max_tree, self.max_tokens, self.heads = dtype, torch.device("cpu"), 8, 64, 6, 4
         self._q_shape, self._kv_shape, self._page_shape = (6, 4, 8), (6, 2, 8), (3, 2, 16, 8)
-        self.masks = torch.zeros(6, 1, dtype=torch.int64)
+        self.masks, self._page_bytes = torch.zeros(6, 1, dtype=torch.int64), 3 * 2 * 16 * 8 * dtype.itemsize
 
     def tensors(self):
         new = lambda shape: torch.zeros(shape, dtype=self.dtype)  # noqa: E731
@@ -263,3 +263,36 @@ def test_serving_refuses_what_needs_a_gradient(name):
     if name == "q":
         with pytest.raises(RuntimeError, match="no gradient"):
             A.paged_tree_afa(plain, t["k_pages"], t["v_pages"], plan, out=out)
+
+
+def test_serving_refuses_shared_places():
+    """Pages that would be written twice, and results over what other workgroups still read."""
+    plan = _StubPlan()
+    t = plan.tensors()
+    append = lambda: _serve(plan, t)[0][1]()  # noqa: E731
+    attend = lambda out: _serve(plan, t, out=out)[1][1]  # noqa: E731
+    for call in (append, attend(torch.zeros(6, 4, 8))):
+        _reaches_the_device(call)
+    n = t["k_pages"].numel()
+    room = torch.zeros(2 * n)
+    apart = room[n:].view(plan._page_shape)
+    t["k_pages"] = room[:n].view(plan._page_shape)
+    for bad in (t["k_pages"], room[8:n + 8].view(plan._page_shape), room[n - 8:2 * n - 8].view(plan._page_shape)):
+        t["v_pages"] = bad
+        with pytest.raises(ValueError, match="overlap"):
+            append()
+    t["v_pages"] = apart
+    _reaches_the_device(append)
+    t["v_pages"] = torch.zeros(3, 1, 16, 8).expand(3, 2, 16, 8)
+    with pytest.raises(ValueError, match="expanded"):
+        append()
+    both = torch.zeros(3, 16, 2, 2, 8)  # keys and values side by side share no place
+    t["k_pages"], t["v_pages"] = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    _reaches_the_device(append)
+    t["v_pages"] = t["k_pages"]
+    with pytest.raises(ValueError, match="overlap"):
+        append()
+    t["k_pages"], t["v_pages"] = room[:n].view(plan._page_shape), apart
+    for at in (0, n - 1, 2 * n - 192):
+        with pytest.raises(ValueError, match="overlap"):
+            attend(room[at:at + 192].view(6, 4, 8))()
