@@ -13,7 +13,6 @@ import struct
 import threading
 
 import torch
-from torch.autograd import forward_ad
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "_build", "libafa_hip.so")
@@ -132,11 +131,6 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)
-
-
-def in_forward_mode() -> bool:
-    """Whether a forward-mode level is open, in which an input may carry a tangent."""
-    return getattr(forward_ad, "_current_level", 0) >= 0
 
 
 _HERE = contextlib.nullcontext()

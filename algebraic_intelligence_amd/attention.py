@@ -13,6 +13,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -487,7 +488,8 @@ class _RotateAxes(torch.autograd.Function):
 
 
 def _rotate_axes(q, k, c, s, positions, cfg, transpose):
-    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or _lib.in_forward_mode():
+    # within a forward-mode level an input may carry a tangent, which autograd refuses
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or forward_ad._current_level >= 0:
         return _RotateAxes.apply(q, k, c, s, positions, cfg, transpose)
     y, z = _axes_launch(q, k, c, s, positions, cfg, transpose)
     return y if k is None else (y, z)

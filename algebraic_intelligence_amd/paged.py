@@ -121,6 +121,7 @@ class DraftPlan:
         self._q_shape = (self.max_tokens, self.heads, self.head_dim)
         self._kv_shape = (self.max_tokens, self.kv_heads, self.head_dim)
         self._page_shape = (pool.num_pages, self.kv_heads, pool.page_size, self.head_dim)
+        self._q_bytes = self.max_tokens * self.heads * self.head_dim * dtype.itemsize
         self._page_bytes = pool.num_pages * self.kv_heads * pool.page_size * self.head_dim * dtype.itemsize
         self._len_shape = (pool.max_requests,)
         c = self._c = _Plan(num_pages=pool.num_pages, page_size=pool.page_size, requests=pool.max_requests,
@@ -191,23 +192,24 @@ def build_block_tables(plan: DraftPlan, cached_lens: torch.Tensor, new_lens: tor
     return plan
 
 
-def _inference_only(name, *tensors):
-    """Refuses tensors that a derivative is asked of, which the call's result would not have."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
-    if _lib.in_forward_mode():
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{name} has no derivative, and a tensor carries a tangent")
+def _no_gradient(name):
+    raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
+
+
+def _no_tangents(name, *tensors):
+    """Refuses tensors that carry a tangent, within a forward-mode level."""
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no derivative, and a tensor carries a tangent")
 
 
 def _pages(plan, k_pages, v_pages):
     """Strides of the pages (page, head, slot of k, then of v), None where both are contiguous."""
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != plan.dtype or t.shape != plan._page_shape or t.device != plan.device:
-            _refuse(plan, name, t, plan._page_shape)
+    dt, shape, dev = plan.dtype, plan._page_shape, plan.device
+    if k_pages.dtype != dt or k_pages.shape != shape or k_pages.device != dev:
+        _refuse(plan, "k_pages", k_pages, shape)
+    if v_pages.dtype != dt or v_pages.shape != shape or v_pages.device != dev:
+        _refuse(plan, "v_pages", v_pages, shape)
     if k_pages.is_contiguous() and v_pages.is_contiguous():
         return None
     k, v = k_pages.stride(), v_pages.stride()
@@ -217,10 +219,15 @@ def _pages(plan, k_pages, v_pages):
 
 
 def _rows(plan, name, t, shape):
-    """t of the plan's dtype and device, of shape (max_tokens, heads, head_dim), with a contiguous head dimension."""
+    """t, of the plan's dtype and device and of shape (max_tokens, heads, head_dim), with a contiguous head dimension,
+    and its strides."""
     if t.dtype != plan.dtype or t.shape != shape or t.device != plan.device:
         _refuse(plan, name, t, shape)
-    return t if t.stride(2) == 1 or plan.head_dim == 1 else t.contiguous()
+    at = t.stride()
+    if at[2] != 1 and plan.head_dim != 1:
+        t = t.contiguous()
+        at = t.stride()
+    return t, at
 
 
 def _like_rows(q):
@@ -229,28 +236,17 @@ def _like_rows(q):
     return y if y.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
-def _span(t):
-    """First byte of t and the one behind its last."""
-    n = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + n * t.element_size()
-
-
-def _overlap(a, b):
-    """Whether the address ranges of a and b meet."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
-
-
-def _own_places(plan, k_pages, v_pages, contiguous):
-    """Refuses pages in which two of a step's rows would be written to one place, as far as addresses and
-    strides tell."""
-    apart = abs(k_pages.data_ptr() - v_pages.data_ptr())
-    if apart < plan._page_bytes if contiguous else apart == 0:
-        raise ValueError("k_pages and v_pages must not overlap")
+def _meet(out, t, contiguous, out_bytes, bytes_):
+    """Whether the address ranges of out, which is contiguous, and t meet."""
+    a, b = out.data_ptr(), t.data_ptr()
     if not contiguous:
-        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
-                raise ValueError(f"{name} must not be an expanded tensor")
+        bytes_ = t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+    return a < b + bytes_ and b < a + out_bytes
+
+
+def _expanded(name, t):
+    if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be an expanded tensor")
 
 
 def _refuse(plan, name, t, shape):
@@ -274,10 +270,21 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
     without a slot are not stored.  The pages hold k and v in places of their own, apart from q, k and v.
     For inference: inputs that require a gradient are refused where gradients are recorded."""
-    _inference_only("append_to_cache", q, k, v, k_pages, v_pages)
-    q, k, v = _rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape), _rows(plan, "v", v, plan._kv_shape)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
+                                    or v_pages.requires_grad):
+        _no_gradient("append_to_cache")
+    if forward_ad._current_level >= 0:
+        _no_tangents("append_to_cache", q, k, v, k_pages, v_pages)
+    (q, sq), (k, sk), (v, sv) = (_rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape),
+                                 _rows(plan, "v", v, plan._kv_shape))
     page_strides = _pages(plan, k_pages, v_pages)
-    _own_places(plan, k_pages, v_pages, page_strides is None)
+    # two of a step's rows must not be written to one place, as far as addresses and strides tell
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if kp == vp or (page_strides is None and abs(kp - vp) < plan._page_bytes):
+        raise ValueError("k_pages and v_pages must not overlap")
+    if page_strides is not None:
+        _expanded("k_pages", k_pages)
+        _expanded("v_pages", v_pages)
     dev = plan.device
     c = s = None
     axes, cuts = 1, None
@@ -294,11 +301,11 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
         raise ValueError("positions and sections need rotary_params")
     strides = None
     if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
-        strides = _lib.pack6(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        strides = _lib.pack6(sq[0], sq[1], sk[0], sk[1], sv[0], sv[1])
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_append(
             plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, None if c is None else q_out.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+            kp, vp, page_strides, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
             _lib.ptr(positions), axes, cuts, _lib.stream_ptr(dev))
     _lib.check(rc, "afa_paged_append")
     return q_out
@@ -318,10 +325,14 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     that it sees is its result in that feature.  Rows behind the last request's are 0, or left as they
     were where ``out`` is given.  For inference: tensors that require a gradient are refused where gradients
     are recorded."""
-    _inference_only("paged_tree_afa", q, k_pages, v_pages)
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
-    q = _rows(plan, "q", q, plan._q_shape)
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or (out is not None and out.requires_grad)):
+        _no_gradient("paged_tree_afa")
+    if forward_ad._current_level >= 0:
+        _no_tangents("paged_tree_afa", q, k_pages, v_pages)
+    q, sq = _rows(plan, "q", q, plan._q_shape)
     page_strides = _pages(plan, k_pages, v_pages)
     dev = plan.device
     if masks is not None:
@@ -330,21 +341,21 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         if masks.dtype != torch.int64 or masks.shape != plan.masks.shape or masks.device != dev:
             raise ValueError(f"masks must be int64 of shape {tuple(plan.masks.shape)} on {dev}")
         masks = masks.contiguous()
+    strides = None if q.is_contiguous() else _lib.pack2(sq[0], sq[1])
     flags = 0
     if out is None:
-        out = _like_rows(q)
+        out = torch.empty_like(q) if strides is None else _like_rows(q)
         flags = _lib.FLAG_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous, of shape {tuple(q.shape)}, {q.dtype} on {dev}")
-    elif _overlap(out, q) or _overlap(out, k_pages) or _overlap(out, v_pages):
+    elif (_meet(out, q, strides is None, plan._q_bytes, plan._q_bytes)
+          or _meet(out, k_pages, page_strides is None, plan._q_bytes, plan._page_bytes)
+          or _meet(out, v_pages, page_strides is None, plan._q_bytes, plan._page_bytes)):
         raise ValueError("out must not overlap q, k_pages or v_pages")
-    else:
-        _inference_only("paged_tree_afa", out)
     den = None
     if return_denominator:
         new = torch.empty if flags else torch.zeros
         den = new((plan.max_tokens, plan.heads), dtype=_lib.accum_dtype(q.dtype), device=dev)
-    strides = None if q.is_contiguous() else _lib.pack2(q.stride(0), q.stride(1))
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_fwd(
             plan._ref, q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(masks),

@@ -212,7 +212,8 @@ class _StubPlan:
     def __init__(self, dtype=torch.float32):
         self.dtype, self.device, self.head_dim, self.max_tree, self.max_tokens, self.heads = dtype, torch.device("cpu"), 8, 64, 6, 4
         self._q_shape, self._kv_shape, self._page_shape = (6, 4, 8), (6, 2, 8), (3, 2, 16, 8)
-        self.masks, self._page_bytes = torch.zeros(6, 1, dtype=torch.int64), 3 * 2 * 16 * 8 * dtype.itemsize
+        self.masks = torch.zeros(6, 1, dtype=torch.int64)
+        self._q_bytes, self._page_bytes = 6 * 4 * 8 * dtype.itemsize, 3 * 2 * 16 * 8 * dtype.itemsize
 
     def tensors(self):
         new = lambda shape: torch.zeros(shape, dtype=self.dtype)  # noqa: E731
