@@ -127,25 +127,28 @@ def test_cached_values_that_are_not_finite(dt, H, K, n, cached, D):
 
 @pytest.mark.parametrize("dt", [BF16, F32, F64])
 @pytest.mark.parametrize("H,K,n", ROWS)
-def test_scores_far_below_zero(dt, H, K, n):
-    """A key whose score's eighth power, and whose square, no longer fit weighs nothing, as one of score -26250
-    does (2^-125 beside weights of about 1): the same results bit for bit.  Its infinity is seen all the same."""
-    x = _Cache(dt, [(40, n), (0, 3)], H, K, 64, 16, seed=n)
+@pytest.mark.parametrize("D,page", [(64, 16), (40, 5)])
+def test_scores_far_below_zero(dt, H, K, n, D, page):
+    """A key whose score's eighth power, and whose square, no longer fit weighs nothing, as one of score -26250 or
+    -33200 does (2^-125 or less beside weights of about 1): the same results bit for bit.  Its infinity is
+    seen all the same."""
+    x = _Cache(dt, [(40, n), (0, 3)], H, K, D, page, seed=n)
     x.q[..., 0] = 300.0
-    _set_keys(x, 16, lambda k: torch.cat((torch.zeros_like(k[..., :1]), k[..., 1:]), -1))
-    at = x.kp[x.tables[0][0], :, 7]
+    _set_keys(x, page, lambda k: torch.cat((torch.zeros_like(k[..., :1]), k[..., 1:]), -1))
+    where, slot = x.tables[0][7 // page], 7 % page
+    at = x.kp[where, :, slot]
     at.zero_()
     at[:, 0] = -700.0
-    x.vp[x.tables[0][0], :, 7, 1] = 1.0
+    x.vp[where, :, slot, 1] = 1.0
     want = _run(x)
     assert all(torch.isfinite(t).all() for t in want)
     for k in (-1200.0, -1e6, -3e30):
         at[:, 0] = k
         for got, ref in zip(_run(x), want):
             assert torch.equal(got, ref), k
-        x.vp[x.tables[0][0], :, 7, 1] = float("inf")
+        x.vp[where, :, slot, 1] = float("inf")
         out, _ = _run(x)
         assert (out[:n, :, 1] == float("inf")).all()
         out[:n, :, 1] = want[0][:n, :, 1]
         assert torch.equal(out, want[0])
-        x.vp[x.tables[0][0], :, 7, 1] = 1.0
+        x.vp[where, :, slot, 1] = 1.0
