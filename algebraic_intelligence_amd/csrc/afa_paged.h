@@ -17,8 +17,10 @@ constexpr int kMaxAxes = 4;
 // A segment is one request's query rows of one block (up to `rows` of its new tokens * group) over all of its
 // keys.  Laid end to end, a segment taking kPagedLead units and one for each of its key tiles, the segments
 // of a key/value head form a line that is cut into `slots` even stretches, one for each workgroup.  Every
-// workgroup so has the same work whatever the lengths; a segment that a cut crosses ends as partial sums,
-// at most two of a slot: of a segment that began earlier and of one that goes on.
+// workgroup so has the same units.  Trees and rows of one block have a tile of work in each.  In a chain of
+// several blocks (a prompt) the units of a block behind its last token's keys are empty, on an empty cache about
+// half of them: there the workgroups of the last blocks have up to twice the mean work.  A segment that a cut
+// crosses ends as partial sums, at most two of a slot: of a segment that began earlier and of one that goes on.
 struct PagedCut {
   int rows;
   int64_t slots;  // per key/value head

@@ -25,8 +25,9 @@
 // joined by adding numerators and denominators in a fixed order (LDS; fp32 parts that the last workgroup of a
 // row block to finish adds up).
 //
-// Weights are the B operand in two planes of the type (w = hi + lo), so no rounding of w is left in
-// the result (the matrix cores idle beside the loads); the row sums are fp32.  fp16 ends at 65504: there
+// Weights are the B operand in two planes of the type (w = hi + lo), so that what is left of their rounding is
+// its square.  With few rows the second plane is free, as the matrix cores idle beside the loads; with 128 rows
+// it is 16 of a tile's 48 products, and is kept all the same.  The row sums are fp32.  fp16 ends at 65504: there
 // a row's weights are scaled by a power of two, lowered when a larger weight comes (kFirstScale).
 //
 // HBM bound where requests are many or long.  96 requests of one token over up to 4096 cached, 16 heads of 64,

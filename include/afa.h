@@ -328,7 +328,8 @@ int afa_paged_build(const afa_paged_plan* plan, const int32_t* cached, const int
  * Rotates q and k of the step's tokens and stores k and v at the tokens' slots (a token without a
  * slot is not stored).  q (max_tokens, heads, head_dim), k and v (max_tokens, kv_heads, head_dim) with
  * strides {q_t, q_h, k_t, k_h, v_t, v_h} in elements (NULL: contiguous); q_out contiguous, nullable
- * without tables.  page_strides {k_page, k_head, k_slot, v_page, v_head, v_slot} (NULL: contiguous).
+ * without tables.  page_strides {k_page, k_head, k_slot, v_page, v_head, v_slot} (NULL: contiguous); no two
+ * places of the pages share memory, nor do they with q, k, v and q_out.
  * rot_cos, rot_sin (rot_len, head_dim / 2) in fp32 (fp64 for AFA_F64), nullable: no rotation.
  * positions (max_tokens, axes) or NULL for the plan's (axes 1); sections: as in ago_rotate_axes.
  */
@@ -342,7 +343,8 @@ int afa_paged_append(const afa_paged_plan* plan, const void* q, const void* k, c
  * with strides {q_t, q_h} (NULL: contiguous); masks: nullable, the plan's; out and denom (nullable,
  * (max_tokens, heads), accumulation type) contiguous.  A row without a visible key is 0; an infinity or a
  * NaN in a value that a row sees is its result in that feature.  Rows behind the last request's are left
- * as they were, or with AFA_FLAG_ZERO_TAIL set to 0.  A page id outside the pool holds no keys.
+ * as they were, or with AFA_FLAG_ZERO_TAIL set to 0.  A page id outside the pool holds no keys.  out and
+ * denom share no memory with q and the pages.
  * workspace: afa_paged_workspace_size() bytes, 16-byte aligned, or NULL.
  */
 #define AFA_FLAG_ZERO_TAIL 0x400u
