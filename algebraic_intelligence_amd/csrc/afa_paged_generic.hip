@@ -58,9 +58,9 @@ __global__ __launch_bounds__(ROW_KEYS) void afa_paged_row_kernel(const PagedFwdA
       for (int d = 0; d < D; ++d) s += q_row[d] * elem<DT, A>(a.k_pages, k + d);
       if constexpr (DT == AFA_F64) w = rho8_f64(s * a.scale);
       else w = rho8_ref(s * (float)a.scale);
-      // above 0 as its formula is, so that a value that is not finite is seen
+      // above 0 as its formula is, so that a value that is not finite is seen; the NaN of a score of -infinity too
       constexpr A LEAST = DT == AFA_F64 ? (A)0x1p-1022 : (A)0x1p-126f;
-      w = w < LEAST ? LEAST : w;
+      if (s < 0 && !(w >= LEAST)) w = LEAST;
       sum += w;
       row[tid] = page * a.ps.v_page + hk * a.ps.v_head + at * a.ps.v_slot;
     } else {

@@ -125,13 +125,13 @@ def test_cached_values_that_are_not_finite(dt, H, K, n, cached, D):
     assert torch.equal(out[~nan], want[~nan])
 
 
-@pytest.mark.parametrize("dt", [BF16, F32, F64])
+@pytest.mark.parametrize("dt", [BF16, F16, F32, F64])
 @pytest.mark.parametrize("H,K,n", ROWS)
 @pytest.mark.parametrize("D,page", [(64, 16), (40, 5)])
 def test_scores_far_below_zero(dt, H, K, n, D, page):
     """A key whose score's eighth power, and whose square, no longer fit weighs nothing, as one of score -26250 or
     -33200 does (2^-125 or less beside weights of about 1): the same results bit for bit.  Its infinity is
-    seen all the same."""
+    seen all the same.  A score of -infinity is the last of them; one of infinity or NaN makes its rows NaN."""
     x = _Cache(dt, [(40, n), (0, 3)], H, K, D, page, seed=n)
     x.q[..., 0] = 300.0
     _set_keys(x, page, lambda k: torch.cat((torch.zeros_like(k[..., :1]), k[..., 1:]), -1))
@@ -142,7 +142,7 @@ def test_scores_far_below_zero(dt, H, K, n, D, page):
     x.vp[where, :, slot, 1] = 1.0
     want = _run(x)
     assert all(torch.isfinite(t).all() for t in want)
-    for k in (-1200.0, -1e6, -3e30):
+    for k in (-1200.0, -1e6, -3e30, float("-inf")):
         at[:, 0] = k
         for got, ref in zip(_run(x), want):
             assert torch.equal(got, ref), k
@@ -152,3 +152,8 @@ def test_scores_far_below_zero(dt, H, K, n, D, page):
         out[:n, :, 1] = want[0][:n, :, 1]
         assert torch.equal(out, want[0])
         x.vp[where, :, slot, 1] = 1.0
+    for k in (float("inf"), float("nan")):
+        at[:, 0] = k
+        out, den = _run(x)
+        assert torch.isnan(out[:n]).all() and not torch.isfinite(den[:n]).any()
+        assert torch.equal(out[n:], want[0][n:])
