@@ -58,6 +58,20 @@ SIGNATURES = {
     "afa_paged_append": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp, _vp]),
     "afa_paged_workspace_size": (_sz, [_vp]),
     "afa_paged_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _uint, _vp, _sz, _vp]),
+    "ago_norm_rotate_axes": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _vp, _vp,
+                                    _i64, _vp, _int, _i64, _int, _vp, _vp]),
+    "ago_norm_rotate_axes_bwd_workspace_size": (_sz, [_int, _i64]),
+    "ago_norm_rotate_axes_bwd": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _vp, _vp, _dbl, _vp, _vp, _i64, _vp, _int, _i64, _int, _vp, _vp, _sz, _vp]),
+    "afa_paged_append_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _vp, _vp, _i64, _vp, _int,
+                                     _vp, _vp]),
+    "afa_paged_prefix_workspace_size": (_sz, [_vp, _i64]),
+    "afa_paged_prefix_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _uint, _vp, _sz,
+                                    _vp]),
+    "afa_paged_weights": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "afa_paged_evict_workspace_size": (_sz, [_i64, _i64]),
+    "afa_paged_evict": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
+                               _i64, _vp, _vp, _vp, _sz, _vp]),
     "oace_workspace_size": (_sz, [_int, _i64, _i64, _i64, _int, _uint]),
     "oace_linear_fwd": (_int, [_int, _i64, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _dbl, _dbl, _vp, _vp,
                                _uint, _vp, _sz, _vp]),
@@ -156,7 +170,7 @@ def workspace_size(name: str, device: torch.device, *sizes) -> int:
 
 
 # int64 values, such as strides, as the bytes a C array of them has
-pack2, pack6, pack12 = (struct.Struct(f"{n}q").pack for n in (2, 6, 12))
+pack2, pack3, pack4, pack6, pack12, pack18 = (struct.Struct(f"{n}q").pack for n in (2, 3, 4, 6, 12, 18))
 
 
 def ptr(t):

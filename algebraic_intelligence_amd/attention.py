@@ -14,12 +14,13 @@ from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 __all__ = [
     "octic_kernel", "algebraic_softmax", "CayleyRotary", "build_cayley_rotary_matrix",
-    "apply_ago_rotations", "apply_ago_axis_rotations", "rotate_tensor",
+    "apply_ago_rotations", "apply_ago_axis_rotations", "apply_ago_norm_rotations", "rotate_tensor",
 ]
 
 
@@ -538,3 +539,185 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
     if k is not None and k.numel() == 0:
         return _rotate_axes(q, None, c, s, positions, cfg, 0), k.clone()
     return _rotate_axes(q, k, c, s, positions, cfg, 0)
+
+
+# ------------------------------------------------------------------- norms of q and k with their rotation
+def _norm_scale(name, scale, head_dim, dtype, dev):
+    """A norm's scale in fp32 (fp64 for fp64 inputs), contiguous."""
+    if not isinstance(scale, torch.Tensor) or not scale.is_floating_point():
+        raise TypeError(f"{name} must be a floating point tensor, got {type(scale) if not isinstance(scale, torch.Tensor) else scale.dtype}")
+    if scale.shape != (head_dim,):
+        raise ValueError(f"{name} must have shape ({head_dim},), got {tuple(scale.shape)}")
+    if scale.device != dev:
+        _lib.require_device(scale)
+        raise ValueError(f"{name} must be on {dev}, got {scale.device}")
+    want = torch.float64 if dtype is torch.float64 else torch.float32
+    if scale.dtype is not want:
+        scale = scale.to(want)
+    return scale if scale.is_contiguous() else scale.contiguous()
+
+
+def _norm_eps(eps):
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and nonnegative, got {eps}")
+    return eps
+
+
+class _NormConfig(NamedTuple):
+    """What a norm and its VJP share beside their tensors."""
+
+    axes: _AxesConfig
+    eps: float
+
+
+def _row_layout(x):
+    """x with a contiguous head dimension, an empty tensor like it, and the strides of both."""
+    sx = x.stride()
+    if sx[3] != 1:
+        x = x.contiguous()
+        sx = x.stride()
+    y = torch.empty_like(x)
+    sy = y.stride()
+    if sy[3] != 1:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        sy = y.stride()
+    return x, y, sx, sy
+
+
+def _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg):
+    q, y, sq, sy = _row_layout(q)
+    B, H, L, D = q.shape
+    K, z, kp, zp, sk, sz = 0, None, None, None, sq, sy
+    if k is not None:
+        k, z, sk, sz = _row_layout(k)
+        K, kp, zp = k.shape[1], k.data_ptr(), z.data_ptr()
+    dev, at = q.device, cfg.axes
+    with _lib.on_device(dev):
+        rc = _lib.lib().ago_norm_rotate_axes(
+            at.dtype, B, H, K, L, D, q.data_ptr(), kp, y.data_ptr(), zp,
+            _lib.pack12(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sy[0], sy[1], sy[2], sz[0], sz[1], sz[2]),
+            q_scale.data_ptr(), _lib.ptr(k_scale), cfg.eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+            _lib.ptr(positions), at.pos_bytes, at.pos_b, at.axes, at.cuts, _lib.stream_ptr(dev))
+    _lib.check(rc, "ago_norm_rotate_axes")
+    return y, z
+
+
+def _norm_backward_launch(q, k, gq, gk, q_scale, k_scale, c, s, positions, cfg):
+    q, dq, sq, sdq = _row_layout(q)
+    gq = gq if gq.stride(3) == 1 else gq.contiguous()
+    sgq = gq.stride()
+    B, H, L, D = q.shape
+    acc = {"dtype": q_scale.dtype, "device": q.device}
+    dqs = torch.empty(D, **acc)
+    K, dk, dks, kp, gkp, dkp, sk, sgk, sdk = 0, None, None, None, None, None, sq, sgq, sdq
+    if k is not None:
+        k, dk, sk, sdk = _row_layout(k)
+        gk = gk if gk.stride(3) == 1 else gk.contiguous()
+        sgk, dks = gk.stride(), torch.empty(D, **acc)
+        K, kp, gkp, dkp = k.shape[1], k.data_ptr(), gk.data_ptr(), dk.data_ptr()
+    dev, at = q.device, cfg.axes
+    with _lib.on_device(dev):
+        size = _lib.workspace_size("ago_norm_rotate_axes_bwd_workspace_size", dev, at.dtype, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        rc = _lib.lib().ago_norm_rotate_axes_bwd(
+            at.dtype, B, H, K, L, D, q.data_ptr(), kp, gq.data_ptr(), gkp, dq.data_ptr(), dkp,
+            _lib.pack18(*sq[:3], *sk[:3], *sgq[:3], *sgk[:3], *sdq[:3], *sdk[:3]), q_scale.data_ptr(), _lib.ptr(k_scale),
+            dqs.data_ptr(), _lib.ptr(dks), cfg.eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+            _lib.ptr(positions), at.pos_bytes, at.pos_b, at.axes, at.cuts, ws.data_ptr(), size, _lib.stream_ptr(dev))
+    _lib.check(rc, "ago_norm_rotate_axes_bwd")
+    return dq, dk, dqs, dks
+
+
+class _NormRotate(torch.autograd.Function):
+    """Norm, scale and rotation of q, and of k where there is one; the VJP forms the norm again from q and k."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_scale, k_scale, c, s, positions, cfg):
+        ctx.save_for_backward(q, k, q_scale, k_scale, c, s, positions)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
+        return y if k is None else (y, z)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk=None):
+        q, k, q_scale, k_scale, *rest = ctx.saved_tensors
+        dq = dk = dqs = dks = None
+        if gq is not None and gk is not None:
+            dq, dk, dqs, dks = _norm_backward_launch(q, k, gq, gk, q_scale, k_scale, *rest, ctx.cfg)
+        elif gq is not None:
+            dq, _, dqs, _ = _norm_backward_launch(q, None, gq, None, q_scale, None, *rest, ctx.cfg)
+        elif gk is not None:
+            dk, _, dks, _ = _norm_backward_launch(k, None, gk, None, k_scale, None, *rest, ctx.cfg)
+        return dq, dk, dqs, dks, None, None, None, None
+
+
+def apply_ago_norm_rotations(q, k, q_scale, k_scale, rotary_params=None, positions=None, sections=None, *, eps=1e-6):
+    """q and k normalised head by head, scaled, and turned by the Cayley rotation, in one pass over each:
+    R(m) (scale * x / sqrt(mean(x^2) + eps)), the mean over the head dimension.
+
+    q (B, H, L, D) and k (B, H_kv, L, D) (None, with k_scale None: q alone).  ``q_scale`` and ``k_scale`` (D,): of any floating
+    type, used in fp32 (fp64 for fp64 inputs).  ``rotary_params``, ``positions`` and ``sections`` as in
+    ``apply_ago_axis_rotations``; positions None: a row's index in its sequence; rotary_params None: no rotation, and any D.
+    No counterpart in the reference, whose model (src/model.py:262-275) rotates q and k as they are.
+
+    Returns (q_out, k_out) (q_out alone without k) in the inputs' dtype and axis order.  Everything between is fp32
+    (fp64) with one rounding: a row whose mean square passes fp32's range gives 0 where it is finite.  Differentiable once, in
+    reverse mode, with respect to q, k and both scales, whose gradients are summed in a fixed order."""
+    q = _float_input(q)
+    shape = q.shape
+    if len(shape) != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != shape[0] or k.shape[2:] != shape[2:])):
+        raise ValueError("q and k must have shapes (batch, heads, sequence, dimension), alike but for the heads, got "
+                         f"{tuple(shape)} and {None if k is None else tuple(k.shape)}")
+    if (k is None) != (k_scale is None):
+        raise ValueError("k and k_scale come together")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"q and k must share a dtype, got {q.dtype} and {k.dtype}")
+    B, _, L, D = shape
+    dt = _lib.dtype_code(q.dtype)
+    dev = _lib.require_device(q, k)
+    eps = _norm_eps(eps)
+    if D == 0:
+        raise ValueError("the norm needs at least one feature")
+    q_scale = _norm_scale("q_scale", q_scale, D, q.dtype, dev)
+    k_scale = None if k is None else _norm_scale("k_scale", k_scale, D, q.dtype, dev)
+    c = s = cuts = None
+    axes, pos_bytes, pos_b = 1, 4, 0
+    if rotary_params is None:
+        if positions is not None or sections is not None:
+            raise ValueError("positions and sections need rotary_params")
+    else:
+        if D % 2 != 0:
+            raise ValueError(f"Feature dimension must be even, got {D}")
+        c, s = _axis_tables(rotary_params, D, q.dtype, dev)
+        if positions is not None:
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+            at = positions.shape
+            if len(at) not in (2, 3) or at[-2] != L or (len(at) == 3 and at[0] not in (1, B)):
+                raise ValueError(f"positions must have shape ({B}, {L}, axes) or ({L}, axes), got {tuple(at)}")
+            _lib.require_device(q, positions)
+            axes, pos_bytes = at[-1], positions.element_size()
+            pos_b = L * axes if len(at) == 3 and at[0] > 1 else 0
+            positions = positions.contiguous()
+        cuts = _axis_sections(sections, axes, D // 2)
+    cfg = _NormConfig(_AxesConfig(dt, pos_bytes, pos_b, axes, cuts), eps)
+
+    def run(q, k, q_scale, k_scale):
+        grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_scale, k_scale))
+        # within a forward-mode level an input may carry a tangent, which autograd refuses
+        if grads or forward_ad._current_level >= 0:
+            return _NormRotate.apply(q, k, q_scale, k_scale, c, s, positions, cfg)
+        y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
+        return y if k is None else (y, z)
+
+    if q.numel() != 0 and (k is None or k.numel() != 0):
+        return run(q, k, q_scale, k_scale)
+    # tensors without rows, whose gradients are as empty
+    none = lambda x, scale: x * scale.to(x.dtype)  # noqa: E731
+    y = none(q, q_scale) if q.numel() == 0 else run(q, None, q_scale, None)
+    if k is None:
+        return y
+    return y, none(k, k_scale) if k.numel() == 0 else run(k, None, k_scale, None)

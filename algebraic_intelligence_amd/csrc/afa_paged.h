@@ -121,6 +121,13 @@ struct AppendArgs {
 };
 hipError_t paged_append_launch(int dtype, const AppendArgs& a, hipStream_t st);
 
+// Keys and values that all requests of a call see before their own: (kv_heads, len, head_dim).
+struct PrefixKeys {
+  const void *k, *v;
+  int64_t k_head, k_key, v_head, v_key;
+  int len;  // 0: none
+};
+
 struct PagedFwdArgs {
   afa_paged_plan plan;
   PagedSchedule sched;
@@ -132,12 +139,44 @@ struct PagedFwdArgs {
   void* denom;           // nullable
   double scale, omega;
   int group, zero_tail;
+  PrefixKeys prefix;
 };
 hipError_t paged_fwd_generic_launch(const PagedFwdArgs& a, hipStream_t st);
 // Matrix-core path (afa_paged_mfma.hip): 16-byte aligned rows of q, pages and out.  ws: paged_fast_workspace bytes.
 bool paged_fast_supported(const afa_paged_plan& p);
 size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c);
 hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, void* ws, hipStream_t st);
+
+// What each cached token was given by the step's rows (afa_paged_weights.hip).
+struct WeightArgs {
+  afa_paged_plan plan;
+  PagedSchedule sched;
+  const void *q, *k_pages;
+  const int64_t* masks;  // nullptr: no trees
+  const void* denom;     // (max_tokens, heads), accumulation type
+  int64_t q_t, q_h, k_page, k_head, k_slot;
+  float* weights;        // (requests, row stride)
+  int64_t row;
+  double scale;
+  int group;
+};
+hipError_t paged_weights_launch(const WeightArgs& a, int cus, hipStream_t st);
+
+// Requests cut back to a budget of tokens (afa_paged_evict.hip).
+struct EvictArgs {
+  int64_t num_pages, page_size, requests, table_width, kv_heads, head_dim;
+  const int32_t *block_tables, *held, *cached;
+  void *k_pages, *v_pages;
+  PageStrides ps;
+  const float* weights;  // (requests, row stride)
+  int64_t row;
+  float* left;           // (requests, table_width * page_size)
+  int32_t* lens;
+  int32_t* kept;         // workspace: (requests, budget) indexes, then the requests' first moved place
+  int budget, first, recent, esz;
+};
+size_t paged_evict_workspace(int64_t requests, int64_t budget);
+hipError_t paged_evict_launch(const EvictArgs& a, hipStream_t st);
 
 struct RotateAxesArgs {
   const void *x[2];
@@ -151,6 +190,29 @@ struct RotateAxesArgs {
   float sign;
 };
 hipError_t rotate_axes_launch(int dtype, const RotateAxesArgs& a, hipStream_t st);
+
+// Norm of q's and k's rows with their rotation (ago_norm.hip).  Scales are fp32 (fp64 for AFA_F64).
+struct HeadNorm {
+  const void* scale[2];  // of q and of k, (dim,)
+  double eps;
+};
+struct NormArgs {
+  const void *x[2];
+  const void *g[2];        // backward: the results' cotangents
+  void* y[2];              // results, or x's gradients
+  int64_t sx[2][3], sg[2][3], sy[2][3];  // b, h, l
+  int heads[2];
+  int64_t batch, seq;
+  int dim;
+  HeadNorm norm;
+  AxisRotation rot;
+  int64_t pos_b;
+};
+hipError_t norm_rotate_launch(int dtype, const NormArgs& a, hipStream_t st);
+// dscale: of q and of k, fp32 (fp64), (dim,); ws: norm_rotate_bwd_workspace bytes
+size_t norm_rotate_bwd_workspace(int dtype, int dim, int cus);
+hipError_t norm_rotate_bwd_launch(int dtype, const NormArgs& a, void* const dscale[2], void* ws, int cus, hipStream_t st);
+hipError_t paged_append_norm_launch(int dtype, const AppendArgs& a, const HeadNorm& n, hipStream_t st);
 
 // The axis whose section holds pair p, or -1 behind the last section.
 __host__ __device__ inline int pair_axis(const AxisRotation& r, int p) {

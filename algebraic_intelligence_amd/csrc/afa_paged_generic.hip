@@ -3,7 +3,8 @@
 //
 //   out = sum_j w_j v_j / (sum_j w_j + Omega),  w_j = rho(q.k_j / sqrt(D))^8
 //
-// over the cached keys and the drafted ones that the token's mask shows.  The sums are additive, so keys
+// over the keys of a prefix that all requests share, where there is one, the cached keys and the drafted ones that
+// the token's mask shows.  The sums are additive, so keys
 // go by in blocks of one key a thread with no running maximum; a masked key is left out of both sums,
 // whatever its page holds.  Latency bounds it (a key row a thread, 126 us for one token over 700 in 12 heads of
 // 64); it is here for the calls that the matrix-core kernel does not take, and to check that one.
@@ -25,8 +26,9 @@ __device__ __forceinline__ A elem(const void* p, int64_t i) {
 template <int DT>
 __global__ __launch_bounds__(ROW_KEYS) void afa_paged_row_kernel(const PagedFwdArgs a) {
   using A = typename std::conditional<DT == AFA_F64, double, float>::type;
+  constexpr int ESZ = DT == AFA_F64 ? 8 : DT == AFA_F32 ? 4 : 2;
   __shared__ A q_row[MAX_DIM], weight[ROW_KEYS];
-  __shared__ int64_t row[ROW_KEYS];  // the key's v row, -1 where it is masked
+  __shared__ const char* row[ROW_KEYS];  // the key's v row, nullptr where it is masked
   const afa_paged_plan& p = a.plan;
   const int D = (int)p.head_dim, H = (int)p.heads, tid = threadIdx.x;
   const int64_t t = blockIdx.x / H;
@@ -40,39 +42,52 @@ __global__ __launch_bounds__(ROW_KEYS) void afa_paged_row_kernel(const PagedFwdA
   const bool tree = a.masks != nullptr && n <= p.max_tree;
   for (int d = tid; d < D; d += ROW_KEYS) q_row[d] = elem<DT, A>(a.q, t * a.q_t + h * a.q_h + d);
   A acc[MAX_DIM / ROW_KEYS] = {}, sum = 0;
-  for (int base = 0; base < keys; base += ROW_KEYS) {
-    __syncthreads();
-    const int pos = base + tid;
-    bool sees = pos < keys;
-    if (sees && pos >= c) {
+  // `count` keys, of which locate(pos, k, v) gives the rows, or leaves nullptr
+  auto meet = [&](int count, auto locate) {
+    for (int base = 0; base < count; base += ROW_KEYS) {
+      __syncthreads();
+      const int pos = base + tid;
+      const char *k = nullptr, *v = nullptr;
+      if (pos < count) locate(pos, k, v);
+      A w = 0;
+      if (k != nullptr) {
+        A s = 0;
+        for (int d = 0; d < D; ++d) s += q_row[d] * elem<DT, A>(k, d);
+        if constexpr (DT == AFA_F64) w = rho8_f64(s * a.scale);
+        else w = rho8_ref(s * (float)a.scale);
+        // above 0 as its formula is, so that a value that is not finite is seen; the NaN of a score of -infinity too
+        constexpr A LEAST = DT == AFA_F64 ? (A)0x1p-1022 : (A)0x1p-126f;
+        if (s < 0 && !(w >= LEAST)) w = LEAST;
+        sum += w;
+      }
+      row[tid] = v;
+      weight[tid] = w;
+      __syncthreads();
+      const int m = min(ROW_KEYS, count - base);
+      for (int d = tid, u = 0; d < D; d += ROW_KEYS, ++u)
+        for (int j = 0; j < m; ++j)
+          if (row[j] != nullptr) acc[u] += weight[j] * elem<DT, A>(row[j], d);
+    }
+  };
+  if (live && a.prefix.len > 0) {
+    const PrefixKeys& x = a.prefix;
+    meet(x.len, [&](int pos, const char*& k, const char*& v) {
+      k = (const char*)x.k + (hk * x.k_head + pos * x.k_key) * ESZ;
+      v = (const char*)x.v + (hk * x.v_head + pos * x.v_key) * ESZ;
+    });
+  }
+  meet(keys, [&](int pos, const char*& k, const char*& v) {
+    bool sees = true;
+    if (pos >= c) {
       const int j = pos - c;
       sees = tree ? (a.masks[t * W + j / 64] >> (j & 63)) & 1 : j <= i;
     }
     const int page = sees ? p.block_tables[r * p.table_width + pos / p.page_size] : -1;
-    sees = page >= 0 && page < p.num_pages;
-    A w = 0;
-    if (sees) {
-      const int64_t at = pos % p.page_size;
-      const int64_t k = page * a.ps.k_page + hk * a.ps.k_head + at * a.ps.k_slot;
-      A s = 0;
-      for (int d = 0; d < D; ++d) s += q_row[d] * elem<DT, A>(a.k_pages, k + d);
-      if constexpr (DT == AFA_F64) w = rho8_f64(s * a.scale);
-      else w = rho8_ref(s * (float)a.scale);
-      // above 0 as its formula is, so that a value that is not finite is seen; the NaN of a score of -infinity too
-      constexpr A LEAST = DT == AFA_F64 ? (A)0x1p-1022 : (A)0x1p-126f;
-      if (s < 0 && !(w >= LEAST)) w = LEAST;
-      sum += w;
-      row[tid] = page * a.ps.v_page + hk * a.ps.v_head + at * a.ps.v_slot;
-    } else {
-      row[tid] = -1;
-    }
-    weight[tid] = w;
-    __syncthreads();
-    const int m = min(ROW_KEYS, keys - base);
-    for (int d = tid, u = 0; d < D; d += ROW_KEYS, ++u)
-      for (int j = 0; j < m; ++j)
-        if (row[j] >= 0) acc[u] += weight[j] * elem<DT, A>(a.v_pages, row[j] + d);
-  }
+    if (page < 0 || page >= p.num_pages) return;
+    const int64_t at = pos % p.page_size;
+    k = (const char*)a.k_pages + (page * a.ps.k_page + hk * a.ps.k_head + at * a.ps.k_slot) * ESZ;
+    v = (const char*)a.v_pages + (page * a.ps.v_page + hk * a.ps.v_head + at * a.ps.v_slot) * ESZ;
+  });
   __syncthreads();
   weight[tid] = sum;
   __syncthreads();

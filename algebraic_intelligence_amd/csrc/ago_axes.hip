@@ -12,29 +12,11 @@
 
 #include "afa_common.h"
 #include "afa_paged.h"
+#include "ago_turn.h"
 
 namespace afa {
 
 namespace {
-
-__device__ __forceinline__ int64_t position(const AxisRotation& r, int64_t i) {
-  return r.pos64 ? ((const int64_t*)r.positions)[i] : ((const int32_t*)r.positions)[i];
-}
-
-// One pair by the table entries of position m of its axis; NaN where the tables have no such row.
-template <typename T>
-__device__ __forceinline__ void turn(const AxisRotation& r, int64_t m, int p, T sign, T x0, T x1, T& y0, T& y1) {
-#pragma clang fp contract(off)
-  T c, s;
-  if (m >= 0 && m < r.len) {
-    c = ((const T*)r.rc)[m * r.pairs + p];
-    s = ((const T*)r.rs)[m * r.pairs + p] * sign;
-  } else {
-    c = s = (T)__builtin_nanf("");
-  }
-  y0 = c * x0 - s * x1;
-  y1 = s * x0 + c * x1;
-}
 
 // One thread a pair, q's rows before k's: fp64, rows that are no whole 16-byte chunks, and any alignment.
 template <int DT>
@@ -64,58 +46,6 @@ __global__ __launch_bounds__(256) void ago_axes_kernel(const RotateAxesArgs a, i
   }
 }
 
-// The same in 16-byte chunks: a thread owns one chunk of a token's rows, holds its table entries and turns
-// it in up to HG heads, `groups` apart, whose loads are in flight together.  Where the heads of a token lie
-// nearer to one another than its neighbours do, lanes run over heads before tokens, so that a wave's
-// accesses stay whole lines side by side either way.
-template <int DT>
-struct ChunkTurn {
-  using R = RowChunk<DT>;
-  static constexpr int NP = R::EPC / 2;
-  float c[NP], s[NP];
-  bool keep[NP];
-
-  __device__ __forceinline__ void load(const AxisRotation& r, int64_t token, int p0, float sign) {
-    const int first = pair_axis(r, p0), last = pair_axis(r, p0 + NP - 1);
-    if (first == last && first >= 0 && r.wide) {
-      const int64_t m = position(r, token + first), at = m * r.pairs + p0;
-      const bool in = m >= 0 && m < r.len;
-      typedef __attribute__((ext_vector_type(NP))) float vec;
-      const vec nan = __builtin_nanf("");
-      const vec cv = in ? *(const vec*)((const float*)r.rc + at) : nan, sv = in ? *(const vec*)((const float*)r.rs + at) : nan;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        c[p] = cv[p];
-        s[p] = sv[p] * sign;
-        keep[p] = false;
-      }
-      return;
-    }
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int axis = pair_axis(r, p0 + p);
-      const int64_t m = axis < 0 ? 0 : position(r, token + axis), at = m * r.pairs + p0 + p;
-      const bool in = m >= 0 && m < r.len;
-      keep[p] = axis < 0;
-      c[p] = in ? ((const float*)r.rc)[at] : __builtin_nanf("");
-      s[p] = in ? ((const float*)r.rs)[at] * sign : __builtin_nanf("");
-    }
-  }
-
-  __device__ __forceinline__ u32x4_t turned(u32x4_t w) const {
-#pragma clang fp contract(off)
-    float v[R::EPC];
-    R::unpack(w, v);
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const float x0 = v[2 * p], x1 = v[2 * p + 1];
-      v[2 * p] = keep[p] ? x0 : c[p] * x0 - s[p] * x1;
-      v[2 * p + 1] = keep[p] ? x1 : s[p] * x0 + c[p] * x1;
-    }
-    return R::pack(v);
-  }
-};
-
 // Thread i of tokens * groups * chunks: its chunk of a row, its token and its first head.
 struct ChunkPlace {
   uint32_t chunk, token, group;
@@ -130,6 +60,10 @@ __device__ __forceinline__ ChunkPlace chunk_place(const ChunkGrid& g, uint32_t i
   return ChunkPlace{i - rest * g.chunks, g.heads_inner ? out : in, g.heads_inner ? in : out};
 }
 
+// The same in 16-byte chunks: a thread owns one chunk of a token's rows, holds its table entries and turns
+// it in up to HG heads, `groups` apart, whose loads are in flight together.  Where the heads of a token lie
+// nearer to one another than its neighbours do, lanes run over heads before tokens, so that a wave's
+// accesses stay whole lines side by side either way.
 template <int DT, int HG, bool STREAM>
 __global__ __launch_bounds__(256) void ago_axes_chunk_kernel(const RotateAxesArgs a, const ChunkGrid g) {
   constexpr int EPC = RowChunk<DT>::EPC;

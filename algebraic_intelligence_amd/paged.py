@@ -21,9 +21,9 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .attention import _axis_sections, _axis_tables
+from .attention import _axis_sections, _axis_tables, _norm_eps, _norm_scale
 
-__all__ = ["PagePool", "DraftPlan", "build_block_tables", "append_to_cache", "paged_tree_afa"]
+__all__ = ["PagePool", "DraftPlan", "build_block_tables", "append_to_cache", "paged_tree_afa", "paged_prefix_afa"]
 
 
 class _Plan(ctypes.Structure):
@@ -78,6 +78,10 @@ class PagePool:
         self.held = torch.zeros(self.max_requests, **new)
         self.ring = torch.arange(self.num_pages, **new)
         self.ring_state = torch.tensor([0, self.num_pages], **new)
+
+    def new_weights(self) -> torch.Tensor:
+        """The accumulated attention weights of one layer's cached tokens, (max_requests, max_len) in fp32, 0."""
+        return torch.zeros((self.max_requests, self.max_len), dtype=torch.float32, device=self.device)
 
     def new_pages(self, kv_heads: int, head_dim: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         """k and v pages of one layer, (num_pages, kv_heads, page_size, head_dim) each, not initialised."""
@@ -260,9 +264,12 @@ def _refuse(plan, name, t, shape):
 
 def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     plan: DraftPlan, rotary_params=None, *, positions: Optional[torch.Tensor] = None,
-                    sections=None) -> torch.Tensor:
+                    sections=None, norms=None, eps: float = 1e-6) -> torch.Tensor:
     """Rotate the step's q (max_tokens, heads, head_dim) and k (max_tokens, kv_heads, head_dim), store k and v
     at the tokens' slots of ``k_pages`` and ``v_pages``, and return the rotated q.
+
+    ``norms``: (q_scale, k_scale), (head_dim,) each; q and k are normalised, scaled and then rotated as in
+    ``apply_ago_norm_rotations``, with its ``eps``, in the same launch.
 
     ``rotary_params``: Cayley tables (positions, head_dim / 2), in fp32 (fp64 for fp64 inputs; others are
     cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
@@ -275,6 +282,16 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
         _no_gradient("append_to_cache")
     if forward_ad._current_level >= 0:
         _no_tangents("append_to_cache", q, k, v, k_pages, v_pages)
+    if norms is not None:
+        eps = _norm_eps(eps)
+        if not isinstance(norms, (tuple, list)) or len(norms) != 2:
+            raise TypeError("norms must be a pair (q_scale, k_scale)")
+        norms = [_norm_scale(name, t, plan.head_dim, plan.dtype, plan.device)
+                 for name, t in zip(("q_scale", "k_scale"), norms)]
+        if torch.is_grad_enabled() and (norms[0].requires_grad or norms[1].requires_grad):
+            _no_gradient("append_to_cache")
+        if forward_ad._current_level >= 0:
+            _no_tangents("append_to_cache", *norms)
     (q, sq), (k, sk), (v, sv) = (_rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape),
                                  _rows(plan, "v", v, plan._kv_shape))
     page_strides = _pages(plan, k_pages, v_pages)
@@ -302,6 +319,16 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     strides = None
     if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
         strides = _lib.pack6(sq[0], sq[1], sk[0], sk[1], sv[0], sv[1])
+    if norms is not None:
+        if c is None:
+            q_out = _like_rows(q)
+        with _lib.on_device(dev):
+            rc = _lib.lib().afa_paged_append_norm(
+                plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, q_out.data_ptr(), kp, vp, page_strides,
+                norms[0].data_ptr(), norms[1].data_ptr(), eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+                _lib.ptr(positions), axes, cuts, _lib.stream_ptr(dev))
+        _lib.check(rc, "afa_paged_append_norm")
+        return q_out
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_append(
             plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, None if c is None else q_out.data_ptr(),
@@ -325,15 +352,55 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     that it sees is its result in that feature.  Rows behind the last request's are 0, or left as they
     were where ``out`` is given.  For inference: tensors that require a gradient are refused where gradients
     are recorded."""
+    return _attend("paged_tree_afa", q, None, k_pages, v_pages, plan, sink_omega, masks, out, return_denominator)
+
+
+def paged_prefix_afa(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_pages: torch.Tensor,
+                     v_pages: torch.Tensor, plan: DraftPlan, sink_omega: float = 0.5, *, masks: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None,
+                     return_denominator: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``paged_tree_afa`` of requests that begin with the same tokens: every row sees the keys and values of
+    ``k_prefix`` and ``v_prefix`` (kv_heads, prefix length, head_dim), of any strides with a contiguous head
+    dimension, and then its request's cached and drafted tokens.
+
+    The prefix is kept once and met once for all rows of the step, whatever the number of requests.  The pool's lengths count a
+    request's own tokens, so that the positions of ``append_to_cache`` are the plan's plus the prefix's length:
+    ``positions=plan.positions + k_prefix.shape[1]``.  The plan, q, masks, out and what is returned are as in
+    ``paged_tree_afa``; rows of requests that were not served are 0."""
+    return _attend("paged_prefix_afa", q, (k_prefix, v_prefix), k_pages, v_pages, plan, sink_omega, masks, out,
+                   return_denominator)
+
+
+def _prefix(plan, k_prefix, v_prefix):
+    """The prefix's strides (head and key of k, then of v), None where both are contiguous, and its length."""
+    if k_prefix.ndim != 3 or k_prefix.shape[1] < 1 or k_prefix.shape[1] > 1 << 29:
+        raise ValueError(f"k_prefix must have shape ({plan.kv_heads}, length, {plan.head_dim}) with a length of 1 to 2^29, got "
+                         f"{tuple(k_prefix.shape)}")
+    shape = (plan.kv_heads, k_prefix.shape[1], plan.head_dim)
+    for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+        if t.dtype != plan.dtype or t.shape != shape or t.device != plan.device:
+            _refuse(plan, name, t, shape)
+    if k_prefix.is_contiguous() and v_prefix.is_contiguous():
+        return None, shape[1]
+    k, v = k_prefix.stride(), v_prefix.stride()
+    if (k[2] != 1 or v[2] != 1) and plan.head_dim != 1:
+        raise ValueError("k_prefix and v_prefix need a contiguous head dimension")
+    return _lib.pack4(k[0], k[1], v[0], v[1]), shape[1]
+
+
+def _attend(name, q, prefix, k_pages, v_pages, plan, sink_omega, masks, out, return_denominator):
     if not 0.0 <= sink_omega < float("inf"):
         raise ValueError("sink_omega must be finite and nonnegative")
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
-                                    or (out is not None and out.requires_grad)):
-        _no_gradient("paged_tree_afa")
+                                    or (out is not None and out.requires_grad)
+                                    or (prefix is not None and (prefix[0].requires_grad or prefix[1].requires_grad))):
+        _no_gradient(name)
     if forward_ad._current_level >= 0:
-        _no_tangents("paged_tree_afa", q, k_pages, v_pages)
+        _no_tangents(name, q, k_pages, v_pages, *(prefix or ()))
     q, sq = _rows(plan, "q", q, plan._q_shape)
     page_strides = _pages(plan, k_pages, v_pages)
+    if prefix is not None:
+        prefix_strides, length = _prefix(plan, *prefix)
     dev = plan.device
     if masks is not None:
         if plan.max_tree == 0:
@@ -352,10 +419,22 @@ def paged_tree_afa(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
           or _meet(out, k_pages, page_strides is None, plan._q_bytes, plan._page_bytes)
           or _meet(out, v_pages, page_strides is None, plan._q_bytes, plan._page_bytes)):
         raise ValueError("out must not overlap q, k_pages or v_pages")
+    elif prefix is not None and any(_meet(out, t, False, plan._q_bytes, 0) for t in prefix):
+        raise ValueError("out must not overlap k_prefix or v_prefix")
     den = None
     if return_denominator:
         new = torch.empty if flags else torch.zeros
         den = new((plan.max_tokens, plan.heads), dtype=_lib.accum_dtype(q.dtype), device=dev)
+    if prefix is not None:
+        with _lib.on_device(dev):
+            size = _lib.lib().afa_paged_prefix_workspace_size(plan._ref, length)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+            rc = _lib.lib().afa_paged_prefix_fwd(
+                plan._ref, q.data_ptr(), strides, prefix[0].data_ptr(), prefix[1].data_ptr(), length, prefix_strides,
+                k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(masks), out.data_ptr(), _lib.ptr(den),
+                sink_omega, flags, _lib.ptr(ws), size, _lib.stream_ptr(dev))
+        _lib.check(rc, "afa_paged_prefix_fwd")
+        return (out, den) if return_denominator else out
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_fwd(
             plan._ref, q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(), page_strides, _lib.ptr(masks),

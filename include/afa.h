@@ -368,6 +368,73 @@ int ago_rotate_axes(int dtype, int64_t batch, int64_t q_heads, int64_t k_heads, 
                     const void* rot_sin, int64_t rot_len, const void* positions, int pos_bytes, int64_t pos_b, int axes,
                     const int32_t* sections, int transpose, void* stream);
 
+/*
+ * Rows of q and k normalised head by head, scaled and rotated: y = R(m) (w . x / sqrt(mean(x^2) + eps)), w = q_scale or
+ * k_scale (head_dim,) in fp32 (fp64 for AFA_F64), m as in ago_rotate_axes.  positions NULL (axes 1, pos_b 0): a row's
+ * index in its sequence.  rot_cos and rot_sin NULL: no rotation, any head_dim.  The mean and all else in fp32 (fp64),
+ * one rounding.  Strides {q_b, q_h, q_l, k.., yq.., yk..} in elements, NULL: contiguous.
+ */
+int ago_norm_rotate_axes(int dtype, int64_t batch, int64_t q_heads, int64_t k_heads, int64_t seq_len, int64_t head_dim,
+                         const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const void* q_scale,
+                         const void* k_scale, double eps, const void* rot_cos, const void* rot_sin, int64_t rot_len,
+                         const void* positions, int pos_bytes, int64_t pos_b, int axes, const int32_t* sections,
+                         void* stream);
+/*
+ * Its VJP: dq and dk in q's type from the cotangents gq and gk, dq_scale and dk_scale (head_dim,) in fp32 (fp64), summed over
+ * all rows in a fixed order.  Strides {q.., k.., gq.., gk.., dq.., dk..}.  workspace:
+ * ago_norm_rotate_axes_bwd_workspace_size() bytes for the current device, 16-byte aligned, or NULL.
+ */
+size_t ago_norm_rotate_axes_bwd_workspace_size(int dtype, int64_t head_dim);
+int ago_norm_rotate_axes_bwd(int dtype, int64_t batch, int64_t q_heads, int64_t k_heads, int64_t seq_len, int64_t head_dim,
+                             const void* q, const void* k, const void* gq, const void* gk, void* dq, void* dk,
+                             const int64_t* strides, const void* q_scale, const void* k_scale, void* dq_scale, void* dk_scale,
+                             double eps, const void* rot_cos, const void* rot_sin, int64_t rot_len, const void* positions,
+                             int pos_bytes, int64_t pos_b, int axes, const int32_t* sections, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/*
+ * afa_paged_append with that norm of q and k before their rotation; q_out is not NULL.  v is stored as it is.
+ */
+int afa_paged_append_norm(const afa_paged_plan* plan, const void* q, const void* k, const void* v, const int64_t* strides,
+                          void* q_out, void* k_pages, void* v_pages, const int64_t* page_strides, const void* q_scale,
+                          const void* k_scale, double eps, const void* rot_cos, const void* rot_sin, int64_t rot_len,
+                          const int32_t* positions, int axes, const int32_t* sections, void* stream);
+/*
+ * afa_paged_fwd of requests that share a prefix: every row sees the prefix_len (up to 2^29) keys of k_prefix and v_prefix
+ * (kv_heads, prefix_len, head_dim), strides {k_head, k_key, v_head, v_key} in elements (NULL: contiguous), and then what it
+ * sees in afa_paged_fwd.  Rows of requests that were not served see neither.
+ * workspace: afa_paged_prefix_workspace_size() bytes, 16-byte aligned, or NULL.
+ */
+size_t afa_paged_prefix_workspace_size(const afa_paged_plan* plan, int64_t prefix_len);
+int afa_paged_prefix_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_prefix,
+                         const void* v_prefix, int64_t prefix_len, const int64_t* prefix_strides, const void* k_pages,
+                         const void* v_pages, const int64_t* page_strides, const int64_t* masks, void* out, void* denom,
+                         double sink_omega, unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * What each token was given by the step's rows: weights[r][j] += sum over the tokens i of request r that see its token j
+ * (as in afa_paged_fwd), and heads, of rho(s_ij)^8 / denom[i][head]; the step's own tokens (j >= cached) are set to
+ * their sums instead.  denom (max_tokens, heads): what the attention of these rows returned; a row whose denom is 0 gives
+ * nothing.  weights (requests, weights_stride), weights_stride >= table_width * page_size: fp32 for every dtype.  Sums are formed in
+ * a fixed order.  Requests without new tokens, and those that were not served, keep their weights.
+ */
+int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
+                      const int64_t* page_strides, const int64_t* masks, const void* denom, float* weights,
+                      int64_t weights_stride, void* stream);
+/*
+ * Requests of more than `budget` cached tokens cut back to it: the `first` oldest stay, the `recent` newest, and those of
+ * the largest weights among the others, the lower index among equal ones (NaN counts as the largest).  Their order stays: k, v and
+ * weight of the i-th that stays move to place i, in place in the pages; left (requests, table_width * page_size) receives the
+ * weights, 0 behind them, and lens (requests,) the lengths.  budget at most table_width * page_size; first + recent at most
+ * budget.  A cached length is taken as at most what the request's pages hold.  Places behind the budget keep their contents; the
+ * pages go back to the pool with the next afa_paged_build.  A page id outside the pool is neither read nor written.
+ * workspace: afa_paged_evict_workspace_size() bytes, 16-byte aligned, or NULL.
+ */
+size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget);
+int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t requests, int64_t table_width, int64_t kv_heads,
+                    int64_t head_dim, const int32_t* block_tables, const int32_t* held, void* k_pages, void* v_pages,
+                    const int64_t* page_strides, const int32_t* cached, int64_t budget, int64_t first, int64_t recent,
+                    const float* weights, int64_t weights_stride, float* left, int32_t* lens, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
