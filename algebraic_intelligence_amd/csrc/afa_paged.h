@@ -160,7 +160,9 @@ struct WeightArgs {
   double scale;
   int group;
 };
-hipError_t paged_weights_launch(const WeightArgs& a, int cus, hipStream_t st);
+// Whether the matrix-core kernel takes the call.  It has `ws`, the attention's workspace; nullptr: the other kernel.
+bool paged_weights_fast(const WeightArgs& a);
+hipError_t paged_weights_launch(const WeightArgs& a, const PagedCut& cut, int cus, void* ws, size_t ws_bytes, hipStream_t st);
 
 // Requests cut back to a budget of tokens (afa_paged_evict.hip).
 struct EvictArgs {

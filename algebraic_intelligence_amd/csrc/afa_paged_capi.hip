@@ -328,7 +328,7 @@ int afa_paged_prefix_fwd(const afa_paged_plan* plan, const void* q, const int64_
 
 int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
                       const int64_t* page_strides, const int64_t* masks, const void* denom, float* weights,
-                      int64_t weights_stride, void* stream) {
+                      int64_t weights_stride, unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_plan(plan);
   if (rc != AFA_OK) return rc;
   if (q == nullptr || k_pages == nullptr || denom == nullptr || weights == nullptr) return AFA_ERR_NULL;
@@ -338,7 +338,8 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
   afa::WeightArgs a = {};
   a.plan = p;
   const int cus = afa::device_cus();
-  a.sched = afa::paged_schedule(p, afa::paged_cut(p, cus).slots);
+  const afa::PagedCut cut = afa::paged_cut(p, cus);
+  a.sched = afa::paged_schedule(p, cut.slots);
   a.q = q; a.k_pages = k_pages;
   a.masks = masks != nullptr ? masks : p.max_tree > 0 ? p.masks : nullptr;
   a.denom = denom;
@@ -354,8 +355,17 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
   a.row = weights_stride;
   a.scale = 1.0 / std::sqrt((double)p.head_dim);
   a.group = (int)(p.heads / p.kv_heads);
-  const hipError_t e = afa::paged_weights_launch(a, cus, (hipStream_t)stream);
-  return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
+  const hipStream_t s = (hipStream_t)stream;
+  if ((flags & AFA_FLAG_GENERIC) != 0 || !afa::paged_weights_fast(a)) {
+    const hipError_t e = afa::paged_weights_launch(a, cut, cus, nullptr, 0, s);
+    return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
+  }
+  const size_t need = afa::paged_fast_workspace(p, cut);
+  void* ws;
+  bool own;
+  const int got = workspace_of(workspace, workspace_bytes, need, s, ws, own);
+  if (got != AFA_OK) return got;
+  return workspace_done(afa::paged_weights_launch(a, cut, cus, ws, need, s), ws, own, s);
 }
 
 size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget) {

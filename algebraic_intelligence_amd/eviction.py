@@ -77,7 +77,8 @@ def accumulate_cache_weights(q: torch.Tensor, k_pages: torch.Tensor, denominator
     with _lib.on_device(dev):
         rc = _lib.lib().afa_paged_weights(
             plan._ref, q.data_ptr(), None if q.is_contiguous() else _lib.pack2(sq[0], sq[1]), k_pages.data_ptr(),
-            page_strides, _lib.ptr(masks), denominator.data_ptr(), weights.data_ptr(), row, _lib.stream_ptr(dev))
+            page_strides, _lib.ptr(masks), denominator.data_ptr(), weights.data_ptr(), row, 0, _lib.ptr(plan._ws),
+            plan._ws_bytes, _lib.stream_ptr(dev))
     _lib.check(rc, "afa_paged_weights")
     return weights
 

@@ -414,11 +414,12 @@ int afa_paged_prefix_fwd(const afa_paged_plan* plan, const void* q, const int64_
  * (as in afa_paged_fwd), and heads, of rho(s_ij)^8 / denom[i][head]; the step's own tokens (j >= cached) are set to
  * their sums instead.  denom (max_tokens, heads): what the attention of these rows returned; a row whose denom is 0 gives
  * nothing.  weights (requests, weights_stride), weights_stride >= table_width * page_size: fp32 for every dtype.  Sums are formed in
- * a fixed order.  Requests without new tokens, and those that were not served, keep their weights.
+ * a fixed order.  Requests without new tokens, and those that were not served, keep their weights.  AFA_FLAG_GENERIC: without
+ * the matrix cores.  workspace: the attention's, afa_paged_workspace_size() bytes, 16-byte aligned, or NULL.
  */
 int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
                       const int64_t* page_strides, const int64_t* masks, const void* denom, float* weights,
-                      int64_t weights_stride, void* stream);
+                      int64_t weights_stride, unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * Requests of more than `budget` cached tokens cut back to it: the `first` oldest stay, the `recent` newest, and those of
  * the largest weights among the others, the lower index among equal ones (NaN counts as the largest).  Their order stays: k, v and
