@@ -145,7 +145,14 @@ hipError_t paged_fwd_generic_launch(const PagedFwdArgs& a, hipStream_t st);
 // Matrix-core path (afa_paged_mfma.hip): 16-byte aligned rows of q, pages and out.  ws: paged_fast_workspace bytes.
 bool paged_fast_supported(const afa_paged_plan& p);
 size_t paged_fast_workspace(const afa_paged_plan& p, const PagedCut& c);
-hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, void* ws, hipStream_t st);
+// Sums over a shared prefix: (max_tokens, heads, head_dim) numerators and (max_tokens, heads) row sums; nullptr: none.
+struct PrefixSums {
+  float *top, *bottom;
+};
+hipError_t paged_fwd_fast_launch(const PagedFwdArgs& a, const PagedCut& c, const PrefixSums& shared, void* ws, hipStream_t st);
+// The prefix's part (afa_prefix.hip), whose sums that call takes.  ws: paged_fast_workspace bytes of the cut.
+PagedCut prefix_cut(const afa_paged_plan& p, int cus);
+hipError_t prefix_sums_launch(const PagedFwdArgs& a, const PagedCut& c, const PrefixSums& shared, void* ws, hipStream_t st);
 
 // What each cached token was given by the step's rows (afa_paged_weights.hip).
 struct WeightArgs {

@@ -159,6 +159,15 @@ bool fast_rows(const afa::PagedFwdArgs& a, unsigned flags) {
   return fast;
 }
 
+// A call behind a prefix: its sums, and the parts of the two launches, which come one after the other.
+size_t prefix_sum_bytes(const afa_paged_plan& p) {
+  return (size_t)((p.max_tokens * p.heads * (p.head_dim + 1) * 4 + 15) / 16 * 16);
+}
+size_t prefix_workspace(const afa_paged_plan& p, int cus) {
+  const size_t a = afa::paged_fast_workspace(p, afa::paged_cut(p, cus)), b = afa::paged_fast_workspace(p, afa::prefix_cut(p, cus));
+  return prefix_sum_bytes(p) + (a > b ? a : b);
+}
+
 // A norm's scales and eps.
 int check_norm(afa::HeadNorm& n, const void* q_scale, const void* k_scale, bool has_k, double eps) {
   if (q_scale == nullptr || (has_k && k_scale == nullptr)) return AFA_ERR_NULL;
@@ -294,12 +303,14 @@ int afa_paged_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_st
   bool own;
   const int got = workspace_of(workspace, workspace_bytes, afa::paged_fast_workspace(*plan, cut), s, ws, own);
   if (got != AFA_OK) return got;
-  return workspace_done(afa::paged_fwd_fast_launch(a, cut, ws, s), ws, own, s);
+  return workspace_done(afa::paged_fwd_fast_launch(a, cut, afa::PrefixSums{}, ws, s), ws, own, s);
 }
 
 size_t afa_paged_prefix_workspace_size(const afa_paged_plan* plan, int64_t prefix_len) {
-  if (plan == nullptr || check_sizes(*plan) != AFA_OK || !within(prefix_len, 1, kMostPrefix)) return 0;
-  return 0;
+  if (plan == nullptr || check_sizes(*plan) != AFA_OK || !within(prefix_len, 1, kMostPrefix) ||
+      !afa::paged_fast_supported(*plan))
+    return 0;
+  return prefix_workspace(*plan, afa::device_cus());
 }
 
 int afa_paged_prefix_fwd(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_prefix,
@@ -322,8 +333,28 @@ int afa_paged_prefix_fwd(const afa_paged_plan* plan, const void* q, const int64_
     x.v_head = prefix_strides[2]; x.v_key = prefix_strides[3];
   }
   const hipStream_t s = (hipStream_t)stream;
-  const hipError_t e = afa::paged_fwd_generic_launch(a, s);
-  return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
+  const afa_paged_plan& p = *plan;
+  // a tile's 32 rows by 32-bit byte offsets
+  const int64_t unit = p.dtype == AFA_F32 ? 4 : 8;
+  bool fast = fast_rows(a, flags) && aligned16(k_prefix) && aligned16(v_prefix);
+  for (int64_t v : {x.k_head, x.k_key, x.v_head, x.v_key}) fast = fast && v % unit == 0;
+  for (int64_t v : {x.k_key, x.v_key}) fast = fast && v >= 0 && v < int64_t(1) << 24;
+  if (!fast) {
+    const hipError_t e = afa::paged_fwd_generic_launch(a, s);
+    return e == hipSuccess ? AFA_OK : afa::hip_status_code(e);
+  }
+  const int cus = afa::device_cus();
+  void* ws;
+  bool own;
+  const int got = workspace_of(workspace, workspace_bytes, prefix_workspace(p, cus), s, ws, own);
+  if (got != AFA_OK) return got;
+  // the sums, then the parts of either launch
+  const int64_t rows = p.max_tokens * p.heads;
+  const afa::PrefixSums sums{(float*)ws, (float*)ws + rows * p.head_dim};
+  void* parts = (char*)ws + prefix_sum_bytes(p);
+  hipError_t e = afa::prefix_sums_launch(a, afa::prefix_cut(p, cus), sums, parts, s);
+  if (e == hipSuccess) e = afa::paged_fwd_fast_launch(a, afa::paged_cut(p, cus), sums, parts, s);
+  return workspace_done(e, ws, own, s);
 }
 
 int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* q_strides, const void* k_pages,
