@@ -181,11 +181,12 @@ struct EvictArgs {
   int64_t row;
   float* left;           // (requests, table_width * page_size)
   int32_t* lens;
-  int32_t* kept;         // workspace: (requests, budget) indexes, then the requests' first moved place
+  int32_t* space;        // paged_evict_workspace bytes
   int budget, first, recent, esz;
+  int rows, chunks;      // set by the launch: places of a chunk, and chunks of a budget
 };
-size_t paged_evict_workspace(int64_t requests, int64_t budget);
-hipError_t paged_evict_launch(const EvictArgs& a, hipStream_t st);
+size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim);
+hipError_t paged_evict_launch(EvictArgs a, hipStream_t st);
 
 struct RotateAxesArgs {
   const void *x[2];

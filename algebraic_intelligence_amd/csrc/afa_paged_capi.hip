@@ -399,9 +399,11 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
   return workspace_done(afa::paged_weights_launch(a, cut, cus, ws, need, s), ws, own, s);
 }
 
-size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget) {
-  if (!within(requests, 1, int64_t(1) << 22) || !within(budget, 1, int64_t(1) << 30)) return 0;
-  return afa::paged_evict_workspace(requests, budget);
+size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim) {
+  if (!within(requests, 1, int64_t(1) << 22) || !within(budget, 1, int64_t(1) << 30) || !within(kv_heads, 1, 1 << 16) ||
+      !within(head_dim, 1, 1024))
+    return 0;
+  return afa::paged_evict_workspace(requests, budget, kv_heads, head_dim);
 }
 
 int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t requests, int64_t table_width, int64_t kv_heads,
@@ -435,9 +437,10 @@ int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t req
   const hipStream_t s = (hipStream_t)stream;
   void* ws;
   bool own;
-  const int got = workspace_of(workspace, workspace_bytes, afa::paged_evict_workspace(requests, budget), s, ws, own);
+  const int got = workspace_of(workspace, workspace_bytes, afa::paged_evict_workspace(requests, budget, kv_heads, head_dim), s,
+                               ws, own);
   if (got != AFA_OK) return got;
-  a.kept = (int32_t*)ws;
+  a.space = (int32_t*)ws;
   return workspace_done(afa::paged_evict_launch(a, s), ws, own, s);
 }
 

@@ -3,9 +3,16 @@
 // order: token kept[i] moves to place i, in k, in v and in the weights.
 //
 // Two launches.  The first finds, one workgroup a request, the weight from which on tokens stay, by its bits from
-// the top (four passes over the weights, eight bits each, in LDS), and lists the tokens that do.  The second moves
-// rows in place: kept[i] >= i and both rise, so that one workgroup that goes through a head's rows in order, reads a
-// batch of them, waits and writes it, never writes over a row that it has still to read.
+// the top (three passes over the weights, up to eleven bits each, counted in LDS), and lists the tokens that do.
+//
+// The second moves rows in place.  A workgroup has one chunk of ROWS places of one head's k or v; its sources are behind its
+// places, in places of later chunks, so it reads all of them, says so, and writes only once the chunks that read from
+// its own places (earlier ones, two at most, as ROWS places hold at most ROWS sources) have said so too.  Chunks are handed
+// out in their order by a counter, and a workgroup reads and says so before it waits: whatever one waits for has begun and
+// waits for nothing before it says so, so every wait ends.
+//
+// HBM bounds the second launch: every row that moves is read and written once.
+#include <algorithm>
 #include <initializer_list>
 
 #include "afa_common.h"
@@ -15,7 +22,27 @@ namespace afa {
 
 namespace {
 
-constexpr int PICK = 1024, BINS = 256;
+constexpr int PICK = 1024, PICK_WAVES = PICK / 64;
+constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // lanes spread over copies: neighbours often share a bin
+constexpr int LOADS = 8;                                  // weights of a thread in flight
+constexpr int MOVE = 256, BATCH = 16;                     // threads of a mover, and units that each holds
+
+// The workspace: tokens that stay (requests, budget); the first place that moves (requests,); sources before each chunk's
+// places, and behind the last's (requests, chunks + 1); chunks handed out (requests, streams) and chunks that are read (requests, streams, chunks), a
+// stream being one head's k or v.
+struct EvictSpace {
+  int32_t *kept, *moved, *before, *next, *read;
+};
+__host__ __device__ inline EvictSpace evict_space(const EvictArgs& a) {
+  const int64_t streams = a.requests * 2 * a.kv_heads;
+  EvictSpace s;
+  s.kept = a.space;
+  s.moved = s.kept + a.requests * a.budget;
+  s.before = s.moved + a.requests;
+  s.next = s.before + a.requests * (a.chunks + 1);
+  s.read = s.next + streams;
+  return s;
+}
 
 // Bits whose unsigned order is that of the weights: -0 and 0 alike, NaN above infinity.
 __device__ __forceinline__ unsigned order_bits(float w) {
@@ -24,158 +51,239 @@ __device__ __forceinline__ unsigned order_bits(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sums of x over the threads before this one; all: over the workgroup.
-__device__ __forceinline__ int before(int x, int* lds, int& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = x;
+// Inclusive sums of x over the lanes up to this one.
+__device__ __forceinline__ int lanes_up_to(int x) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(s, o);
-    if (lane >= o) s += u;
+    const int u = __shfl_up(x, o);
+    if ((int)(threadIdx.x & 63) >= o) x += u;
   }
-  __syncthreads();
-  if (lane == 63) lds[wave] = s;
-  __syncthreads();
-  int base = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < PICK / 64; ++w) {
-    if (w == wave) base = all;
-    all += lds[w];
-  }
-  return base + s - x;
+  return x;
 }
 
 __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a) {
-  __shared__ int bins[BINS], scan[PICK / 64], found[2];
-  const int r = blockIdx.x, tid = threadIdx.x;
+  __shared__ int bins[COPIES * BINS], wave_sum[PICK_WAVES], found[2];
+  __shared__ int2 counts[LOADS * PICK_WAVES];
+  const EvictSpace s = evict_space(a);
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t width = a.table_width * a.page_size;
   const int held = (int)min(max((int64_t)a.held[r], (int64_t)0) * a.page_size, width);
   const int c = min(max(a.cached[r], 0), held), budget = a.budget, m = min(c, budget);
   const float* w = a.weights + r * a.row;
   float* left = a.left + r * width;
-  int32_t* kept = a.kept + (int64_t)r * budget;
-  int32_t* moved = a.kept + a.requests * budget + r;
+  int32_t* kept = s.kept + (int64_t)r * budget;
+  const int streams = (int)(2 * a.kv_heads);
+  for (int i = tid; i < streams; i += PICK) s.next[(int64_t)r * streams + i] = 0;
+  for (int64_t i = tid; i < (int64_t)streams * a.chunks; i += PICK) s.read[(int64_t)r * streams * a.chunks + i] = 0;
   if (tid == 0) a.lens[r] = m;
   for (int64_t i = m + tid; i < width; i += PICK) left[i] = 0.0f;
   if (c <= budget) {
     for (int i = tid; i < m; i += PICK) left[i] = w[i];
-    if (tid == 0) *moved = m;
+    if (tid == 0) s.moved[r] = m;
     return;
   }
+  int32_t* before = s.before + (int64_t)r * (a.chunks + 1);
+  for (int i = tid; i <= a.chunks; i += PICK)
+    if ((int64_t)i * a.rows >= c) before[i] = m;
   // tokens [lo, hi) are chosen from; `need` of them stay
   const int lo = a.first, hi = c - a.recent;
   int need = budget - a.first - a.recent;
-  unsigned prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
+  unsigned top = 0;  // the bits of the least weight that stays, as far as they are known
+  for (int shift = 32 - DIGIT; ; shift = shift > DIGIT ? shift - DIGIT : 0) {
+    const int above = shift == 32 - DIGIT ? 32 : shift == 0 ? 32 - 2 * DIGIT : 32 - DIGIT;
+    const unsigned mask = (1u << (above - shift)) - 1;
+    for (int i = tid; i < COPIES * BINS; i += PICK) bins[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += PICK) {
-      const unsigned u = order_bits(w[i]);
-      if (shift == 24 || u >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&bins[u >> shift & 255], 1);
+    for (int base = lo; base < hi; base += LOADS * PICK) {
+      unsigned u[LOADS];
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k) u[k] = order_bits(w[min(base + k * PICK + tid, hi - 1)]);
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k)
+        if (base + k * PICK + tid < hi && (above == 32 || u[k] >> above == top >> above))
+          atomicAdd(&bins[(lane % COPIES) * BINS + (u[k] >> shift & mask)], 1);
     }
     __syncthreads();
-    // the bin in which the need-th largest lies
-    if (tid == 0) {
-      int b = BINS - 1, above = 0;
-      while (b > 0 && above + bins[b] < need) above += bins[b--];
-      found[0] = b;
-      found[1] = above;
+    // the bin in which the need-th largest lies: thread t has bins of rank 2 t and 2 t + 1 from the top
+    static_assert(BINS == 2 * PICK, "two bins a thread");
+    int n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      n[k] = 0;
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) n[k] += bins[i * BINS + BINS - 1 - 2 * tid - k];
+    }
+    const int upto = lanes_up_to(n[0] + n[1]);
+    if (lane == 63) wave_sum[wave] = upto;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    int earlier = upto - n[0] - n[1];
+    for (int v = 0; v < wave; ++v) earlier += wave_sum[v];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (earlier < need && need <= earlier + n[k]) {
+        found[0] = BINS - 1 - 2 * tid - k;
+        found[1] = earlier;
+      }
+      earlier += n[k];
     }
     __syncthreads();
-    prefix |= (unsigned)found[0] << shift;
+    if (found[0] < 0) {  // none is needed
+      top = 0xffffffffu;
+      need = 0;
+      break;
+    }
+    top |= (unsigned)found[0] << shift;
     need -= found[1];
+    if (shift == 0) break;
     __syncthreads();
   }
-  // above `prefix` all stay, and the first `need` that equal it
-  int at = 0, equal = 0, start = budget;
-  for (int base = 0; base < c; base += PICK) {
-    const int i = base + tid;
-    const bool in = i < c, sure = in && (i < lo || i >= hi);
-    const unsigned u = in && !sure ? order_bits(w[i]) : 0;
-    const bool same = in && !sure && u == prefix;
-    int all;
-    const int rank = equal + before(same, scan, all);
-    equal += all;
-    const bool stays = sure || (in && !sure && (u > prefix || (same && rank < need)));
-    const int to = at + before(stays, scan, all);
-    at += all;
-    if (stays) {
-      kept[to] = i;
-      left[to] = w[i];
-      if (to != i) start = min(start, to);
+  // those above `top` stay, and the first `need` that equal it
+  int over = 0, equal = 0, start = budget;  // of the tokens before this batch: above and sure ones, and equal ones
+  for (int base = 0; base < c; base += LOADS * PICK) {
+    float v[LOADS];
+    int kind[LOADS];  // 2: stays, 1: equal, 0: neither
+    unsigned long long overs[LOADS], equals[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) v[k] = w[min(base + k * PICK + tid, c - 1)];
+    __syncthreads();  // counts is free
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int i = base + k * PICK + tid;
+      const unsigned u = order_bits(v[k]);
+      kind[k] = i >= c ? 0 : i < lo || i >= hi || u > top ? 2 : u == top ? 1 : 0;
+      overs[k] = __ballot(kind[k] == 2);
+      equals[k] = __ballot(kind[k] == 1);
+      if (lane == 0) counts[k * PICK_WAVES + wave] = int2{__popcll(overs[k]), __popcll(equals[k])};
     }
+    __syncthreads();
+    // sums before each wave's, in place; the last two entries' sums are the batch's
+    static_assert(LOADS * PICK_WAVES == 128, "two entries a lane");
+    if (wave == 0) {
+      const int2 x = counts[2 * lane], y = counts[2 * lane + 1];
+      const int o = lanes_up_to(x.x + y.x), e = lanes_up_to(x.y + y.y);
+      counts[2 * lane] = int2{o - x.x - y.x, e - x.y - y.y};
+      counts[2 * lane + 1] = int2{o - y.x, e - y.y};
+      if (lane == 63) {
+        found[0] = o;
+        found[1] = e;
+      }
+    }
+    __syncthreads();
+    const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int i = base + k * PICK + tid;
+      const int2 b = counts[k * PICK_WAVES + wave];
+      const int o = over + b.x + __popcll(overs[k] & below), e = equal + b.y + __popcll(equals[k] & below);
+      const int to = o + min(e, need);
+      if (i < c && i % a.rows == 0 && i / a.rows <= a.chunks) before[i / a.rows] = to;
+      if (kind[k] == 2 || (kind[k] == 1 && e < need)) {
+        kept[to] = i;
+        left[to] = v[k];
+        if (to != i) start = min(start, to);
+      }
+    }
+    over += found[0];
+    equal += found[1];
   }
   // the first place whose token moves
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) start = min(start, __shfl_xor(start, o));
-  __syncthreads();
-  if ((tid & 63) == 0) scan[tid >> 6] = start;
+  if (lane == 0) wave_sum[wave] = start;
   __syncthreads();
   if (tid == 0) {
-    for (int k = 1; k < PICK / 64; ++k) start = min(start, scan[k]);
-    *moved = start;
+    for (int k = 1; k < PICK_WAVES; ++k) start = min(start, wave_sum[k]);
+    s.moved[r] = start;
   }
 }
 
-// Rows as `units` of type T each; U of them a thread and batch.
+// Rows as `units` of type T each; a chunk is BATCH units a thread, a.rows rows.
 template <typename T>
-__global__ __launch_bounds__(256) void afa_paged_move_kernel(const EvictArgs a, int units) {
-  constexpr int U = 8;
-  int64_t item = blockIdx.x;
-  const bool is_v = item & 1;
-  item >>= 1;
-  const int hk = (int)(item % a.kv_heads), r = (int)(item / a.kv_heads);
-  const int m = a.lens[r], start = a.kept[a.requests * a.budget + r];
-  const int32_t *kept = a.kept + (int64_t)r * a.budget, *table = a.block_tables + (int64_t)r * a.table_width;
-  char* pages = (char*)(is_v ? a.v_pages : a.k_pages);
+__global__ __launch_bounds__(MOVE) void afa_paged_move_kernel(const EvictArgs a, int units) {
+  __shared__ int ticket;
+  const EvictSpace s = evict_space(a);
+  const int64_t streams = a.requests * 2 * a.kv_heads, stream = blockIdx.x % streams;
+  const int r = (int)(stream / (2 * a.kv_heads)), which = (int)(stream % (2 * a.kv_heads)), hk = which >> 1;
+  const bool is_v = which & 1;
+  const int m = a.lens[r], start = s.moved[r];
+  // chunks in which a token moves
+  const int begin = start / a.rows, end = (m + a.rows - 1) / a.rows;
+  if (start >= m) return;
+  const int32_t *kept = s.kept + (int64_t)r * a.budget, *table = a.block_tables + (int64_t)r * a.table_width;
+  const int32_t* before = s.before + (int64_t)r * (a.chunks + 1);
+  int32_t* read = s.read + stream * a.chunks;
+  char* pages = (char*)(is_v ? a.v_pages : a.k_pages) + hk * (is_v ? a.ps.v_head : a.ps.k_head) * a.esz;
   const int64_t page = (is_v ? a.ps.v_page : a.ps.k_page) * a.esz, slot = (is_v ? a.ps.v_slot : a.ps.k_slot) * a.esz;
-  pages += hk * (is_v ? a.ps.v_head : a.ps.k_head) * a.esz;
+  const unsigned P = (unsigned)a.page_size;
   auto place = [&](int pos) -> char* {
-    const int at = (int)(pos / a.page_size), id = table[at];
-    return id < 0 || id >= a.num_pages ? nullptr : pages + id * page + (pos - at * a.page_size) * slot;
+    const unsigned at = (unsigned)pos / P;
+    const int id = table[at];
+    return id < 0 || id >= a.num_pages ? nullptr : pages + id * page + ((unsigned)pos - at * P) * slot;
   };
-  const int64_t all = (int64_t)(m - start) * units;
-  for (int64_t base = 0; base < all; base += 256 * U) {
-    T x[U];
-    char* to[U];
+  for (;;) {
+    __syncthreads();  // ticket has been read
+    if (threadIdx.x == 0) ticket = begin + atomicAdd(s.next + stream, 1);
+    __syncthreads();
+    const int chunk = ticket;
+    if (chunk >= end) return;
+    const int first = chunk * a.rows, count = min(a.rows, m - first) * units;
+    T x[BATCH];
+    unsigned moves = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t e = base + u * 256 + threadIdx.x;
-      to[u] = nullptr;
-      if (e >= all) continue;
-      const int i = start + (int)(e / units), in = (int)(e % units);
-      const char* from = place(kept[i]);
-      if (from == nullptr) continue;
-      to[u] = place(i);
-      if (to[u] == nullptr) continue;
-      to[u] += in * sizeof(T);
-      x[u] = *(const T*)(from + in * sizeof(T));
+    for (int u = 0; u < BATCH; ++u) {
+      const int e = u * MOVE + (int)threadIdx.x;
+      if (e >= count) continue;
+      const int i = e / units, from = kept[first + i];
+      const char* p = place(from);
+      if (from == first + i || p == nullptr) continue;
+      moves |= 1u << u;
+      x[u] = *(const T*)(p + (e - i * units) * sizeof(T));
     }
-    // read by all before any is written
+    // every read of the chunk is done
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+    if (threadIdx.x == 0) __hip_atomic_store(read + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // sources [low, high) lie in this chunk's places: the first's chunk and the last's
+    if (threadIdx.x < 2) {
+      const int low = before[chunk], high = before[chunk + 1];
+      const int other = (threadIdx.x == 0 ? low : high - 1) / a.rows;
+      if (low < high && other < chunk && other >= begin)
+        while (__hip_atomic_load(read + other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(1);
+    }
+    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (to[u] != nullptr) *(T*)to[u] = x[u];
+    for (int u = 0; u < BATCH; ++u) {
+      if (!(moves >> u & 1)) continue;
+      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
+      char* q = place(first + i);
+      if (q != nullptr) *(T*)(q + (e - i * units) * sizeof(T)) = x[u];
+    }
   }
 }
 
 }  // namespace
 
-size_t paged_evict_workspace(int64_t requests, int64_t budget) { return (size_t)(requests * (budget + 1)) * 4; }
+// Chunks are shortest where units are elements.
+size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim) {
+  const int64_t rows = std::max<int64_t>(1, MOVE * BATCH / head_dim), chunks = (budget + rows - 1) / rows;
+  return (size_t)(requests * (budget + 2 + chunks + 2 * kv_heads * (1 + chunks))) * 4;
+}
 
-hipError_t paged_evict_launch(const EvictArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(afa_paged_pick_kernel, dim3((unsigned)a.requests), dim3(PICK), 0, st, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(2 * a.requests * a.kv_heads)), block(256);
+hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
   int64_t unit = 16;
   const int64_t bytes = a.head_dim * a.esz;
   for (int64_t v : {(int64_t)(uintptr_t)a.k_pages, (int64_t)(uintptr_t)a.v_pages, bytes, a.ps.k_page * a.esz, a.ps.k_head * a.esz,
                     a.ps.k_slot * a.esz, a.ps.v_page * a.esz, a.ps.v_head * a.esz, a.ps.v_slot * a.esz})
     while (v % unit != 0) unit /= 2;
   const int units = (int)(bytes / unit);
+  a.rows = MOVE * BATCH / units;
+  a.chunks = (a.budget + a.rows - 1) / a.rows;
+  hipLaunchKernelGGL(afa_paged_pick_kernel, dim3((unsigned)a.requests), dim3(PICK), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t streams = 2 * a.requests * a.kv_heads, most = std::max<int64_t>(1, (int64_t(1) << 20) / streams);
+  const dim3 grid((unsigned)(streams * std::min<int64_t>(a.chunks, most))), block(MOVE);
   switch (unit) {
     case 16: hipLaunchKernelGGL((afa_paged_move_kernel<u32x4_t>), grid, block, 0, st, a, units); break;
     case 8: hipLaunchKernelGGL((afa_paged_move_kernel<u32x2_t>), grid, block, 0, st, a, units); break;

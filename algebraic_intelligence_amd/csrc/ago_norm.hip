@@ -61,59 +61,50 @@ struct RotateRows {
 };
 
 struct AppendRows {
-  AppendArgs a;
+  // q, k and v.  k and v lie in pages; q's page is its token, and its place there 0
+  const void* x[3];
+  void* y[3];
+  int64_t xt[3], xh[3], page[3], head[3], slot[3];
+  int count[3];
+  const int32_t* slots;
+  int64_t capacity;
+  int page_size, features;
   HeadNorm n;
+  AxisRotation rot;
   static constexpr int KINDS = 3;
   struct Token {
     int64_t t, at, page, place;
     bool stored;
   };
-  __device__ __forceinline__ int heads(int which) const { return which == 0 ? a.heads : a.kv_heads; }
+  __device__ __forceinline__ int heads(int which) const { return count[which]; }
   __device__ __forceinline__ Token token(uint32_t t) const {
-    const int64_t slot = a.slots[t];
-    const bool stored = slot >= 0 && slot < a.capacity;
-    const uint32_t page = stored ? (uint32_t)slot / (uint32_t)a.page_size : 0;
-    return Token{t, (int64_t)t * a.rot.axes, page, stored ? slot - (int64_t)page * a.page_size : 0, stored};
+    const int64_t slot = slots[t];
+    const bool stored = slot >= 0 && slot < capacity;
+    const uint32_t page = stored ? (uint32_t)slot / (uint32_t)page_size : 0;
+    return Token{t, (int64_t)t * rot.axes, page, stored ? slot - (int64_t)page * page_size : 0, stored};
   }
   template <typename S>
   __device__ __forceinline__ const S* src(const Token& t, int which, int h) const {
-    return which == 0 ? (const S*)a.q + (t.t * a.q_t + h * a.q_h)
-           : which == 1 ? (const S*)a.k + (t.t * a.k_t + h * a.k_h)
-                        : (const S*)a.v + (t.t * a.v_t + h * a.v_h);
+    return (const S*)x[which] + (t.t * xt[which] + h * xh[which]);
   }
   template <typename S>
   __device__ __forceinline__ S* dst(const Token& t, int which, int h) const {
-    if (which == 0) return (S*)a.q_out + (t.t * a.heads + h) * a.dim;
-    if (!t.stored) return nullptr;
-    return which == 1 ? (S*)a.k_pages + (t.page * a.ps.k_page + h * a.ps.k_head + t.place * a.ps.k_slot)
-                      : (S*)a.v_pages + (t.page * a.ps.v_page + h * a.ps.v_head + t.place * a.ps.v_slot);
+    const bool in_pages = which > 0;
+    if (in_pages && !t.stored) return nullptr;
+    return (S*)y[which] + ((in_pages ? t.page : t.t) * page[which] + h * head[which] + (in_pages ? t.place : 0) * slot[which]);
   }
-  __device__ __forceinline__ const AxisRotation& rotation() const { return a.rot; }
+  __device__ __forceinline__ const AxisRotation& rotation() const { return rot; }
   __device__ __forceinline__ const HeadNorm& norm() const { return n; }
-  __device__ __forceinline__ int dim() const { return a.dim; }
+  __device__ __forceinline__ int dim() const { return features; }
 };
 
 // ------------------------------------------------------------------ rows in 16-byte chunks
-// Groups of LPR lanes, each for up to HG heads of one kind of one token, `groups[which]` apart.
+// Groups of LPR lanes, each for up to HG heads of one token, `groups[which]` apart.  A workgroup has rows of one kind, that
+// of the last of `begin` that it does not precede: what differs by kind stays in scalar registers.
 struct NormGrid {
-  uint32_t chunks, tokens, groups[3], all;
+  uint32_t chunks, tokens, groups[3], begin[4];
   int heads_inner;
 };
-
-__device__ __forceinline__ void norm_group(const NormGrid& g, uint32_t i, uint32_t& token, int& which, uint32_t& first) {
-  const uint32_t inner = g.heads_inner ? g.all : g.tokens, out = i / inner, in = i - out * inner;
-  token = g.heads_inner ? out : in;
-  first = g.heads_inner ? in : out;
-  which = 0;
-  if (first >= g.groups[0]) {
-    first -= g.groups[0];
-    which = 1;
-    if (first >= g.groups[1]) {
-      first -= g.groups[1];
-      which = 2;
-    }
-  }
-}
 
 template <int DT>
 struct ChunkScale {
@@ -130,14 +121,15 @@ __global__ __launch_bounds__(256) void ago_norm_chunk_kernel(const Rows rows, co
   using R = RowChunk<DT>;
   using S = typename Elem<DT>::storage;
   constexpr int EPC = R::EPC;
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, c = i % LPR;
-  if (i / LPR >= g.tokens * g.all) return;  // whole rows of lanes
-  uint32_t t, first;
-  int which;
-  norm_group(g, i / LPR, t, which, first);
+  int which = 0;
+#pragma unroll
+  for (int k = 1; k < Rows::KINDS; ++k) which += blockIdx.x >= g.begin[k];
+  const uint32_t i = (blockIdx.x - g.begin[which]) * 256 + threadIdx.x, c = i % LPR, set = i / LPR, step = g.groups[which];
+  if (set >= g.tokens * step) return;  // whole rows of lanes
+  const uint32_t inner = g.heads_inner ? step : g.tokens, out = set / inner, in = set - out * inner;
+  const uint32_t t = g.heads_inner ? out : in, first = g.heads_inner ? in : out;
   const typename Rows::Token token = rows.token(t);
   const int heads = rows.heads(which), d = (int)c * EPC;
-  const uint32_t step = g.groups[which];
   const bool mine = c < g.chunks;
   u32x4_t w[HG];
 #pragma unroll
@@ -177,17 +169,18 @@ __global__ __launch_bounds__(256) void ago_norm_chunk_kernel(const Rows rows, co
 }
 
 // The gradients.  Workgroups below `parts[0]` have q's rows, the others k's; a group of lanes goes through every
-// parts * (256 / LPR)-th set of heads, and its sums of back . xh stay in registers.
+// parts * (BWD / LPR)-th set of heads, and its sums of back . xh stay in registers.
 struct NormParts {
   uint32_t parts[2];
   void* sums;  // (parts[0] + parts[1], dim)
 };
 
+constexpr int BWD = 512;
 template <int DT, int LPR, int HG>
-__global__ __launch_bounds__(256) void ago_norm_bwd_chunk_kernel(const NormArgs a, const NormGrid g, const NormParts p) {
+__global__ __launch_bounds__(BWD) void ago_norm_bwd_chunk_kernel(const NormArgs a, const NormGrid g, const NormParts p) {
   using R = RowChunk<DT>;
   using S = typename Elem<DT>::storage;
-  constexpr int EPC = R::EPC, SLOTS = 256 / LPR;
+  constexpr int EPC = R::EPC, SLOTS = BWD / LPR;
   __shared__ float sums[SLOTS][LPR * EPC];
   const int which = blockIdx.x >= p.parts[0];
   const uint32_t part = which ? blockIdx.x - p.parts[0] : blockIdx.x;
@@ -246,7 +239,7 @@ __global__ __launch_bounds__(256) void ago_norm_bwd_chunk_kernel(const NormArgs 
 #pragma unroll
   for (int e = 0; e < EPC; ++e) sums[slot][d + e] = acc[e];
   __syncthreads();
-  for (int e = threadIdx.x; e < a.dim; e += 256) {
+  for (int e = threadIdx.x; e < a.dim; e += BWD) {
     float x = 0.0f;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) x += sums[s][e];
@@ -431,15 +424,17 @@ inline NormGrid norm_grid(int64_t tokens, std::initializer_list<int> heads, int 
   int i = 0;
   for (int h : heads) {
     g.groups[i] = (uint32_t)(many ? (h + per - 1) / per : h);
-    g.all += g.groups[i++];
+    g.begin[i + 1] = g.begin[i] + (uint32_t)((tokens * g.groups[i] * lanes_of(chunks) + 255) / 256);
+    ++i;
   }
+  for (; i < 3; ++i) g.begin[i + 1] = g.begin[i];
   return g;
 }
 
 template <int DT, int HG, bool STREAM, typename Rows>
 hipError_t norm_chunks_go(const Rows& rows, const NormGrid& g, hipStream_t st) {
   const int lanes = lanes_of((int)g.chunks);
-  const dim3 grid((unsigned)(((int64_t)g.tokens * g.all * lanes + 255) / 256)), block(256);
+  const dim3 grid(g.begin[Rows::KINDS]), block(256);
   switch (lanes) {
     case 4: hipLaunchKernelGGL((ago_norm_chunk_kernel<DT, 4, HG, STREAM, Rows>), grid, block, 0, st, rows, g); break;
     case 8: hipLaunchKernelGGL((ago_norm_chunk_kernel<DT, 8, HG, STREAM, Rows>), grid, block, 0, st, rows, g); break;
@@ -496,7 +491,10 @@ hipError_t norm_go(const NormArgs& a, hipStream_t st) {
 
 template <int DT>
 hipError_t append_norm_go(const AppendArgs& a, const HeadNorm& n, hipStream_t st) {
-  const AppendRows rows{a, n};
+  const AppendRows rows{{a.q, a.k, a.v}, {a.q_out, a.k_pages, a.v_pages}, {a.q_t, a.k_t, a.v_t}, {a.q_h, a.k_h, a.v_h},
+                        {(int64_t)a.heads * a.dim, a.ps.k_page, a.ps.v_page}, {a.dim, a.ps.k_head, a.ps.v_head},
+                        {0, a.ps.k_slot, a.ps.v_slot}, {a.heads, a.kv_heads, a.kv_heads}, a.slots, a.capacity, a.page_size,
+                        a.dim, n, a.rot};
   const int64_t heads = (int64_t)a.heads + 2 * a.kv_heads;
   if constexpr (DT != AFA_F64) {
     constexpr int EPC = RowChunk<DT>::EPC;
@@ -520,11 +518,11 @@ inline void parts_of(NormParts& p, int64_t most, int64_t q, int64_t k, int64_t p
   p.parts[0] = (uint32_t)(a < nq ? a : nq);
   p.parts[1] = k == 0 ? 0 : (uint32_t)(b < nk ? b : nk);
 }
-inline int64_t most_parts(int cus) { return 8 * (int64_t)cus; }
+inline int64_t most_parts(int cus) { return 2 * (int64_t)cus; }
 
 template <int DT, int HG>
 hipError_t norm_bwd_chunks_go(const NormArgs& a, const NormGrid& g, const NormParts& p, hipStream_t st) {
-  const dim3 grid(p.parts[0] + p.parts[1]), block(256);
+  const dim3 grid(p.parts[0] + p.parts[1]), block(BWD);
   switch (lanes_of((int)g.chunks)) {
     case 4: hipLaunchKernelGGL((ago_norm_bwd_chunk_kernel<DT, 4, HG>), grid, block, 0, st, a, g, p); break;
     case 8: hipLaunchKernelGGL((ago_norm_bwd_chunk_kernel<DT, 8, HG>), grid, block, 0, st, a, g, p); break;
@@ -553,7 +551,7 @@ hipError_t norm_bwd_go(const NormArgs& a, void* const dscale[2], void* ws, int c
       bool many;
       constexpr int HG = 2;
       const NormGrid g = norm_grid(tokens, {a.heads[0], a.heads[1]}, a.dim / EPC, a.sx[0][1] < a.sx[0][2], HG, many);
-      parts_of(p, most_parts(cus), tokens * g.groups[0], tokens * g.groups[1], 256 / lanes_of(a.dim / EPC));
+      parts_of(p, most_parts(cus), tokens * g.groups[0], tokens * g.groups[1], BWD / lanes_of(a.dim / EPC));
       e = many ? norm_bwd_chunks_go<DT, HG>(a, g, p, st) : norm_bwd_chunks_go<DT, 1>(a, g, p, st);
     }
   }
