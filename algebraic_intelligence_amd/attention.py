@@ -544,17 +544,18 @@ def apply_ago_axis_rotations(q, k, rotary_params, positions, sections=None):
 # ------------------------------------------------------------------- norms of q and k with their rotation
 def _norm_scale(name, scale, head_dim, dtype, dev):
     """A norm's scale in fp32 (fp64 for fp64 inputs), contiguous."""
+    want = torch.float64 if dtype is torch.float64 else torch.float32
+    if (isinstance(scale, torch.Tensor) and scale.dtype is want and scale.shape == (head_dim,) and scale.device == dev
+            and scale.is_contiguous()):
+        return scale  # as the kernel takes it
     if not isinstance(scale, torch.Tensor) or not scale.is_floating_point():
-        raise TypeError(f"{name} must be a floating point tensor, got {type(scale) if not isinstance(scale, torch.Tensor) else scale.dtype}")
+        raise TypeError(f"{name} must be a floating point tensor, got {scale.dtype if isinstance(scale, torch.Tensor) else type(scale)}")
     if scale.shape != (head_dim,):
         raise ValueError(f"{name} must have shape ({head_dim},), got {tuple(scale.shape)}")
     if scale.device != dev:
         _lib.require_device(scale)
         raise ValueError(f"{name} must be on {dev}, got {scale.device}")
-    want = torch.float64 if dtype is torch.float64 else torch.float32
-    if scale.dtype is not want:
-        scale = scale.to(want)
-    return scale if scale.is_contiguous() else scale.contiguous()
+    return scale.to(want).contiguous()
 
 
 def _norm_eps(eps):
@@ -605,53 +606,88 @@ def _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg):
 
 def _norm_backward_launch(q, k, gq, gk, q_scale, k_scale, c, s, positions, cfg):
     q, dq, sq, sdq = _row_layout(q)
-    gq = gq if gq.stride(3) == 1 else gq.contiguous()
     sgq = gq.stride()
+    if sgq[3] != 1:
+        gq = gq.contiguous()
+        sgq = gq.stride()
     B, H, L, D = q.shape
-    acc = {"dtype": q_scale.dtype, "device": q.device}
-    dqs = torch.empty(D, **acc)
-    K, dk, dks, kp, gkp, dkp, sk, sgk, sdk = 0, None, None, None, None, None, sq, sgq, sdq
-    if k is not None:
+    dqs = torch.empty_like(q_scale)
+    if k is None:
+        K, dk, dks, kp, gkp, dkp, ksp, dksp, sk, sgk, sdk = 0, None, None, None, None, None, None, None, sq, sgq, sdq
+    else:
         k, dk, sk, sdk = _row_layout(k)
-        gk = gk if gk.stride(3) == 1 else gk.contiguous()
-        sgk, dks = gk.stride(), torch.empty(D, **acc)
-        K, kp, gkp, dkp = k.shape[1], k.data_ptr(), gk.data_ptr(), dk.data_ptr()
+        sgk = gk.stride()
+        if sgk[3] != 1:
+            gk = gk.contiguous()
+            sgk = gk.stride()
+        dks = torch.empty_like(k_scale)
+        K, kp, gkp, dkp, ksp, dksp = k.shape[1], k.data_ptr(), gk.data_ptr(), dk.data_ptr(), k_scale.data_ptr(), dks.data_ptr()
     dev, at = q.device, cfg.axes
     with _lib.on_device(dev):
         size = _lib.workspace_size("ago_norm_rotate_axes_bwd_workspace_size", dev, at.dtype, D)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         rc = _lib.lib().ago_norm_rotate_axes_bwd(
             at.dtype, B, H, K, L, D, q.data_ptr(), kp, gq.data_ptr(), gkp, dq.data_ptr(), dkp,
-            _lib.pack18(*sq[:3], *sk[:3], *sgq[:3], *sgk[:3], *sdq[:3], *sdk[:3]), q_scale.data_ptr(), _lib.ptr(k_scale),
-            dqs.data_ptr(), _lib.ptr(dks), cfg.eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+            _lib.pack18(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sgq[0], sgq[1], sgq[2], sgk[0], sgk[1], sgk[2],
+                        sdq[0], sdq[1], sdq[2], sdk[0], sdk[1], sdk[2]),
+            q_scale.data_ptr(), ksp, dqs.data_ptr(), dksp, cfg.eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
             _lib.ptr(positions), at.pos_bytes, at.pos_b, at.axes, at.cuts, ws.data_ptr(), size, _lib.stream_ptr(dev))
     _lib.check(rc, "ago_norm_rotate_axes_bwd")
     return dq, dk, dqs, dks
 
 
 class _NormRotate(torch.autograd.Function):
-    """Norm, scale and rotation of q, and of k where there is one; the VJP forms the norm again from q and k."""
+    """Norm, scale and rotation of q, and of k where there is one; the VJP forms the norm again from q and k.
+
+    The tables and positions have no gradient and are kept beside the saved tensors, which is half the time of saving
+    them; their versions are compared as autograd compares those."""
 
     @staticmethod
     def forward(ctx, q, k, q_scale, k_scale, c, s, positions, cfg):
-        ctx.save_for_backward(q, k, q_scale, k_scale, c, s, positions)
-        ctx.cfg = cfg
+        ctx.save_for_backward(q, k, q_scale, k_scale)
+        ctx.cfg = c, s, positions, cfg
+        ctx.versions = _versions(c, s, positions)
         ctx.set_materialize_grads(False)
         y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
         return y if k is None else (y, z)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk=None):
-        q, k, q_scale, k_scale, *rest = ctx.saved_tensors
-        dq = dk = dqs = dks = None
-        if gq is not None and gk is not None:
-            dq, dk, dqs, dks = _norm_backward_launch(q, k, gq, gk, q_scale, k_scale, *rest, ctx.cfg)
-        elif gq is not None:
-            dq, _, dqs, _ = _norm_backward_launch(q, None, gq, None, q_scale, None, *rest, ctx.cfg)
-        elif gk is not None:
-            dk, _, dks, _ = _norm_backward_launch(k, None, gk, None, k_scale, None, *rest, ctx.cfg)
-        return dq, dk, dqs, dks, None, None, None, None
+        # recorded for a second derivative, which there is not: what follows it raises an error
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, gq, gk)
+
+
+def _versions(*tensors):
+    return [t._version for t in tensors if t is not None]
+
+
+def _norm_backward(ctx, gq, gk):
+    q, k, q_scale, k_scale = ctx.saved_tensors
+    c, s, positions, cfg = ctx.cfg
+    if ctx.versions != _versions(c, s, positions):
+        raise RuntimeError("the rotary tables or the positions of apply_ago_norm_rotations have been modified by an inplace "
+                           "operation before its backward pass")
+    dq = dk = dqs = dks = None
+    if gq is not None and gk is not None:
+        dq, dk, dqs, dks = _norm_backward_launch(q, k, gq, gk, q_scale, k_scale, c, s, positions, cfg)
+    elif gq is not None:
+        dq, _, dqs, _ = _norm_backward_launch(q, None, gq, None, q_scale, None, c, s, positions, cfg)
+    elif gk is not None:
+        dk, _, dks, _ = _norm_backward_launch(k, None, gk, None, k_scale, None, c, s, positions, cfg)
+    return dq, dk, dqs, dks, None, None, None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
+
+
+def _norm_rotate(q, k, q_scale, k_scale, c, s, positions, cfg):
+    # within a forward-mode level an input may carry a tangent, which autograd refuses
+    if (torch.is_grad_enabled() and (q.requires_grad or q_scale.requires_grad
+                                     or (k is not None and (k.requires_grad or k_scale.requires_grad)))
+            or forward_ad._current_level >= 0):
+        return _NormRotate.apply(q, k, q_scale, k_scale, c, s, positions, cfg)
+    y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
+    return y if k is None else (y, z)
 
 
 def apply_ago_norm_rotations(q, k, q_scale, k_scale, rotary_params=None, positions=None, sections=None, *, eps=1e-6):
@@ -705,19 +741,11 @@ def apply_ago_norm_rotations(q, k, q_scale, k_scale, rotary_params=None, positio
         cuts = _axis_sections(sections, axes, D // 2)
     cfg = _NormConfig(_AxesConfig(dt, pos_bytes, pos_b, axes, cuts), eps)
 
-    def run(q, k, q_scale, k_scale):
-        grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_scale, k_scale))
-        # within a forward-mode level an input may carry a tangent, which autograd refuses
-        if grads or forward_ad._current_level >= 0:
-            return _NormRotate.apply(q, k, q_scale, k_scale, c, s, positions, cfg)
-        y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
-        return y if k is None else (y, z)
-
     if q.numel() != 0 and (k is None or k.numel() != 0):
-        return run(q, k, q_scale, k_scale)
+        return _norm_rotate(q, k, q_scale, k_scale, c, s, positions, cfg)
     # tensors without rows, whose gradients are as empty
     none = lambda x, scale: x * scale.to(x.dtype)  # noqa: E731
-    y = none(q, q_scale) if q.numel() == 0 else run(q, None, q_scale, None)
+    y = none(q, q_scale) if q.numel() == 0 else _norm_rotate(q, None, q_scale, None, c, s, positions, cfg)
     if k is None:
         return y
-    return y, none(k, k_scale) if k.numel() == 0 else run(k, None, k_scale, None)
+    return y, none(k, k_scale) if k.numel() == 0 else _norm_rotate(k, None, k_scale, None, c, s, positions, cfg)

@@ -23,9 +23,9 @@ namespace afa {
 namespace {
 
 constexpr int PICK = 1024, PICK_WAVES = PICK / 64;
-constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // lanes spread over copies: neighbours often share a bin
+constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // of a bin, in banks of their own: neighbours often share one
 constexpr int LOADS = 8;                                  // weights of a thread in flight
-constexpr int MOVE = 256, BATCH = 16;                     // threads of a mover, and units that each holds
+constexpr int MOVE = 256, BATCH = 8;                      // threads of a mover, and units that each holds
 
 // The workspace: tokens that stay (requests, budget); the first place that moves (requests,); sources before each chunk's
 // places, and behind the last's (requests, chunks + 1); chunks handed out (requests, streams) and chunks that are read (requests, streams, chunks), a
@@ -94,14 +94,22 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
     const unsigned mask = (1u << (above - shift)) - 1;
     for (int i = tid; i < COPIES * BINS; i += PICK) bins[i] = 0;
     __syncthreads();
+    // the next batch comes while this one is counted
+    float v[LOADS], next[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) next[k] = w[min(lo + k * PICK + tid, hi - 1)];
     for (int base = lo; base < hi; base += LOADS * PICK) {
-      unsigned u[LOADS];
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k) u[k] = order_bits(w[min(base + k * PICK + tid, hi - 1)]);
+      for (int k = 0; k < LOADS; ++k) {
+        v[k] = next[k];
+        next[k] = w[min(base + (LOADS + k) * PICK + tid, hi - 1)];
+      }
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k)
-        if (base + k * PICK + tid < hi && (above == 32 || u[k] >> above == top >> above))
-          atomicAdd(&bins[(lane % COPIES) * BINS + (u[k] >> shift & mask)], 1);
+      for (int k = 0; k < LOADS; ++k) {
+        const unsigned u = order_bits(v[k]);
+        if (base + k * PICK + tid < hi && (above == 32 || u >> above == top >> above))
+          atomicAdd(&bins[(u >> shift & mask) * COPIES + lane % COPIES], 1);
+      }
     }
     __syncthreads();
     // the bin in which the need-th largest lies: thread t has bins of rank 2 t and 2 t + 1 from the top
@@ -111,7 +119,7 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
     for (int k = 0; k < 2; ++k) {
       n[k] = 0;
 #pragma unroll
-      for (int i = 0; i < COPIES; ++i) n[k] += bins[i * BINS + BINS - 1 - 2 * tid - k];
+      for (int i = 0; i < COPIES; ++i) n[k] += bins[(BINS - 1 - 2 * tid - k) * COPIES + i];
     }
     const int upto = lanes_up_to(n[0] + n[1]);
     if (lane == 63) wave_sum[wave] = upto;
@@ -140,12 +148,17 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
   }
   // those above `top` stay, and the first `need` that equal it
   int over = 0, equal = 0, start = budget;  // of the tokens before this batch: above and sure ones, and equal ones
+  float v[LOADS], next[LOADS];
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) next[k] = w[min(k * PICK + tid, c - 1)];
   for (int base = 0; base < c; base += LOADS * PICK) {
-    float v[LOADS];
     int kind[LOADS];  // 2: stays, 1: equal, 0: neither
     unsigned long long overs[LOADS], equals[LOADS];
 #pragma unroll
-    for (int k = 0; k < LOADS; ++k) v[k] = w[min(base + k * PICK + tid, c - 1)];
+    for (int k = 0; k < LOADS; ++k) {
+      v[k] = next[k];
+      next[k] = w[min(base + (LOADS + k) * PICK + tid, c - 1)];
+    }
     __syncthreads();  // counts is free
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
@@ -200,7 +213,7 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
 
 // Rows as `units` of type T each; a chunk is BATCH units a thread, a.rows rows.
 template <typename T>
-__global__ __launch_bounds__(MOVE) void afa_paged_move_kernel(const EvictArgs a, int units) {
+__global__ __launch_bounds__(MOVE, 5) void afa_paged_move_kernel(const EvictArgs a, int units) {
   __shared__ int ticket;
   const EvictSpace s = evict_space(a);
   const int64_t streams = a.requests * 2 * a.kv_heads, stream = blockIdx.x % streams;

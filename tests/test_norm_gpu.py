@@ -324,3 +324,13 @@ def test_norm_refusals():
         A.append_to_cache(q, k, k, kp, vp, plan, tab, norms=(w, w), eps=-1)
     with pytest.raises(RuntimeError, match="gradient"):
         A.append_to_cache(q, k, k, kp, vp, plan, tab, norms=(w.clone().requires_grad_(True), w))
+
+
+def test_norm_changed_positions_are_noticed():
+    """Positions changed between the two passes are an error, not another gradient."""
+    q, w = torch.randn(1, 2, 3, 64, device="cuda", requires_grad=True), torch.ones(64, device="cuda")
+    pos = torch.zeros(3, 1, device="cuda", dtype=torch.int64)
+    y = A.apply_ago_norm_rotations(q, None, w, None, _tables(20, 64), pos)
+    pos += 1
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
