@@ -183,7 +183,8 @@ struct EvictArgs {
   int32_t* lens;
   int32_t* space;        // paged_evict_workspace bytes
   int budget, first, recent, esz;
-  int rows, chunks;      // set by the launch: places of a chunk, and chunks of a budget
+  int rows, chunks;      // set by the launch: places of a chunk, a power of two; chunks of a budget; and the
+  int log_page;          // logarithm of a page_size that is one, or -1
 };
 size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim);
 hipError_t paged_evict_launch(EvictArgs a, hipStream_t st);

@@ -27,7 +27,7 @@ constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // of a bin, in banks 
 constexpr int LOADS = 8;                                  // weights of a thread in flight
 constexpr int MOVE = 256, BATCH = 8;                      // threads of a mover, and units that each holds
 
-// The workspace: tokens that stay (requests, budget); the first place that moves (requests,); sources before each chunk's
+// The workspace: slots of the tokens that stay, page * page_size + offset, or -1 for a page of no pool (requests, budget); the first place that moves (requests,); sources before each chunk's
 // places, and behind the last's (requests, chunks + 1); chunks handed out (requests, streams) and chunks that are read (requests, streams, chunks), a
 // stream being one head's k or v.
 struct EvictSpace {
@@ -49,6 +49,13 @@ __device__ __forceinline__ unsigned order_bits(float w) {
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.0f);
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Slot of a request's token.
+__device__ __forceinline__ int slot_of(const EvictArgs& a, const int32_t* table, int pos) {
+  const unsigned P = (unsigned)a.page_size, at = a.log_page >= 0 ? (unsigned)pos >> a.log_page : (unsigned)pos / P;
+  const int page = table[at];
+  return page < 0 || page >= a.num_pages ? -1 : page * (int)P + (int)((unsigned)pos - at * P);
 }
 
 // Inclusive sums of x over the lanes up to this one.
@@ -82,6 +89,8 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
     if (tid == 0) s.moved[r] = m;
     return;
   }
+  const int32_t* table = a.block_tables + (int64_t)r * a.table_width;
+  const int log_rows = __builtin_ctz((unsigned)a.rows);
   int32_t* before = s.before + (int64_t)r * (a.chunks + 1);
   for (int i = tid; i <= a.chunks; i += PICK)
     if ((int64_t)i * a.rows >= c) before[i] = m;
@@ -190,9 +199,9 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
       const int2 b = counts[k * PICK_WAVES + wave];
       const int o = over + b.x + __popcll(overs[k] & below), e = equal + b.y + __popcll(equals[k] & below);
       const int to = o + min(e, need);
-      if (i < c && i % a.rows == 0 && i / a.rows <= a.chunks) before[i / a.rows] = to;
+      if (i < c && (i & (a.rows - 1)) == 0 && i >> log_rows <= a.chunks) before[i >> log_rows] = to;
       if (kind[k] == 2 || (kind[k] == 1 && e < need)) {
-        kept[to] = i;
+        kept[to] = slot_of(a, table, i);
         left[to] = v[k];
         if (to != i) start = min(start, to);
       }
@@ -219,58 +228,63 @@ __global__ __launch_bounds__(MOVE, 5) void afa_paged_move_kernel(const EvictArgs
   const int64_t streams = a.requests * 2 * a.kv_heads, stream = blockIdx.x % streams;
   const int r = (int)(stream / (2 * a.kv_heads)), which = (int)(stream % (2 * a.kv_heads)), hk = which >> 1;
   const bool is_v = which & 1;
-  const int m = a.lens[r], start = s.moved[r];
-  // chunks in which a token moves
-  const int begin = start / a.rows, end = (m + a.rows - 1) / a.rows;
-  if (start >= m) return;
   const int32_t *kept = s.kept + (int64_t)r * a.budget, *table = a.block_tables + (int64_t)r * a.table_width;
   const int32_t* before = s.before + (int64_t)r * (a.chunks + 1);
   int32_t* read = s.read + stream * a.chunks;
   char* pages = (char*)(is_v ? a.v_pages : a.k_pages) + hk * (is_v ? a.ps.v_head : a.ps.k_head) * a.esz;
-  const int64_t page = (is_v ? a.ps.v_page : a.ps.k_page) * a.esz, slot = (is_v ? a.ps.v_slot : a.ps.k_slot) * a.esz;
+  const int64_t page = (is_v ? a.ps.v_page : a.ps.k_page) * a.esz, step = (is_v ? a.ps.v_slot : a.ps.k_slot) * a.esz;
   const unsigned P = (unsigned)a.page_size;
-  auto place = [&](int pos) -> char* {
-    const unsigned at = (unsigned)pos / P;
-    const int id = table[at];
-    return id < 0 || id >= a.num_pages ? nullptr : pages + id * page + ((unsigned)pos - at * P) * slot;
+  const int log_rows = __builtin_ctz((unsigned)a.rows);
+  auto row = [&](int slot) {
+    const unsigned at = a.log_page >= 0 ? (unsigned)slot >> a.log_page : (unsigned)slot / P;
+    return pages + at * page + ((unsigned)slot - at * P) * step;
   };
+  const int m = a.lens[r], start = s.moved[r];  // from place `start` on every token moves
+  const int begin = start >> log_rows, end = start < m ? (m + a.rows - 1) >> log_rows : 0;
   for (;;) {
-    __syncthreads();  // ticket has been read
-    if (threadIdx.x == 0) ticket = begin + atomicAdd(s.next + stream, 1);
+    // begin and end come with the counter, not before it: what a workgroup reads one after the other is what bounds it
+    if (threadIdx.x == 0) ticket = atomicAdd(s.next + stream, 1);
     __syncthreads();
-    const int chunk = ticket;
+    const int chunk = begin + ticket;
     if (chunk >= end) return;
-    const int first = chunk * a.rows, count = min(a.rows, m - first) * units;
+    const int first = chunk << log_rows, count = min(a.rows, m - first) * units;
+    // sources [low, high) lie in this chunk's places: the first's chunk and the last's have to be read
+    int other = -1;
+    if (threadIdx.x < 2) {
+      const int low = before[chunk], high = before[chunk + 1];
+      if (low < high) other = (threadIdx.x == 0 ? low : high - 1) >> log_rows;
+      if (other >= chunk || other < begin) other = -1;
+    }
     T x[BATCH];
     unsigned moves = 0;
+    int from[BATCH];
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int e = u * MOVE + (int)threadIdx.x;
-      if (e >= count) continue;
-      const int i = e / units, from = kept[first + i];
-      const char* p = place(from);
-      if (from == first + i || p == nullptr) continue;
-      moves |= 1u << u;
-      x[u] = *(const T*)(p + (e - i * units) * sizeof(T));
+      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
+      from[u] = e < count && first + i >= start ? kept[first + i] : -1;
     }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
+      if (from[u] < 0) continue;
+      moves |= 1u << u;
+      x[u] = *(const T*)(row(from[u]) + (e - i * units) * sizeof(T));
+    }
+    bool ready = other < 0 || __hip_atomic_load(read + other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
     // every read of the chunk is done
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) __hip_atomic_store(read + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // sources [low, high) lie in this chunk's places: the first's chunk and the last's
-    if (threadIdx.x < 2) {
-      const int low = before[chunk], high = before[chunk + 1];
-      const int other = (threadIdx.x == 0 ? low : high - 1) / a.rows;
-      if (low < high && other < chunk && other >= begin)
-        while (__hip_atomic_load(read + other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(1);
+    while (!ready) {
+      __builtin_amdgcn_s_sleep(1);
+      ready = __hip_atomic_load(read + other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       if (!(moves >> u & 1)) continue;
-      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
-      char* q = place(first + i);
-      if (q != nullptr) *(T*)(q + (e - i * units) * sizeof(T)) = x[u];
+      const int e = u * MOVE + (int)threadIdx.x, i = e / units, to = slot_of(a, table, first + i);
+      if (to >= 0) *(T*)(row(to) + (e - i * units) * sizeof(T)) = x[u];
     }
   }
 }
@@ -279,7 +293,9 @@ __global__ __launch_bounds__(MOVE, 5) void afa_paged_move_kernel(const EvictArgs
 
 // Chunks are shortest where units are elements.
 size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim) {
-  const int64_t rows = std::max<int64_t>(1, MOVE * BATCH / head_dim), chunks = (budget + rows - 1) / rows;
+  int64_t rows = 1;
+  while (2 * rows * head_dim <= MOVE * BATCH) rows *= 2;
+  const int64_t chunks = (budget + rows - 1) / rows;
   return (size_t)(requests * (budget + 2 + chunks + 2 * kv_heads * (1 + chunks))) * 4;
 }
 
@@ -290,7 +306,9 @@ hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
                     a.ps.k_slot * a.esz, a.ps.v_page * a.esz, a.ps.v_head * a.esz, a.ps.v_slot * a.esz})
     while (v % unit != 0) unit /= 2;
   const int units = (int)(bytes / unit);
-  a.rows = MOVE * BATCH / units;
+  a.rows = 1;  // a power of two
+  while (2 * a.rows * units <= MOVE * BATCH) a.rows *= 2;
+  a.log_page = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)a.page_size) : -1;
   a.chunks = (a.budget + a.rows - 1) / a.rows;
   hipLaunchKernelGGL(afa_paged_pick_kernel, dim3((unsigned)a.requests), dim3(PICK), 0, st, a);
   hipError_t e = hipGetLastError();
