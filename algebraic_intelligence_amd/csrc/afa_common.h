@@ -305,6 +305,23 @@ __device__ __forceinline__ void lds_dma16(const void* src, const void* lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(m0) : "memory", "m0");
 }
 
+// ------------------------------------------------------------------ LDS tiles of 32 keys
+// K chunk c of tile row r sits at c ^ k_key(r).  At DP = 128 a 256-byte row is one bank period and
+// r & 15 spreads the 16 rows of a fragment read's pass (16 lanes x 16 bytes) over its 16 slots; at
+// DP = 64 an even and an odd row share a period, and (r >> 1) & 7 takes all 8 positions over the
+// even rows and over the odd ones (r & 7 took them over 8 rows only: 2-way conflicts).
+template <int DP>
+__device__ __forceinline__ int k_key(int r) {
+  if constexpr (DP == 128) return r & 15;
+  else return (r >> 1) & 7;
+}
+
+template <int D>
+__device__ __forceinline__ int v_swizzle(int r, int c) {
+  if constexpr (D == 128) return c ^ ((r & 3) << 2);
+  else return c ^ (((r >> 1) & 1) << 2);
+}
+
 // s_waitcnt immediate that waits for vmcnt <= n only (gfx9: vmcnt [3:0] and [15:14]; expcnt and
 // lgkmcnt at their no-wait maxima).
 __host__ __device__ constexpr int vmcnt_only(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4) | (0xF << 8); }

@@ -88,22 +88,6 @@ __device__ __forceinline__ float tree16x(const float (&p)[16]) {
   return a[0] + a[2];
 }
 
-// K chunk c of tile row r sits at c ^ k_key(r).  At DP = 128 a 256-byte row is one bank period and
-// r & 15 spreads the 16 rows of a fragment read's pass (16 lanes x 16 bytes) over its 16 slots; at
-// DP = 64 an even and an odd row share a period, and (r >> 1) & 7 takes all 8 positions over the
-// even rows and over the odd ones (r & 7 took them over 8 rows only: 2-way conflicts).
-template <int DP>
-__device__ __forceinline__ int k_key(int r) {
-  if constexpr (DP == 128) return r & 15;
-  else return (r >> 1) & 7;
-}
-
-template <int D>
-__device__ __forceinline__ int v_swizzle(int r, int c) {
-  if constexpr (D == 128) return c ^ ((r & 3) << 2);
-  else return c ^ (((r >> 1) & 1) << 2);
-}
-
 template <int DP>
 struct PipeShape {
   static constexpr int NB = 4;                  // ring of tile buffers

@@ -818,8 +818,8 @@ hipError_t tile_go(const PagedFast& f, int rows, hipStream_t st) {
   // 32 rows: a wave's own where two row blocks fit its registers, else two waves that meet the same keys
   if (rows == 32) return tile_launch<DT, D, ROW <= 128 ? 2 : 1, ROW <= 128 ? 1 : 2, PREFIX>(f, st);
   if (rows == 64) return tile_launch<DT, D, 1, 4, PREFIX>(f, st);
-  if constexpr (ROW <= 256) return tile_launch<DT, D, 2, 4, PREFIX>(f, st);
-  return hipErrorInvalidValue;  // no plan has more than 64 rows of these
+  if constexpr (ROW <= 256 && !(PREFIX && DT != AFA_F32)) return tile_launch<DT, D, 2, 4, PREFIX>(f, st);
+  return hipErrorInvalidValue;  // no plan has more than 64 rows of these, or a kernel of their own has them
 }
 
 template <int DT, bool PREFIX>

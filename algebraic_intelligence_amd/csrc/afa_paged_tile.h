@@ -54,6 +54,14 @@ __device__ __forceinline__ float rho8_by_score(float s) {
   return low ? __builtin_amdgcn_rcpf(__builtin_fminf(p8, kMostPower)) : p8;  // a NaN stays one
 }
 
+// Makes values new ones to the compiler, at no cost.  In one side of a branch over both forms of the weights it keeps what
+// they share from being formed once for both, and the branch from turning into a select, which would cost every tile both.
+template <int N>
+__device__ __forceinline__ void apart(float (&w)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm volatile("" : "+v"(w[e]));
+}
+
 // The power of two by which a row's fp16 weights begin.  It is only ever lowered, so it decides how small weights may
 // be that have a row to themselves: 2^-120, a score of -16384, is 1 then.  A first weight of about 1 lowers it
 // at once, as any start does; its inverse and that of the lowest, 2^-123, are normal numbers.

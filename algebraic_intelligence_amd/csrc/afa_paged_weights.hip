@@ -257,6 +257,8 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
                 for (int i = 0; i < 4; ++i) w[u][i] = rho8_fast(w[u][i]);
             } else {
 #pragma unroll
+              for (int u = 0; u < NG; ++u) apart(w[u]);
+#pragma unroll
               for (int u = 0; u < NG; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[u][i] = rho8_by_score(w[u][i]);

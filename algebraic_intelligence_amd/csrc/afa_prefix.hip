@@ -1,9 +1,348 @@
 // A prefix that all requests share, met once by the rows of all the step's tokens: sum_j w_ij v_j and sum_j w_ij over its
-// keys in fp32 (afa_paged_attend.h, PREFIX), for the attention of the requests' own keys to start from.  The sums are
-// additive, so that nothing else passes between the two launches.
+// keys in fp32, for the attention of the requests' own keys to start from.  The sums are additive, so that nothing else
+// passes between the two launches.
+//
+// Up to 64 rows a key head, fp32, and head_dim 256 run on the paged kernel (afa_paged_attend.h, PREFIX).  More rows of bf16
+// and fp16 are a product of matrices, which the kernel below is for: four waves of 32 rows each share a ring of four tiles of
+// 32 keys in LDS, filled by direct loads three tiles ahead.
+//
+//   S^T = K Q^T    32 keys x 32 rows; a lane ends with 16 keys' scores of row lane % 32
+//   w = rho^8      in place, the B operand of
+//   O^T += V^T w   V's columns by transposing LDS reads, in the order of keys that S^T leaves
+//
+// While a wave forms the weights of a tile, the scores of the next one are on the matrix cores, and the other wave of its
+// SIMD has its products there.  Weights enter the product rounded to the type, as in the training forward: vector and matrix
+// instructions bound this kernel, and the second plane that the paged kernel keeps would be a third of its products and a
+// sixth of its vector instructions.  The rounding is as large as the result's own.  Row sums are of the weights in fp32.
+// The line of a key head's tiles over all row blocks is cut into even stretches, one for each resident workgroup, and what a
+// cut leaves of a row block is joined as in the paged kernel.
 #include "afa_paged_attend.h"
 
 namespace afa {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+template <int DT>
+__device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (DT == AFA_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0,
+                                                   0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+constexpr int WIDE_ROWS = 32 * WAVES, RING = 4;
+
+template <int DT, int D>
+__global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const PagedFast f) {
+  constexpr int DP = D <= 64 ? 64 : 128;
+  constexpr int CH = DP / 8, CHD = D / 8;          // 16-byte chunks of a row in LDS, and of data
+  constexpr int LPT = kPagedTile * CH / THREADS;   // direct loads of a thread for K of a tile, and for V
+  constexpr int LOADS = 2 * LPT;
+  constexpr int NK = DP / 16, NDB = DP / 32;
+  __shared__ __attribute__((aligned(1024))) unsigned short lds_k[RING][kPagedTile * DP], lds_v[RING][kPagedTile * DP];
+  __shared__ float sums[WIDE_ROWS];
+  __shared__ int flag;
+  const PagedFwdArgs& a = f.a;
+  const afa_paged_plan& p = a.plan;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5, l16 = lane & 15, m16 = lane >> 4 & 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int H = (int)p.heads, G = a.group, L = a.prefix.len;
+  // bf16 at head_dim 128: q carries 2^-4, x = s / sqrt(2), and the weights 1/16: (rho(s) / sqrt(2))^8 is formed from x without s.
+  // Powers of two are exact there; in fp16 they would cost small numbers their digits.
+  constexpr bool HALF = DT == AFA_BF16 && D == 128;
+  const float scale = (float)a.scale;
+  // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
+  const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads), hk = (int)(blockIdx.x - (unsigned)slot * (unsigned)p.kv_heads);
+  const char* k_base = (const char*)a.prefix.k + hk * a.prefix.k_head * 2;
+  const char* v_base = (const char*)a.prefix.v + hk * a.prefix.v_head * 2;
+  const int nrows = p.starts[p.requests] * G, tiles = (L + kPagedTile - 1) / kPagedTile, cost = kPagedLead + tiles;
+  const int64_t end = (int64_t)((nrows + WIDE_ROWS - 1) / WIDE_ROWS) * cost;
+  const int64_t stretch = max((end + f.slots - 1) / f.slots, (int64_t)kPagedMin);
+  int64_t pos = slot * stretch;
+  const int64_t stop = min(pos + stretch, end);
+  int block = (int)(pos / cost), unit0 = (int)(pos - (int64_t)block * cost);
+  const int64_t head0 = (int64_t)hk * 2 * f.slots * WIDE_ROWS;
+  float *part_den = f.part_den + head0, *part_sum = f.part_sum + head0;
+  const __amdgpu_buffer_rsrc_t buffer =
+      __builtin_amdgcn_make_buffer_rsrc(f.part + head0 * D, 0, (int)(2 * f.slots * WIDE_ROWS * D * 4), 0x00020000);
+
+  while (pos < stop) {
+    const int row0 = block * WIDE_ROWS, take = (int)min((int64_t)(cost - unit0), stop - pos);
+    const int t0 = max(unit0 - kPagedLead, 0), t1 = unit0 + take - kPagedLead;
+    // the slots that hold keys of this row block
+    const int64_t key0 = pos - unit0 + kPagedLead;
+    const int from_slot = (int)(key0 / stretch), parts = (int)((key0 + tiles - 1) / stretch) - from_slot + 1;
+    pos += take;
+    unit0 += take;
+    if (unit0 == cost) {
+      unit0 = 0;
+      ++block;
+    }
+    if (t0 >= t1) continue;
+
+    // this lane's row, features 16 kc + 8 g .. of chunk kc
+    const int row = min(row0 + 32 * wave + l32, nrows - 1), token = row / G;
+    const int64_t q_row = (int64_t)token * H + hk * G + (row - token * G);
+    u32x4_t qf[NK];
+    {
+      const char* x = (const char*)a.q + ((int64_t)token * a.q_t + (hk * G + row - token * G) * a.q_h) * 2;
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc)
+        qf[kc] = CHD == CH || 2 * kc + g < CHD ? *(const u32x4_t*)(x + (2 * kc + g) * 16) : u32x4_t{0, 0, 0, 0};
+    }
+    if constexpr (HALF) {
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned u = qf[kc][e];
+          qf[kc][e] = Elem<DT>::pack(Elem<DT>::lo(u) * 0.0625f, Elem<DT>::hi(u) * 0.0625f);
+        }
+    }
+    // they are here before the ring's first loads, which the compiler does not count
+#pragma unroll
+    for (int kc = 0; kc < NK; ++kc) asm volatile("" : "+v"(qf[kc]));
+    __syncthreads();  // the ring is free of the row block before
+
+    // Tile t into buffer buf.  What lies behind the prefix's last row, and chunks behind a row's features, is out of the
+    // resource's range and comes as zeros.
+    auto issue = [&](int t, int buf) {
+      const uint32_t rows = (uint32_t)min(L - t * kPagedTile, kPagedTile) - 1;
+      const i32x4_t k = raw_buffer_srd(k_base + (uint64_t)(uint32_t)(t * kPagedTile) * f.k_slot, rows * f.k_slot + D * 2);
+      const i32x4_t v = raw_buffer_srd(v_base + (uint64_t)(uint32_t)(t * kPagedTile) * f.v_slot, rows * f.v_slot + D * 2);
+#pragma unroll
+      for (int i = 0; i < LPT; ++i) {
+        const int s = tid + THREADS * i, r = s / CH, c = s % CH, ck = c ^ k_key<DP>(r), cv = v_swizzle<DP>(r, c);
+        const uint32_t ko = CHD == CH || ck < CHD ? (uint32_t)r * f.k_slot + 16 * ck : 0xfffffff0u;
+        const uint32_t vo = CHD == CH || cv < CHD ? (uint32_t)r * f.v_slot + 16 * cv : 0xfffffff0u;
+        lds_dma16_buf(k, ko, &lds_k[buf][(THREADS * i + wave * 64) * 8]);
+        lds_dma16_buf(v, vo, &lds_v[buf][(THREADS * i + wave * 64) * 8]);
+      }
+    };
+    f32x16_t o[NDB], s_even, s_odd;
+    float den = 0.0f, sc = kFirstScale;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
+
+    auto scores = [&](int buf, f32x16_t& s) {
+      u32x4_t kf[NK];
+      const unsigned short* at = &lds_k[buf][l32 * DP];
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc) kf[kc] = *(const u32x4_t*)(at + (((2 * kc + g) ^ k_key<DP>(l32)) * 8));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int kc = 0; kc < NK; ++kc) s = mma32<DT>(kf[kc], qf[kc], s);
+    };
+    // weights of a tile's scores and its products; MASK: keys from L on weigh nothing
+    auto meet = [&](int t, int buf, const f32x16_t& s, auto mask) {
+      u32x4_t vf[NDB][2];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const int r = kk * 16 + hh * 8 + 4 * g + (l16 >> 2), col = db * 32 + m16 * 16 + 4 * (l16 & 3);
+            const unsigned short* at = &lds_v[buf][r * DP + v_swizzle<DP>(r, col >> 3) * 8 + (col & 7)];
+            const u32x2_t w = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)at));
+            vf[db][kk][2 * hh] = w[0];
+            vf[db][kk][2 * hh + 1] = w[1];
+          }
+      __builtin_amdgcn_sched_barrier(0);
+      float w[16];
+      float least = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        w[e] = HALF ? s[e] : s[e] * scale;
+        least = __builtin_fminf(least, w[e]);
+      }
+      // a score that is no number takes either form
+      if (__ballot(!(least > (HALF ? kLowScore * 0.70710678f : kLowScore))) == 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = HALF ? rho8_fast_half(w[e]) : rho8_fast(w[e]);
+      } else {
+        apart(w);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = HALF ? 0.0625f * rho8_by_score(w[e] * 1.41421356f) : rho8_by_score(w[e]);
+      }
+      if constexpr (decltype(mask)::value) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = t * kPagedTile + (e >> 2) * 8 + 4 * g + (e & 3) < L ? w[e] : 0.0f;
+      }
+      float tree[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tree[e] = w[e] + w[e + 8];
+      den += ((tree[0] + tree[4]) + (tree[1] + tree[5])) + ((tree[2] + tree[6]) + (tree[3] + tree[7]));
+      if constexpr (DT == AFA_F16) {
+        float top = w[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = __builtin_fmaxf(top, w[e]);
+        if (__ballot(!(top * sc <= 32768.0f)) != 0) {
+          // a row's largest weight so far now lies in [16, 32)
+          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+          if (top * sc > 32768.0f && top < __builtin_inff()) {
+            const int e = (__builtin_bit_cast(int, top) >> 23) - 127;
+            const float to = __builtin_bit_cast(float, (127 + 4 - e) << 23);
+            const float ratio = to / sc;
+            sc = to;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[db] *= ratio;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] *= sc;
+      }
+      u32x4_t wp[2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wp[kk][e] = Elem<DT>::pack(w[kk * 8 + 2 * e], w[kk * 8 + 2 * e + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db] = mma32<DT>(vf[db][kk], wp[kk], o[db]);
+    };
+
+    const int n = t1 - t0;
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+      if (i < n) issue(t0 + i, i);
+    if (n >= RING - 1) __builtin_amdgcn_s_waitcnt(vmcnt_only(LOADS * (RING - 2)));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    __syncthreads();
+    scores(0, s_even);
+    // before tile u's weights: this wave's loads of tile u + 1 are done, those of u + 2 may go on; then every wave's, and every
+    // wave has read tile u - 1, whose place the next one takes
+    auto step = [&](int u, int buf) {
+      if (u + 2 < n) __builtin_amdgcn_s_waitcnt(vmcnt_only(LOADS * (RING - 3)));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      __syncthreads();
+      if (u + RING - 1 < n) issue(t0 + u + RING - 1, (buf + RING - 1) & (RING - 1));
+    };
+    auto more = [&](int u, int buf, const f32x16_t& now, f32x16_t& next) {  // tile u has a next one
+      step(u, buf);
+      scores((buf + 1) & (RING - 1), next);
+      meet(t0 + u, buf, now, std::false_type());
+    };
+    auto last = [&](int u, int buf, const f32x16_t& now) {
+      step(u, buf);
+      if (t1 * kPagedTile > L) meet(t0 + u, buf, now, std::true_type());
+      else meet(t0 + u, buf, now, std::false_type());
+    };
+    int u = 0;
+    for (; u + 4 < n; u += 4) {
+      more(u, 0, s_even, s_odd);
+      more(u + 1, 1, s_odd, s_even);
+      more(u + 2, 2, s_even, s_odd);
+      more(u + 3, 3, s_odd, s_even);
+    }
+    if (u + 2 < n) {
+      more(u, u & 3, s_even, s_odd);
+      more(u + 1, (u + 1) & 3, s_odd, s_even);
+      u += 2;
+    }
+    if (u + 1 < n) {
+      more(u, u & 3, s_even, s_odd);
+      last(u + 1, (u + 1) & 3, s_odd);
+    } else {
+      last(u, u & 3, s_even);
+    }
+
+    den += __shfl_xor(den, 32);
+    if constexpr (HALF) den *= 16.0f;
+    // a power of two takes the weights' back
+    const float back = HALF ? 16.0f : DT == AFA_F16 ? __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc)) : 1.0f;
+    auto part_of = [&](int i) { return (int64_t)2 * (from_slot + i) + (i == 0); };
+    const int64_t my_part = part_of(slot - from_slot);
+    const bool mine = row0 + 32 * wave + l32 < nrows;
+    float zero = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int d = db * 32 + r4 * 8 + 4 * g;
+        f32x4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = o[db][4 * r4 + i] * back;
+          zero = __builtin_fmaf(x[i], 0.0f, zero);
+        }
+        if (!mine || (D < DP && d >= D)) continue;
+        if (parts > 1) put4(buffer, (uint32_t)((my_part * WIDE_ROWS + 32 * wave + l32) * D + d) * 4, x);
+        else *(f32x4_t*)(f.shared.top + q_row * D + d) = x;
+      }
+    if (mine && g == 0) {
+      if (parts > 1) put1(part_den + my_part * WIDE_ROWS + 32 * wave + l32, den);
+      else f.shared.bottom[q_row] = den;
+    }
+    // A value that is not finite is the sum of every row, as weights are above 0.  It may have become NaN in the product, where
+    // a weight may be rounded to 0: such sums are formed again, from these values alone.
+    if (mine && zero != 0.0f) {
+      float* to = parts > 1 ? f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D : f.shared.top + q_row * D;
+      for (int d = 4 * g; d < D; d += 8)
+        for (int i = d; i < d + 4; ++i) {
+          float y = 0.0f;
+          for (int key = t0 * kPagedTile; key < min(t1 * kPagedTile, L); ++key) {
+            const float z = Elem<DT>::load(v_base + (uint64_t)(uint32_t)key * f.v_slot, i);
+            if (!(__builtin_fabsf(z) < __builtin_inff())) y += z;
+          }
+          if (!(__builtin_fabsf(y) < __builtin_inff())) put1(to + i, y);
+        }
+    }
+    if (parts == 1) continue;
+
+    const int size = group_size(parts), groups = (parts + size - 1) / size, g0 = (slot - from_slot) / size * size;
+    const int here = min(size, parts - g0), all = min(WIDE_ROWS, nrows - row0);
+    int* count = a.sched.count + (int64_t)hk * 4 * f.slots;
+    if (!arrived(count + part_of(g0), here, &flag)) continue;
+    auto store4 = [&](int r, int d, f32x4_t x) {
+      const int who = (row0 + r) / G;
+      const int64_t at = (int64_t)who * H + hk * G + (row0 + r - who * G);
+      *(f32x4_t*)(f.shared.top + at * D + d) = x;
+      if (d == 0) f.shared.bottom[at] = sums[r];
+    };
+    const int64_t to = part_of(g0) * WIDE_ROWS;
+    sum_parts<THREADS>(buffer, part_den, here, all, D, sums, [&](int i) { return part_of(g0 + i) * WIDE_ROWS; },
+                       [&](int r, int d, f32x4_t x) {
+                         if (groups == 1) {
+                           store4(r, d, x);
+                         } else {
+                           // over the group's first part, of which this thread alone reads these features
+                           put4(buffer, (uint32_t)((to + r) * D + d) * 4, x);
+                           if (d == 0) put1(part_sum + to + r, sums[r]);
+                         }
+                       });
+    if (groups == 1 || !arrived(count + 2 * f.slots + part_of(0), groups, &flag)) continue;
+    sum_parts<THREADS>(buffer, part_sum, groups, all, D, sums, [&](int i) { return part_of(i * size) * WIDE_ROWS; }, store4);
+  }
+}
+
+template <int DT, int D>
+hipError_t wide_launch(const PagedFast& f, hipStream_t st) {
+  hipLaunchKernelGGL((afa_prefix_wide_kernel<DT, D>), dim3((unsigned)(f.slots * f.a.plan.kv_heads)), dim3(THREADS), 0, st, f);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t wide_go(const PagedFast& f, hipStream_t st) {
+  switch (f.dim) {
+    case 32: return wide_launch<DT, 32>(f, st);
+    case 48: return wide_launch<DT, 48>(f, st);
+    case 64: return wide_launch<DT, 64>(f, st);
+    case 96: return wide_launch<DT, 96>(f, st);
+    default: return wide_launch<DT, 128>(f, st);
+  }
+}
+
+}  // namespace
 
 PagedCut prefix_cut(const afa_paged_plan& p, int cus) {
   afa_paged_plan all = p;
@@ -13,7 +352,10 @@ PagedCut prefix_cut(const afa_paged_plan& p, int cus) {
 
 hipError_t prefix_sums_launch(const PagedFwdArgs& a, const PagedCut& c, const PrefixSums& shared, void* ws, hipStream_t st) {
   const PrefixKeys& x = a.prefix;
-  return fast_launch<true>(paged_fast_args(a, c, PageStrides{0, x.k_head, x.k_key, 0, x.v_head, x.v_key}, shared, ws), c.rows, st);
+  const PagedFast f = paged_fast_args(a, c, PageStrides{0, x.k_head, x.k_key, 0, x.v_head, x.v_key}, shared, ws);
+  if (c.rows == WIDE_ROWS && a.plan.dtype != AFA_F32)
+    return a.plan.dtype == AFA_BF16 ? wide_go<AFA_BF16>(f, st) : wide_go<AFA_F16>(f, st);
+  return fast_launch<true>(f, c.rows, st);
 }
 
 }  // namespace afa
