@@ -14,8 +14,9 @@
 // SIMD has its products there.  Weights enter the product rounded to the type, as in the training forward: vector and matrix
 // instructions bound this kernel, and the second plane that the paged kernel keeps would be a third of its products and a
 // sixth of its vector instructions.  The rounding is as large as the result's own.  Row sums are of the weights in fp32.
-// The line of a key head's tiles over all row blocks is cut into even stretches, one for each resident workgroup, and what a
-// cut leaves of a row block is joined as in the paged kernel.
+// The line of a key head's tiles over all row blocks is cut into even stretches, one for each resident workgroup.  What a cut
+// leaves of a row block is added up by a launch of its own, which has all of the device for it: the last workgroup of a row block
+// alone takes longer (84 us in all for 40 and 7, 256 rows of 4 heads behind 8192), and so does the own keys' launch (16 us more).
 #include "afa_paged_attend.h"
 
 namespace afa {
@@ -36,6 +37,15 @@ __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 
 constexpr int WIDE_ROWS = 32 * WAVES, RING = 4;
 
+// Parts of a row block that the join adds up; of more, groups are added up first, each by its last workgroup.
+constexpr int WIDE_PARTS = 16;
+__host__ __device__ inline int wide_group(int parts) { return (parts + WIDE_PARTS - 1) / WIDE_PARTS; }
+// The length of a slot's stretch of a key head's line.
+__device__ __forceinline__ int64_t wide_stretch(int nrows, int cost, int64_t slots) {
+  const int64_t end = (int64_t)((nrows + WIDE_ROWS - 1) / WIDE_ROWS) * cost;
+  return max((end + slots - 1) / slots, (int64_t)kPagedMin);
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const PagedFast f) {
   constexpr int DP = D <= 64 ? 64 : 128;
@@ -50,7 +60,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   const afa_paged_plan& p = a.plan;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5, l16 = lane & 15, m16 = lane >> 4 & 1;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int H = (int)p.heads, G = a.group, L = a.prefix.len;
+  const int G = a.group, L = a.prefix.len;
   // bf16 at head_dim 128: q carries 2^-4, x = s / sqrt(2), and the weights 1/16: (rho(s) / sqrt(2))^8 is formed from x without s.
   // Powers of two are exact there; in fp16 they would cost small numbers their digits.
   constexpr bool HALF = DT == AFA_BF16 && D == 128;
@@ -61,7 +71,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   const char* v_base = (const char*)a.prefix.v + hk * a.prefix.v_head * 2;
   const int nrows = p.starts[p.requests] * G, tiles = (L + kPagedTile - 1) / kPagedTile, cost = kPagedLead + tiles;
   const int64_t end = (int64_t)((nrows + WIDE_ROWS - 1) / WIDE_ROWS) * cost;
-  const int64_t stretch = max((end + f.slots - 1) / f.slots, (int64_t)kPagedMin);
+  const int64_t stretch = wide_stretch(nrows, cost, f.slots);
   int64_t pos = slot * stretch;
   const int64_t stop = min(pos + stretch, end);
   int block = (int)(pos / cost), unit0 = (int)(pos - (int64_t)block * cost);
@@ -86,7 +96,6 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
 
     // this lane's row, features 16 kc + 8 g .. of chunk kc
     const int row = min(row0 + 32 * wave + l32, nrows - 1), token = row / G;
-    const int64_t q_row = (int64_t)token * H + hk * G + (row - token * G);
     u32x4_t qf[NK];
     {
       const char* x = (const char*)a.q + ((int64_t)token * a.q_t + (hk * G + row - token * G) * a.q_h) * 2;
@@ -262,6 +271,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     const float back = HALF ? 16.0f : DT == AFA_F16 ? __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc)) : 1.0f;
     auto part_of = [&](int i) { return (int64_t)2 * (from_slot + i) + (i == 0); };
     const int64_t my_part = part_of(slot - from_slot);
+    const int size = wide_group(parts);
     const bool mine = row0 + 32 * wave + l32 < nrows;
     float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
@@ -276,17 +286,15 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
           zero = __builtin_fmaf(x[i], 0.0f, zero);
         }
         if (!mine || (D < DP && d >= D)) continue;
-        if (parts > 1) put4(buffer, (uint32_t)((my_part * WIDE_ROWS + 32 * wave + l32) * D + d) * 4, x);
-        else *(f32x4_t*)(f.shared.top + q_row * D + d) = x;
+        // a part that is added up here goes where every XCD sees it
+        if (size > 1) put4(buffer, (uint32_t)((my_part * WIDE_ROWS + 32 * wave + l32) * D + d) * 4, x);
+        else *(f32x4_t*)(f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D + d) = x;
       }
-    if (mine && g == 0) {
-      if (parts > 1) put1(part_den + my_part * WIDE_ROWS + 32 * wave + l32, den);
-      else f.shared.bottom[q_row] = den;
-    }
+    if (mine && g == 0) put1(part_den + my_part * WIDE_ROWS + 32 * wave + l32, den);
     // A value that is not finite is the sum of every row, as weights are above 0.  It may have become NaN in the product, where
     // a weight may be rounded to 0: such sums are formed again, from these values alone.
     if (mine && zero != 0.0f) {
-      float* to = parts > 1 ? f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D : f.shared.top + q_row * D;
+      float* to = f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D;
       for (int d = 4 * g; d < D; d += 8)
         for (int i = d; i < d + 4; ++i) {
           float y = 0.0f;
@@ -297,31 +305,61 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
           if (!(__builtin_fabsf(y) < __builtin_inff())) put1(to + i, y);
         }
     }
-    if (parts == 1) continue;
+    if (size == 1) continue;
 
-    const int size = group_size(parts), groups = (parts + size - 1) / size, g0 = (slot - from_slot) / size * size;
-    const int here = min(size, parts - g0), all = min(WIDE_ROWS, nrows - row0);
-    int* count = a.sched.count + (int64_t)hk * 4 * f.slots;
-    if (!arrived(count + part_of(g0), here, &flag)) continue;
-    auto store4 = [&](int r, int d, f32x4_t x) {
-      const int who = (row0 + r) / G;
-      const int64_t at = (int64_t)who * H + hk * G + (row0 + r - who * G);
-      *(f32x4_t*)(f.shared.top + at * D + d) = x;
-      if (d == 0) f.shared.bottom[at] = sums[r];
-    };
+    // the last of a group to finish adds its parts up, over the first of them
+    const int g0 = (slot - from_slot) / size * size, here = min(size, parts - g0);
+    if (!arrived(a.sched.count + (int64_t)hk * 4 * f.slots + part_of(g0), here, &flag)) continue;
     const int64_t to = part_of(g0) * WIDE_ROWS;
-    sum_parts<THREADS>(buffer, part_den, here, all, D, sums, [&](int i) { return part_of(g0 + i) * WIDE_ROWS; },
+    sum_parts<THREADS>(buffer, part_den, here, min(WIDE_ROWS, nrows - row0), D, sums,
+                       [&](int i) { return part_of(g0 + i) * WIDE_ROWS; },
                        [&](int r, int d, f32x4_t x) {
-                         if (groups == 1) {
-                           store4(r, d, x);
-                         } else {
-                           // over the group's first part, of which this thread alone reads these features
-                           put4(buffer, (uint32_t)((to + r) * D + d) * 4, x);
-                           if (d == 0) put1(part_sum + to + r, sums[r]);
-                         }
+                         // of the first part this thread alone reads these features
+                         put4(buffer, (uint32_t)((to + r) * D + d) * 4, x);
+                         if (d == 0) put1(part_sum + to + r, sums[r]);
                        });
-    if (groups == 1 || !arrived(count + 2 * f.slots + part_of(0), groups, &flag)) continue;
-    sum_parts<THREADS>(buffer, part_sum, groups, all, D, sums, [&](int i) { return part_of(i * size) * WIDE_ROWS; }, store4);
+  }
+}
+
+// The parts of every row added up in their order: a thread has four features of a row.
+__global__ __launch_bounds__(THREADS) void afa_prefix_join_kernel(const PagedFast f) {
+  const afa_paged_plan& p = f.a.plan;
+  const int D = f.dim, quads = D / 4, G = f.a.group, H = (int)p.heads;
+  const int nrows = p.starts[p.requests] * G, tiles = (f.a.prefix.len + kPagedTile - 1) / kPagedTile, cost = kPagedLead + tiles;
+  const int64_t stretch = wide_stretch(nrows, cost, f.slots), all = (int64_t)nrows * (int)p.kv_heads * quads;
+  for (int64_t e = (int64_t)blockIdx.x * THREADS + threadIdx.x; e < all; e += (int64_t)gridDim.x * THREADS) {
+    // rows of the call one after the other: token, then head
+    const int d = 4 * (int)(e % quads), at = (int)(e / quads), token = at / H, hk = (at - token * H) / G;
+    const int row = token * G + (at - token * H - hk * G), block = row / WIDE_ROWS, r = row - block * WIDE_ROWS;
+    const int64_t key0 = (int64_t)block * cost + kPagedLead, from = key0 / stretch;
+    const int parts = (int)((key0 + tiles - 1) / stretch - from) + 1, size = wide_group(parts), n = (parts + size - 1) / size;
+    const float* den = size > 1 ? f.part_sum : f.part_den;
+    // part i of the row block: a slot's second where it begins there, else its first
+    auto place = [&](int i) {
+      return ((int64_t)hk * 2 * f.slots + 2 * (from + (int64_t)i * size) + (i == 0)) * WIDE_ROWS + r;
+    };
+    f32x4_t x = {0, 0, 0, 0};
+    float sum = 0.0f;
+    constexpr int N = 8;
+    for (int i0 = 0; i0 < n; i0 += N) {
+      f32x4_t y[N];
+      float z[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        y[i] = f32x4_t{0, 0, 0, 0};
+        z[i] = 0.0f;
+        if (i0 + i >= n) continue;
+        y[i] = *(const f32x4_t*)(f.part + place(i0 + i) * D + d);
+        if (d == 0) z[i] = den[place(i0 + i)];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x += y[i];
+        sum += z[i];
+      }
+    }
+    *(f32x4_t*)(f.shared.top + (int64_t)at * D + d) = x;
+    if (d == 0) f.shared.bottom[at] = sum;
   }
 }
 
@@ -353,9 +391,12 @@ PagedCut prefix_cut(const afa_paged_plan& p, int cus) {
 hipError_t prefix_sums_launch(const PagedFwdArgs& a, const PagedCut& c, const PrefixSums& shared, void* ws, hipStream_t st) {
   const PrefixKeys& x = a.prefix;
   const PagedFast f = paged_fast_args(a, c, PageStrides{0, x.k_head, x.k_key, 0, x.v_head, x.v_key}, shared, ws);
-  if (c.rows == WIDE_ROWS && a.plan.dtype != AFA_F32)
-    return a.plan.dtype == AFA_BF16 ? wide_go<AFA_BF16>(f, st) : wide_go<AFA_F16>(f, st);
-  return fast_launch<true>(f, c.rows, st);
+  if (c.rows != WIDE_ROWS || a.plan.dtype == AFA_F32) return fast_launch<true>(f, c.rows, st);
+  const hipError_t e = a.plan.dtype == AFA_BF16 ? wide_go<AFA_BF16>(f, st) : wide_go<AFA_F16>(f, st);
+  if (e != hipSuccess) return e;
+  const int64_t groups = (a.plan.max_tokens * a.plan.heads * (a.plan.head_dim / 4) + THREADS - 1) / THREADS;
+  hipLaunchKernelGGL(afa_prefix_join_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(THREADS), 0, st, f);
+  return hipGetLastError();
 }
 
 }  // namespace afa
