@@ -36,6 +36,7 @@ __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 }
 
 constexpr int WIDE_ROWS = 32 * WAVES, RING = 4;
+constexpr float kFirstRoot = 0x1p15f;  // the eighth root of kFirstScale
 
 // Parts of a row block that the join adds up; of more, groups are added up first, each by its last workgroup.
 constexpr int WIDE_PARTS = 16;
@@ -61,10 +62,11 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5, l16 = lane & 15, m16 = lane >> 4 & 1;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.group, L = a.prefix.len;
-  // bf16 at head_dim 128: q carries 2^-4, x = s / sqrt(2), and the weights 1/16: (rho(s) / sqrt(2))^8 is formed from x without s.
-  // Powers of two are exact there; in fp16 they would cost small numbers their digits.
-  constexpr bool HALF = DT == AFA_BF16 && D == 128;
-  const float scale = (float)a.scale;
+  // With y = c s, (c rho(s))^8 = (y + sqrt(y^2 + c^2))^8: a factor of the weights costs nothing where the scores carry its eighth
+  // root.  In bf16 q carries 1/8, exactly, so that y is what the products give and c^2 = D / 64.  In fp16, where small
+  // numbers would lose digits, y = kappa q.k, and kappa takes the power of two by which a row's weights are scaled too.
+  constexpr bool F16 = DT == AFA_F16;
+  constexpr float C2 = (float)D / 64, LOW = kLowScore * (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
   // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
   const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads), hk = (int)(blockIdx.x - (unsigned)slot * (unsigned)p.kv_heads);
   const char* k_base = (const char*)a.prefix.k + hk * a.prefix.k_head * 2;
@@ -103,13 +105,13 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       for (int kc = 0; kc < NK; ++kc)
         qf[kc] = CHD == CH || 2 * kc + g < CHD ? *(const u32x4_t*)(x + (2 * kc + g) * 16) : u32x4_t{0, 0, 0, 0};
     }
-    if constexpr (HALF) {
+    if constexpr (!F16) {
 #pragma unroll
       for (int kc = 0; kc < NK; ++kc)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned u = qf[kc][e];
-          qf[kc][e] = Elem<DT>::pack(Elem<DT>::lo(u) * 0.0625f, Elem<DT>::hi(u) * 0.0625f);
+          qf[kc][e] = Elem<DT>::pack(Elem<DT>::lo(u) * 0.125f, Elem<DT>::hi(u) * 0.125f);
         }
     }
     // they are here before the ring's first loads, which the compiler does not count
@@ -133,7 +135,8 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       }
     };
     f32x16_t o[NDB], s_even, s_odd;
-    float den = 0.0f, sc = kFirstScale;
+    float den = 0.0f;
+    float kappa = kFirstRoot * 0.125f, c2 = C2 * kFirstRoot * kFirstRoot;  // fp16: 2^k / 8 and 4^k C2
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -150,7 +153,12 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       for (int kc = 0; kc < NK; ++kc) s = mma32<DT>(kf[kc], qf[kc], s);
     };
     // weights of a tile's scores and its products; MASK: keys from L on weigh nothing
-    auto meet = [&](int t, int buf, const f32x16_t& s, auto mask) {
+    auto meet = [&](int t, int buf, f32x16_t s, auto mask) {
+      auto behind = [&](int e) { return t * kPagedTile + (e >> 2) * 8 + 4 * g + (e & 3) >= L; };
+      if constexpr (decltype(mask)::value) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = behind(e) ? -__builtin_inff() : s[e];
+      }
       u32x4_t vf[NDB][2];
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -166,48 +174,72 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
           }
       __builtin_amdgcn_sched_barrier(0);
       float w[16];
+      if constexpr (F16) {
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          w[e] = s[e] * kappa;
+          top = __builtin_fmaxf(top, w[e]);
+        }
+        // weights end at kMost^8 = 32768: y ends where y + sqrt(y^2 + c2) is kMost
+        constexpr float kMost = 3.6680162f;
+        if (__ballot(!(top <= __builtin_fmaf(c2, -0.5f / kMost, 0.5f * kMost))) != 0) {
+          // a row's largest weight so far now lies in [1, 256)
+          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+          const float z = top + __builtin_sqrtf(__builtin_fmaf(top, top, c2));
+          if (z > kMost && z < __builtin_inff()) {
+            const int j = (__builtin_bit_cast(int, z) >> 23) - 127;  // 0 to 2^7 and more
+            const float root = __builtin_bit_cast(float, max(127 - j, 1) << 23);
+            const float ratio = 8 * j < 127 ? __builtin_bit_cast(float, (127 - 8 * j) << 23) : 0.0f;
+            kappa *= root;
+            c2 *= root * root;
+            den *= ratio;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] *= root;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[db] *= ratio;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = s[e];
+      }
+      const float cc = F16 ? c2 : C2, low = F16 ? LOW * 8.0f * kappa : LOW;
       float least = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        w[e] = HALF ? s[e] : s[e] * scale;
-        least = __builtin_fminf(least, w[e]);
-      }
+      for (int e = 0; e < 16; ++e) least = __builtin_fminf(least, w[e]);
       // a score that is no number takes either form
-      if (__ballot(!(least > (HALF ? kLowScore * 0.70710678f : kLowScore))) == 0) {
+      if (__ballot(!(least > low)) == 0) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = HALF ? rho8_fast_half(w[e]) : rho8_fast(w[e]);
+        for (int e = 0; e < 16; ++e) {
+          const float t = __builtin_fmaf(w[e], w[e], cc);
+          const float rho = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), w[e]);
+          const float p2 = rho * rho;
+          const float p4 = p2 * p2;
+          w[e] = p4 * p4;
+        }
       } else {
         apart(w);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = HALF ? 0.0625f * rho8_by_score(w[e] * 1.41421356f) : rho8_by_score(w[e]);
+        for (int e = 0; e < 16; ++e) {
+          // far below 0 without cancellation, and above 0 to the end: -infinity weighs 2^-126 too; a NaN stays one
+          const float y = w[e], t = __builtin_fmaf(y, y, cc);
+          const float far = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), y <= low ? __builtin_fabsf(y) : y);
+          const float rho = y <= low ? cc * __builtin_amdgcn_rcpf(far) : far;
+          const float p2 = rho * rho;
+          const float p4 = p2 * p2;
+          const float p8 = p4 * p4;
+          w[e] = y < -0x1p60f || p8 < 0x1p-126f ? 0x1p-126f : p8;
+        }
       }
       if constexpr (decltype(mask)::value) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = t * kPagedTile + (e >> 2) * 8 + 4 * g + (e & 3) < L ? w[e] : 0.0f;
+        for (int e = 0; e < 16; ++e) w[e] = behind(e) ? 0.0f : w[e];
       }
       float tree[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) tree[e] = w[e] + w[e + 8];
       den += ((tree[0] + tree[4]) + (tree[1] + tree[5])) + ((tree[2] + tree[6]) + (tree[3] + tree[7]));
-      if constexpr (DT == AFA_F16) {
-        float top = w[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = __builtin_fmaxf(top, w[e]);
-        if (__ballot(!(top * sc <= 32768.0f)) != 0) {
-          // a row's largest weight so far now lies in [16, 32)
-          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-          if (top * sc > 32768.0f && top < __builtin_inff()) {
-            const int e = (__builtin_bit_cast(int, top) >> 23) - 127;
-            const float to = __builtin_bit_cast(float, (127 + 4 - e) << 23);
-            const float ratio = to / sc;
-            sc = to;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) o[db] *= ratio;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] *= sc;
-      }
       u32x4_t wp[2];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -266,9 +298,14 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     }
 
     den += __shfl_xor(den, 32);
-    if constexpr (HALF) den *= 16.0f;
-    // a power of two takes the weights' back
-    const float back = HALF ? 16.0f : DT == AFA_F16 ? __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, sc)) : 1.0f;
+    // the factor is taken back: c^8, and in fp16 the rows' powers of two
+    constexpr float C8 = C2 * C2 * C2 * C2;
+    float back = 1.0f / C8;
+    if constexpr (F16) {
+      const int k = (__builtin_bit_cast(int, kappa) >> 23) - 127 + 3;
+      back *= __builtin_bit_cast(float, min(max(127 - 8 * k, 1), 254) << 23);
+    }
+    den *= back;
     auto part_of = [&](int i) { return (int64_t)2 * (from_slot + i) + (i == 0); };
     const int64_t my_part = part_of(slot - from_slot);
     const int size = wide_group(parts);
