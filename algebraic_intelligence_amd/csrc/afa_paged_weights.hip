@@ -5,10 +5,10 @@
 // with d the denominators that the step's attention returned, sink and prefix included.  A token of the step
 // itself has no weight yet: its place is set, not added to.
 //
-// On the matrix cores (bf16, fp16, fp32; head_dim 32, 48, 64, 96, 128, 256; pages of a power of two) a workgroup takes 32
-// keys of one request.  S = Q K^T with 16 rows of Q as A and two times 16 keys as B leaves each lane with the scores
-// of one key in a group, so that the sum over the rows stays in the lane; K is in registers for all rows of its head, and
-// Q comes from the caches.  The four waves share a head's row blocks, or the heads where these are few, and add up in
+// On the matrix cores (bf16, fp16, fp32; head_dim 32, 48, 64, 96, 128, 256; pages of a power of two) a workgroup takes 64
+// keys of one request (32 where rows are longer than 256 bytes).  S = Q K^T with 16 rows of Q as A and four times 16 keys as
+// B leaves each lane with the scores of one key in a group, so that the sum over the rows stays in the lane; K is in registers
+// for all rows of its head, and Q comes from the caches.  The four waves share a head's row blocks, or the heads where these are few, and add up in
 // LDS.  Where the requests' tiles are too few to fill the device, workgroups share a tile's heads too, and the last one
 // of a tile adds their parts in order.  So every sum has one order, which atomics would not give it.
 #include <algorithm>
@@ -76,21 +76,22 @@ hipError_t weight_keys_go(const WeightArgs& a, int cus, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------ matrix cores
-// parts of tiles that share their heads
+// parts of tiles that share their heads, and the most keys of a tile
 constexpr int64_t kWeightParts = 4096;
-constexpr int WTILE = 32, WAVES = 4, THREADS = 64 * WAVES;
+constexpr int MOST_KEYS = 64;
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr int SCAN = 4 * THREADS;  // requests whose tiles a workgroup counts at a time
 
 struct WeightFast {
   WeightArgs a;
-  float* part;      // (tiles * splits, WTILE)
+  float* part;      // (tiles * splits, keys of a tile)
   int* count;       // of a tile's parts; 0 between calls
   int most;         // parts that there is room for
   int log_page;
 };
 
-// Sums of x over the threads before this one; all: over the workgroup.
-__device__ __forceinline__ int tiles_before(int x, int* lds, int& all) {
+// Sums of x over the threads before this one.
+__device__ __forceinline__ int tiles_before(int x, int* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int s = x;
 #pragma unroll
@@ -101,26 +102,37 @@ __device__ __forceinline__ int tiles_before(int x, int* lds, int& all) {
   if (lane == 63) lds[wave] = s;
   __syncthreads();
   int base = 0;
-  all = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w == wave) base = all;
-    all += lds[w];
-  }
+  for (int w = 0; w < WAVES - 1; ++w)
+    if (w < wave) base += lds[w];
   return base + s - x;
 }
 
+// Groups of 16 keys of a tile: as many as leave their rows of K room in the registers.
 template <int DT, int D>
-__global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const WeightFast f) {
+constexpr int key_groups() {
+  return D * (DT == AFA_F32 ? 4 : 2) <= 256 ? 4 : 2;
+}
+
+// Workgroups that a CU's registers hold, and as many are launched for each: with a third more, which wait for the first to
+// end, 64 requests of one token over up to 8192 take 111 us for 78.
+template <int DT, int D>
+constexpr int resident() {
+  constexpr int bytes = D * (DT == AFA_F32 ? 4 : 2);
+  return bytes <= 128 ? 3 : bytes <= 512 ? 2 : 1;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight_tile_kernel(const WeightFast f) {
   constexpr bool F32 = DT == AFA_F32;
   constexpr int ESZ = F32 ? 4 : 2;
   constexpr int EPC = 16 / ESZ;           // features of a 16-byte chunk
   constexpr int KB = 4 * EPC;             // of a chunk over the four lane groups
   constexpr int KS = (D + KB - 1) / KB;   // chunks of a row a lane
   constexpr bool FULL = D % KB == 0;
-  constexpr int NG = WTILE / 16;
+  constexpr int NG = key_groups<DT, D>(), TILE = 16 * NG;
   __shared__ int first[SCAN + 1], scan[WAVES], flag;
-  __shared__ float red[WAVES][WTILE];
+  __shared__ float red[WAVES][TILE];
   const WeightArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
@@ -138,12 +150,11 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
         n[u] = 0;
         if (r < R && p.status[r] == AFA_PAGED_OK) {
           const int fresh = p.starts[r + 1] - p.starts[r];
-          if (fresh > 0) n[u] = (int)((unsigned)(a.sched.cached[r] + fresh + WTILE - 1) / WTILE);
+          if (fresh > 0) n[u] = (int)((unsigned)(a.sched.cached[r] + fresh + TILE - 1) / TILE);
         }
         sum += n[u];
       }
-      int all;
-      int at = tiles_before(sum, scan, all);
+      int at = tiles_before(sum, scan);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         first[4 * tid + u] = at;
@@ -153,19 +164,18 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
       __syncthreads();
     }
     const int tiles = first[SCAN];
+    const int coarse = first[SCAN / 64 * lane];
     // heads of a tile over so many workgroups; requests beyond the first SCAN would need counts of their own
     const int splits = R <= SCAN && tiles > 0 ? max(1, min(K, f.most / tiles)) : 1;
     const int64_t items = (int64_t)tiles * splits;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
       const int tile = (int)(item / splits), split = (int)(item - (int64_t)tile * splits);
-      // the request: the last whose first tile is not behind this one
-      int lo = 0, hi = SCAN;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= tile) lo = mid;
-        else hi = mid;
-      }
-      const int r = r0 + lo, kb = (tile - first[lo]) * WTILE;
+      // the request: the last whose first tile is not behind this one, in two steps of the lanes
+      static_assert(SCAN / 64 <= 64, "entries between two coarse ones");
+      const int step = SCAN / 64, at0 = (__popcll(__ballot(coarse <= tile)) - 1) * step;
+      const int mine = first[at0 + min(lane, step - 1)];
+      const int lo = __builtin_amdgcn_readfirstlane(at0 + __popcll(__ballot(lane < step && mine <= tile)) - 1);
+      const int r = r0 + lo, kb = (tile - first[lo]) * TILE;
       const int start = p.starts[r], n = p.starts[r + 1] - start, c = a.sched.cached[r], keys = c + n, nrows = n * G;
       const bool tree = a.masks != nullptr && n <= p.max_tree;
       // this lane's keys, and where their rows lie
@@ -178,12 +188,19 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
         krow[u] = (const char*)a.k_pages +
                   ((lost[u] ? 0 : page) * a.k_page + (int64_t)(pos & in_page) * a.k_slot + EPC * g) * ESZ;
       }
+      // what the tile's tokens had, which is needed last
+      const int pos = kb + tid;
+      float* to = a.weights + r * a.row + pos;
+      const float old = tid < TILE && pos < c ? *to : 0.0f;
       // chains: row blocks whose last token is before the tile see nothing of it
       const int blocks = (nrows + 15) / 16;
-      const int block0 = tree || kb <= c ? 0 : (kb - c) * G / 16;
+      const int block0 = tree || kb <= c ? 0 : (int)((int64_t)(kb - c) * G / 16);
       // waves that share a head's row blocks
       const int share = blocks - block0 >= WAVES ? WAVES : blocks - block0 >= 2 ? 2 : 1;
       const int heads_at_once = WAVES / share, rsub = wave % share;
+      // a lane's row, 16 * share further on each time: its token and head of the group
+      const int row0 = 16 * (block0 + rsub) + m, token0 = row0 / G, in0 = row0 - token0 * G;
+      const int more_tokens = 16 * share / G, more_in = 16 * share - more_tokens * G;
       float acc[NG];
 #pragma unroll
       for (int u = 0; u < NG; ++u) acc[u] = 0.0f;
@@ -198,24 +215,36 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
         float head[NG];
 #pragma unroll
         for (int u = 0; u < NG; ++u) head[u] = 0.0f;
-        for (int b = block0 + rsub; b < blocks; b += share) {
-          const int row = min(16 * b + m, nrows - 1), token = row / G;
-          const char* x = (const char*)a.q +
-                          ((int64_t)(start + token) * a.q_t + (hk * G + row - token * G) * a.q_h + EPC * g) * ESZ;
-          u32x4_t qf[KS];
+        int token = token0, in = in0;
+        u32x4_t next[KS];
+        float next_den;
+        // the row's features and its denominator; behind the last row that one's
+        auto load = [&]() {
+          const int t = start + min(token, n - 1), h = hk * G + (token < n ? in : G - 1);
+          const char* x = (const char*)a.q + ((int64_t)t * a.q_t + h * a.q_h + EPC * g) * ESZ;
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks)
-            qf[ks] = FULL || KB * ks + EPC * g < D ? *(const u32x4_t*)(x + KB * ks * ESZ) : u32x4_t{0, 0, 0, 0};
-          // over the rows' denominators; rows behind the last have none, nor has one that saw no key
-          float over[4];
-          int who[4];
+            next[ks] = FULL || KB * ks + EPC * g < D ? *(const u32x4_t*)(x + KB * ks * ESZ) : u32x4_t{0, 0, 0, 0};
+          next_den = ((const float*)a.denom)[(int64_t)t * H + h];
+        };
+        load();
+        for (int b = block0 + rsub; b < blocks; b += share) {
+          u32x4_t qf[KS];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = 16 * b + 4 * g + i, at = min(rr, nrows - 1);
-            who[i] = at / G;
-            const float d = ((const float*)a.denom)[(int64_t)(start + who[i]) * H + hk * G + (at - who[i] * G)];
-            over[i] = rr < nrows && d != 0.0f ? __builtin_amdgcn_rcpf(d) : 0.0f;
+          for (int ks = 0; ks < KS; ++ks) qf[ks] = next[ks];
+          // over the row's denominator; rows behind the last have none, nor has one that saw no key
+          const float den = next_den, over_m = token < n && den != 0.0f ? __builtin_amdgcn_rcpf(den) : 0.0f;
+          const int token_m = token;
+          token += more_tokens;
+          in += more_in;
+          if (in >= G) {
+            in -= G;
+            ++token;
           }
+          if (b + share < blocks) load();
+          float over[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) over[i] = __shfl(over_m, 4 * g + i);
           f32x4_t s4[NG];
 #pragma unroll
           for (int u = 0; u < NG; ++u) {
@@ -234,58 +263,48 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
               }
             }
           }
-          float w[NG][4];
+          float w[4 * NG];
+#pragma unroll
+          for (int e = 0; e < 4 * NG; ++e) w[e] = s4[e >> 2][e & 3] * scale;
           if constexpr (F32) {
 #pragma unroll
-            for (int u = 0; u < NG; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[u][i] = rho8_refined(s4[u][i] * scale);
+            for (int e = 0; e < 4 * NG; ++e) w[e] = rho8_refined(w[e]);
           } else {
             float least = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NG; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                w[u][i] = s4[u][i] * scale;
-                least = __builtin_fminf(least, w[u][i]);
-              }
+            for (int e = 0; e < 4 * NG; ++e) least = __builtin_fminf(least, w[e]);
             // a score that is no number takes either form
             if (__ballot(!(least > kLowScore)) == 0) {
 #pragma unroll
-              for (int u = 0; u < NG; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[u][i] = rho8_fast(w[u][i]);
+              for (int e = 0; e < 4 * NG; ++e) w[e] = rho8_fast(w[e]);
             } else {
+              apart(w);
 #pragma unroll
-              for (int u = 0; u < NG; ++u) apart(w[u]);
-#pragma unroll
-              for (int u = 0; u < NG; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[u][i] = rho8_by_score(w[u][i]);
+              for (int e = 0; e < 4 * NG; ++e) w[e] = rho8_by_score(w[e]);
             }
           }
           // every key of the tile is seen by these rows, which all give something, or each by its own
-          const bool some = (over[0] != 0.0f && over[1] != 0.0f) && (over[2] != 0.0f && over[3] != 0.0f);
-          const bool whole = kb + WTILE <= (tree ? c : c + 1 + 16 * b / G) && __ballot(!some) == 0;
+          const bool whole = kb + TILE <= (tree ? c : c + 1 + 16 * b / G) && __ballot(over_m == 0.0f) == 0;
           if (!whole) {
 #pragma unroll
-            for (int u = 0; u < NG; ++u) {
-              const int pos = kb + 16 * u + m, j = pos - c;
+            for (int i = 0; i < 4; ++i) {
+              const int who = __shfl(token_m, 4 * g + i);
+              const int64_t* words = tree ? a.masks + (int64_t)(start + min(who, n - 1)) * W : nullptr;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                bool sees = pos < keys && over[i] != 0.0f;
-                if (sees && j >= 0)
-                  sees = tree ? a.masks[(int64_t)(start + who[i]) * W + (j >> 6)] >> (j & 63) & 1 : j <= who[i];
-                w[u][i] = sees ? w[u][i] : 0.0f;
+              for (int u = 0; u < NG; ++u) {
+                const int at = kb + 16 * u + m, j = at - c;
+                bool sees = at < keys && over[i] != 0.0f;
+                if (sees && j >= 0) sees = tree ? words[j >> 6] >> (j & 63) & 1 : j <= who;
+                w[4 * u + i] = sees ? w[4 * u + i] : 0.0f;
               }
             }
           }
 #pragma unroll
           for (int u = 0; u < NG; ++u) {
-            float x4 = w[u][0] * over[0];
+            float x = w[4 * u] * over[0];
 #pragma unroll
-            for (int i = 1; i < 4; ++i) x4 = __builtin_fmaf(w[u][i], over[i], x4);
-            head[u] += x4;
+            for (int i = 1; i < 4; ++i) x = __builtin_fmaf(w[4 * u + i], over[i], x);
+            head[u] += x;
           }
         }
 #pragma unroll
@@ -300,28 +319,24 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
         if (g == 0) red[wave][16 * u + m] = x;
       }
       __syncthreads();
-      const int pos = kb + tid;
       float sum = 0.0f;
-      if (tid < WTILE) sum = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+      if (tid < TILE) sum = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
       if (splits > 1) {
-        float* part = f.part + (int64_t)tile * splits * WTILE;
-        if (tid < WTILE) put1(part + split * WTILE + tid, sum);
+        float* part = f.part + (int64_t)tile * splits * TILE;
+        if (tid < TILE) put1(part + split * TILE + tid, sum);
         if (!arrived(f.count + tile, splits, &flag)) continue;
-        if (tid < WTILE) {
+        if (tid < TILE) {
           sum = 0.0f;
           for (int i0 = 0; i0 < splits; i0 += 8) {
             float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = get1(part + min(i0 + i, splits - 1) * WTILE + tid);
+            for (int i = 0; i < 8; ++i) y[i] = get1(part + min(i0 + i, splits - 1) * TILE + tid);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum += i0 + i < splits ? y[i] : 0.0f;
           }
         }
       }
-      if (tid < WTILE && pos < keys) {
-        float* to = a.weights + r * a.row + pos;
-        *to = pos < c ? *to + sum : sum;
-      }
+      if (tid < TILE && pos < keys) *to = old + sum;
     }
     __syncthreads();  // first is free
   }
@@ -329,7 +344,7 @@ __global__ __launch_bounds__(THREADS) void afa_paged_weight_tile_kernel(const We
 
 template <int DT, int D>
 hipError_t weight_tiles_launch(const WeightFast& f, int cus, hipStream_t st) {
-  hipLaunchKernelGGL((afa_paged_weight_tile_kernel<DT, D>), dim3((unsigned)(4 * cus)), dim3(THREADS), 0, st, f);
+  hipLaunchKernelGGL((afa_paged_weight_tile_kernel<DT, D>), dim3((unsigned)(resident<DT, D>() * cus)), dim3(THREADS), 0, st, f);
   return hipGetLastError();
 }
 
@@ -361,7 +376,7 @@ hipError_t paged_weights_launch(const WeightArgs& a, const PagedCut& cut, int cu
     f.part = (float*)ws;
     f.count = a.sched.count;
     // a tile has two parts at least where it is split
-    const int64_t counts = 2 * a.plan.kv_heads * 4 * cut.slots, room = (int64_t)(ws_bytes / (WTILE * 4));
+    const int64_t counts = 2 * a.plan.kv_heads * 4 * cut.slots, room = (int64_t)(ws_bytes / (MOST_KEYS * 4));
     f.most = (int)std::min<int64_t>(kWeightParts, std::min(counts, room));
     f.log_page = __builtin_ctzll((unsigned long long)a.plan.page_size);
     switch ((int)a.plan.dtype) {
