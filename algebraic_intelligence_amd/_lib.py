@@ -69,7 +69,7 @@ SIGNATURES = {
     "afa_paged_prefix_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _uint, _vp, _sz,
                                     _vp]),
     "afa_paged_weights": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _uint, _vp, _sz, _vp]),
-    "afa_paged_evict_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "afa_paged_evict_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "afa_paged_evict": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
                                _i64, _vp, _vp, _vp, _sz, _vp]),
     "oace_workspace_size": (_sz, [_int, _i64, _i64, _i64, _int, _uint]),

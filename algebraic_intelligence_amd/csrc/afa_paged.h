@@ -181,12 +181,12 @@ struct EvictArgs {
   int64_t row;
   float* left;           // (requests, table_width * page_size)
   int32_t* lens;
-  int32_t* space;        // paged_evict_workspace bytes
+  int32_t* space;        // paged_evict_workspace bytes, 16-byte aligned
   int budget, first, recent, esz;
   int rows, chunks;      // set by the launch: places of a chunk, a power of two; chunks of a budget; and the
-  int log_page;          // logarithm of a page_size that is one, or -1
+  int log_page, slices;  // logarithm of a page_size that is one, or -1; workgroups of a long request, or 0
 };
-size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim);
+size_t paged_evict_workspace(int64_t requests, int64_t max_len, int64_t budget, int64_t kv_heads, int64_t head_dim);
 hipError_t paged_evict_launch(EvictArgs a, hipStream_t st);
 
 struct RotateAxesArgs {

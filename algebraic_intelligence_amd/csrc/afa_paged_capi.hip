@@ -399,11 +399,11 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
   return workspace_done(afa::paged_weights_launch(a, cut, cus, ws, need, s), ws, own, s);
 }
 
-size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim) {
-  if (!within(requests, 1, int64_t(1) << 22) || !within(budget, 1, int64_t(1) << 30) || !within(kv_heads, 1, 1 << 16) ||
+size_t afa_paged_evict_workspace_size(int64_t requests, int64_t max_len, int64_t budget, int64_t kv_heads, int64_t head_dim) {
+  if (!within(requests, 1, int64_t(1) << 22) || !within(max_len, 1, int64_t(1) << 30) || !within(budget, 1, max_len) || !within(kv_heads, 1, 1 << 16) ||
       !within(head_dim, 1, 1024))
     return 0;
-  return afa::paged_evict_workspace(requests, budget, kv_heads, head_dim);
+  return afa::paged_evict_workspace(requests, max_len, budget, kv_heads, head_dim);
 }
 
 int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t requests, int64_t table_width, int64_t kv_heads,
@@ -423,7 +423,8 @@ int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t req
   const int64_t width = table_width * page_size;
   if (!within(budget, 1, width) || first < 0 || recent < 0 || first > budget || recent > budget - first) return AFA_ERR_SHAPE;
   if (weights_stride < width && requests > 1) return AFA_ERR_SHAPE;
-  if (requests > (kLaunchThreads - 1) / 512 / kv_heads || requests > (kLaunchThreads - 1) / 1024) return AFA_ERR_SHAPE;
+  if (requests > (kLaunchThreads - 1) / 512 / kv_heads || requests > (kLaunchThreads - 1) / 1024 / ((width + 8191) / 8192))
+    return AFA_ERR_SHAPE;
   afa::EvictArgs a = {};
   a.num_pages = num_pages; a.page_size = page_size; a.requests = requests; a.table_width = table_width;
   a.kv_heads = kv_heads; a.head_dim = head_dim;
@@ -437,7 +438,7 @@ int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t req
   const hipStream_t s = (hipStream_t)stream;
   void* ws;
   bool own;
-  const int got = workspace_of(workspace, workspace_bytes, afa::paged_evict_workspace(requests, budget, kv_heads, head_dim), s,
+  const int got = workspace_of(workspace, workspace_bytes, afa::paged_evict_workspace(requests, width, budget, kv_heads, head_dim), s,
                                ws, own);
   if (got != AFA_OK) return got;
   a.space = (int32_t*)ws;

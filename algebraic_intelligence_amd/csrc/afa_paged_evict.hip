@@ -2,16 +2,17 @@
 // newest, and of the others those of the largest weight, the lower index among equal ones.  What stays keeps its
 // order: token kept[i] moves to place i, in k, in v and in the weights.
 //
-// Two launches.  The first finds, one workgroup a request, the weight from which on tokens stay, by its bits from
-// the top (three passes over the weights, up to eleven bits each, counted in LDS), and lists the tokens that do.
+// First the weight is found from which on tokens stay, by its bits from the top (three passes over the weights, up to eleven
+// bits each, counted in LDS), and the tokens that stay are listed: in one launch of a workgroup a request, or, where caches are
+// long, in five launches of a workgroup for every 8192 tokens.
 //
-// The second moves rows in place.  A workgroup has one chunk of ROWS places of one head's k or v; its sources are behind its
+// The last launch moves rows in place.  A workgroup has one chunk of ROWS places of one head's k or v; its sources are behind its
 // places, in places of later chunks, so it reads all of them, says so, and writes only once the chunks that read from
 // its own places (earlier ones, two at most, as ROWS places hold at most ROWS sources) have said so too.  Chunks are handed
 // out in their order by a counter, and a workgroup reads and says so before it waits: whatever one waits for has begun and
 // waits for nothing before it says so, so every wait ends.
 //
-// HBM bounds the second launch: every row that moves is read and written once.
+// HBM bounds the last launch: every row that moves is read and written once.
 #include <algorithm>
 #include <initializer_list>
 
@@ -27,20 +28,30 @@ constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // of a bin, in banks 
 constexpr int LOADS = 8;                                  // weights of a thread in flight
 constexpr int MOVE = 256, BATCH = 8;                      // threads of a mover, and units that each holds
 
-// The workspace: slots of the tokens that stay, page * page_size + offset, or -1 for a page of no pool (requests, budget); the first place that moves (requests,); sources before each chunk's
-// places, and behind the last's (requests, chunks + 1); chunks handed out (requests, streams) and chunks that are read (requests, streams, chunks), a
-// stream being one head's k or v.
+constexpr int SLICE = LOADS * PICK;                       // tokens of a workgroup where a request has several
+constexpr int PASSES = 3;
+
+// The workspace: slots of the tokens that stay, page * page_size + offset, or -1 for a page of no pool (requests, budget); the
+// first place that moves (requests,); sources before each chunk's places, and behind the last's (requests, chunks + 1); chunks
+// handed out (requests, streams) and chunks that are read (requests, streams, chunks), a stream being one head's k or v.
+// With slices: counts of the digits (requests, PASSES, BINS), the digits found before each but the first pass and how many
+// tokens of the last are needed (requests, PASSES - 1, 2), slices handed out (requests,), and each one's counts (requests, slices).
 struct EvictSpace {
-  int32_t *kept, *moved, *before, *next, *read;
+  int64_t* counted;
+  int32_t *kept, *moved, *before, *next, *read, *bins, *state, *slice;
 };
 __host__ __device__ inline EvictSpace evict_space(const EvictArgs& a) {
   const int64_t streams = a.requests * 2 * a.kv_heads;
   EvictSpace s;
-  s.kept = a.space;
+  s.counted = (int64_t*)a.space;
+  s.kept = a.space + 2 * a.requests * a.slices;
   s.moved = s.kept + a.requests * a.budget;
   s.before = s.moved + a.requests;
   s.next = s.before + a.requests * (a.chunks + 1);
   s.read = s.next + streams;
+  s.bins = s.read + streams * a.chunks;
+  s.state = s.bins + a.requests * PASSES * BINS;
+  s.slice = s.state + 2 * (PASSES - 1) * a.requests;
   return s;
 }
 
@@ -68,61 +79,158 @@ __device__ __forceinline__ int lanes_up_to(int x) {
   return x;
 }
 
+// What a request asks for: its tokens, those that are chosen from, and how many of them stay.
+struct Choice {
+  int c, m, lo, hi, need;
+  bool over;  // more than the budget
+};
+__device__ __forceinline__ Choice choice(const EvictArgs& a, int r) {
+  const int held = (int)min(max((int64_t)a.held[r], (int64_t)0) * a.page_size, a.table_width * a.page_size);
+  const int c = min(max(a.cached[r], 0), held);
+  return Choice{c, min(c, a.budget), a.first, c - a.recent, a.budget - a.first - a.recent, c > a.budget};
+}
+
+// Digit `pass` of the weights: its lowest bit, and the lowest of the digits above it.
+__device__ __forceinline__ int shift_of(int pass) { return pass == 0 ? 32 - DIGIT : pass == 1 ? 32 - 2 * DIGIT : 0; }
+__device__ __forceinline__ int above_of(int pass) { return pass == 0 ? 32 : shift_of(pass - 1); }
+
+__device__ __forceinline__ void clear(int* bins) {
+  for (int i = threadIdx.x; i < COPIES * BINS; i += PICK) bins[i] = 0;
+}
+// Counts weights [base, base + SLICE) of [lo, hi), of which v are this thread's, whose digits above are those of `top`.
+__device__ __forceinline__ void count_digits(const float (&v)[LOADS], int base, int hi, int pass, unsigned top, int* bins) {
+  const int shift = shift_of(pass), above = above_of(pass);
+  const unsigned mask = (1u << (above - shift)) - 1;
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const unsigned u = order_bits(v[k]);
+    if (base + k * PICK + (int)threadIdx.x < hi && (above == 32 || u >> above == top >> above))
+      atomicAdd(&bins[(u >> shift & mask) * COPIES + threadIdx.x % COPIES], 1);
+  }
+}
+// The bin in which the need-th largest lies, from the counts n of bins BINS - 1 - 2 t and the one below, t this thread: found =
+// {bin, those above it}, bin -1 where none is needed.
+__device__ __forceinline__ void find_digit(const int (&n)[2], int need, int* wave_sum, int* found) {
+  static_assert(BINS == 2 * PICK, "two bins a thread");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, upto = lanes_up_to(n[0] + n[1]);
+  if (lane == 63) wave_sum[wave] = upto;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  int earlier = upto - n[0] - n[1];
+  for (int v = 0; v < wave; ++v) earlier += wave_sum[v];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (earlier < need && need <= earlier + n[k]) {
+      found[0] = BINS - 1 - 2 * tid - k;
+      found[1] = earlier;
+    }
+    earlier += n[k];
+  }
+  __syncthreads();
+}
+
+// Lists those of tokens [base, base + SLICE) that stay: those above `top`, and of those that equal it the first `need` of the
+// request.  before(over, equal), called by all threads with the batch's counts, gives those of the tokens before it.
+struct Lists {
+  float* left;
+  int32_t *kept, *before;
+  const int32_t* table;
+};
+template <typename B>
+__device__ __forceinline__ void list_tokens(const EvictArgs& a, const Choice& q, const Lists& to, const float (&v)[LOADS], int base,
+                                            unsigned top, int need, int2* counts, int* found, int& first_gone, const B& before) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, log_rows = __builtin_ctz((unsigned)a.rows);
+  int kind[LOADS];  // 2: stays, 1: equal, 0: neither
+  unsigned long long overs[LOADS], equals[LOADS];
+  __syncthreads();  // counts is free
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const int i = base + k * PICK + tid;
+    const unsigned u = order_bits(v[k]);
+    kind[k] = i >= q.c ? 0 : i < q.lo || i >= q.hi || u > top ? 2 : u == top ? 1 : 0;
+    overs[k] = __ballot(kind[k] == 2);
+    equals[k] = __ballot(kind[k] == 1);
+    if (lane == 0) counts[k * PICK_WAVES + wave] = int2{__popcll(overs[k]), __popcll(equals[k])};
+  }
+  __syncthreads();
+  // sums before each wave's, in place, and the batch's
+  static_assert(LOADS * PICK_WAVES == 128, "two entries a lane");
+  if (wave == 0) {
+    const int2 x = counts[2 * lane], y = counts[2 * lane + 1];
+    const int o = lanes_up_to(x.x + y.x), e = lanes_up_to(x.y + y.y);
+    counts[2 * lane] = int2{o - x.x - y.x, e - x.y - y.y};
+    counts[2 * lane + 1] = int2{o - y.x, e - y.y};
+    if (lane == 63) {
+      found[0] = o;
+      found[1] = e;
+    }
+  }
+  __syncthreads();
+  const int2 earlier = before(found[0], found[1]);
+  const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const int i = base + k * PICK + tid;
+    const int2 b = counts[k * PICK_WAVES + wave];
+    const int o = earlier.x + b.x + __popcll(overs[k] & below), e = earlier.y + b.y + __popcll(equals[k] & below);
+    const int at = o + min(e, need);
+    if (i < q.c && (i & (a.rows - 1)) == 0 && i >> log_rows <= a.chunks) to.before[i >> log_rows] = at;
+    if (kind[k] == 2 || (kind[k] == 1 && e < need)) {
+      to.kept[at] = slot_of(a, to.table, i);
+      to.left[at] = v[k];
+    } else if (i < q.c) {
+      first_gone = min(first_gone, i);
+    }
+  }
+}
+
+__device__ __forceinline__ Lists lists_of(const EvictArgs& a, const EvictSpace& s, int r) {
+  return Lists{a.left + r * a.table_width * a.page_size, s.kept + (int64_t)r * a.budget, s.before + (int64_t)r * (a.chunks + 1),
+               a.block_tables + (int64_t)r * a.table_width};
+}
+
 __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a) {
   __shared__ int bins[COPIES * BINS], wave_sum[PICK_WAVES], found[2];
   __shared__ int2 counts[LOADS * PICK_WAVES];
   const EvictSpace s = evict_space(a);
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t width = a.table_width * a.page_size;
-  const int held = (int)min(max((int64_t)a.held[r], (int64_t)0) * a.page_size, width);
-  const int c = min(max(a.cached[r], 0), held), budget = a.budget, m = min(c, budget);
+  const Choice q = choice(a, r);
+  const Lists to = lists_of(a, s, r);
   const float* w = a.weights + r * a.row;
-  float* left = a.left + r * width;
-  int32_t* kept = s.kept + (int64_t)r * budget;
   const int streams = (int)(2 * a.kv_heads);
   for (int i = tid; i < streams; i += PICK) s.next[(int64_t)r * streams + i] = 0;
   for (int64_t i = tid; i < (int64_t)streams * a.chunks; i += PICK) s.read[(int64_t)r * streams * a.chunks + i] = 0;
-  if (tid == 0) a.lens[r] = m;
-  for (int64_t i = m + tid; i < width; i += PICK) left[i] = 0.0f;
-  if (c <= budget) {
-    for (int i = tid; i < m; i += PICK) left[i] = w[i];
-    if (tid == 0) s.moved[r] = m;
+  if (tid == 0) a.lens[r] = q.m;
+  for (int64_t i = q.m + tid; i < width; i += PICK) to.left[i] = 0.0f;
+  if (!q.over) {
+    for (int i = tid; i < q.m; i += PICK) to.left[i] = w[i];
+    if (tid == 0) s.moved[r] = q.m;
     return;
   }
-  const int32_t* table = a.block_tables + (int64_t)r * a.table_width;
-  const int log_rows = __builtin_ctz((unsigned)a.rows);
-  int32_t* before = s.before + (int64_t)r * (a.chunks + 1);
   for (int i = tid; i <= a.chunks; i += PICK)
-    if ((int64_t)i * a.rows >= c) before[i] = m;
-  // tokens [lo, hi) are chosen from; `need` of them stay
-  const int lo = a.first, hi = c - a.recent;
-  int need = budget - a.first - a.recent;
+    if ((int64_t)i * a.rows >= q.c) to.before[i] = q.m;
+  int need = q.need;
   unsigned top = 0;  // the bits of the least weight that stays, as far as they are known
-  for (int shift = 32 - DIGIT; ; shift = shift > DIGIT ? shift - DIGIT : 0) {
-    const int above = shift == 32 - DIGIT ? 32 : shift == 0 ? 32 - 2 * DIGIT : 32 - DIGIT;
-    const unsigned mask = (1u << (above - shift)) - 1;
-    for (int i = tid; i < COPIES * BINS; i += PICK) bins[i] = 0;
+  float v[LOADS], next[LOADS];  // the next batch comes while this one is counted
+  auto load = [&](int base, int end) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) next[k] = w[min(base + k * PICK + tid, end - 1)];
+  };
+  auto take = [&](int base, int end) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) v[k] = next[k];
+    load(base + SLICE, end);
+  };
+  for (int pass = 0; pass < PASSES; ++pass) {
+    clear(bins);
+    load(q.lo, q.hi > q.lo ? q.hi : q.lo + 1);
     __syncthreads();
-    // the next batch comes while this one is counted
-    float v[LOADS], next[LOADS];
-#pragma unroll
-    for (int k = 0; k < LOADS; ++k) next[k] = w[min(lo + k * PICK + tid, hi - 1)];
-    for (int base = lo; base < hi; base += LOADS * PICK) {
-#pragma unroll
-      for (int k = 0; k < LOADS; ++k) {
-        v[k] = next[k];
-        next[k] = w[min(base + (LOADS + k) * PICK + tid, hi - 1)];
-      }
-#pragma unroll
-      for (int k = 0; k < LOADS; ++k) {
-        const unsigned u = order_bits(v[k]);
-        if (base + k * PICK + tid < hi && (above == 32 || u >> above == top >> above))
-          atomicAdd(&bins[(u >> shift & mask) * COPIES + lane % COPIES], 1);
-      }
+    for (int base = q.lo; base < q.hi; base += SLICE) {
+      take(base, q.hi);
+      count_digits(v, base, q.hi, pass, top, bins);
     }
     __syncthreads();
-    // the bin in which the need-th largest lies: thread t has bins of rank 2 t and 2 t + 1 from the top
-    static_assert(BINS == 2 * PICK, "two bins a thread");
     int n[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -130,94 +238,180 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
 #pragma unroll
       for (int i = 0; i < COPIES; ++i) n[k] += bins[(BINS - 1 - 2 * tid - k) * COPIES + i];
     }
-    const int upto = lanes_up_to(n[0] + n[1]);
-    if (lane == 63) wave_sum[wave] = upto;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    int earlier = upto - n[0] - n[1];
-    for (int v = 0; v < wave; ++v) earlier += wave_sum[v];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (earlier < need && need <= earlier + n[k]) {
-        found[0] = BINS - 1 - 2 * tid - k;
-        found[1] = earlier;
-      }
-      earlier += n[k];
-    }
-    __syncthreads();
+    find_digit(n, need, wave_sum, found);
     if (found[0] < 0) {  // none is needed
       top = 0xffffffffu;
       need = 0;
       break;
     }
-    top |= (unsigned)found[0] << shift;
+    top |= (unsigned)found[0] << shift_of(pass);
     need -= found[1];
-    if (shift == 0) break;
     __syncthreads();
   }
-  // those above `top` stay, and the first `need` that equal it
-  int over = 0, equal = 0, start = budget;  // of the tokens before this batch: above and sure ones, and equal ones
-  float v[LOADS], next[LOADS];
-#pragma unroll
-  for (int k = 0; k < LOADS; ++k) next[k] = w[min(k * PICK + tid, c - 1)];
-  for (int base = 0; base < c; base += LOADS * PICK) {
-    int kind[LOADS];  // 2: stays, 1: equal, 0: neither
-    unsigned long long overs[LOADS], equals[LOADS];
-#pragma unroll
-    for (int k = 0; k < LOADS; ++k) {
-      v[k] = next[k];
-      next[k] = w[min(base + (LOADS + k) * PICK + tid, c - 1)];
-    }
-    __syncthreads();  // counts is free
-#pragma unroll
-    for (int k = 0; k < LOADS; ++k) {
-      const int i = base + k * PICK + tid;
-      const unsigned u = order_bits(v[k]);
-      kind[k] = i >= c ? 0 : i < lo || i >= hi || u > top ? 2 : u == top ? 1 : 0;
-      overs[k] = __ballot(kind[k] == 2);
-      equals[k] = __ballot(kind[k] == 1);
-      if (lane == 0) counts[k * PICK_WAVES + wave] = int2{__popcll(overs[k]), __popcll(equals[k])};
-    }
-    __syncthreads();
-    // sums before each wave's, in place; the last two entries' sums are the batch's
-    static_assert(LOADS * PICK_WAVES == 128, "two entries a lane");
-    if (wave == 0) {
-      const int2 x = counts[2 * lane], y = counts[2 * lane + 1];
-      const int o = lanes_up_to(x.x + y.x), e = lanes_up_to(x.y + y.y);
-      counts[2 * lane] = int2{o - x.x - y.x, e - x.y - y.y};
-      counts[2 * lane + 1] = int2{o - y.x, e - y.y};
-      if (lane == 63) {
-        found[0] = o;
-        found[1] = e;
-      }
-    }
-    __syncthreads();
-    const unsigned long long below = (1ull << lane) - 1;
-#pragma unroll
-    for (int k = 0; k < LOADS; ++k) {
-      const int i = base + k * PICK + tid;
-      const int2 b = counts[k * PICK_WAVES + wave];
-      const int o = over + b.x + __popcll(overs[k] & below), e = equal + b.y + __popcll(equals[k] & below);
-      const int to = o + min(e, need);
-      if (i < c && (i & (a.rows - 1)) == 0 && i >> log_rows <= a.chunks) before[i >> log_rows] = to;
-      if (kind[k] == 2 || (kind[k] == 1 && e < need)) {
-        kept[to] = slot_of(a, table, i);
-        left[to] = v[k];
-        if (to != i) start = min(start, to);
-      }
-    }
-    over += found[0];
-    equal += found[1];
+  int2 earlier = {0, 0};
+  int gone = q.m;
+  load(0, q.c);
+  for (int base = 0; base < q.c; base += SLICE) {
+    take(base, q.c);
+    list_tokens(a, q, to, v, base, top, need, counts, found, gone, [&](int over, int equal) {
+      const int2 was = earlier;
+      earlier.x += over;
+      earlier.y += equal;
+      return was;
+    });
   }
-  // the first place whose token moves
+  // the first place whose token moves: that of the first token that does not stay
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) start = min(start, __shfl_xor(start, o));
-  if (lane == 0) wave_sum[wave] = start;
+  for (int o = 32; o > 0; o >>= 1) gone = min(gone, __shfl_xor(gone, o));
+  if (lane == 0) wave_sum[wave] = gone;
   __syncthreads();
   if (tid == 0) {
-    for (int k = 1; k < PICK_WAVES; ++k) start = min(start, wave_sum[k]);
-    s.moved[r] = start;
+    for (int k = 1; k < PICK_WAVES; ++k) gone = min(gone, wave_sum[k]);
+    s.moved[r] = gone;
   }
+}
+
+// ------------------------------------------------------------------ a workgroup for every SLICE tokens
+// What the other launches count in is cleared, and the lengths and first places set.
+__global__ __launch_bounds__(256) void afa_paged_slice_clear_kernel(const EvictArgs a) {
+  const EvictSpace s = evict_space(a);
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  const int64_t streams = a.requests * 2 * a.kv_heads;
+  for (int64_t i = i0; i < streams * (a.chunks + 1); i += step) s.next[i] = 0;  // read lies behind it
+  for (int64_t i = i0; i < a.requests * PASSES * BINS; i += step) s.bins[i] = 0;
+  for (int64_t i = i0; i < a.requests * a.slices; i += step) s.counted[i] = 0;
+  for (int64_t r = i0; r < a.requests; r += step) {
+    const Choice q = choice(a, (int)r);
+    a.lens[r] = s.moved[r] = q.m;
+    s.slice[r] = 0;
+  }
+}
+
+// The digits of the passes before `pass`, from their counts: top and need.
+__device__ __forceinline__ bool digits_before(const EvictArgs& a, const EvictSpace& s, int r, int pass, const Choice& q, unsigned& top,
+                                              int& need, int* wave_sum, int* found) {
+  top = 0;
+  need = q.need;
+  if (pass >= 2) {
+    const int32_t* state = s.state + 2 * ((PASSES - 1) * r + pass - 2);
+    top = (unsigned)state[0];
+    need = state[1];
+  }
+  if (pass >= 1 && need > 0) {
+    const int* bins = s.bins + ((int64_t)r * PASSES + pass - 1) * BINS;
+    const int n[2] = {bins[BINS - 1 - 2 * (int)threadIdx.x], bins[BINS - 2 - 2 * (int)threadIdx.x]};
+    find_digit(n, need, wave_sum, found);
+    top |= (unsigned)found[0] << shift_of(pass - 1);
+    need -= found[1];
+    __syncthreads();  // found is free
+  }
+  if (need <= 0) {  // none is needed
+    top = 0xffffffffu;
+    need = 0;
+  }
+  return need > 0;
+}
+
+__global__ __launch_bounds__(PICK) void afa_paged_slice_count_kernel(const EvictArgs a, int pass) {
+  __shared__ int bins[COPIES * BINS], wave_sum[PICK_WAVES], found[2];
+  const EvictSpace s = evict_space(a);
+  const int r = blockIdx.x / a.slices, slice = blockIdx.x % a.slices, tid = threadIdx.x;
+  const Choice q = choice(a, r);
+  const int base = slice * SLICE;
+  if (!q.over || (base >= q.hi && slice > 0)) return;
+  const float* w = a.weights + r * a.row;
+  float v[LOADS];
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) v[k] = w[min(base + k * PICK + tid, q.c - 1)];
+  clear(bins);
+  unsigned top;
+  int need;
+  const bool some = digits_before(a, s, r, pass, q, top, need, wave_sum, found);
+  // for the next pass, which reads it in another launch
+  if (slice == 0 && tid == 0 && pass >= 1) {
+    int32_t* state = s.state + 2 * ((PASSES - 1) * r + pass - 1);
+    state[0] = (int)top;
+    state[1] = need;
+  }
+  if (!some) return;
+  __syncthreads();
+  const int shift = shift_of(pass), above = above_of(pass);
+  const unsigned mask = (1u << (above - shift)) - 1;
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const int i = base + k * PICK + tid;
+    const unsigned u = order_bits(v[k]);
+    if (i >= q.lo && i < q.hi && (above == 32 || u >> above == top >> above))
+      atomicAdd(&bins[(u >> shift & mask) * COPIES + tid % COPIES], 1);
+  }
+  __syncthreads();
+  int* to = s.bins + ((int64_t)r * PASSES + pass) * BINS;
+  for (int b = tid; b < BINS; b += PICK) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) n += bins[b * COPIES + i];
+    if (n > 0) atomicAdd(to + b, n);
+  }
+}
+
+// A request's slices are handed out in their order; each says what it counts before it waits for the earlier ones' counts,
+// so every wait ends.
+__global__ __launch_bounds__(PICK) void afa_paged_slice_list_kernel(const EvictArgs a) {
+  __shared__ int wave_sum[PICK_WAVES], wave_more[PICK_WAVES], found[2], ticket;
+  __shared__ int2 counts[LOADS * PICK_WAVES];
+  const EvictSpace s = evict_space(a);
+  const int r = blockIdx.x / a.slices, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Choice q = choice(a, r);
+  const Lists to = lists_of(a, s, r);
+  const float* w = a.weights + r * a.row;
+  if (tid == 0) ticket = atomicAdd(s.slice + r, 1);
+  __syncthreads();
+  const int slice = ticket, base = slice * SLICE;
+  const int64_t width = a.table_width * a.page_size, end = min((int64_t)base + SLICE, width);
+  for (int64_t i = max((int64_t)base, (int64_t)q.m) + tid; i < end; i += PICK) to.left[i] = 0.0f;
+  if (!q.over) {
+    for (int64_t i = base + tid; i < min(end, (int64_t)q.m); i += PICK) to.left[i] = w[i];
+    return;
+  }
+  if (slice == 0)
+    for (int i = tid; i <= a.chunks; i += PICK)
+      if ((int64_t)i * a.rows >= q.c) to.before[i] = q.m;
+  if (base >= q.c) return;
+  float v[LOADS];
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) v[k] = w[min(base + k * PICK + tid, q.c - 1)];
+  unsigned top;
+  int need;
+  digits_before(a, s, r, PASSES, q, top, need, wave_sum, found);
+  int gone = q.m;
+  list_tokens(a, q, to, v, base, top, need, counts, found, gone, [&](int over, int equal) {
+    int64_t* counted = s.counted + (int64_t)r * a.slices;
+    if (tid == 0)
+      __hip_atomic_store(counted + slice, (int64_t)1 << 62 | (int64_t)over << 31 | equal, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    int2 sum = {0, 0};
+    for (int j = tid; j < slice; j += PICK) {
+      int64_t x;
+      while ((x = __hip_atomic_load(counted + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == 0) __builtin_amdgcn_s_sleep(1);
+      sum.x += (int)(x >> 31 & 0x7fffffff);
+      sum.y += (int)(x & 0x7fffffff);
+    }
+    const int o = lanes_up_to(sum.x), e = lanes_up_to(sum.y);
+    if (lane == 63) {
+      wave_sum[wave] = o;
+      wave_more[wave] = e;
+    }
+    __syncthreads();
+    sum = int2{0, 0};
+    for (int k = 0; k < PICK_WAVES; ++k) {
+      sum.x += wave_sum[k];
+      sum.y += wave_more[k];
+    }
+    return sum;
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) gone = min(gone, __shfl_xor(gone, o));
+  if (lane == 0 && gone < q.m) atomicMin(s.moved + r, gone);
 }
 
 // Rows as `units` of type T each; a chunk is BATCH units a thread, a.rows rows.
@@ -289,14 +483,23 @@ __global__ __launch_bounds__(MOVE, 5) void afa_paged_move_kernel(const EvictArgs
   }
 }
 
+// Slices of a request, 0 where one workgroup has all of its tokens.  That takes about 20 us and 7 for every slice, requests side
+// by side; five launches about 30 and 0.1 for every slice of all requests.  4 requests of 131072 tokens take 122 us and 35, 256 of
+// 16384 with the rows' launch 59 and (of 16448) 104.
+int64_t slices_of(int64_t requests, int64_t max_len) {
+  const int64_t slices = (max_len + SLICE - 1) / SLICE;
+  return requests < 70 && slices * (70 - requests) > 100 ? slices : 0;
+}
+
 }  // namespace
 
 // Chunks are shortest where units are elements.
-size_t paged_evict_workspace(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim) {
+size_t paged_evict_workspace(int64_t requests, int64_t max_len, int64_t budget, int64_t kv_heads, int64_t head_dim) {
   int64_t rows = 1;
   while (2 * rows * head_dim <= MOVE * BATCH) rows *= 2;
-  const int64_t chunks = (budget + rows - 1) / rows;
-  return (size_t)(requests * (budget + 2 + chunks + 2 * kv_heads * (1 + chunks))) * 4;
+  const int64_t chunks = (budget + rows - 1) / rows, slices = slices_of(requests, max_len);
+  return (size_t)(requests * (budget + 2 + chunks + 2 * kv_heads * (1 + chunks) +
+                              (slices > 0 ? 2 * slices + PASSES * BINS + 2 * (PASSES - 1) + 1 : 0))) * 4;
 }
 
 hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
@@ -310,7 +513,17 @@ hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
   while (2 * a.rows * units <= MOVE * BATCH) a.rows *= 2;
   a.log_page = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)a.page_size) : -1;
   a.chunks = (a.budget + a.rows - 1) / a.rows;
-  hipLaunchKernelGGL(afa_paged_pick_kernel, dim3((unsigned)a.requests), dim3(PICK), 0, st, a);
+  a.slices = (int)slices_of(a.requests, a.table_width * a.page_size);
+  if (a.slices == 0) {
+    hipLaunchKernelGGL(afa_paged_pick_kernel, dim3((unsigned)a.requests), dim3(PICK), 0, st, a);
+  } else {
+    const dim3 grid((unsigned)(a.requests * a.slices)), block(PICK);
+    const int64_t ints = a.requests * (PASSES * BINS + a.slices + 2 * a.kv_heads * (a.chunks + 1));
+    hipLaunchKernelGGL(afa_paged_slice_clear_kernel, dim3((unsigned)std::min<int64_t>((ints + 1023) / 1024, 4096)), dim3(256), 0, st,
+                       a);
+    for (int pass = 0; pass < PASSES; ++pass) hipLaunchKernelGGL(afa_paged_slice_count_kernel, grid, block, 0, st, a, pass);
+    hipLaunchKernelGGL(afa_paged_slice_list_kernel, grid, block, 0, st, a);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t streams = 2 * a.requests * a.kv_heads, most = std::max<int64_t>(1, (int64_t(1) << 20) / streams);

@@ -139,8 +139,8 @@ def evict_from_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, pool: PagePoo
     lens = torch.empty(pool.max_requests, dtype=torch.int32, device=dev)
     left = torch.empty((pool.max_requests, pool.max_len), dtype=torch.float32, device=dev)
     with _lib.on_device(dev):
-        size = _lib.workspace_size("afa_paged_evict_workspace_size", dev, pool.max_requests, budget, kv_heads,
-                                   head_dim)
+        size = _lib.workspace_size("afa_paged_evict_workspace_size", dev, pool.max_requests, pool.max_len, budget,
+                                   kv_heads, head_dim)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         rc = _lib.lib().afa_paged_evict(
             dt, pool.num_pages, pool.page_size, pool.max_requests, pool.block_tables.shape[1], kv_heads, head_dim,

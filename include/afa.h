@@ -427,9 +427,9 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
  * weights, 0 behind them, and lens (requests,) the lengths.  budget at most table_width * page_size; first + recent at most
  * budget.  A cached length is taken as at most what the request's pages hold.  Places behind the budget keep their contents; the
  * pages go back to the pool with the next afa_paged_build.  A page id outside the pool is neither read nor written.
- * workspace: afa_paged_evict_workspace_size() bytes, 16-byte aligned, or NULL.
+ * workspace: afa_paged_evict_workspace_size() bytes (max_len: table_width * page_size), 16-byte aligned, or NULL.
  */
-size_t afa_paged_evict_workspace_size(int64_t requests, int64_t budget, int64_t kv_heads, int64_t head_dim);
+size_t afa_paged_evict_workspace_size(int64_t requests, int64_t max_len, int64_t budget, int64_t kv_heads, int64_t head_dim);
 int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t requests, int64_t table_width, int64_t kv_heads,
                     int64_t head_dim, const int32_t* block_tables, const int32_t* held, void* k_pages, void* v_pages,
                     const int64_t* page_strides, const int32_t* cached, int64_t budget, int64_t first, int64_t recent,

@@ -239,6 +239,24 @@ def test_evict_weights(what):
         x.check(budget, first, recent)
 
 
+@pytest.mark.parametrize("budget,first,recent,weights", [(9000, 10, 500, "plain"), (9000, 0, 0, "equal"), (1, 0, 0, "plain"),
+                                                         (20000, 12000, 8000, "plain"), (16385, 9000, 1, "odd"), (33000, 3, 8192, "zero"),
+                                                         (8192, 0, 8192, "plain"), (24576, 0, 17, "bits")])
+def test_evict_long(budget, first, recent, weights):
+    """Caches of several workgroups a request, beside short ones and lengths on both sides of a workgroup's tokens."""
+    x = _Held(BF16, [40000, 24576, 8192, 8193, 100, 0, 16384, 16385, 36000], 1, 16, 64, seed=budget % 100)
+    rng = np.random.default_rng(1)
+    if weights == "equal":
+        x.w.fill_(0.75)
+    if weights == "zero":
+        x.w = torch.where(torch.tensor(rng.random(x.w.shape) < 0.9, device="cuda"), 0.0, x.w)
+    if weights == "odd":
+        x.w = torch.tensor(rng.choice(np.array([np.nan, np.inf, -np.inf, 1, -1, 1e-45, 3e38], np.float32), x.w.shape), device="cuda")
+    if weights == "bits":
+        x.w = (0x3f800000 + torch.randint(0, 3000, x.w.shape, device="cuda", dtype=torch.int32)).view(torch.float32)
+    x.check(budget, first, recent)
+
+
 def test_evict_odd_lengths():
     """Lengths below 0 and past what a request's pages hold; weights in a wider buffer; a page of no pool is let be."""
     x = _Held(BF16, [100, 33, 64, 20], 2, 64, 16, seed=1, slack=4)
@@ -255,8 +273,10 @@ def test_evict_odd_lengths():
     assert torch.equal(x.kp[lost], k[lost])
 
 
-def test_evict_captured_and_on_a_stream():
-    x = _Held(BF16, [3000, 200, 1500], 2, 64, 16, seed=1)
+@pytest.mark.parametrize("slack", [1, 2000])
+def test_evict_captured_and_on_a_stream(slack):
+    """One workgroup a request, and several where max_len is long."""
+    x = _Held(BF16, [3000, 200, 1500], 2, 64, 16, seed=1, slack=slack)
     k0, v0 = x.kp.clone(), x.vp.clone()
     lens = _i32(x.lens)
     graph = torch.cuda.CUDAGraph()
