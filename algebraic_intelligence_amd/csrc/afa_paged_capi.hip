@@ -423,7 +423,7 @@ int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t req
   const int64_t width = table_width * page_size;
   if (!within(budget, 1, width) || first < 0 || recent < 0 || first > budget || recent > budget - first) return AFA_ERR_SHAPE;
   if (weights_stride < width && requests > 1) return AFA_ERR_SHAPE;
-  if (requests > (kLaunchThreads - 1) / 512 / kv_heads || requests > (kLaunchThreads - 1) / 1024 / ((width + 8191) / 8192))
+  if (requests > (kLaunchThreads - 1) / 2048 / kv_heads || requests > (kLaunchThreads - 1) / 1024 / ((width + 8191) / 8192))
     return AFA_ERR_SHAPE;
   afa::EvictArgs a = {};
   a.num_pages = num_pages; a.page_size = page_size; a.requests = requests; a.table_width = table_width;

@@ -239,6 +239,20 @@ def test_evict_weights(what):
         x.check(budget, first, recent)
 
 
+@pytest.mark.parametrize("dt,K,D,page,layout", [(F32, 2, 256, 16, "plain"), (F64, 1, 512, 64, "side"), (BF16, 3, 1000, 5, "plain"),
+                                                (F16, 1, 1024, 32, "gap"), (F64, 2, 3, 7, "gap")])
+def test_evict_rows_in_many_chunks(dt, K, D, page, layout):
+    """Rows so long that a request's are moved by many workgroups, whose places are each other's sources: tokens that stay
+    spread evenly, at the end, at the front, and at random."""
+    x = _Held(dt, [4000, 3999, 1500, 2100], K, D, page, seed=D, layout=layout)
+    n = x.w.shape[1]
+    at = torch.arange(n, device="cuda")
+    for weights in ((at % 2).float(), (at >= 1000).float(), (at % 64 < 32).float(), torch.rand(n, device="cuda")):
+        x.w = weights.expand_as(x.w).contiguous()
+        x.check(1000, 1, 3)
+    x.check(1999)
+
+
 @pytest.mark.parametrize("budget,first,recent,weights", [(9000, 10, 500, "plain"), (9000, 0, 0, "equal"), (1, 0, 0, "plain"),
                                                          (20000, 12000, 8000, "plain"), (16385, 9000, 1, "odd"), (33000, 3, 8192, "zero"),
                                                          (8192, 0, 8192, "plain"), (24576, 0, 17, "bits")])
