@@ -649,7 +649,14 @@ class _NormRotate(torch.autograd.Function):
         ctx.versions = _versions(c, s, positions)
         ctx.set_materialize_grads(False)
         y, z = _norm_launch(q, k, q_scale, k_scale, c, s, positions, cfg)
-        return y if k is None else (y, z)
+        if k is None:
+            return y
+        need = ctx.needs_input_grad
+        if not (need[0] or need[2]):
+            ctx.mark_non_differentiable(y)
+        elif not (need[1] or need[3]):
+            ctx.mark_non_differentiable(z)
+        return y, z
 
     @staticmethod
     def backward(ctx, gq, gk=None):

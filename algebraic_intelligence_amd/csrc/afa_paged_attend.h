@@ -743,8 +743,11 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void afa_paged_tile_kern
           for (int i = 0; i < 4; ++i)
             if (!(__builtin_fabsf(y[i]) < __builtin_inff())) x[i] = y[i];
         } else if constexpr (!F32) {
+          // (a prefix's rows may be those of requests that were not served: whatever they hold, they cost nothing)
+          if (!PREFIX || __builtin_fabsf(sum) < __builtin_inff()) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(x[i], 0.0f, zero[i]);
+            for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(x[i], 0.0f, zero[i]);
+          }
         }
         if (parts > 1) {
           put4(buffer, (uint32_t)((my_part * ROWS + row) * D + d) * 4, x);

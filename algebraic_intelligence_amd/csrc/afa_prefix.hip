@@ -329,18 +329,29 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       }
     if (mine && g == 0) put1(part_den + my_part * WIDE_ROWS + 32 * wave + l32, den);
     // A value that is not finite is the sum of every row, as weights are above 0.  It may have become NaN in the product, where
-    // a weight may be rounded to 0: such sums are formed again, from these values alone.
-    if (mine && zero != 0.0f) {
+    // a weight may be rounded to 0: each feature's sum of such values, the same for all rows, takes its place.  (Where the row
+    // sum is not finite either the row is NaN already.)
+    if (__syncthreads_or(mine && zero != 0.0f && __builtin_fabsf(den) < __builtin_inff())) {
+      float* odd = (float*)&lds_k[0][0];
+      for (int d = tid; d < D; d += THREADS) odd[d] = 0.0f;
+      __syncthreads();
+      for (int e = tid; e < (min(t1 * kPagedTile, L) - t0 * kPagedTile) * CHD; e += THREADS) {
+        const int key = e / CHD, c = e - key * CHD;
+        float x[8];
+        RowChunk<DT>::unpack(*(const u32x4_t*)(v_base + (uint64_t)(uint32_t)(t0 * kPagedTile + key) * f.v_slot + 16 * c), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(__builtin_fabsf(x[i]) < __builtin_inff())) atomicAdd(&odd[8 * c + i], x[i]);
+      }
+      __syncthreads();
       float* to = f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D;
-      for (int d = 4 * g; d < D; d += 8)
-        for (int i = d; i < d + 4; ++i) {
-          float y = 0.0f;
-          for (int key = t0 * kPagedTile; key < min(t1 * kPagedTile, L); ++key) {
-            const float z = Elem<DT>::load(v_base + (uint64_t)(uint32_t)key * f.v_slot, i);
-            if (!(__builtin_fabsf(z) < __builtin_inff())) y += z;
+      if (mine)
+        for (int d = 4 * g; d < D; d += 8)
+          for (int i = d; i < d + 4; ++i) {
+            if (__builtin_fabsf(odd[i]) < __builtin_inff()) continue;
+            if (size > 1) put1(to + i, odd[i]);
+            else to[i] = odd[i];
           }
-          if (!(__builtin_fabsf(y) < __builtin_inff())) put1(to + i, y);
-        }
     }
     if (size == 1) continue;
 

@@ -123,6 +123,40 @@ def test_weights_edges(dt):
     assert (w[:2] == 3).all() and (w[2, 10:] == 3).all()
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_weights_of_many_requests(dt):
+    """More requests than a workgroup counts at a time, most of them short, some without new tokens."""
+    lens = [(r % 7, (r % 3 != 0) * 1) for r in range(2500)]
+    lens[1200] = (150, 2)
+    x = _Cache(dt, lens, 2, 1, 32, 8, seed=1, max_tree=0, parents=False)
+    _check(x, _den(x))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_weights_over_other_strides(dt):
+    """Pages as (pages, slots, heads, dim) in memory, q inside a wider buffer, weights in wider rows; and without the matrix cores or a
+    workspace, through the C call."""
+    import ctypes
+
+    from algebraic_intelligence_amd import _lib
+    x = _Cache(dt, [(100, 3), (0, 20), (300, 1)], 4, 2, 64, 16, seed=5)
+    den = _den(x)
+    want = A.accumulate_cache_weights(x.q, x.kp, den, x.plan, x.pool.new_weights())
+    q = torch.zeros(x.q.shape[0], 8, 64, device="cuda", dtype=dt)
+    q[:, 2:6] = x.q
+    pages = x.kp.transpose(1, 2).contiguous().transpose(1, 2)
+    wide = torch.zeros(3, x.pool.max_len + 5, device="cuda")
+    got = A.accumulate_cache_weights(q[:, 2:6], pages, den, x.plan, wide[:, :x.pool.max_len])
+    assert torch.equal(got, want) and (wide[:, x.pool.max_len:] == 0).all()
+    for flags in (0, _lib.FLAG_GENERIC):
+        w = x.pool.new_weights()
+        rc = _lib.lib().afa_paged_weights(x.plan._ref, x.q.data_ptr(), None, x.kp.data_ptr(), None, None, den.data_ptr(), w.data_ptr(),
+                                          x.pool.max_len, flags, None, 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0 and (flags or torch.equal(w, want))
+        given, bound = _given(x, den)
+        _close(w, given, bound + 2 * U * given, flags)
+
+
 def test_weights_repeat_on_streams_and_in_graphs():
     x = _Cache(BF16, [(100 + 70 * r, 1 + r % 3) for r in range(30)], 8, 2, 128, 16, seed=1, max_tree=0, parents=False)
     den = _den(x)
@@ -309,6 +343,45 @@ def test_evict_captured_and_on_a_stream(slack):
             b = [*A.evict_from_cache(x.kp, x.vp, x.pool, x.w, lens, 128, first=4, recent=16), x.kp, x.vp]
         side.synchronize()
         assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_evict_in_the_librarys_own_workspace():
+    from algebraic_intelligence_amd import _lib
+    x = _Held(BF16, [300, 20, 100], 2, 64, 16, seed=1)
+    k, v, lens = x.kp.clone(), x.vp.clone(), _i32(x.lens)
+    want = A.evict_from_cache(k, v, x.pool, x.w, lens, 64, first=2, recent=8)
+    got, left, p = torch.empty_like(lens), torch.empty_like(x.w), x.pool
+    rc = _lib.lib().afa_paged_evict(_lib.AFA_BF16, p.num_pages, p.page_size, 3, p.block_tables.shape[1], 2, 64, p.block_tables.data_ptr(),
+                                    p.held.data_ptr(), x.kp.data_ptr(), x.vp.data_ptr(), None, lens.data_ptr(), 64, 2, 8, x.w.data_ptr(),
+                                    x.w.shape[1], left.data_ptr(), got.data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(got, want[0]) and torch.equal(left, want[1])
+    assert torch.equal(x.kp, k) and torch.equal(x.vp, v)
+
+
+def test_evict_twice_and_at_once():
+    """Two pools on two streams at a time; a layer cut back, filled on and cut back again."""
+    xs = [_Held(F32, [3000, 2000, 2500], 2, 256, 16, seed=s) for s in (1, 2)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    kept = [(x.kp.clone(), x.vp.clone()) for x in xs]
+    for round_ in range(3):
+        got = []
+        for x, s, (k, v) in zip(xs, sides, kept):
+            x.kp.copy_(k), x.vp.copy_(v)
+        torch.cuda.synchronize()
+        for x, s in zip(xs, sides):
+            with torch.cuda.stream(s):
+                got.append(A.evict_from_cache(x.kp, x.vp, x.pool, x.w, _i32(x.lens), 700, first=3, recent=60))
+        torch.cuda.synchronize()
+        for x, (k, v), (lens, left) in zip(xs, kept, got):
+            again_k, again_v = k.clone(), v.clone()
+            a, b = A.evict_from_cache(again_k, again_v, x.pool, x.w, _i32(x.lens), 700, first=3, recent=60)
+            assert torch.equal(a, lens) and torch.equal(b, left) and torch.equal(again_k, x.kp) and torch.equal(again_v, x.vp)
+    x = xs[0]
+    x.w = torch.rand_like(x.w)
+    x.check(900, 5, 5)
+    x.w = torch.rand_like(x.w)
+    x.check(300, 5, 5, lens=[900, 900, 900])
 
 
 def test_refusals():

@@ -77,7 +77,7 @@ def _layouts(arrays, layout, D, dt):
     (2, 2, 1, 5, 36, (3, 4), True, "gap", F32), (1, 9, 4, 130, 64, (32,), True, "shared", F32),
     (1, 3, 2, 6, 256, (128,), False, "blhd", F32), (2, 1, 5, 9, 512, (256,), False, "bhld", F32),
     (1, 2, 1, 3, 1000, None, False, "bhld", F32), (1, 3, 2, 11, 7, "none", False, "blhd", F32),
-    (5, 2, 2, 1, 64, "rows", False, "bhld", F32), (2, 3, 2, 300, 80, "rows", False, "blhd", F32),
+    (5, 2, 2, 1, 64, "rows", False, "bhld", F32), (2, 2, 3, 9, 8, (2, 2), True, "blhd", F32), (2, 3, 2, 300, 80, "rows", False, "blhd", F32),
 ])
 def test_norm_rotation_and_gradients(dt, B, H, K, L, D, sections, long, layout, scale_dt):
     """Chunked and ragged rows, shared positions, a row's index for a position, no rotation at all."""
@@ -113,6 +113,7 @@ def test_norm_rotation_and_gradients(dt, B, H, K, L, D, sections, long, layout, 
     # q alone, the same bits; one gradient of the two
     assert torch.equal(A.apply_ago_norm_rotations(q, None, qs, None, tab, pos, cuts, eps=eps), y)
     y, z = A.apply_ago_norm_rotations(q.detach(), k, qs.detach(), ks, tab, pos, cuts, eps=eps)
+    assert not y.requires_grad and z.requires_grad
     again = torch.autograd.grad(z, (k, ks), gk)
     assert torch.equal(again[0], dk)
     _close(again[1], *(lambda p: (p[0], p[1] + _half(scale_dt) * np.abs(p[0])))(_backward(
@@ -334,3 +335,18 @@ def test_norm_changed_positions_are_noticed():
     pos += 1
     with pytest.raises(RuntimeError, match="modified"):
         y.sum().backward()
+
+
+def test_norm_in_the_librarys_own_workspace():
+    """The C call without a workspace: the same bits."""
+    from algebraic_intelligence_amd import _lib
+    B, H, L, D = 2, 4, 50, 64
+    q, g = (torch.randn(B, H, L, D, device="cuda", dtype=BF16) for _ in range(2))
+    w = 1 + torch.randn(D, device="cuda") / 4
+    leaf, scale = q.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    want = torch.autograd.grad(A.apply_ago_norm_rotations(leaf, None, scale, None), (leaf, scale), g)
+    dq, dw = torch.empty_like(q), torch.empty_like(w)
+    rc = _lib.lib().ago_norm_rotate_axes_bwd(_lib.AFA_BF16, B, H, 0, L, D, q.data_ptr(), None, g.data_ptr(), None, dq.data_ptr(), None,
+                                             None, w.data_ptr(), None, dw.data_ptr(), None, 1e-6, None, None, 0, None, 4, 0, 1, None,
+                                             None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(dq, want[0]) and torch.equal(dw, want[1])

@@ -146,9 +146,11 @@ def test_prefix_of_hidden_drafts(dt):
 
 
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
-def test_prefix_values_that_are_not_finite(dt):
-    """An infinity or a NaN in a prefix value is every row's result in that feature; NaN in a key is the row's."""
-    x = _Shared(dt, [(50, 3), (0, 30), (1, 1)], 4, 2, 64, 16, 200, seed=2)
+@pytest.mark.parametrize("new", [9, 30, 130])
+def test_prefix_values_that_are_not_finite(dt, new):
+    """An infinity or a NaN in a prefix value is every row's result in that feature; NaN in a key is the row's.  Few and many
+    rows a key head, in one block and in several."""
+    x = _Shared(dt, [(50, 3), (0, new), (1, 1)], 4, 2, 64, 16, 200, seed=2)
     plain = x.call()
     x.pv[0, 17, 5], x.pv[1, 199, 63], x.pv[0, 3, 40] = float("inf"), float("-inf"), float("nan")
     got = x.call()
@@ -224,3 +226,57 @@ def test_prefix_refusals():
         call(k, v, out=k.view(-1)[:x.q.numel()].view_as(x.q))
     with pytest.raises(ValueError, match="sink"):
         call(k, v, sink_omega=-1.0)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D,L", [(128, 20000), (32, 9001), (96, 7000)])
+def test_prefix_of_many_rows_in_many_parts(dt, D, L):
+    """One block of rows, whose keys all workgroups share, and a few of them: more parts than are added up at once; values that are
+    not finite in some of the parts; the same bits each time."""
+    for R in (70, 150):
+        x = _Shared(dt, [(r % 3, 1) for r in range(R)], 1, 1, D, 16, L, seed=R, max_tree=0, parents=False)
+        out, den = x.check(what=(D, L, R))
+        assert torch.equal(x.call(), out)
+        x.pv[0, L // 2, 3], x.pv[0, L - 1, D - 1] = float("inf"), float("nan")
+        got = x.call()
+        assert (got[:R, 0, 3] == float("inf")).all() and torch.isnan(got[:R, 0, D - 1]).all()
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[..., 3] = same[..., D - 1] = False
+        assert torch.equal(got[same], out[same])
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("R", [3, 60])
+def test_prefix_beside_rows_of_nan(dt, R):
+    """Rows of NaN, and those of requests that are not served, whatever they hold: their own results alone."""
+    x = _Shared(dt, [(r % 5, 2) for r in range(R)], 4, 2, 64, 16, 500, seed=R, max_tree=0, parents=False)
+    out, den = x.check()
+    x.q[2, 1] = float("nan")
+    cached = _i32([10 ** 6 if r == 0 else r % 5 for r in range(R)])
+    A.build_block_tables(x.plan, cached, _i32([2] * R))
+    x.q[0] = float("nan")
+    got = x.call()
+    assert (got[:2] == 0).all() and torch.isnan(got[2, 1]).all()
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[:2], same[2, 1] = False, False
+    assert torch.equal(got[same], out[same])
+
+
+@pytest.mark.parametrize("dt", [BF16, F32, F64])
+def test_prefix_in_the_librarys_own_workspace(dt):
+    """The C call without a workspace: the same bits; and without the matrix cores, within the bounds."""
+    import ctypes
+
+    from algebraic_intelligence_amd import _lib
+    x = _Shared(dt, [(5, 2), (40, 3)], 4, 2, 64, 16, 300, seed=3)
+    want, _ = x.check()
+    for flags in (_lib.FLAG_ZERO_TAIL, _lib.FLAG_ZERO_TAIL | _lib.FLAG_GENERIC):
+        out = torch.empty_like(x.q)
+        rc = _lib.lib().afa_paged_prefix_fwd(x.plan._ref, x.q.data_ptr(), None, x.pk.data_ptr(), x.pv.data_ptr(), 300, None,
+                                             x.kp.data_ptr(), x.vp.data_ptr(), None, None, out.data_ptr(), None, 0.5, flags, None, 0,
+                                             ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0
+        if flags == _lib.FLAG_ZERO_TAIL or dt == F64:
+            assert torch.equal(out, want)
+        ref, _, size, e = x.want(0.5)
+        _close(out, ref, 2 * e[..., None] * size + (_half(dt) + 4 * U) * np.abs(ref) + _tiny(dt), flags)
