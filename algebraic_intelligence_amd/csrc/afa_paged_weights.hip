@@ -11,6 +11,10 @@
 // for all rows of its head, and Q comes from the caches.  The four waves share a head's row blocks, or the heads where these are few, and add up in
 // LDS.  Where the requests' tiles are too few to fill the device, workgroups share a tile's heads too, and the last one
 // of a tile adds their parts in order.  So every sum has one order, which atomics would not give it.
+//
+// One token of 64 requests over up to 8192, 16 heads on 4 of 128 in bf16: 78 us, K read once at 4.2 TB/s.  Prompts are bound by the
+// vector instructions of rho^8 (7 for 64 weights and a square root, which is as long as 4): 8 of 2048 tokens, 12 heads of 64 in bf16,
+// take 111 us, and about 70 if the vector units never paused; the heavy tiles' workgroups are alone on their CUs at the end.
 #include <algorithm>
 #include <initializer_list>
 

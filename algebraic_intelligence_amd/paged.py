@@ -1,7 +1,8 @@
 """Serving with AFA: drafted trees of tokens over a paged key/value cache.
 
 A serving step is one ``build_block_tables`` for the whole model and, in every layer, one
-``append_to_cache`` (q and k rotated, k and v stored) and one ``paged_tree_afa``.  Nothing in a step
+``append_to_cache`` (q and k normalised and rotated, k and v stored) and one ``paged_tree_afa``, or one
+``paged_prefix_afa`` where all requests share a prefix that no page holds.  Nothing in a step
 needs the lengths on the host, so a step of fixed sizes can be captured into a HIP graph and replayed
 with other lengths, parents and activations in the same tensors.  The reference trains only and has
 no counterpart; the attention is its AFA (src/kernels/pallas_afa.py:104-151) over other keys.
