@@ -18,9 +18,9 @@
 // leaves of a row block is added up by a launch of its own, which has all of the device for it: the last workgroup of a row block
 // alone takes longer (84 us in all for 40 and 7, 256 rows of 4 heads behind 8192), and so does the own keys' launch (16 us more).
 //
-// 32 requests of up to 32 tokens, 16 heads on 4 of 128 in fp16, behind 30001 tokens: 291 us and 13 for the parts, 0.7 PFLOP/s; matrix
-// instructions take 34% of the SIMDs' cycles and vector ones 51%, an eighth of them at once.  256 of one token behind 8192: 41 and
-// 10, half of it parts and the first tiles.  The paged kernel takes 435 us for the former.
+// 32 requests of up to 32 tokens, 16 heads on 4 of 128 in fp16, behind 30001 tokens: 330 us, 65 of them for the own keys and 12 for the
+// parts, so 0.8 PFLOP/s; matrix instructions take 34% of the SIMDs' cycles and vector ones 51%, an eighth of them at once.  The
+// paged kernel takes 435 us for the prefix alone.  256 requests of one token behind 8192: 41 us and 10, a third of it parts.
 #include "afa_paged_attend.h"
 
 namespace afa {
