@@ -342,8 +342,8 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       float* odd = (float*)&lds_k[0][0];
       for (int d = tid; d < D; d += THREADS) odd[d] = 0.0f;
       __syncthreads();
-      for (int e = tid; e < (min(t1 * kPagedTile, L) - t0 * kPagedTile) * CHD; e += THREADS) {
-        const int key = e / CHD, c = e - key * CHD;
+      for (int64_t e = tid; e < (int64_t)(min(t1 * kPagedTile, L) - t0 * kPagedTile) * CHD; e += THREADS) {
+        const int key = (int)(e / CHD), c = (int)(e - (int64_t)key * CHD);
         float x[8];
         RowChunk<DT>::unpack(*(const u32x4_t*)(v_base + (uint64_t)(uint32_t)(t0 * kPagedTile + key) * f.v_slot + 16 * c), x);
 #pragma unroll

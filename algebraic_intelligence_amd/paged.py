@@ -287,12 +287,12 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
         eps = _norm_eps(eps)
         if not isinstance(norms, (tuple, list)) or len(norms) != 2:
             raise TypeError("norms must be a pair (q_scale, k_scale)")
-        norms = [_norm_scale(name, t, plan.head_dim, plan.dtype, plan.device)
-                 for name, t in zip(("q_scale", "k_scale"), norms)]
-        if torch.is_grad_enabled() and (norms[0].requires_grad or norms[1].requires_grad):
+        q_scale = _norm_scale("q_scale", norms[0], plan.head_dim, plan.dtype, plan.device)
+        k_scale = _norm_scale("k_scale", norms[1], plan.head_dim, plan.dtype, plan.device)
+        if torch.is_grad_enabled() and (q_scale.requires_grad or k_scale.requires_grad):
             _no_gradient("append_to_cache")
         if forward_ad._current_level >= 0:
-            _no_tangents("append_to_cache", *norms)
+            _no_tangents("append_to_cache", q_scale, k_scale)
     (q, sq), (k, sk), (v, sv) = (_rows(plan, "q", q, plan._q_shape), _rows(plan, "k", k, plan._kv_shape),
                                  _rows(plan, "v", v, plan._kv_shape))
     page_strides = _pages(plan, k_pages, v_pages)
@@ -326,7 +326,7 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
         with _lib.on_device(dev):
             rc = _lib.lib().afa_paged_append_norm(
                 plan._ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, q_out.data_ptr(), kp, vp, page_strides,
-                norms[0].data_ptr(), norms[1].data_ptr(), eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
+                q_scale.data_ptr(), k_scale.data_ptr(), eps, _lib.ptr(c), _lib.ptr(s), 0 if c is None else c.shape[0],
                 _lib.ptr(positions), axes, cuts, _lib.stream_ptr(dev))
         _lib.check(rc, "afa_paged_append_norm")
         return q_out
