@@ -14,7 +14,7 @@
 //
 // One token of 64 requests over up to 8192, 16 heads on 4 of 128 in bf16: 78 us, K read once at 4.2 TB/s.  Prompts are bound by the
 // vector instructions of rho^8 (7 for 64 weights and a square root, which is as long as 4): 8 of 2048 tokens, 12 heads of 64 in bf16,
-// take 111 us, and about 70 if the vector units never paused; the heavy tiles' workgroups are alone on their CUs at the end.
+// take 104 us, and about 70 if the vector units never paused.
 #include <algorithm>
 #include <initializer_list>
 
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight
   constexpr int KS = (D + KB - 1) / KB;   // chunks of a row a lane
   constexpr bool FULL = D % KB == 0;
   constexpr int NG = key_groups<DT, D>(), TILE = 16 * NG;
-  __shared__ int first[SCAN + 1], scan[WAVES], flag;
+  __shared__ int first[SCAN + 1], scan[WAVES], longest[WAVES], flag;
   __shared__ float red[WAVES][TILE];
   const WeightArgs& a = f.a;
   const afa_paged_plan& p = a.plan;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight
   for (int r0 = 0; r0 < R; r0 += SCAN) {
     // tiles of the requests before each of these
     {
-      int n[4], sum = 0;
+      int n[4], sum = 0, most = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int r = r0 + 4 * tid + u;
@@ -160,7 +160,11 @@ __global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight
           if (fresh > 0) n[u] = (int)((unsigned)(a.sched.cached[r] + fresh + TILE - 1) / TILE);
         }
         sum += n[u];
+        most = max(most, n[u]);
       }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+      if (lane == 0) longest[wave] = most;
       int at = tiles_before(sum, scan);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -170,19 +174,32 @@ __global__ __launch_bounds__(THREADS, (resident<DT, D>())) void afa_paged_weight
       if (tid == THREADS - 1) first[SCAN] = at;
       __syncthreads();
     }
-    const int tiles = first[SCAN];
+    const int tiles = __builtin_amdgcn_readfirstlane(first[SCAN]);
     const int coarse = first[SCAN / 64 * lane];
     // heads of a tile over so many workgroups; requests beyond the first SCAN would need counts of their own
     const int splits = R <= SCAN && tiles > 0 ? max(1, min(K, f.most / tiles)) : 1;
-    const int64_t items = (int64_t)tiles * splits;
-    // there and back, as the later tiles of a prompt are seen by fewer rows: 8 prompts of 2048 took 124 us, 131 without
+    // Long prompts (1024 rows of a key head or more, on average) of about one length go by columns: all requests' first tiles, then
+    // their second, for the later tiles of a prompt are seen by fewer rows.  8 of 2048 tokens take 104 us, one after the other 111;
+    // 8 of 1024 to 2048 90 and 92; 32 of 512 to 1024, two rows each, 71 and 69; 64 of 256 take 56 either way.
+    const int tall = __builtin_amdgcn_readfirstlane(max(max(longest[0], longest[1]), max(longest[2], longest[3])));
+    const bool columns = R <= SCAN && (int64_t)p.starts[R] * G >= 1024 * R && 3 * (int64_t)tall * R <= 4 * (int64_t)tiles;
+    const int64_t items = (columns ? (int64_t)tall * R : tiles) * splits;
+    // there and back, for the same reason: 124 us for 131 without, one after the other
     for (int64_t k = 0, item; (item = k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x)) < items; ++k) {
-      const int tile = (int)(item / splits), split = (int)(item - (int64_t)tile * splits);
-      // the request: the last whose first tile is not behind this one, in two steps of the lanes
-      static_assert(SCAN / 64 <= 64, "entries between two coarse ones");
-      const int step = SCAN / 64, at0 = (__popcll(__ballot(coarse <= tile)) - 1) * step;
-      const int mine = first[at0 + min(lane, step - 1)];
-      const int lo = __builtin_amdgcn_readfirstlane(at0 + __popcll(__ballot(lane < step && mine <= tile)) - 1);
+      int tile = (int)(item / splits), lo;
+      const int split = (int)(item - (int64_t)tile * splits);
+      if (columns) {
+        const int column = tile / R;
+        lo = tile - column * R;
+        tile = __builtin_amdgcn_readfirstlane(first[lo]) + column;
+        if (tile >= __builtin_amdgcn_readfirstlane(first[lo + 1])) continue;
+      } else {
+        // the request: the last whose first tile is not behind this one, in two steps of the lanes
+        static_assert(SCAN / 64 <= 64, "entries between two coarse ones");
+        const int step = SCAN / 64, at0 = (__popcll(__ballot(coarse <= tile)) - 1) * step;
+        const int mine = first[at0 + min(lane, step - 1)];
+        lo = __builtin_amdgcn_readfirstlane(at0 + __popcll(__ballot(lane < step && mine <= tile)) - 1);
+      }
       const int r = r0 + lo, kb = (tile - first[lo]) * TILE;
       const int start = p.starts[r], n = p.starts[r + 1] - start, c = a.sched.cached[r], keys = c + n, nrows = n * G;
       const bool tree = a.masks != nullptr && n <= p.max_tree;

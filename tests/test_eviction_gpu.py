@@ -77,6 +77,17 @@ def test_weights_of_long_drafts(dt, new, max_tree, parents, G):
     _check(x, _den(x), what=(new, G))
 
 
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 48), (BF16, 256)])
+@pytest.mark.parametrize("lens,G", [([(5, 200), (0, 150), (33, 190), (64, 170)], 1), ([(0, 64)] * 3, 1),
+                                    ([(70, 130), (0, 0), (64, 129), (3, 140), (66, 131)], 2), ([(0, 300)], 3),
+                                    ([(10, 130), (0, 0), (900, 1), (3, 140)], 4), ([(5, 300), (0, 220), (33, 290), (9, 0), (64, 270)], 4),
+                                    ([(40, 600)], 2)])
+def test_weights_of_prompts_alike(dt, D, lens, G):
+    """Prompts of about one length, some with a request without tokens among them, and of other lengths."""
+    x = _Cache(dt, lens, 2 * G, 2, D, 16, max_tree=0, seed=D + G, parents=False, tail=1)
+    _check(x, _den(x), what=(lens, G))
+
+
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("scale", [0.05, 3.0, 8.0])
 def test_weights_of_far_scores(dt, scale):
