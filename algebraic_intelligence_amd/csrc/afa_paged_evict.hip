@@ -27,7 +27,7 @@ namespace {
 constexpr int PICK = 1024, PICK_WAVES = PICK / 64;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT, COPIES = 8;  // of a bin, in banks of their own: neighbours often share one
 constexpr int LOADS = 8;                                  // weights of a thread in flight
-constexpr int MOVE = 1024, BATCH = 8;                     // threads of a mover, and units that each holds
+constexpr int MOVE = 1024, FEW = 256, BATCH = 8;          // threads of a mover, or of one for short streams, and units that each holds
 
 constexpr int SLICE = LOADS * PICK;                       // tokens of a workgroup where a request has several
 constexpr int PASSES = 3;
@@ -118,7 +118,8 @@ __device__ __forceinline__ void find_digit(const int (&n)[2], int need, int* wav
   if (tid == 0) found[0] = -1;
   __syncthreads();
   int earlier = upto - n[0] - n[1];
-  for (int v = 0; v < wave; ++v) earlier += wave_sum[v];
+#pragma unroll
+  for (int v = 0; v < PICK_WAVES; ++v) earlier += v < wave ? wave_sum[v] : 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (earlier < need && need <= earlier + n[k]) {
@@ -191,8 +192,10 @@ __device__ __forceinline__ Lists lists_of(const EvictArgs& a, const EvictSpace& 
 }
 
 __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a) {
-  __shared__ int bins[COPIES * BINS], wave_sum[PICK_WAVES], found[2];
+  __shared__ __attribute__((aligned(16))) int bins[COPIES * BINS];
+  __shared__ int wave_sum[PICK_WAVES], found[2];
   __shared__ int2 counts[LOADS * PICK_WAVES];
+  static_assert(COPIES == 8, "pieces of 16 bytes");
   const EvictSpace s = evict_space(a);
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t width = a.table_width * a.page_size;
@@ -232,12 +235,14 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
       count_digits(v, base, q.hi, pass, top, bins);
     }
     __syncthreads();
-    int n[2];
+    // two bins are 64 bytes, four pieces of 16; lanes four apart, which would meet in their banks, begin with another piece
+    int n[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      n[k] = 0;
-#pragma unroll
-      for (int i = 0; i < COPIES; ++i) n[k] += bins[(BINS - 1 - 2 * tid - k) * COPIES + i];
+    for (int i = 0; i < 4; ++i) {
+      const int piece = (i + (lane >> 2)) & 3;
+      const int4 x = *(const int4*)&bins[(BINS - 2 - 2 * tid) * COPIES + 4 * piece];
+      n[0] += piece >= 2 ? (x.x + x.y) + (x.z + x.w) : 0;
+      n[1] += piece >= 2 ? 0 : (x.x + x.y) + (x.z + x.w);
     }
     find_digit(n, need, wave_sum, found);
     if (found[0] < 0) {  // none is needed
@@ -418,8 +423,8 @@ __global__ __launch_bounds__(PICK) void afa_paged_slice_list_kernel(const EvictA
 // Rows as `units` of type T each; a chunk is up to BATCH units a thread, a.rows rows.  Long chunks wait for one another less: with
 // 256, 512 and 1024 threads 4 requests of up to 131072 tokens take 170, 142 and 133 us in all, 64 of up to 8192 126, 124 and 124.
 // Rows pass by the caches (5 us less in each): what is moved is not read again soon.
-template <typename T>
-__global__ __launch_bounds__(MOVE, 4) void afa_paged_move_kernel(const EvictArgs a, int units) {
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void afa_paged_move_kernel(const EvictArgs a, int units) {
   __shared__ int ticket;
   const EvictSpace s = evict_space(a);
   const int64_t streams = a.requests * 2 * a.kv_heads, stream = blockIdx.x % streams;
@@ -457,12 +462,12 @@ __global__ __launch_bounds__(MOVE, 4) void afa_paged_move_kernel(const EvictArgs
     int from[BATCH];
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
+      const int e = u * THREADS + (int)threadIdx.x, i = e / units;
       from[u] = e < count && first + i >= start ? kept[first + i] : -1;
     }
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int e = u * MOVE + (int)threadIdx.x, i = e / units;
+      const int e = u * THREADS + (int)threadIdx.x, i = e / units;
       if (from[u] < 0) continue;
       moves |= 1u << u;
       x[u] = __builtin_nontemporal_load((const T*)(row(from[u]) + (e - i * units) * sizeof(T)));
@@ -480,10 +485,16 @@ __global__ __launch_bounds__(MOVE, 4) void afa_paged_move_kernel(const EvictArgs
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       if (!(moves >> u & 1)) continue;
-      const int e = u * MOVE + (int)threadIdx.x, i = e / units, to = slot_of(a, table, first + i);
+      const int e = u * THREADS + (int)threadIdx.x, i = e / units, to = slot_of(a, table, first + i);
       if (to >= 0) __builtin_nontemporal_store(x[u], (T*)(row(to) + (e - i * units) * sizeof(T)));
     }
   }
+}
+
+template <typename T>
+void move_go(const EvictArgs& a, int units, bool few, dim3 grid, hipStream_t st) {
+  if (few) hipLaunchKernelGGL((afa_paged_move_kernel<T, FEW>), grid, dim3(FEW), 0, st, a, units);
+  else hipLaunchKernelGGL((afa_paged_move_kernel<T, MOVE>), grid, dim3(MOVE), 0, st, a, units);
 }
 
 // Slices of a request, 0 where one workgroup has all of its tokens.  That takes about 20 us and 7 for every slice, requests side
@@ -512,8 +523,13 @@ hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
                     a.ps.k_slot * a.esz, a.ps.v_page * a.esz, a.ps.v_head * a.esz, a.ps.v_slot * a.esz})
     while (v % unit != 0) unit /= 2;
   const int units = (int)(bytes / unit);
-  a.rows = 1;  // a power of two
-  while (2 * a.rows * units <= MOVE * BATCH) a.rows *= 2;
+  auto rows_of = [&](int threads) {  // a power of two
+    int rows = 1;
+    while (2 * rows * units <= threads * BATCH) rows *= 2;
+    return rows;
+  };
+  const bool few = a.budget <= rows_of(FEW);  // one chunk
+  a.rows = rows_of(few ? FEW : MOVE);
   a.log_page = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)a.page_size) : -1;
   a.chunks = (a.budget + a.rows - 1) / a.rows;
   a.slices = (int)slices_of(a.requests, a.table_width * a.page_size);
@@ -530,12 +546,12 @@ hipError_t paged_evict_launch(EvictArgs a, hipStream_t st) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t streams = 2 * a.requests * a.kv_heads, most = std::max<int64_t>(1, (int64_t(1) << 20) / streams);
-  const dim3 grid((unsigned)(streams * std::min<int64_t>(a.chunks, most))), block(MOVE);
+  const dim3 grid((unsigned)(streams * std::min<int64_t>(a.chunks, most)));
   switch (unit) {
-    case 16: hipLaunchKernelGGL((afa_paged_move_kernel<u32x4_t>), grid, block, 0, st, a, units); break;
-    case 8: hipLaunchKernelGGL((afa_paged_move_kernel<u32x2_t>), grid, block, 0, st, a, units); break;
-    case 4: hipLaunchKernelGGL((afa_paged_move_kernel<unsigned>), grid, block, 0, st, a, units); break;
-    default: hipLaunchKernelGGL((afa_paged_move_kernel<unsigned short>), grid, block, 0, st, a, units); break;
+    case 16: move_go<u32x4_t>(a, units, few, grid, st); break;
+    case 8: move_go<u32x2_t>(a, units, few, grid, st); break;
+    case 4: move_go<unsigned>(a, units, few, grid, st); break;
+    default: move_go<unsigned short>(a, units, few, grid, st); break;
   }
   return hipGetLastError();
 }
