@@ -104,6 +104,7 @@ __device__ __forceinline__ void count_digits(const float (&v)[LOADS], int base, 
   const unsigned mask = (1u << (above - shift)) - 1;
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
+    if (base + k * PICK >= hi) break;  // code that is not run is not fetched, which short requests wait for
     const unsigned u = order_bits(v[k]);
     if (base + k * PICK + (int)threadIdx.x < hi && (above == 32 || u >> above == top >> above))
       atomicAdd(&bins[(u >> shift & mask) * COPIES + threadIdx.x % COPIES], 1);
@@ -147,6 +148,9 @@ __device__ __forceinline__ void list_tokens(const EvictArgs& a, const Choice& q,
   __syncthreads();  // counts is free
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
+    kind[k] = 0;
+    overs[k] = equals[k] = 0;
+    if (base + k * PICK >= q.c) continue;
     const int i = base + k * PICK + tid;
     const unsigned u = order_bits(v[k]);
     kind[k] = i >= q.c ? 0 : i < q.lo || i >= q.hi || u > top ? 2 : u == top ? 1 : 0;
@@ -158,7 +162,8 @@ __device__ __forceinline__ void list_tokens(const EvictArgs& a, const Choice& q,
   // sums before each wave's, in place, and the batch's
   static_assert(LOADS * PICK_WAVES == 128, "two entries a lane");
   if (wave == 0) {
-    const int2 x = counts[2 * lane], y = counts[2 * lane + 1];
+    const bool some = base + 2 * lane / PICK_WAVES * PICK < q.c;
+    const int2 x = some ? counts[2 * lane] : int2{0, 0}, y = some ? counts[2 * lane + 1] : int2{0, 0};
     const int o = lanes_up_to(x.x + y.x), e = lanes_up_to(x.y + y.y);
     counts[2 * lane] = int2{o - x.x - y.x, e - x.y - y.y};
     counts[2 * lane + 1] = int2{o - y.x, e - y.y};
@@ -172,6 +177,7 @@ __device__ __forceinline__ void list_tokens(const EvictArgs& a, const Choice& q,
   const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
+    if (base + k * PICK >= q.c) break;
     const int i = base + k * PICK + tid;
     const int2 b = counts[k * PICK_WAVES + wave];
     const int o = earlier.x + b.x + __popcll(overs[k] & below), e = earlier.y + b.y + __popcll(equals[k] & below);
