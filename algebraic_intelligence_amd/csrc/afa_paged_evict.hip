@@ -222,10 +222,13 @@ __global__ __launch_bounds__(PICK) void afa_paged_pick_kernel(const EvictArgs a)
     if ((int64_t)i * a.rows >= q.c) to.before[i] = q.m;
   int need = q.need;
   unsigned top = 0;  // the bits of the least weight that stays, as far as they are known
-  float v[LOADS], next[LOADS];  // the next batch comes while this one is counted
+  float v[LOADS], next[LOADS] = {};  // the next batch comes while this one is counted
   auto load = [&](int base, int end) {
 #pragma unroll
-    for (int k = 0; k < LOADS; ++k) next[k] = w[min(base + k * PICK + tid, end - 1)];
+    for (int k = 0; k < LOADS; ++k) {
+      if (base + k * PICK >= end) break;
+      next[k] = w[min(base + k * PICK + tid, end - 1)];
+    }
   };
   auto take = [&](int base, int end) {
 #pragma unroll
