@@ -13,7 +13,8 @@
 // waits for nothing before it says so, so every wait ends.
 //
 // HBM bounds the last launch: every row that moves is read and written once.  64 requests of up to 8192 tokens cut back to 2048, 4 heads
-// of 128 in bf16: 19 us for the choice and 104 for the rows (4.6 TB/s); 4 of up to 131072 cut back to 32768: 34 and 100.
+// of 128 in bf16: 18 us for the choice and 104 for the rows (4.6 TB/s); 4 of up to 131072 cut back to 32768: 33 and 100.  Short
+// requests, 2 of 124 tokens: 11 and 6, a chain of barriers and of code that is fetched once.
 #include <algorithm>
 #include <initializer_list>
 
@@ -431,6 +432,7 @@ __global__ __launch_bounds__(PICK) void afa_paged_slice_list_kernel(const EvictA
 
 // Rows as `units` of type T each; a chunk is up to BATCH units a thread, a.rows rows.  Long chunks wait for one another less: with
 // 256, 512 and 1024 threads 4 requests of up to 131072 tokens take 170, 142 and 133 us in all, 64 of up to 8192 126, 124 and 124.
+// A stream that one chunk of 256 threads holds has no more of them: 68 requests of 23 tokens, 8 heads of 48, take 7 us and not 20.
 // Rows pass by the caches (5 us less in each): what is moved is not read again soon.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void afa_paged_move_kernel(const EvictArgs a, int units) {
@@ -506,12 +508,12 @@ void move_go(const EvictArgs& a, int units, bool few, dim3 grid, hipStream_t st)
   else hipLaunchKernelGGL((afa_paged_move_kernel<T, MOVE>), grid, dim3(MOVE), 0, st, a, units);
 }
 
-// Slices of a request, 0 where one workgroup has all of its tokens.  That takes about 20 us and 7 for every slice, requests side
-// by side; five launches about 30 and 0.1 for every slice of all requests.  4 requests of 131072 tokens take 122 us and 35, 256 of
-// 16384 with the rows' launch 59 and (of 16448) 104.
+// Slices of a request, 0 where one workgroup has all of its tokens.  With the rows' launch that takes about 16 us and 8 for every slice,
+// requests side by side; five launches 35, and 0.1 for a request and 0.04 for its every slice.  48 requests in three slices (up to
+// 16384 tokens and a page) take 32 us and 38, in four 40 and 39, in five 49 and 39; 80 in five 49 and 54; 84 in nine 82 and 69, in 17 146 and 96.
 int64_t slices_of(int64_t requests, int64_t max_len) {
   const int64_t slices = (max_len + SLICE - 1) / SLICE;
-  return requests < 70 && slices * (70 - requests) > 100 ? slices : 0;
+  return requests * (3 + 2 * slices) < 385 * slices - 1285 ? slices : 0;
 }
 
 }  // namespace
