@@ -147,6 +147,26 @@ def test_norm_sums_many_rows_the_same_way_each_time():
         _close(dw, ww, bw, "dw")
 
 
+@pytest.mark.parametrize("dt,B,H,K,L,D,layout", [(BF16, 5, 6, 3, 7001, 64, "blhd"), (F32, 1, 5, 2, 9501, 128, "bhld"),
+                                                 (F16, 3, 7, 2, 2901, 48, "blhd"), (BF16, 2, 5, 5, 3601, 96, "bhld")])
+def test_norm_of_many_rows(dt, B, H, K, L, D, layout):
+    """Groups of heads with a ragged last one, and results larger than the caches."""
+    rng = np.random.default_rng(L)
+    q, k, gq, gk = _layouts([torch.tensor(rng.standard_normal((B, n, L, D), dtype=np.float32), device="cuda").to(dt)
+                             for n in (H, K, H, K)], layout, D, dt)
+    qs, ks = (torch.tensor(1 + 0.3 * rng.standard_normal(D), device="cuda").float() for _ in range(2))
+    leaves = [t.requires_grad_(True) for t in (q, k, qs, ks)]
+    tab = _tables(L, D)
+    y = A.apply_ago_norm_rotations(*leaves, tab)
+    dx, dw = (g[2 * i:2 * i + 2] for g in [torch.autograd.grad(y, leaves, (gq, gk))] for i in range(2))
+    c, s, at = _f64(tab[0]), _f64(tab[1]), np.broadcast_to(np.arange(L)[None, :, None], (B, L, 1))
+    for i, (x, w, g) in enumerate(((q, qs, gq), (k, ks, gk))):
+        _close(y[i], *_forward(_f64(x), _f64(w), 1e-6, c, s, at, (D // 2,), dt), i)
+        (wx, bx), (ww, bw) = _backward(_f64(x), _f64(w), 1e-6, _f64(g), c, s, at, (D // 2,), dt)
+        _close(dx[i], wx, bx, ("dx", i))
+        _close(dw[i], ww, bw, ("dw", i))
+
+
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 def test_norm_edges(dt):
     """Rows of zeros with and without eps, infinities and NaN, positions outside the tables, empty tensors, expanded cotangents."""
