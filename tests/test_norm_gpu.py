@@ -302,6 +302,24 @@ def test_append_with_norms_is_the_training_call():
     assert torch.equal(vp[slots // 16, :, slots % 16], v)
 
 
+def test_append_with_norms_of_many_tokens_is_the_training_call():
+    """Groups of heads, the same bits as apply_ago_norm_rotations gives: serving meets what training made."""
+    T, H, K, D = 3300, 6, 2, 128
+    pool = A.PagePool(220, 16, 2, 2100)
+    plan = _plan(pool, T, T, 0, H, K, D, BF16)
+    A.build_block_tables(plan, _i32([3, 0]), _i32([2000, 1300]))
+    q, k, v = (torch.randn(T, n, D, device="cuda", dtype=BF16) for n in (H, K, K))
+    qs, ks = (1 + torch.randn(D, device="cuda") / 4 for _ in range(2))
+    kp, vp = _pages(pool, K, D, BF16)
+    tab = _tables(2100, D)
+    out = A.append_to_cache(q, k, v, kp, vp, plan, tab, norms=(qs, ks))
+    y, z = A.apply_ago_norm_rotations(q.transpose(0, 1)[None], k.transpose(0, 1)[None], qs, ks, tab, plan.positions[None, :, None])
+    assert torch.equal(out, y[0].transpose(0, 1))
+    slots = plan.slots.long()
+    assert torch.equal(kp[slots // 16, :, slots % 16], z[0].transpose(0, 1))
+    assert torch.equal(vp[slots // 16, :, slots % 16], v)
+
+
 def test_norm_refusals():
     q, w = torch.zeros(1, 2, 3, 64, device="cuda", dtype=BF16), torch.ones(64, device="cuda")
     tab = _tables(20, 64)

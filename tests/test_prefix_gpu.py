@@ -94,6 +94,24 @@ def test_prefix_scores(dt, scale, pscale):
     _Shared(dt, [(200, 4), (33, 9), (0, 3)], 4, 2, 64, 32, 250, seed=3, scale=scale, pscale=pscale).check(what=scale)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 48])
+@pytest.mark.parametrize("scale,pscale,how", [(3.0, 1.0, None), (0.05, 1.0, None), (4.0, 2.0, None), (1.0, 0.0, None), (1.0, 8.0, None),
+                                              (1.0, 6.0, "rising"), (1.0, 6.0, "falling"), (1.0, 1.0, "negative"),
+                                              (6.0, 6.0, "negative")])
+def test_prefix_scores_of_many_rows(dt, D, scale, pscale, how):
+    """Scores near 0 and beyond 100 of both signs over more than 64 rows a key head; larger and smaller ones from tile to tile; a
+    prefix that points away from all queries.  In fp16 a weight far below its row's largest is off by up to 2^-25 of that: 300
+    of them by 9e-6, within the error of the weights (_weight_error)."""
+    x = _Shared(dt, [(20, 40), (0, 33), (3, 9)], 4, 2, D, 16, 300, seed=6, scale=scale, pscale=pscale)
+    if how in ("rising", "falling"):
+        steps = torch.linspace(0.02, 1, 300, device="cuda")[None, :, None]
+        x.pk = (x.pk.float() * (steps if how == "rising" else steps.flip(1))).to(dt)
+    if how == "negative":
+        x.q, x.pk = (x.q.abs() + 0.25).to(dt), -x.pk.abs()
+    x.check(what=(D, scale, pscale, how))
+
+
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 def test_prefix_negative_scores(dt):
     """A prefix that all points away from the queries: weights far below 1, no sink."""
