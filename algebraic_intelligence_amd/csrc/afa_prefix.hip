@@ -317,6 +317,15 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     const int64_t my_part = part_of(slot - from_slot);
     const int size = wide_group(parts);
     const bool mine = row0 + 32 * wave + l32 < nrows;
+    // All of a row block's keys are the sums themselves: their place is the row's.  Only a row block that goes on behind this
+    // stretch has a part in it that is the first, so that a slot has room for one of these; where row blocks are more than slots,
+    // several lie within a stretch.
+    int mine_at = row0 + 32 * wave + l32;
+    asm volatile("" : "+v"(mine_at));  // formed again: no register holds it over the keys
+    const int mine_token = mine_at / G;
+    const int64_t at = (int64_t)mine_token * (int)p.heads + (hk * G + mine_at - mine_token * G);
+    float* const to = parts == 1 ? f.shared.top + at * D : f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D;
+    float* const to_den = parts == 1 ? f.shared.bottom + at : part_den + my_part * WIDE_ROWS + 32 * wave + l32;
     float zero = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -332,9 +341,9 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
         if (!mine || (D < DP && d >= D)) continue;
         // a part that is added up here goes where every XCD sees it
         if (size > 1) put4(buffer, (uint32_t)((my_part * WIDE_ROWS + 32 * wave + l32) * D + d) * 4, x);
-        else *(f32x4_t*)(f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D + d) = x;
+        else *(f32x4_t*)(to + d) = x;
       }
-    if (mine && g == 0) put1(part_den + my_part * WIDE_ROWS + 32 * wave + l32, den);
+    if (mine && g == 0) put1(to_den, den);
     // A value that is not finite is the sum of every row, as weights are above 0.  It may have become NaN in the product, where
     // a weight may be rounded to 0: each feature's sum of such values, the same for all rows, takes its place.  (Where the row
     // sum is not finite either the row is NaN already.)
@@ -351,7 +360,6 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
           if (!(__builtin_fabsf(x[i]) < __builtin_inff())) atomicAdd(&odd[8 * c + i], x[i]);
       }
       __syncthreads();
-      float* to = f.part + head0 * D + (my_part * WIDE_ROWS + 32 * wave + l32) * D;
       if (mine)
         for (int d = 4 * g; d < D; d += 8)
           for (int i = d; i < d + 4; ++i) {
@@ -365,18 +373,18 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     // the last of a group to finish adds its parts up, over the first of them
     const int g0 = (slot - from_slot) / size * size, here = min(size, parts - g0);
     if (!arrived(a.sched.count + (int64_t)hk * 4 * f.slots + part_of(g0), here, &flag)) continue;
-    const int64_t to = part_of(g0) * WIDE_ROWS;
+    const int64_t sum_at = part_of(g0) * WIDE_ROWS;
     sum_parts<THREADS>(buffer, part_den, here, min(WIDE_ROWS, nrows - row0), D, sums,
                        [&](int i) { return part_of(g0 + i) * WIDE_ROWS; },
                        [&](int r, int d, f32x4_t x) {
                          // of the first part this thread alone reads these features
-                         put4(buffer, (uint32_t)((to + r) * D + d) * 4, x);
-                         if (d == 0) put1(part_sum + to + r, sums[r]);
+                         put4(buffer, (uint32_t)((sum_at + r) * D + d) * 4, x);
+                         if (d == 0) put1(part_sum + sum_at + r, sums[r]);
                        });
   }
 }
 
-// The parts of every row added up in their order: a thread has four features of a row.
+// The parts of every row that has several, added up in their order: a thread has four features of a row.
 __global__ __launch_bounds__(THREADS) void afa_prefix_join_kernel(const PagedFast f) {
   const afa_paged_plan& p = f.a.plan;
   const int D = f.dim, quads = D / 4, G = f.a.group, H = (int)p.heads;
@@ -388,6 +396,7 @@ __global__ __launch_bounds__(THREADS) void afa_prefix_join_kernel(const PagedFas
     const int row = token * G + (at - token * H - hk * G), block = row / WIDE_ROWS, r = row - block * WIDE_ROWS;
     const int64_t key0 = (int64_t)block * cost + kPagedLead, from = key0 / stretch;
     const int parts = (int)((key0 + tiles - 1) / stretch - from) + 1, size = wide_group(parts), n = (parts + size - 1) / size;
+    if (parts == 1) continue;  // these are in their places
     const float* den = size > 1 ? f.part_sum : f.part_den;
     // part i of the row block: a slot's second where it begins there, else its first
     auto place = [&](int i) {
