@@ -190,7 +190,9 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
         if (__ballot(!(top <= __builtin_fmaf(c2, -0.5f / kMost, 0.5f * kMost))) != 0) {
           // a row's largest weight so far now lies in [1, 256)
           top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-          const float z = top + __builtin_sqrtf(__builtin_fmaf(top, top, c2));
+          // below 0 without cancellation: a row begins with c2 so large that its scores may lie far down and weigh much
+          const float far = __builtin_sqrtf(__builtin_fmaf(top, top, c2)) + __builtin_fabsf(top);
+          const float z = top < 0.0f ? c2 * __builtin_amdgcn_rcpf(far) : far;
           if (z > kMost && z < __builtin_inff()) {
             const int j = (__builtin_bit_cast(int, z) >> 23) - 127;  // 0 to 2^7 and more
             const float root = __builtin_bit_cast(float, max(127 - j, 1) << 23);
