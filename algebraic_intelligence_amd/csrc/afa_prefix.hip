@@ -13,7 +13,9 @@
 // While a wave forms the weights of a tile, the scores of the next one are on the matrix cores, and the other wave of its
 // SIMD has its products there.  Weights enter the product rounded to the type, as in the training forward: vector and matrix
 // instructions bound this kernel, and the second plane that the paged kernel keeps would be a third of its products and a
-// sixth of its vector instructions.  The rounding is as large as the result's own.  Row sums are of the weights in fp32.
+// sixth of its vector instructions.  The rounding is as large as the result's own in bf16, and in fp16 for weights of 2^-18 of the row's
+// largest and more.  Smaller ones are off by up to 2^-29 of the largest each: of very many keys far below one that is 2^-11, as the
+// result's own rounding, for 2^18 keys, and grows with them.  Row sums are of the weights in fp32.
 // The line of a key head's tiles over all row blocks is cut into even stretches, one for each resident workgroup.  What a cut
 // leaves of a row block is added up by a launch of its own, which has all of the device for it: the last workgroup of a row block
 // alone takes longer (84 us in all for 40 and 7, 256 rows of 4 heads behind 8192), and so does the own keys' launch (16 us more).
@@ -40,7 +42,9 @@ __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 }
 
 constexpr int WIDE_ROWS = 32 * WAVES, RING = 4;
-constexpr float kFirstRoot = 0x1p15f;  // the eighth root of kFirstScale
+// kFirstScale's eighth root and logarithm
+constexpr float kFirstRoot = 0x1p15f;
+constexpr int kFirstPower = 120;
 
 // Parts of a row block that the join adds up; of more, groups are added up first, each by its last workgroup.
 constexpr int WIDE_PARTS = 16;
@@ -68,7 +72,8 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   const int G = a.group, L = a.prefix.len;
   // With y = c s, (c rho(s))^8 = (y + sqrt(y^2 + c^2))^8: a factor of the weights costs nothing where the scores carry its eighth
   // root.  In bf16 q carries 1/8, exactly, so that y is what the products give and c^2 = D / 64.  In fp16, where small
-  // numbers would lose digits, y = kappa q.k, and kappa takes the power of two by which a row's weights are scaled too.
+  // numbers would lose digits, y = kappa q.k, and kappa takes the eighth root of the power of two by which a row's weights are
+  // scaled too: lowered n times it is off by up to n 2^-23, which is 2^-20 n of a part's weights.
   constexpr bool F16 = DT == AFA_F16;
   constexpr float C2 = (float)D / 64, LOW = kLowScore * (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
   // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
@@ -140,7 +145,8 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     };
     f32x16_t o[NDB], s_even, s_odd;
     float den = 0.0f;
-    float kappa = kFirstRoot * 0.125f, c2 = C2 * kFirstRoot * kFirstRoot;  // fp16: 2^k / 8 and 4^k C2
+    int power = kFirstPower;  // fp16: the row's weights are scaled by 2^power; kappa is an eighth of its eighth root, and c2 with it
+    float kappa = kFirstRoot * 0.125f, c2 = F16 ? C2 * kFirstRoot * kFirstRoot : C2;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -188,15 +194,18 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
         // weights end at kMost^8 = 32768: y ends where y + sqrt(y^2 + c2) is kMost
         constexpr float kMost = 3.6680162f;
         if (__ballot(!(top <= __builtin_fmaf(c2, -0.5f / kMost, 0.5f * kMost))) != 0) {
-          // a row's largest weight so far now lies in [1, 256)
+          // A row's largest weight so far now lies in [16, 32), as in the paged kernel: weights below the normal numbers are off
+          // by up to 2^-25 / 16 = 2^-29 of it each, and it may grow by 2^10 before the row comes here again.  32 drafts behind 30001
+          // tokens take 329 us with it in [1, 2), 337 in [16, 32), 352 in [128, 256) and 361 in [1024, 2048).
           top = __builtin_fmaxf(top, __shfl_xor(top, 32));
           // below 0 without cancellation: a row begins with c2 so large that its scores may lie far down and weigh much
-          const float far = __builtin_sqrtf(__builtin_fmaf(top, top, c2)) + __builtin_fabsf(top);
+          const float t = __builtin_fmaf(top, top, c2), far = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), __builtin_fabsf(top));
           const float z = top < 0.0f ? c2 * __builtin_amdgcn_rcpf(far) : far;
           if (z > kMost && z < __builtin_inff()) {
-            const int j = (__builtin_bit_cast(int, z) >> 23) - 127;  // 0 to 2^7 and more
-            const float root = __builtin_bit_cast(float, max(127 - j, 1) << 23);
-            const float ratio = 8 * j < 127 ? __builtin_bit_cast(float, (127 - 8 * j) << 23) : 0.0f;
+            const int j = (int)(8.0f * __builtin_amdgcn_logf(z)) - 4;  // 10 and more
+            const float root = __builtin_amdgcn_exp2f(-0.125f * (float)j);
+            const float ratio = j < 127 ? __builtin_bit_cast(float, (127 - j) << 23) : 0.0f;
+            power -= j;
             kappa *= root;
             c2 *= root * root;
             den *= ratio;
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = s[e];
       }
-      const float cc = F16 ? c2 : C2, low = F16 ? LOW * 8.0f * kappa : LOW;
+      const float low = F16 ? LOW * 8.0f * kappa : LOW;
       float least = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) least = __builtin_fminf(least, w[e]);
@@ -218,7 +227,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
       if (__ballot(!(least > low)) == 0) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float t = __builtin_fmaf(w[e], w[e], cc);
+          const float t = __builtin_fmaf(w[e], w[e], c2);
           const float rho = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), w[e]);
           const float p2 = rho * rho;
           const float p4 = p2 * p2;
@@ -229,9 +238,9 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           // far below 0 without cancellation, and above 0 to the end: -infinity weighs 2^-126 too; a NaN stays one
-          const float y = w[e], t = __builtin_fmaf(y, y, cc);
+          const float y = w[e], t = __builtin_fmaf(y, y, c2);
           const float far = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), y <= low ? __builtin_fabsf(y) : y);
-          const float rho = y <= low ? cc * __builtin_amdgcn_rcpf(far) : far;
+          const float rho = y <= low ? c2 * __builtin_amdgcn_rcpf(far) : far;
           const float p2 = rho * rho;
           const float p4 = p2 * p2;
           const float p8 = p4 * p4;
@@ -310,10 +319,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
     // the factor is taken back: c^8, and in fp16 the rows' powers of two
     constexpr float C8 = C2 * C2 * C2 * C2;
     float back = 1.0f / C8;
-    if constexpr (F16) {
-      const int k = (__builtin_bit_cast(int, kappa) >> 23) - 127 + 3;
-      back *= __builtin_bit_cast(float, min(max(127 - 8 * k, 1), 254) << 23);
-    }
+    if constexpr (F16) back *= __builtin_bit_cast(float, min(max(127 - power, 1), 254) << 23);
     den *= back;
     auto part_of = [&](int i) { return (int64_t)2 * (from_slot + i) + (i == 0); };
     const int64_t my_part = part_of(slot - from_slot);

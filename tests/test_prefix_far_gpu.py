@@ -75,3 +75,45 @@ def test_prefix_far_below(dt, D, where, few):
     for size in [*(sizes if dt == F16 else sizes[::3]), mixed]:
         x.place(m * size, prefix.transpose(1, 0, 2), lambda r, n: (far if where == "all" else near)(n))
         x.compare(0.0 if where == "all" else 0.5, (where, "mixed" if size is mixed else size))
+
+
+@pytest.mark.parametrize("L", [30001, 65536])
+@pytest.mark.parametrize("D", [32, 128])
+def test_prefix_of_one_key_above_very_many_in_fp16(D, L):
+    """A first key of large weight and value 0, then keys of one weight and value 1, which so are all of a row's result: rows with
+    from 2^-14 to 2^-26 of the first one's weight for each of them.
+
+    A row's factor leaves its largest weight at 16 or above, so that fp16 holds the others to half a step of it, 2^-11, or to half of
+    its smallest one: 2^-25 / 16 of the largest.  Equal weights of 11 bits add up without a rounding within the 16 keys of a
+    product, whose result is added to the sum by one rounding or a cut, 2^-23: L / 16 of them.  The row sums add L / 32 of
+    fp32 weights by u each, and those of a tile by 5 u."""
+    K = 2 * torch.cuda.get_device_properties(0).multi_processor_count  # one workgroup has all of a head's prefix
+    T = 96
+    x = _Shared(F16, [(0, 1)] * T, K, K, D, 16, 16, seed=1, max_tree=0, parents=False)
+    a = 1.0 + np.arange(T) / 64
+    first, small = 5.0, np.exp2(-(14 + 12 * np.arange(T) / (T - 1)) / 8)  # (rho's eighth root of the shares)
+    rho = first * a + np.sqrt(1 + (first * a) ** 2)
+    s = (rho * small - 1 / (rho * small)) / 2  # rho(s) = rho * small
+    q = np.zeros((T, 1, D))
+    q[:, 0, 0], q[:, 0, 1] = a * np.sqrt(D), s * np.sqrt(D)
+    x.q = torch.tensor(q, device="cuda").half().expand(T, K, D).contiguous()
+    pk = torch.zeros(1, L, D, device="cuda", dtype=F16)
+    pk[:, 0, 0], pk[:, 1:, 1] = first, 1.0
+    pv = torch.ones(1, L, D, device="cuda", dtype=F16)
+    pv[:, 0] = 0.0
+    x.pk, x.pv = pk.expand(K, L, D), pv.expand(K, L, D)
+    x.kp.zero_(), x.vp.zero_()  # a row's own key weighs 1, its value is 0
+    out, den = x.call(0.5, return_denominator=True)
+    assert torch.equal(out, out[:, :1].expand_as(out)) and torch.equal(den, den[:, :1].expand_as(den))
+    q = x.q[:, 0].double().cpu().numpy()
+    weigh = lambda score: P.rho8(score / np.sqrt(D))  # noqa: E731
+    top, low = weigh(q[:, 0] * first), weigh(q[:, 1])
+    wden = top + (L - 1) * low + 1.5
+    want = (L - 1) * low / wden
+    e = (121 + 16 + L / 32 + 5) * U + 2.2e-4
+    got, gden = out[:, 0].double().cpu().numpy(), den[:, 0].double().cpu().numpy()
+    bound = (2 * e + L / 16 * 2.0 ** -23 + 2.0 ** -11 + 2.0 ** -11) * want + (L - 1) * 2.0 ** -29 * np.maximum(top, low) / wden
+    off = np.abs(got - want[:, None]) - bound[:, None]
+    at = int(np.argmax(off.max(1)))
+    assert off.max() <= 0, ("row", at, got[at, 0], want[at], bound[at], low[at] / top[at])
+    assert (np.abs(gden - wden) <= e * wden).all()
