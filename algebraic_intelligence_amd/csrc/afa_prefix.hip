@@ -71,11 +71,13 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.group, L = a.prefix.len;
   // With y = c s, (c rho(s))^8 = (y + sqrt(y^2 + c^2))^8: a factor of the weights costs nothing where the scores carry its eighth
-  // root.  In bf16 q carries 1/8, exactly, so that y is what the products give and c^2 = D / 64.  In fp16, where small
+  // root.  In bf16 q carries 1/8, exactly, so that y is what the products give and c^2 = D / 64; 1/16 where that would be above 1
+  // and weights would leave fp32 before the formula's do, by c^8 = 16 for D = 128 (scores from 23000 on).  In fp16, where small
   // numbers would lose digits, y = kappa q.k, and kappa takes the eighth root of the power of two by which a row's weights are
   // scaled too: lowered n times it is off by up to n 2^-23, which is 2^-20 n of a part's weights.
   constexpr bool F16 = DT == AFA_F16;
-  constexpr float C2 = (float)D / 64, LOW = kLowScore * (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
+  constexpr float CARRIED = F16 || D <= 64 ? 0.125f : 0.0625f;
+  constexpr float C2 = (float)D * CARRIED * CARRIED, LOW = kLowScore * 8 * CARRIED * (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
   // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
   const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads), hk = (int)(blockIdx.x - (unsigned)slot * (unsigned)p.kv_heads);
   const char* k_base = (const char*)a.prefix.k + hk * a.prefix.k_head * 2;
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned u = qf[kc][e];
-          qf[kc][e] = Elem<DT>::pack(Elem<DT>::lo(u) * 0.125f, Elem<DT>::hi(u) * 0.125f);
+          qf[kc][e] = Elem<DT>::pack(Elem<DT>::lo(u) * CARRIED, Elem<DT>::hi(u) * CARRIED);
         }
     }
     // they are here before the ring's first loads, which the compiler does not count

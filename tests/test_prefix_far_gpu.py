@@ -77,6 +77,26 @@ def test_prefix_far_below(dt, D, where, few):
         x.compare(0.0 if where == "all" else 0.5, (where, "mixed" if size is mixed else size))
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("D", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("few", [False, True])
+def test_prefix_far_above(dt, D, few):
+    """One key of a score up to 30000, whose weight of up to 2^127 is a row's, beside ordinary ones; v is at most 1."""
+    rng = np.random.default_rng(D)
+    x = _Exact(dt, [(0, 9), (5, 13)] if few else LENS, 4, 2, D, 70)
+    T = x.q.shape[0]
+    x.pv.clamp_(-1, 1)
+    prefix = np.zeros((2, 70, D))
+    prefix[:, :, 0] = rng.choice([-1.0, 1.0], (2, 70))
+    prefix[:, 40, 0] = 64.0
+    q = np.zeros((T, 4, D))
+    for score in (3000, 14000, 22000, 25000, 29000):
+        # q's first feature in steps that bf16 holds
+        q[..., 0] = np.floor(score * np.sqrt(D) / 64 / 32) * 32 if dt == BF16 else np.floor(score * np.sqrt(D) / 64)
+        x.place(q, prefix, lambda r, n: np.where(np.arange(D) == 0, rng.choice([-1.0, 0.0], (n, 2, 1)), 0.0))
+        x.compare(0.5, score)
+
+
 @pytest.mark.parametrize("L", [30001, 65536])
 @pytest.mark.parametrize("D", [32, 128])
 def test_prefix_of_one_key_above_very_many_in_fp16(D, L):
