@@ -408,6 +408,17 @@ __device__ __forceinline__ float rho8_ref(float s) {
   return k4 * k4;
 }
 
+// The weight of the score s * scale over the paged cache: above 0 as its formula is, so that a value that is not finite is seen,
+// also where it or a square on its way passes the type's range, the NaN of a score of -infinity among them.
+__device__ __forceinline__ float rho8_above_0(float s, double scale) {
+  const float w = rho8_ref(s * (float)scale);
+  return s < 0.0f && !(w >= 0x1p-126f) ? 0x1p-126f : w;
+}
+__device__ __forceinline__ double rho8_above_0(double s, double scale) {
+  const double w = rho8_f64(s * scale);
+  return s < 0.0 && !(w >= 0x1p-1022) ? 0x1p-1022 : w;
+}
+
 // Workgroup id -> (b*h, query block) for the causal/non-causal attention grids
 // (B*H*nqb workgroups).  Dispatch order is heaviest query block first across all heads, so list
 // scheduling approximates longest-processing-time-first; block id b runs on XCD b mod 8, and

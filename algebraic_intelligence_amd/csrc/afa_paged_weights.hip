@@ -60,8 +60,7 @@ __global__ __launch_bounds__(KEYS) void afa_paged_weight_key_kernel(const Weight
           const int64_t k = page * a.k_page + h / a.group * a.k_head + pos % p.page_size * a.k_slot;
           A s = 0;
           for (int e = 0; e < D; ++e) s += elem_of<DT, A>(a.q, q + e) * elem_of<DT, A>(a.k_pages, k + e);
-          if constexpr (DT == AFA_F64) sum += rho8_f64(s * a.scale) / d;
-          else sum += (double)(rho8_ref(s * (float)a.scale) / d);
+          sum += (double)(rho8_above_0(s, a.scale) / d);
         }
       }
     }
