@@ -7,7 +7,8 @@ import torch
 
 import algebraic_intelligence_amd as A
 from algebraic_intelligence_amd import _lib
-from tests.test_paged_gpu import BF16, F32, F64, _Cache
+from oracle import paged_oracle as P
+from tests.test_paged_gpu import BF16, F16, F32, F64, U, _Cache, _f64
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +57,49 @@ def test_weights_of_a_score_of_minus_infinity(dt, D):
         assert (w[0, :7] > 0).all() and (w[0, 8:42] > 0).all()
     lens, kept = A.evict_from_cache(x.kp, x.vp, x.pool, got[1], torch.tensor([42, 10], dtype=torch.int32, device="cuda"), 41)
     assert lens.tolist() == [41, 10] and torch.equal(kept[0, :41], torch.cat((got[1][0, :7], got[1][0, 8:42])))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("flags", [0, _lib.FLAG_GENERIC])
+def test_weights_of_rows_with_large_denominators(dt, D, flags):
+    """Denominators up to fp32's end: a row gives its largest key 1, whatever the denominator, and others their shares.
+
+    Scores are exact but for their scaling (16 u of a weight), the denominator is off by (121 + keys) u and 2.2e-4 on 16-bit inputs, as a
+    weight is; the inverse of a denominator above 2^126 is a subnormal number with 22 bits or more: 2^-22.  Two keys of one score
+    have half each."""
+    x = _Cache(dt, [(37, 2), (70, 3), (0, 5)], 4, 2, D, 16, max_tree=0, parents=False, seed=D)
+    T = x.q.shape[0]
+    score = np.array([3000, 14000, 25000, 27600, 28500, 29500, 30500, 31500, 32500, 32700])[:T, None]
+    unit = 4 if dt == F16 else 64
+    first = np.floor(score * np.sqrt(D) / 64 / unit) * unit
+    if dt == BF16:  # 8 bits
+        first = torch.tensor(first).bfloat16().double().numpy()
+        first = np.where(first * 64 / np.sqrt(D) > 32700, first - 64, first)
+    q = np.zeros((T, 4, D))
+    q[..., 0] = first
+    x.q = torch.tensor(q, device="cuda").to(dt)
+
+    def own(r, n):
+        k = np.zeros((n, 2, D))
+        k[0, :, 0] = 64.0
+        k[min(2, n - 1):3, 1, 0] = 64.0  # the second head has two such keys in a request
+        return k
+
+    _keys(x, own)
+    # the largest denominators are twice a weight in the second head: those that pass fp32 are left out below
+    _, den = A.paged_tree_afa(x.q, x.kp, x.vp, x.plan, 0.5, return_denominator=True)
+    w = _f64(_weights(x, den, flags))
+    for r, (c, n) in enumerate(x.lens):
+        want = np.zeros(c + n)
+        k = _f64(x.k[r])
+        for i in range(n):
+            t = x.starts[r] + i
+            for h in range(4):
+                if not torch.isfinite(den[t, h]):
+                    continue
+                weight = np.where(np.arange(c + n) <= c + i, P.rho8(k[:, h // 2] @ _f64(x.q[t, h]) / np.sqrt(D)), 0)
+                want += weight / (weight.sum() + 0.5)
+        e = 2 * ((121 + c + n) * U + (2.2e-4 if dt != F32 else 0)) + 2.0 ** -22 + (4 * n + 4) * U
+        assert (np.abs(w[r, :c + n] - want) <= e * want + 4 * n * 2.0 ** -126).all(), (r, w[r, :4], want[:4])
+    assert (_f64(den) > 2.0 ** 126).any()
