@@ -23,7 +23,7 @@ FLAG_ACCUMULATE, FLAG_PARTIAL = 0x100, 0x200
 FLAG_ZERO_TAIL = 0x400
 
 (OK, ERR_NULL, ERR_DTYPE, ERR_SHAPE, ERR_HEAD_DIM, ERR_SINK, ERR_VALID_LEN, ERR_EPS, ERR_ROTARY,
- ERR_ALIGN, ERR_WORKSPACE, ERR_UNSUPPORTED, ERR_GAMMA, ERR_SCRATCH_LIMIT) = range(14)
+ ERR_ALIGN, ERR_WORKSPACE, ERR_UNSUPPORTED, ERR_GAMMA, ERR_SCRATCH_LIMIT, ERR_OVERLAP) = range(15)
 NOALLOC_SCRATCH_BYTES = 64 << 20
 ERR_HIP = 100
 

@@ -123,6 +123,7 @@ const char* afa_status_string(int status) {
     case AFA_ERR_UNSUPPORTED: return "combination not supported by this build";
     case AFA_ERR_GAMMA: return "gamma must be finite and strictly positive";
     case AFA_ERR_SCRATCH_LIMIT: return "the call needs more workspace than afa_fwd_noalloc's fixed scratch";
+    case AFA_ERR_OVERLAP: return "k and v pages must not overlap";
     case AFA_ERR_HIP: return "HIP runtime error";
     default: return "unknown status";
   }

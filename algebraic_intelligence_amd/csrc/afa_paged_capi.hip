@@ -1,7 +1,9 @@
 // C ABI of the paged-cache serving operators (include/afa.h): argument checks and dispatch.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
+#include <utility>
 
 #include "../../include/afa.h"
 #include "afa_launch.h"
@@ -81,6 +83,68 @@ afa::PageStrides page_strides_of(const afa_paged_plan& p, const int64_t* s) {
   return afa::PageStrides{page, head, p.head_dim, page, head, p.head_dim};
 }
 
+// Whether `left` is a sum of the axes' steps (bytes), each taken between `least` and `most` times.  The axes come in falling order of
+// their steps, and reach[i] is what those from i on come to at least and at most: of steps that each pass what the later ones
+// come to, as strides of arrays whose elements lie apart do, two numbers at most are left to try of each.
+struct Axis {
+  int64_t step, least, most;
+};
+struct Reach {
+  int64_t low, high;
+};
+bool sum_of_steps(const Axis* a, const Reach* reach, int count, int64_t left, int& tries) {
+  if (left < reach[0].low || left > reach[0].high) return false;
+  if (count == 0) return true;  // both are 0
+  if (--tries < 0) return false;
+  // multiples of the step that leave what the later axes reach
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t low = std::max(-floor_div(reach[1].high - left, a->step), a->least);
+  const int64_t high = std::min(floor_div(left - reach[1].low, a->step), a->most);
+  for (int64_t n = low; n <= high && tries > 0; ++n)
+    if (sum_of_steps(a + 1, reach + 1, count - 1, left - n * a->step, tries)) return true;
+  return false;
+}
+
+// Whether k and v pages of these strides share a byte, as far as 4096 steps tell, which is to the end where an array's own
+// elements lie apart and both have the same strides, or lie in places of their own altogether.
+bool pages_share(const afa_paged_plan& p, const void* k_pages, const void* v_pages, const int64_t* strides) {
+  const int64_t esz = p.dtype == AFA_F64 ? 8 : p.dtype == AFA_F32 ? 4 : 2;
+  const int64_t sizes[4] = {p.num_pages, p.kv_heads, p.page_size, p.head_dim};
+  Axis a[9];
+  int count = 0;
+  auto add = [&](int64_t step, int64_t least, int64_t most) {
+    if (step < 0) {
+      step = -step;
+      std::swap(least, most);
+      least = -least;
+      most = -most;
+    }
+    if (step == 0 || least == most) return true;
+    a[count++] = Axis{step, least, most};
+    return step < int64_t(1) << 50 && (double)step * (double)(most - least) < 0x1p58;  // sums of them fit
+  };
+  bool fits = add(1, 1 - esz, esz - 1);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = (i < 3 ? strides[i] : 1), v = (i < 3 ? strides[3 + i] : 1), n = sizes[i] - 1;
+    const int64_t most = int64_t(1) << 46;
+    if (!within(k, -most, most) || !within(v, -most, most)) return false;
+    if (k == v) {
+      fits = fits && add(k * esz, -n, n);
+    } else {
+      fits = fits && add(k * esz, 0, n);
+      fits = fits && add(v * esz, -n, 0);
+    }
+  }
+  if (!fits) return false;
+  std::sort(a, a + count, [](const Axis& x, const Axis& y) { return x.step > y.step; });
+  Reach reach[10];
+  reach[count] = Reach{0, 0};
+  for (int i = count - 1; i >= 0; --i)
+    reach[i] = Reach{reach[i + 1].low + a[i].step * a[i].least, reach[i + 1].high + a[i].step * a[i].most};
+  int tries = 4096;
+  return sum_of_steps(a, reach, count, (int64_t)((uintptr_t)v_pages - (uintptr_t)k_pages), tries);
+}
+
 // The arguments of a cache write; `turned`: q_out is written.
 int check_append(afa::AppendArgs& a, const afa_paged_plan* plan, const void* q, const void* k, const void* v,
                  const int64_t* strides, void* q_out, void* k_pages, void* v_pages, const int64_t* page_strides,
@@ -106,6 +170,7 @@ int check_append(afa::AppendArgs& a, const afa_paged_plan* plan, const void* q, 
     a.k_t = strides[2]; a.k_h = strides[3];
     a.v_t = strides[4]; a.v_h = strides[5];
   }
+  if (page_strides != nullptr && pages_share(p, k_pages, v_pages, page_strides)) return AFA_ERR_OVERLAP;
   a.ps = page_strides_of(p, page_strides);
   a.slots = p.slots;
   a.tokens = (int)p.max_tokens; a.heads = (int)p.heads; a.kv_heads = (int)p.kv_heads; a.dim = (int)p.head_dim;
@@ -423,6 +488,7 @@ int afa_paged_evict(int dtype, int64_t num_pages, int64_t page_size, int64_t req
   const int64_t width = table_width * page_size;
   if (!within(budget, 1, width) || first < 0 || recent < 0 || first > budget || recent > budget - first) return AFA_ERR_SHAPE;
   if (weights_stride < width && requests > 1) return AFA_ERR_SHAPE;
+  if (page_strides != nullptr && pages_share(p, k_pages, v_pages, page_strides)) return AFA_ERR_OVERLAP;
   if (requests > (kLaunchThreads - 1) / 2048 / kv_heads || requests > (kLaunchThreads - 1) / 1024 / ((width + 8191) / 8192))
     return AFA_ERR_SHAPE;
   afa::EvictArgs a = {};

@@ -44,6 +44,7 @@ enum afa_status {
   AFA_ERR_GAMMA = 12,        /* OACE gamma not finite or not positive (src/loss.py:33-34) */
   AFA_ERR_SCRATCH_LIMIT = 13, /* afa_fwd_noalloc: the call needs more workspace than the fixed
                                  per-device scratch (AFA_NOALLOC_SCRATCH_BYTES) */
+  AFA_ERR_OVERLAP = 14,      /* k and v pages share places */
   AFA_ERR_HIP = 100          /* a HIP runtime call failed; afa_last_hip_error() has the code */
 };
 
@@ -329,7 +330,8 @@ int afa_paged_build(const afa_paged_plan* plan, const int32_t* cached, const int
  * slot is not stored).  q (max_tokens, heads, head_dim), k and v (max_tokens, kv_heads, head_dim) with
  * strides {q_t, q_h, k_t, k_h, v_t, v_h} in elements (NULL: contiguous); q_out contiguous, nullable
  * without tables.  page_strides {k_page, k_head, k_slot, v_page, v_head, v_slot} (NULL: contiguous); no two
- * places of the pages share memory, nor do they with q, k, v and q_out.
+ * places of the pages share memory (AFA_ERR_OVERLAP where page_strides and the addresses say that k's and v's do), nor do
+ * they with q, k, v and q_out.
  * rot_cos, rot_sin (rot_len, head_dim / 2) in fp32 (fp64 for AFA_F64), nullable: no rotation.
  * positions (max_tokens, axes) or NULL for the plan's (axes 1); sections: as in ago_rotate_axes.
  */
@@ -427,6 +429,7 @@ int afa_paged_weights(const afa_paged_plan* plan, const void* q, const int64_t* 
  * weights, 0 behind them, and lens (requests,) the lengths.  budget at most table_width * page_size; first + recent at most
  * budget.  A cached length is taken as at most what the request's pages hold.  Places behind the budget keep their contents; the
  * pages go back to the pool with the next afa_paged_build.  A page id outside the pool is neither read nor written.
+ * page_strides and places that k and v share: as in afa_paged_append.
  * workspace: afa_paged_evict_workspace_size() bytes (max_len: table_width * page_size), 16-byte aligned, or NULL.
  */
 size_t afa_paged_evict_workspace_size(int64_t requests, int64_t max_len, int64_t budget, int64_t kv_heads, int64_t head_dim);
