@@ -29,11 +29,14 @@ namespace afa {
 
 namespace {
 
-// 1 / sqrt(x) in fp32, the hardware's approximation refined by one Newton step.
+// 1 / sqrt(x) in fp32, the hardware's approximation refined by one Newton step.  Numbers below the normal ones, which it takes for 0, go
+// through it times 2^80.
 __device__ __forceinline__ float inverse_root(float x) {
-  const float r = __builtin_amdgcn_rsqf(x);
-  const float y = r * __builtin_fmaf(-0.5f * x * r, r, 1.5f);
-  return r > 0.0f && r < __builtin_inff() ? y : r;  // x = 0 and infinity
+  const bool small = x < 0x1p-100f;
+  const float z = small ? x * 0x1p80f : x;
+  const float r = __builtin_amdgcn_rsqf(z);
+  const float y = r * __builtin_fmaf(-0.5f * z * r, r, 1.5f);
+  return (r > 0.0f && r < __builtin_inff() ? y : r) * (small ? 0x1p40f : 1.0f);  // x = 0 and infinity
 }
 __device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
 
