@@ -231,7 +231,7 @@ __global__ __launch_bounds__(BWD) void ago_norm_bwd_chunk_kernel(const NormArgs 
       sum = group_sum<LPR>(sum);
       dot = group_sum<LPR>(dot);
       const float r = inverse_root(sum / (float)a.dim + (float)a.norm.eps);
-      const float mean = dot * r * over;  // of h . xh
+      const float mean = r == 0.0f ? 0.0f : dot * r * over;  // of h . xh: 0 past the range, where dot may be infinite
 #pragma unroll
       for (int e = 0; e < EPC; ++e) {
         const float xh = x[e] * r;
@@ -392,7 +392,8 @@ __global__ __launch_bounds__(64) void ago_norm_bwd_row_kernel(const NormArgs a, 
       dot += g0 * w[2 * q] * x0;
       if (two) dot += g1 * w[2 * q + 1] * x1;
     }
-    const A r = inverse_root(wave_sum(sum) / (A)D + (A)a.norm.eps), mean = wave_sum(dot) * r / (A)D;
+    const A r = inverse_root(wave_sum(sum) / (A)D + (A)a.norm.eps), all = wave_sum(dot);
+    const A mean = r == 0 ? (A)0 : all * r / (A)D;
     for (int q = lane; 2 * q < D; q += 64) {
       const bool two = 2 * q + 1 < D;
       A x0 = take<DT>(x, 2 * q), x1 = two ? take<DT>(x, 2 * q + 1) : (A)0;

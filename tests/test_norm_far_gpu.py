@@ -55,3 +55,34 @@ def test_small_rows_on_their_way_into_the_cache(dt, D):
         want, bound = _forward(x, np.ones(D), 0.0, None, None, None, None, dt)
         r = (2.0 ** -149 + 2.0 ** -150) / np.mean(x ** 2, -1, keepdims=True) / 2
         _close(got[None], want, bound + 1.1 * r * np.abs(want), "cache")
+
+
+@pytest.mark.parametrize("dt", [BF16, F32, F64])
+@pytest.mark.parametrize("D", [64, 7, 600])
+@pytest.mark.parametrize("size", [1e20, 1e37, 2e38])
+def test_gradient_of_rows_past_the_range(dt, D, size):
+    """Rows whose mean square passes fp32's range give 0, and so do their gradients, whose true values are |g| / |x|; they add nothing to a
+    scale's gradient.  Infinities and NaN stay visible."""
+    x = torch.full((1, 2, 3, D), size, device="cuda", dtype=dt)
+    x[0, 0, 1] = 0.5
+    g = torch.full_like(x, 8.0)
+    scale = torch.linspace(0.5, 2, D, device="cuda", dtype=F64 if dt == F64 else F32)
+    leaves = x.clone().requires_grad_(True), scale.requires_grad_(True)
+    y = A.apply_ago_norm_rotations(leaves[0], None, leaves[1], None)
+    dx, dw = torch.autograd.grad(y, leaves, g)
+    if dt == F64:
+        assert torch.isfinite(y).all() and torch.isfinite(dx).all() and torch.isfinite(dw).all()
+        return
+    rest = torch.ones(1, 2, 3, dtype=torch.bool, device="cuda")
+    rest[0, 0, 1] = False
+    assert (y[rest] == 0).all() and (dx[rest] == 0).all()
+    alone = x[:, :1, 1:2].clone()
+    (wx, bx), (ww, bw) = _backward(_f64(alone), _f64(scale), 1e-6, _f64(g[:, :1, 1:2]), None, None, None, None, dt)
+    _close(dx[:, :1, 1:2], wx, bx, "the ordinary row")
+    _close(dw, ww, bw, "its scale's gradient")
+    x[0, 1, 2, 3] = float("inf")
+    g[0, 1, 0, 2] = float("nan")
+    leaves = x.clone().requires_grad_(True), scale.detach().requires_grad_(True)
+    y = A.apply_ago_norm_rotations(leaves[0], None, leaves[1], None)
+    dx, dw = torch.autograd.grad(y, leaves, g)
+    assert torch.isnan(y[0, 1, 2, 3]) and torch.isnan(dx[0, 1, 2, 3]) and torch.isnan(dx[0, 1, 0, 2]) and torch.isnan(dw[2])
