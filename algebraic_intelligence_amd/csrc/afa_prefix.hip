@@ -237,16 +237,19 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
         }
       } else {
         apart(w);
+        // Weights end at 2^-126, as those of the requests' own keys do, while the row's factor leaves that a normal number.  In bf16 it is
+        // that of the scaled weights: 2^-122 for heads of 32 and 128, 2^-120 for 96 (scores of -16800 and below).
+        const float end = F16 ? __builtin_fmaxf(C2 * C2 * C2 * C2 * __builtin_bit_cast(float, max(power + 1, 1) << 23), 0x1p-126f) : 0x1p-126f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          // far below 0 without cancellation, and above 0 to the end: -infinity weighs 2^-126 too; a NaN stays one
+          // far below 0 without cancellation, and above 0 to the end: -infinity weighs the least there is too; a NaN stays one
           const float y = w[e], t = __builtin_fmaf(y, y, c2);
           const float far = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), y <= low ? __builtin_fabsf(y) : y);
           const float rho = y <= low ? c2 * __builtin_amdgcn_rcpf(far) : far;
           const float p2 = rho * rho;
           const float p4 = p2 * p2;
           const float p8 = p4 * p4;
-          w[e] = y < -0x1p60f || p8 < 0x1p-126f ? 0x1p-126f : p8;
+          w[e] = y < -0x1p60f || p8 < end ? end : p8;
         }
       }
       if constexpr (decltype(mask)::value) {

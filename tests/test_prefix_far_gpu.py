@@ -77,7 +77,7 @@ def test_prefix_far_below(dt, D, where, few):
         x.compare(0.0 if where == "all" else 0.5, (where, "mixed" if size is mixed else size))
 
 
-@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("D", [32, 48, 64, 96, 128])
 @pytest.mark.parametrize("few", [False, True])
 def test_prefix_far_above(dt, D, few):
@@ -95,6 +95,31 @@ def test_prefix_far_above(dt, D, few):
         q[..., 0] = np.floor(score * np.sqrt(D) / 64 / 32) * 32 if dt == BF16 else np.floor(score * np.sqrt(D) / 64)
         x.place(q, prefix, lambda r, n: np.where(np.arange(D) == 0, rng.choice([-1.0, 0.0], (n, 2, 1)), 0.0))
         x.compare(0.5, score)
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 32), (F16, 48), (F16, 96), (F16, 128), (F32, 48)])
+@pytest.mark.parametrize("few", [False, True])
+def test_prefix_where_weights_end(dt, D, few):
+    """Keys of one score beyond -27554, prefix and own, weigh 2^-126 each: without a sink a row is the mean of all values, however far
+    the keys are.  The mean of N values is off by N u of their sizes and its own rounding."""
+    x = _Exact(dt, [(0, 9), (5, 13)] if few else LENS, 4, 2, D, 90)
+    T = x.q.shape[0]
+    one = lambda n: np.broadcast_to(np.where(np.arange(D) == 0, -64.0, 0.0), (n, 2, D))  # noqa: E731
+    for score in (29000, 1e5, 7e5) if dt == F16 else (29000, 1e5, 1e9, 1e17, 1e36):
+        q = score * np.sqrt(D) / 64
+        x.place(np.full((T, 4, D), min(q, 60000.0) if dt == F16 else q), one(90).transpose(1, 0, 2), lambda r, n: one(n))
+        out, den = (t.double().cpu().numpy() for t in x.call(0.0, return_denominator=True))
+        pv = x.pv.double().cpu().numpy()
+        for r, (c, n) in enumerate(x.lens):
+            v = x.v[r].double().cpu().numpy()
+            for i in range(n):
+                t, seen = x.starts[r] + i, c + i + 1
+                for h in range(4):
+                    values = np.concatenate((pv[h // 2], v[:seen, h // 2]))
+                    want, size = values.mean(0), np.abs(values).mean(0)
+                    bound = 2 * len(values) * U * size + (_half(dt) + 4 * U) * np.abs(want) + _tiny(dt)
+                    assert (np.abs(out[t, h] - want) <= bound).all(), (score, t, h, out[t, h, :3], want[:3])
+                    assert abs(den[t, h] / 2.0 ** -126 - len(values)) <= 2 * len(values) ** 2 * U, (score, den[t, h])
 
 
 @pytest.mark.parametrize("L", [30001, 65536])
