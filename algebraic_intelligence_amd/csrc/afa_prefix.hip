@@ -20,7 +20,7 @@
 // leaves of a row block is added up by a launch of its own, which has all of the device for it: the last workgroup of a row block
 // alone takes longer (84 us in all for 40 and 7, 256 rows of 4 heads behind 8192), and so does the own keys' launch (16 us more).
 //
-// 32 requests of up to 32 tokens, 16 heads on 4 of 128 in fp16, behind 30001 tokens: 330 us, 65 of them for the own keys and 12 for the
+// 32 requests of up to 32 tokens, 16 heads on 4 of 128 in fp16, behind 30001 tokens: 340 us, 65 of them for the own keys and 12 for the
 // parts, so 0.8 PFLOP/s; matrix instructions take 34% of the SIMDs' cycles and vector ones 51%, an eighth of them at once.  The
 // paged kernel takes 435 us for the prefix alone.  256 requests of one token behind 8192: 41 us and 10, a third of it parts.
 #include "afa_paged_attend.h"
@@ -45,6 +45,12 @@ constexpr int WIDE_ROWS = 32 * WAVES, RING = 4;
 // kFirstScale's eighth root and logarithm
 constexpr float kFirstRoot = 0x1p15f;
 constexpr int kFirstPower = 120;
+
+// 2^(p / 8)
+__device__ __forceinline__ float eighth_root_of_2(int p) {
+  const float half = p & 4 ? 1.41421356f : 1.0f, quarter = p & 2 ? 1.18920712f : 1.0f, eighth = p & 1 ? 1.09050773f : 1.0f;
+  return __builtin_bit_cast(float, (127 + (p >> 3)) << 23) * (half * (quarter * eighth));
+}
 
 // Parts of a row block that the join adds up; of more, groups are added up first, each by its last workgroup.
 constexpr int WIDE_PARTS = 16;
@@ -74,10 +80,12 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
   // root.  In bf16 q carries 1/8, exactly, so that y is what the products give and c^2 = D / 64; 1/16 where that would be above 1
   // and weights would leave fp32 before the formula's do, by c^8 = 16 for D = 128 (scores from 23000 on).  In fp16, where small
   // numbers would lose digits, y = kappa q.k, and kappa takes the eighth root of the power of two by which a row's weights are
-  // scaled too: lowered n times it is off by up to n 2^-23, which is 2^-20 n of a part's weights.
+  // scaled too: off by up to 2^-22, which is 2^-19 of a part's weights.
   constexpr bool F16 = DT == AFA_F16;
   constexpr float CARRIED = F16 || D <= 64 ? 0.125f : 0.0625f;
-  constexpr float C2 = (float)D * CARRIED * CARRIED, LOW = kLowScore * 8 * CARRIED * (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
+  constexpr float C2 = (float)D * CARRIED * CARRIED;
+  constexpr float LOW = kLowScore * 8 * CARRIED *
+                        (D == 32 ? 0.70710678f : D == 48 ? 0.8660254f : D == 64 ? 1.0f : D == 96 ? 1.2247449f : 1.4142136f);
   // heads run fastest: with 8 key heads the row blocks of one meet its keys in the same XCD's L2
   const int slot = (int)(blockIdx.x / (unsigned)p.kv_heads), hk = (int)(blockIdx.x - (unsigned)slot * (unsigned)p.kv_heads);
   const char* k_base = (const char*)a.prefix.k + hk * a.prefix.k_head * 2;
@@ -204,12 +212,15 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
           const float t = __builtin_fmaf(top, top, c2), far = __builtin_fmaf(t, __builtin_amdgcn_rsqf(t), __builtin_fabsf(top));
           const float z = top < 0.0f ? c2 * __builtin_amdgcn_rcpf(far) : far;
           if (z > kMost && z < __builtin_inff()) {
-            const int j = (int)(8.0f * __builtin_amdgcn_logf(z)) - 4;  // 10 and more
-            const float root = __builtin_amdgcn_exp2f(-0.125f * (float)j);
+            // z^8 = 2^(8 e) m^8, m in [1, 2): j is its logarithm, rounded down, less 4, which is 11 and more
+            const int bits = __builtin_bit_cast(int, z), e8 = 8 * ((bits >> 23) - 127);
+            const float m = __builtin_bit_cast(float, (bits & 0x7fffff) | 0x3f800000), m2 = m * m, m4 = m2 * m2, m8 = m4 * m4;
+            const int j = e8 + (__builtin_bit_cast(int, m8) >> 23) - 127 - 4;
+            const float root = eighth_root_of_2(-j);
             const float ratio = j < 127 ? __builtin_bit_cast(float, (127 - j) << 23) : 0.0f;
             power -= j;
-            kappa *= root;
-            c2 *= root * root;
+            kappa = 0.125f * eighth_root_of_2(power);
+            c2 = 64 * C2 * kappa * kappa;
             den *= ratio;
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] *= root;
@@ -239,7 +250,8 @@ __global__ __launch_bounds__(THREADS, 2) void afa_prefix_wide_kernel(const Paged
         apart(w);
         // Weights end at 2^-126, as those of the requests' own keys do, while the row's factor leaves that a normal number.  In bf16 it is
         // that of the scaled weights: 2^-122 for heads of 32 and 128, 2^-120 for 96 (scores of -16800 and below).
-        const float end = F16 ? __builtin_fmaxf(C2 * C2 * C2 * C2 * __builtin_bit_cast(float, max(power + 1, 1) << 23), 0x1p-126f) : 0x1p-126f;
+        constexpr float C8 = C2 * C2 * C2 * C2;
+        const float end = F16 ? __builtin_fmaxf(C8 * __builtin_bit_cast(float, max(power + 1, 1) << 23), 0x1p-126f) : 0x1p-126f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           // far below 0 without cancellation, and above 0 to the end: -infinity weighs the least there is too; a NaN stays one
