@@ -707,7 +707,8 @@ def apply_ago_norm_rotations(q, k, q_scale, k_scale, rotary_params=None, positio
     No counterpart in the reference, whose model (src/model.py:262-275) rotates q and k as they are.
 
     Returns (q_out, k_out) (q_out alone without k) in the inputs' dtype and axis order.  Everything between is fp32
-    (fp64) with one rounding: a row whose mean square passes fp32's range gives 0 where it is finite.  Differentiable once, in
+    (fp64) with one rounding, ``eps`` too: a row whose sum of squares passes fp32's range gives 0, and a gradient of 0, where it is
+    finite; squares below fp32's normal numbers keep the digits that it has for them.  Differentiable once, in
     reverse mode, with respect to q, k and both scales, whose gradients are summed in a fixed order."""
     q = _float_input(q)
     shape = q.shape

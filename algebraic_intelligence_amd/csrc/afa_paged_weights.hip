@@ -14,7 +14,7 @@
 //
 // One token of 64 requests over up to 8192, 16 heads on 4 of 128 in bf16: 78 us, K read once at 4.2 TB/s.  Prompts are bound by the
 // vector instructions of rho^8 (7 for 64 weights and a square root, which is as long as 4): 8 of 2048 tokens, 12 heads of 64 in bf16,
-// take 104 us, and about 70 if the vector units never paused.
+// take 105 us, and about 70 if the vector units never paused.
 #include <algorithm>
 #include <initializer_list>
 

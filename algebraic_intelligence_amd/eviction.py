@@ -44,8 +44,9 @@ def accumulate_cache_weights(q: torch.Tensor, k_pages: torch.Tensor, denominator
     q (max_tokens, heads, head_dim), ``k_pages`` and ``masks`` are those of the step's attention, and ``denominator``
     (max_tokens, heads) is what it returned, sink and shared prefix included.  The step's own tokens are set rather than
     added to, so that a place needs no clearing when it is taken again.  Requests without new tokens, and those that were not
-    served, keep their weights.  Tokens of a drafted tree that is not kept count as rows too: for the accepted ones alone,
-    call it with the plan by which they are stored again.  The sums are formed in a fixed order.  Returns weights."""
+    served, keep their weights.  A key whose score is -infinity weighs the least there is.  Tokens of a drafted tree that is not
+    kept count as rows too: for the accepted ones alone, call it with the plan by which they are stored again.  The sums are formed
+    in a fixed order.  Returns weights."""
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or denominator.requires_grad
                                     or weights.requires_grad):
         _no_gradient("accumulate_cache_weights")
@@ -91,8 +92,9 @@ def evict_from_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, pool: PagePoo
     Its ``first`` oldest tokens stay, its ``recent`` newest (first + recent at most budget), and of the others those of the
     largest ``weights`` (max_requests, max_len), the lower place among equal ones; NaN counts as the largest.  What stays keeps its
     order and moves to places 0 .. budget - 1 of the request's pages, in place in ``k_pages`` and ``v_pages`` (num_pages,
-    kv_heads, page_size, head_dim).  Places behind them keep their contents; pages go back to the pool with the next
-    ``build_block_tables`` for the lengths that this returns.  A length is taken as at most what the request's pages hold.
+    kv_heads, page_size, head_dim); pages of k and v that share places are refused, as far as addresses and strides tell.  Places
+    behind the budget keep their contents; pages go back to the pool with the next ``build_block_tables`` for the lengths that this
+    returns.  A length is taken as at most what the request's pages hold.
 
     Returns (lens, weights): the lengths, (max_requests,) int32, and a new (max_requests, max_len) tensor of what the
     tokens that stay had, 0 behind them.  With the same budget every layer of a pool returns the same lengths."""

@@ -276,7 +276,8 @@ def append_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: 
     cast); a position outside them gives NaN.  None: k is stored and q returned as they are.
     ``positions`` (max_tokens, A) int32 with ``sections`` gives positions of A axes as in
     ``apply_ago_axis_rotations``; (max_tokens,) or None, the plan's positions, is one axis.  Tokens
-    without a slot are not stored.  The pages hold k and v in places of their own, apart from q, k and v.
+    without a slot are not stored.  The pages hold k and v in places of their own, apart from q, k and v: k_pages and v_pages
+    that share places are refused, as far as addresses and strides tell.
     For inference: inputs that require a gradient are refused where gradients are recorded."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
                                     or v_pages.requires_grad):
@@ -367,7 +368,12 @@ def paged_prefix_afa(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     The prefix is kept once and met once for all rows of the step, whatever the number of requests.  The pool's lengths count a
     request's own tokens, so that the positions of ``append_to_cache`` are the plan's plus the prefix's length:
     ``positions=plan.positions + k_prefix.shape[1]``.  The plan, q, masks, out and what is returned are as in
-    ``paged_tree_afa``; rows of requests that were not served are 0."""
+    ``paged_tree_afa``; rows of requests that were not served are 0.
+
+    A plan of more than 64 rows a key head (max_tokens * heads / kv_heads) with bf16 or fp16 and head_dim up to 128 rounds the
+    weights over the prefix to that type once, in all of its steps; others, and the weights of the requests' own keys, keep
+    twice its digits.  In fp16 a weight far below a row's largest is off by up to 2^-29 of that: very many such keys, 2^18 and
+    more, can be seen in the result."""
     return _attend("paged_prefix_afa", q, (k_prefix, v_prefix), k_pages, v_pages, plan, sink_omega, masks, out,
                    return_denominator)
 
