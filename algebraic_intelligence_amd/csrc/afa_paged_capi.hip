@@ -106,7 +106,7 @@ bool sum_of_steps(const Axis* a, const Reach* reach, int count, int64_t left, in
 }
 
 // Whether k and v pages of these strides share a byte, as far as 4096 steps tell, which is to the end where an array's own
-// elements lie apart and both have the same strides, or lie in places of their own altogether.
+// elements lie apart and both have the same strides, in any order, or lie in places of their own altogether.
 bool pages_share(const afa_paged_plan& p, const void* k_pages, const void* v_pages, const int64_t* strides) {
   const int64_t esz = p.dtype == AFA_F64 ? 8 : p.dtype == AFA_F32 ? 4 : 2;
   const int64_t sizes[4] = {p.num_pages, p.kv_heads, p.page_size, p.head_dim};
@@ -120,8 +120,15 @@ bool pages_share(const afa_paged_plan& p, const void* k_pages, const void* v_pag
       most = -most;
     }
     if (step == 0 || least == most) return true;
+    if (step >= int64_t(1) << 50 || (double)step * (double)(most - least) >= 0x1p58) return false;  // sums of them fit
+    for (int i = 0; i < count; ++i)
+      if (a[i].step == step) {  // also of k's and v's arrays in another order
+        a[i].least += least;
+        a[i].most += most;
+        return true;
+      }
     a[count++] = Axis{step, least, most};
-    return step < int64_t(1) << 50 && (double)step * (double)(most - least) < 0x1p58;  // sums of them fit
+    return true;
   };
   bool fits = add(1, 1 - esz, esz - 1);
   for (int i = 0; i < 4; ++i) {

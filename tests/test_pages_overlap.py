@@ -84,6 +84,16 @@ def test_large_pages_side_by_side(lib, order):
             _lib.ERR_OVERLAP if off < 0 or strides[3] < span // 2 else _lib.ERR_WORKSPACE)
 
 
+def test_large_pages_in_two_orders(lib):
+    """k by heads and then slots, v by slots and then heads, in the halves of each page of one array."""
+    shape, half = (20000, 8, 64, 128), 8 * 64 * 128
+    s = [2 * half, 64 * 128, 128, 2 * half, 128, 8 * 128]
+    k = 1 << 30
+    assert _evict(lib, _lib.AFA_BF16, shape, k, k + 2 * half, s) == _lib.ERR_WORKSPACE
+    for off in (-1, 1, -half, half, 15000 * 2 * half - 1, -15000 * 2 * half + 1):
+        assert _evict(lib, _lib.AFA_BF16, shape, k, k + 2 * (half + off), s) == _lib.ERR_OVERLAP
+
+
 def test_strides_of_any_size(lib):
     """Numbers that no array has: an answer, and no overflow."""
     for s in (2 ** 62, -2 ** 63, 2 ** 46, 2 ** 45, 0, -1):
